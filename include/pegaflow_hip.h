@@ -559,6 +559,120 @@ int pf_host_wait_word(const uint64_t* word, uint64_t value, uint64_t timeout_us,
                       int* reached);
 
 /* ------------------------------------------------------------------------ */
+/* Paged-cache operators: what a model does with a registered layer's blocks  */
+/* between the transfers above.  No counterpart in the reference, whose       */
+/* blocks are filled and read by the inference engine.                        */
+/*                                                                            */
+/* Rows are [tokens, heads, head_dim] tensors of 16-bit values; a slot is     */
+/* block * block_size + position in the block.  Every call is asynchronous on */
+/* the caller's stream (NULL: the current device's null stream), allocates    */
+/* nothing and may be captured into a graph.  Tensors must lie on the stream's */
+/* device.                                                                    */
+/* ------------------------------------------------------------------------ */
+/* What rows and pages hold.  Rows are BF16 or FP16; pages the same type as    */
+/* the rows, or 8-bit codes with an fp32 scale for each token and head.        */
+enum { PF_KV_BF16 = 1, PF_KV_FP16 = 2, PF_KV_E4M3 = 3, PF_KV_INT8 = 4 };
+/* Order of a block's values: [block_size, heads, head_dim], or               */
+/* [heads, block_size, head_dim].                                              */
+enum { PF_KV_TOKEN_MAJOR = 0, PF_KV_HEAD_MAJOR = 1 };
+#define PF_KV_MAX_HEAD_DIM 256
+
+/* A registered layer as pages of a cache.  A block's K (or V) segment holds its
+ * values in the given order; 8-bit pages then hold [heads, block_size] fp32
+ * scales.  Two-segment layouts whose segments do not overlap (KV-first, K blocks
+ * then V blocks), or one segment whose first half is K and second half V
+ * (blocks-first).  head_dim is a multiple of 16 up to PF_KV_MAX_HEAD_DIM;
+ * data_ptr, bytes_per_block (half of it for one segment) and kv_stride_bytes are
+ * multiples of 16.  Such a layer moves through saves and loads like any other:
+ * its scales travel with its codes. */
+typedef struct pf_kv_pages {
+  pf_kv_layout layout;
+  uint32_t block_size; /* tokens of a block */
+  uint32_t num_heads;  /* KV heads */
+  uint32_t head_dim;
+  uint32_t type;  /* PF_KV_* */
+  uint32_t order; /* PF_KV_TOKEN_MAJOR or PF_KV_HEAD_MAJOR */
+  uint32_t reserved;
+} pf_kv_pages;
+/* Bytes of K (or V) of one block: the values, the scales of 8-bit types, padded
+ * to 16. */
+int pf_kv_segment_bytes(uint32_t block_size, uint32_t num_heads, uint32_t head_dim,
+                        uint32_t type, uint64_t* out);
+
+/* Rows: value (token, head, d) at data + 2 * (token * token_stride + head *
+ * head_stride + d).  Any strides; 16-byte aligned rows move 16 bytes a lane.
+ * Rows that a call writes must not overlap. */
+typedef struct pf_kv_rows {
+  uint64_t data;
+  uint64_t token_stride; /* in values */
+  uint64_t head_stride;  /* in values */
+  uint32_t type;         /* PF_KV_BF16 or PF_KV_FP16 */
+  uint32_t reserved;
+} pf_kv_rows;
+
+/* Writes num_rows rows of K and of V into the pages: row i into slots[i] (int64,
+ * device memory).  A row whose slot is negative, or past the last block, is
+ * padding and written nowhere.  The slots of one call are distinct: of rows
+ * given the same slot, parts of each may stay.
+ *
+ * 8-bit pages: scale = max|x| / 448 (E4M3) or / 127 (INT8) over the head_dim
+ * values of a token and head, code = x / scale rounded to nearest, ties to even,
+ * both in fp32.  Zeros have scale 0; values with an infinity or NaN among them
+ * have scale NaN and codes 0, and read back as NaN. */
+int pf_kv_write(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* v,
+                uint64_t slots, uint64_t num_rows, pf_stream stream);
+/* The reverse: the values at slots[i] into row i of k and v, code * scale rounded
+ * once to the rows' type.  Rows of padding slots are left as they were. */
+int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* v,
+               uint64_t slots, uint64_t num_rows, pf_stream stream);
+
+/* Attention of new tokens over the pages.
+ *
+ * The batch's num_rows query rows are those of num_seqs sequences one after
+ * another: sequence b has rows query_starts[b] to query_starts[b+1], and
+ * seq_lens[b] tokens in all, the new ones last, their K and V already in the
+ * pages.  Its token t lies in block block_table[b * table_stride + t /
+ * block_size].  Query head h reads KV head h / (num_q_heads / num_heads).  The row
+ * at position p attends the tokens t with t <= p (causal), t > p - window (if
+ * window, which needs causal), in blocks that exist: an entry that is negative or
+ * past the last block hides its tokens, whatever they hold.  A row that attends
+ * nothing is 0 (lse -infinity); rows before the first or behind the last sequence
+ * stay as they were.  A length beyond the table is cut to it.
+ *
+ * Scores, softmax statistics and sums are held in fp32; the weights are rounded
+ * to 16 bits (those of FP16 rows, else BF16) for the product with V. */
+typedef struct pf_attend_args {
+  pf_kv_rows q;          /* [num_rows, num_q_heads, head_dim] */
+  pf_kv_rows out;        /* the same shape and type; may not overlap q */
+  uint64_t num_rows;
+  uint64_t block_table;  /* int32, device */
+  uint64_t table_stride; /* entries from one sequence to the next */
+  uint64_t seq_lens;     /* int32 [num_seqs], device */
+  uint64_t query_starts; /* int32 [num_seqs + 1], device */
+  uint64_t lse;          /* fp32 [num_rows, num_q_heads] (natural log), or 0 */
+  uint32_t num_q_heads;  /* a multiple of the pages' num_heads */
+  uint32_t num_seqs;
+  uint32_t table_width;  /* entries of a sequence */
+  uint32_t window;       /* 0: none */
+  uint32_t causal;
+  float scale;           /* of the scores */
+  uint32_t max_seq_len;  /* hints that shape the launch, not limits: the longest */
+  uint32_t max_query_len; /* sequence and query; 0: table_width * block_size, num_rows */
+} pf_attend_args;
+
+/* Device memory in which calls with few rows and long sequences join the shares
+ * of a split sequence.  Calls that share a workspace must be ordered (one stream,
+ * or events between streams), replays of captured calls included: use one
+ * workspace a stream.  Destroying it waits for the device. */
+typedef struct pf_attend_workspace pf_attend_workspace;
+#define PF_ATTEND_WORKSPACE_DEFAULT (64ull << 20)
+int pf_attend_workspace_create(int device, uint64_t bytes, pf_attend_workspace** out);
+int pf_attend_workspace_destroy(pf_attend_workspace* workspace);
+/* workspace may be NULL: no sequence is split then. */
+int pf_kv_attend(const pf_kv_pages* pages, const pf_attend_args* args,
+                 pf_attend_workspace* workspace, pf_stream stream);
+
+/* ------------------------------------------------------------------------ */
 /* Synthetic data and verification kernels (benchmarks and parity tests).     */
 /* ------------------------------------------------------------------------ */
 /* Fill size_bytes (multiple of 8) at dst_dev with splitmix64 words:

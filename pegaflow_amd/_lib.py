@@ -172,6 +172,63 @@ class LayerWords(ctypes.Structure):
     ]
 
 
+# What rows and pages of a paged cache hold (PF_KV_*), and the order of a block's
+# values.
+KV_BF16, KV_FP16, KV_E4M3, KV_INT8 = 1, 2, 3, 4
+KV_TOKEN_MAJOR, KV_HEAD_MAJOR = 0, 1
+KV_MAX_HEAD_DIM = 256
+ATTEND_WORKSPACE_DEFAULT = 64 << 20
+
+
+class KVPages(ctypes.Structure):
+    """pf_kv_pages — a registered layer as pages of a cache."""
+
+    _fields_ = [
+        ("layout", KVLayout),
+        ("block_size", ctypes.c_uint32),
+        ("num_heads", ctypes.c_uint32),
+        ("head_dim", ctypes.c_uint32),
+        ("type", ctypes.c_uint32),
+        ("order", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class KVRows(ctypes.Structure):
+    """pf_kv_rows — [tokens, heads, head_dim] values with any strides."""
+
+    _fields_ = [
+        ("data", ctypes.c_uint64),
+        ("token_stride", ctypes.c_uint64),
+        ("head_stride", ctypes.c_uint64),
+        ("type", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class AttendArgs(ctypes.Structure):
+    """pf_attend_args — one batch's attention over the pages."""
+
+    _fields_ = [
+        ("q", KVRows),
+        ("out", KVRows),
+        ("num_rows", ctypes.c_uint64),
+        ("block_table", ctypes.c_uint64),
+        ("table_stride", ctypes.c_uint64),
+        ("seq_lens", ctypes.c_uint64),
+        ("query_starts", ctypes.c_uint64),
+        ("lse", ctypes.c_uint64),
+        ("num_q_heads", ctypes.c_uint32),
+        ("num_seqs", ctypes.c_uint32),
+        ("table_width", ctypes.c_uint32),
+        ("window", ctypes.c_uint32),
+        ("causal", ctypes.c_uint32),
+        ("scale", ctypes.c_float),
+        ("max_seq_len", ctypes.c_uint32),
+        ("max_query_len", ctypes.c_uint32),
+    ]
+
+
 class SaveLayer(ctypes.Structure):
     """pf_save_layer — one (layer_name, block_ids, block_hashes) of a save batch."""
 
@@ -289,6 +346,14 @@ SIGNATURES = {
                                     ctypes.POINTER(LayerSignal), u32]),
     "pf_stream_wait_word": (i32, [vp, u64, u64, u32, u64]),
     "pf_host_wait_word": (i32, [vp, u64, u64, pi32]),
+    "pf_kv_segment_bytes": (i32, [u32, u32, u32, u32, pu64]),
+    "pf_kv_write": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(KVRows),
+                          ctypes.POINTER(KVRows), u64, u64, vp]),
+    "pf_kv_read": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(KVRows),
+                         ctypes.POINTER(KVRows), u64, u64, vp]),
+    "pf_attend_workspace_create": (i32, [i32, u64, pvp]),
+    "pf_attend_workspace_destroy": (i32, [vp]),
+    "pf_kv_attend": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(AttendArgs), vp, vp]),
     "pf_fill_random": (i32, [u64, u64, u64, u64, vp]),
     "pf_verify_random": (i32, [u64, u64, u64, u64, pu64]),
     "pf_verify_random_chunks": (i32, [pu64, pu64, u64, u64, u64, pu64]),

@@ -25,6 +25,9 @@ SOURCES = [
     "pf_runtime.cpp",
     "pf_kernels.hip",
     "pf_transfer.cpp",
+    "pf_paged.cpp",
+    "pf_paged.hip",
+    "pf_attend.hip",
     "pf_load_state.cpp",
     "pf_engine.cpp",
     "pf_disk.cpp",
@@ -33,8 +36,7 @@ SOURCES = [
     "pf_grpc.cpp",
 ]
 
-# Packed-FP32 instructions are disabled for all device code (this library
-# has no floating-point arithmetic, so the flag costs nothing).
+# Packed-FP32 instructions are disabled for all device code.
 HIP_FLAGS = [
     f"--offload-arch={ARCH}",
     "-O3",

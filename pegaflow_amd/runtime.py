@@ -200,6 +200,49 @@ class DeviceBuffer:
             pass
 
 
+# Bytes of a DeviceArray's values, by name.
+DTYPE_BYTES = {"bf16": 2, "fp16": 2, "fp32": 4, "int32": 4, "int64": 8, "uint8": 1}
+
+
+class DeviceArray:
+    """A typed, shaped view of device memory, with the ``data_ptr()``, ``shape``,
+    ``stride()`` and ``dtype`` that the paged-cache operators ask of a tensor: what
+    a process without torch passes in its place.  ``dtype`` is one of DTYPE_BYTES;
+    strides are in values (default: contiguous); ``offset`` is in bytes.  Without a
+    ``buffer`` it owns a new one."""
+
+    def __init__(self, shape, dtype: str, buffer: DeviceBuffer | None = None, offset: int = 0,
+                 strides=None):
+        self.shape = tuple(int(n) for n in shape)
+        self.dtype = dtype
+        if strides is None:
+            strides, n = [], 1
+            for size in reversed(self.shape):
+                strides.insert(0, n)
+                n *= size
+        self._strides = tuple(int(s) for s in strides)
+        last = sum((n - 1) * s for n, s in zip(self.shape, self._strides))
+        self.nbytes = (last + 1) * DTYPE_BYTES[dtype] if 0 not in self.shape else 0
+        self.buffer = buffer or DeviceBuffer(max(self.nbytes, 1))
+        self._offset = offset
+        if offset + self.nbytes > self.buffer.nbytes:
+            raise ValueError("the array exceeds its buffer")
+
+    def data_ptr(self) -> int:
+        return self.buffer.ptr + self._offset
+
+    def stride(self) -> tuple:
+        return self._strides
+
+    def upload(self, arr: np.ndarray) -> None:
+        """The bytes of ``arr`` from the array's first value on."""
+        self.buffer.upload(arr, self._offset)
+
+    def download(self) -> np.ndarray:
+        """The bytes from the array's first value to its last."""
+        return self.buffer.download(self.nbytes, self._offset)
+
+
 class PinnedBuffer:
     """Pinned host memory from hipHostMalloc, mapped for device access.
 
