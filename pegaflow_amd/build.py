@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -27,7 +28,8 @@ SOURCES = [
     "pf_transfer.cpp",
     "pf_paged.cpp",
     "pf_paged.hip",
-    "pf_attend.hip",
+    "pf_attend_bf16.hip",
+    "pf_attend_fp16.hip",
     "pf_load_state.cpp",
     "pf_engine.cpp",
     "pf_disk.cpp",
@@ -61,13 +63,10 @@ def build(verbose: bool = False) -> str:
     cc = hipcc()
     objs_dir = os.path.join(ROOT, "_build")
     os.makedirs(objs_dir, exist_ok=True)
-    objs = []
-    for src in SOURCES:
-        path = os.path.join(CSRC, src)
-        if not os.path.exists(path):
-            continue
+
+    def compile_one(src: str) -> str:
         obj = os.path.join(objs_dir, src + ".o")
-        cmd = [cc, *HIP_FLAGS, "-c", path, "-o", obj]
+        cmd = [cc, *HIP_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         if not src.endswith(".hip"):
             cmd[1:1] = ["-x", "hip"]
         if verbose:
@@ -75,7 +74,13 @@ def build(verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed on {src}:\n{r.stdout}\n{r.stderr}")
-        objs.append(obj)
+        return obj
+
+    # The attention kernels take the longest: first.
+    sources = sorted((s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))),
+                     key=lambda s: not s.startswith("pf_attend_"))
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, sources))
     tmp = LIB + ".tmp"
     cmd = [cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
            "-Wl,-rpath,/opt/rocm/lib", "-Wl,--no-undefined", "-L/opt/rocm/lib",

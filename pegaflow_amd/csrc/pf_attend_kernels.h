@@ -1,0 +1,1103 @@
+// pf_attend_kernels.h — attention of new tokens over a paged cache: the kernels,
+// included once for each row type (pf_attend_bf16.hip, pf_attend_fp16.hip).
+//
+// Row r (one new token at position p of a sequence of L tokens, one query head)
+// attends the tokens t with t < L, t <= p (causal) and t > p - window:
+//   z_t = scale * q . k_t,  m = max z,  w_t = exp(z_t - m),
+//   o = sum w_t v_t / sum w_t,  lse = m + log(sum w_t);
+// a row that attends none has o = 0 and lse = -inf.  8-bit pages hold codes and a
+// scale for each token, which multiplies z_t and w_t instead of the codes: the codes
+// are exact in 16 bits.
+//
+// The rows of a sequence and KV head, its new tokens times the `group` query heads
+// that share the head, are one matrix of rows, cut into tiles; a tile passes once over
+// the tokens it attends with a running maximum and sum.  Both products are taken
+// transposed, S^T = K Q^T and O^T = V^T W^T, so that a lane of the matrix core's result
+// holds one row's scores: its maximum and sum need one exchange between two (or four)
+// lanes, and the weights are already where the second product reads them.  That product
+// reads V^T from LDS with the transposing 16-bit loads.
+//
+// Weights are rounded to 16 bits for the product with V (bf16, or fp16 for 16-bit
+// pages of fp16 rows): the matrix core takes no more, and the rounding, at most half a
+// step of each weight, is of the size of the output's own.  Scores, maxima, sums and
+// outputs stay in fp32 until the end.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "pf_paged_device.h"
+
+namespace pf {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) uint8_t l_u8;
+typedef __attribute__((address_space(3))) u32x4 l_u32x4;
+typedef __attribute__((address_space(3))) s16x4 l_s16x4;
+typedef __attribute__((address_space(3))) f32x4 l_f32x4;
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_inff();
+
+template <class T>
+struct Mat;
+template <>
+struct Mat<BF16> {
+  static __device__ __forceinline__ f32x16 mul32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mul16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+  }
+};
+template <>
+struct Mat<FP16> {
+  static __device__ __forceinline__ f32x16 mul32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mul16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t,
+                              f16x2{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+  }
+};
+
+constexpr bool is_codes(uint32_t type) { return type == PF_KV_E4M3 || type == PF_KV_INT8; }
+
+// The four codes of a word as 16-bit values of M (exact: 4 and 8 significant bits).
+template <class M, uint32_t TYPE>
+__device__ __forceinline__ u32x2 codes_to_16(uint32_t word) {
+  if constexpr (TYPE == PF_KV_E4M3) {
+    if constexpr (M::kType == PF_KV_BF16)
+      return u32x2{
+          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, false)),
+          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, true))};
+    else
+      return u32x2{
+          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, false)),
+          __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, 1.0f, true))};
+  } else if constexpr (M::kType == PF_KV_BF16) {
+    // The high halves of the floats hold all of them.
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = __builtin_bit_cast(uint32_t,
+                                static_cast<float>(static_cast<int8_t>(word >> (8 * i))));
+    return u32x2{__builtin_amdgcn_perm(f[1], f[0], 0x07060302u),
+                 __builtin_amdgcn_perm(f[3], f[2], 0x07060302u)};
+  } else {
+    // 0x6400 | u is 1024 + u in fp16; u = code + 128.
+    const uint32_t u = word ^ 0x80808080u;
+    const f16x2 bias{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const uint32_t lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    const uint32_t hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, lo) - bias),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, hi) - bias)};
+  }
+}
+
+// x of lanes l and l ^ 32, in both lanes and the same order.
+__device__ __forceinline__ f32x2 both_halves(float x) {
+  const uint32_t y = __builtin_bit_cast(uint32_t, x);
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];  // a bit_cast of a vector's element takes its first
+  return f32x2{__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1)};
+}
+__device__ __forceinline__ float max32(float x) {
+  const f32x2 b = both_halves(x);
+  return fmaxf(b[0], b[1]);
+}
+__device__ __forceinline__ float sum32(float x) {
+  const f32x2 b = both_halves(x);
+  return b[0] + b[1];
+}
+
+// 8 values of a query row (zeros past its end), negated where the scale is negative.
+__device__ __forceinline__ u32x4 load_q8(uint64_t row, uint32_t d, const AttendParams& a,
+                                         bool valid) {
+  u32x4 v{0, 0, 0, 0};
+  if (valid && d < a.pages.dim) {
+    if (a.aligned) {
+      v = *reinterpret_cast<const g_u32x4*>(row + d * 2);
+    } else {
+      const g_u16* p = reinterpret_cast<const g_u16*>(row + d * 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = p[2 * i] | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+    }
+  }
+  return v ^ a.q_sign;
+}
+
+// 4 values of an output row.
+template <class Row>
+__device__ __forceinline__ void store_out4(uint64_t row, uint32_t d, const AttendParams& a,
+                                           f32x4 o) {
+  if (d >= a.pages.dim) return;
+  const u32x2 v{Mat<Row>::pack(o[0], o[1]), Mat<Row>::pack(o[2], o[3])};
+  if (a.aligned) {
+    *reinterpret_cast<g_u32x2*>(row + d * 2) = v;
+  } else {
+    g_u16* p = reinterpret_cast<g_u16*>(row + d * 2);
+    p[0] = static_cast<uint16_t>(v[0]);
+    p[1] = static_cast<uint16_t>(v[0] >> 16);
+    p[2] = static_cast<uint16_t>(v[1]);
+    p[3] = static_cast<uint16_t>(v[1] >> 16);
+  }
+}
+
+// V in a tile that some row attends only in part: a weight of 0 must not meet an
+// infinity or NaN, so those values are zero in LDS, and the tile's caller returns for
+// them at the end (add_odd).  Returns whether there were any.
+template <class VM>
+__device__ __forceinline__ bool clear_odd(u32x4& v) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = max(top, max(v[w] & 0x7fffu, (v[w] >> 16) & 0x7fffu));
+  if (top < VM::kInf) return false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if ((v[w] & 0x7fffu) >= VM::kInf) v[w] &= 0xffff0000u;
+    if (((v[w] >> 16) & 0x7fffu) >= VM::kInf) v[w] &= 0xffffu;
+  }
+  return true;
+}
+
+// Adds the infinities and NaN among values d to d + 3 of V of the token at `at` (their
+// weights are positive, and infinite either way) to 4 outputs.
+template <class Row, uint32_t TYPE>
+__device__ __forceinline__ void add_odd(uint64_t at, uint32_t d, uint32_t dim, float* o) {
+  if (d + 4 > dim) return;
+  float v[4];
+  if constexpr (is_codes(TYPE)) {
+    codes_to_float<TYPE>(*reinterpret_cast<const g_u32*>(at + d), v);
+  } else {
+    const u32x2 x = *reinterpret_cast<const g_u32x2*>(at + d * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = Row::to_float((x[i / 2] >> (16 * (i & 1))) & 0xffffu);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (!__builtin_isfinite(v[i])) o[i] += v[i];
+}
+
+// A sequence of the batch: its first row, its rows, its tokens.  Starts and lengths
+// come from device memory and are bounded here.
+struct Seq {
+  int32_t first, rows, len;
+};
+__device__ __forceinline__ Seq seq_of(const AttendParams& a, uint32_t b) {
+  const int32_t total = static_cast<int32_t>(a.num_rows);
+  const int32_t first = min(max(a.query_starts[b], 0), total);
+  const int32_t last = min(max(a.query_starts[b + 1], 0), total);
+  const int32_t room = static_cast<int32_t>(a.table_width * a.pages.block_size);
+  return {first, max(last - first, 0), min(max(a.seq_lens[b], 0), room)};
+}
+
+// Tokens that the row at position `pos` attends: [begin, end).
+__device__ __forceinline__ int32_t row_end(const AttendParams& a, int32_t len, int32_t pos) {
+  return a.causal ? max(min(len, pos + 1), 0) : len;
+}
+__device__ __forceinline__ int32_t row_begin(const AttendParams& a, int32_t pos) {
+  const int32_t w = static_cast<int32_t>(a.window);
+  return w && pos >= w ? pos - w + 1 : 0;
+}
+
+// The share [begin, end) of a tile's tokens that split `split` of `splits` passes over,
+// in pieces of `piece` tokens; the last split takes what is left.  Returns the number
+// of splits that have a share (at least 1); begin and end mean nothing for the others.
+__device__ __forceinline__ uint32_t split_range(int32_t& begin, int32_t& end, uint32_t split,
+                                                uint32_t splits, uint32_t piece) {
+  const uint32_t n = static_cast<uint32_t>(max(end - begin, 0));
+  const uint32_t used = min(max((n + piece - 1) / piece, 1u), splits);
+  if (split < used) {
+    begin += static_cast<int32_t>(split * piece);
+    if (split + 1 < used) end = begin + static_cast<int32_t>(piece);
+  }
+  return used;
+}
+
+// Byte offset of token t's values in K's (or V's) pages, and of its scale; false where
+// its block does not exist.
+__device__ __forceinline__ bool token_at(const PagedView& p, int32_t block, uint32_t t,
+                                         uint32_t page, uint32_t h, uint64_t* at,
+                                         uint64_t* scale_at) {
+  const uint32_t off = t - page * p.block_size;
+  const uint64_t base = static_cast<uint64_t>(static_cast<uint32_t>(block)) * p.block_bytes;
+  *at = base + off * p.token_bytes + h * p.head_bytes;
+  *scale_at = base + p.scale_offset + (h * p.block_size + off) * 4u;
+  return static_cast<uint32_t>(block) < p.num_blocks;
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and 64 tokens at a
+// time.  K and V of those tokens go through registers into LDS, converted to 16 bits,
+// under the previous tile's products; each wave then multiplies its rows with them.
+//
+// Bound by the matrix cores and, close behind, by the softmax on the vector units: 64
+// tokens x 32 rows take a wave 32 products of 32 cycles at head size 128, and 2,048
+// weights 32 times (multiply-add, exponential, maximum, sum, rounding).  Two workgroups
+// share a compute unit so that one's products run under the other's softmax.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kTileRows = 128;
+constexpr uint32_t kTileTokens = 64;
+constexpr uint32_t kManyThreads = 256;
+
+// Bytes from one token to the next in LDS.  K: 16-byte reads of 16 neighbouring tokens
+// fall into different banks.  V: a transposing read takes 64 bytes of each of 4 tokens.
+constexpr uint32_t k_pitch(uint32_t dp) { return 2 * dp + 16; }
+constexpr uint32_t v_pitch(uint32_t dp) {
+  uint32_t p = 2 * dp;
+  while (p % 256 != 64 && p % 256 != 192) p += 16;
+  return p;
+}
+
+template <uint32_t DP>
+struct ManyLds {
+  // Two tiles in turn where two workgroups still fit the compute unit's 160 KB.
+  static constexpr uint32_t kBuffers = DP <= 128 ? 2 : 1;
+  struct Tile {
+    __attribute__((aligned(16))) uint8_t k[kTileTokens * k_pitch(DP)];
+    __attribute__((aligned(16))) uint8_t v[kTileTokens * v_pitch(DP)];
+    __attribute__((aligned(16))) float k_scale[kTileTokens];
+    __attribute__((aligned(16))) float v_scale[kTileTokens];
+  } tile[kBuffers];
+  // Tokens of a tile whose block is missing, in turn over four tiles: a slot is cleared
+  // two tiles before its next use.
+  unsigned long long hole[4];
+  uint32_t odd;  // some tile attended in part holds V that is not finite
+};
+
+// The rows tile `index` of the batch (tiles of all sequences in order, of sequences
+// with more than `least` rows): its sequence and tile in it, false if there is none.
+__device__ __forceinline__ bool find_tile(const AttendParams& a, uint32_t index, uint32_t tile_rows,
+                                          uint32_t least, uint32_t* seq, uint32_t* tile) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
+    uint32_t tiles = 0;
+    if (b0 + lane < a.num_seqs) {
+      const uint32_t rows = static_cast<uint32_t>(seq_of(a, b0 + lane).rows) * a.group;
+      if (rows > least) tiles = (rows + tile_rows - 1) / tile_rows;
+    }
+    uint32_t sum = tiles;  // of lanes 0 .. lane
+#pragma unroll
+    for (uint32_t step = 1; step < 64; step *= 2) {
+      const uint32_t x = __shfl_up(sum, step);
+      if (lane >= step) sum += x;
+    }
+    const uint64_t past = __ballot(sum > index);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      *seq = b0 + at;
+      *tile = index - __shfl(sum - tiles, at);
+      return true;
+    }
+    index -= __shfl(sum, 63);
+  }
+  return false;
+}
+
+// A tile of rows: its sequence, the tokens it passes over and this lane's row.
+struct ManyTile {
+  Seq s;
+  uint32_t seq, head, rows, row;  // rows of the sequence and head, and this lane's
+  int32_t begin, end;             // tokens of the tile
+  int32_t pos0;                   // position of the sequence's first new token
+  bool valid;
+};
+__device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, uint32_t head,
+                                          ManyTile* t) {
+  uint32_t tile = 0;
+  if (!find_tile(a, unit, kTileRows, a.few_rows, &t->seq, &tile)) return false;
+  t->seq = __builtin_amdgcn_readfirstlane(t->seq);
+  tile = __builtin_amdgcn_readfirstlane(tile);
+  t->s = seq_of(a, t->seq);
+  t->head = head;
+  t->rows = static_cast<uint32_t>(t->s.rows) * a.group;
+  const uint32_t row0 = tile * kTileRows, last = min(row0 + kTileRows, t->rows) - 1;
+  t->pos0 = t->s.len - t->s.rows;
+  t->begin = row_begin(a, t->pos0 + static_cast<int32_t>(row0 / a.group)) &
+             ~static_cast<int32_t>(kTileTokens - 1);
+  t->end = row_end(a, t->s.len, t->pos0 + static_cast<int32_t>(last / a.group));
+  t->row = row0 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+  t->valid = t->row < t->rows;
+  return true;
+}
+
+__device__ __forceinline__ uint64_t row_address(const AttendParams& a, const RowsView& v,
+                                                const ManyTile& t) {
+  const uint32_t token = t.row / a.group, g = t.row - token * a.group;
+  return v.data + ((t.s.first + static_cast<uint64_t>(token)) * v.token_stride +
+                   static_cast<uint64_t>(t.head * a.group + g) * v.head_stride) *
+                      2;
+}
+
+// Outputs of this lane's row: o / l and the log-sum-exp.  m is in units of the raw scores.
+template <class Row, uint32_t DP>
+__device__ __forceinline__ void many_store(const AttendParams& a, const ManyTile& t,
+                                           const f32x16* o, float m, float l) {
+  if (!t.valid) return;
+  const uint32_t half = (threadIdx.x >> 5) & 1;
+  const float inv = l == 0 ? 0.0f : 1.0f / l;
+  const uint64_t row = row_address(a, a.out, t);
+#pragma unroll
+  for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      store_out4<Row>(row, dt * 32 + 8 * i + 4 * half, a,
+                      f32x4{o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv,
+                            o[dt][4 * i + 3] * inv});
+  if (a.lse && half == 0) {
+    const uint32_t token = t.row / a.group, g = t.row - token * a.group;
+    a.lse[(t.s.first + static_cast<uint64_t>(token)) * a.q_heads + t.head * a.group + g] =
+        l == 0 ? kNegInf : m * a.scale_log2 * kLn2 + logf(l);
+  }
+}
+
+template <class Row, uint32_t TYPE, uint32_t DP>
+__global__ void __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1)
+attend_many_kernel(AttendParams a) {
+  constexpr bool kCodes = is_codes(TYPE);
+  using KM = Row;                                          // K as multiplied
+  using VM = typename std::conditional<kCodes, BF16, Row>::type;  // V and the weights
+  constexpr uint32_t kPer = kCodes ? 16 : 8;               // values of a 16-byte load
+  constexpr uint32_t kCols = DP / kPer;
+  constexpr uint32_t kLoads = (kTileTokens * kCols + kManyThreads - 1) / kManyThreads;
+  constexpr bool kWhole = kTileTokens * kCols % kManyThreads == 0;
+  constexpr uint32_t kKP = k_pitch(DP), kVP = v_pitch(DP);
+  using Lds = ManyLds<DP>;
+  __shared__ Lds lds;
+  const PagedView& pg = a.pages;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, half = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // Heads of one tile are neighbours: with 8 of them each has an XCD's L2 for its pages.
+  const uint32_t head = blockIdx.x % pg.heads;
+  const uint32_t rest = blockIdx.x / pg.heads;
+  const uint32_t split = rest % a.many_splits;
+  // Later tiles of a sequence attend more tokens: they start first.
+  const uint32_t unit = a.many_units - 1 - rest / a.many_splits;
+  ManyTile t;
+  if (!many_tile(a, unit, head, &t)) return;
+  int32_t begin = t.begin, end = t.end;
+  const uint32_t used = split_range(begin, end, split, a.many_splits, a.many_piece);
+  if (split >= used) return;
+  const int32_t* table = a.block_table + t.seq * a.table_stride;
+
+  // Tokens that every row of the workgroup attends, and this wave's and row's.
+  const uint32_t wave0 = t.row - (lane & 31u), group = a.group;
+  const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + kTileRows, t.rows) - 1;
+  const int32_t all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
+  const int32_t all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
+  const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
+  const int32_t my_begin = row_begin(a, pos);
+  const int32_t my_end = t.valid ? row_end(a, t.s.len, pos) : 0;
+  const bool wave_valid = wave0 < t.rows;
+  const uint32_t wave_last = min(wave0 + 32, t.rows) - 1;
+  const int32_t wave_end =
+      wave_valid ? row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(wave_last / group)) : 0;
+
+  u32x4 q[DP / 16];
+  const uint64_t q_row = row_address(a, a.q, t);
+#pragma unroll
+  for (uint32_t kk = 0; kk < DP / 16; ++kk) q[kk] = load_q8(q_row, kk * 16 + half * 8, a, t.valid);
+
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+  float m = kNegInf, l = 0.0f;
+
+  // This thread's part of a tile: 16 bytes of kLoads tokens, and of 8-bit pages the K or
+  // V scale of one token (threads 0 to 127).
+  int32_t block[kLoads], s_block = 0;
+  u32x4 kr[kLoads], vr[kLoads];
+  float sr = 0.0f;
+  auto token_of = [&](uint32_t i) { return (tid + i * kManyThreads) / kCols; };
+  auto col_of = [&](uint32_t i) { return (tid + i * kManyThreads) % kCols; };
+  auto load_blocks = [&](int32_t t0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const int32_t tok = t0 + static_cast<int32_t>(token_of(i));
+      block[i] = tok < end ? table[page_of(pg, tok)] : -1;
+    }
+    if constexpr (kCodes) {
+      const int32_t tok = t0 + static_cast<int32_t>(tid & 63u);
+      s_block = tok < end && tid < 128 ? table[page_of(pg, tok)] : -1;
+    }
+  };
+  auto load_tile = [&](int32_t t0) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const int32_t tok = t0 + static_cast<int32_t>(token_of(i));
+      const uint32_t d = col_of(i) * kPer;
+      uint64_t at, scale_at;
+      const bool in = token_at(pg, block[i], tok, page_of(pg, tok), head, &at, &scale_at);
+      kr[i] = u32x4{0, 0, 0, 0};
+      vr[i] = u32x4{0, 0, 0, 0};
+      if (tok < end && in && d < pg.dim && (kWhole || token_of(i) < kTileTokens)) {
+        at += d * (kCodes ? 1 : 2);
+        kr[i] = *reinterpret_cast<const g_u32x4*>(pg.k + at);
+        vr[i] = *reinterpret_cast<const g_u32x4*>(pg.v + at);
+      }
+    }
+    if constexpr (kCodes) {
+      const int32_t tok = t0 + static_cast<int32_t>(tid & 63u);
+      uint64_t at, scale_at;
+      const bool in = token_at(pg, s_block, tok, page_of(pg, tok), head, &at, &scale_at);
+      sr = 0.0f;
+      if (tid < 128 && tok < end && in)
+        sr = *reinterpret_cast<const g_f32*>((tid < 64 ? pg.k : pg.v) + scale_at);
+    }
+  };
+  // Into LDS.  `partial`: some row does not attend every token.
+  auto store_tile = [&](int32_t t0, uint32_t slot, bool partial, typename Lds::Tile& tile) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const uint32_t tok = token_of(i), col = col_of(i);
+      if (!kWhole && tok >= kTileTokens) continue;
+      if (t0 + static_cast<int32_t>(tok) < end && static_cast<uint32_t>(block[i]) >= pg.num_blocks)
+        atomicOr(&lds.hole[slot], 1ull << tok);
+      u32x4 v0, v1{0, 0, 0, 0};
+      if constexpr (kCodes) {
+        const u32x2 a0 = codes_to_16<KM, TYPE>(kr[i][0]), a1 = codes_to_16<KM, TYPE>(kr[i][1]);
+        const u32x2 a2 = codes_to_16<KM, TYPE>(kr[i][2]), a3 = codes_to_16<KM, TYPE>(kr[i][3]);
+        u32x4* kd = reinterpret_cast<u32x4*>(tile.k + tok * kKP + col * 32);
+        kd[0] = u32x4{a0[0], a0[1], a1[0], a1[1]};
+        kd[1] = u32x4{a2[0], a2[1], a3[0], a3[1]};
+        const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
+        const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
+        v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
+        v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
+      } else {
+        *reinterpret_cast<u32x4*>(tile.k + tok * kKP + col * 16) = kr[i];
+        v0 = vr[i];
+      }
+      if (partial && TYPE != PF_KV_INT8) {
+        bool odd = clear_odd<VM>(v0);
+        if constexpr (kCodes) odd |= clear_odd<VM>(v1);
+        if (odd) lds.odd = 1;
+      }
+      if constexpr (kCodes) {
+        u32x4* vd = reinterpret_cast<u32x4*>(tile.v + tok * kVP + col * 32);
+        vd[0] = v0;
+        vd[1] = v1;
+      } else {
+        *reinterpret_cast<u32x4*>(tile.v + tok * kVP + col * 16) = v0;
+      }
+    }
+    if constexpr (kCodes)
+      if (tid < 128) (tid < 64 ? tile.k_scale : tile.v_scale)[tid & 63u] = sr;
+  };
+
+  if (tid < 4) lds.hole[tid] = 0;
+  if (tid == 4) lds.odd = 0;
+  load_blocks(begin);
+  load_tile(begin);
+  __syncthreads();
+  uint32_t n = 0;
+  for (int32_t t0 = begin; t0 < end; t0 += kTileTokens, ++n) {
+    const uint32_t slot = n & 3u;
+    const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kTileTokens) > all_end;
+    typename Lds::Tile& tile = lds.tile[n % Lds::kBuffers];
+    if (Lds::kBuffers == 1 && n) __syncthreads();  // the tile before has been read
+    store_tile(t0, slot, partial, tile);
+    __syncthreads();
+    if (tid == 0) lds.hole[(slot + 2) & 3u] = 0;
+    const int32_t next = t0 + static_cast<int32_t>(kTileTokens);
+    if (next < end) {
+      load_blocks(next);
+      load_tile(next);
+    }
+    if (t0 >= wave_end) continue;  // this wave's rows end before the tile
+
+    // S^T: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.
+    f32x16 s[2];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[tt][i] = 0.0f;
+    const uint8_t* k_at = tile.k + (lane & 31u) * kKP + half * 16;
+#pragma unroll
+    for (uint32_t kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+        s[tt] = Mat<KM>::mul32(*reinterpret_cast<const u32x4*>(k_at + tt * 32 * kKP + kk * 32),
+                               q[kk], s[tt]);
+    if constexpr (kCodes) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(tile.k_scale + tt * 32 + i * 8 + half * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[tt][4 * i + j] *= x[j];
+        }
+    }
+    const uint64_t hole = lds.hole[slot];
+    const bool masked = partial || hole;
+    if (masked) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t j = tt * 32 + 8 * (i / 4) + 4 * half + i % 4;
+          const int32_t tok = t0 + static_cast<int32_t>(j);
+          if (tok < my_begin || tok >= my_end || (hole >> j & 1)) s[tt][i] = kNegInf;
+        }
+    }
+    float top = kNegInf;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tt][i]);
+    top = max32(top);
+    // The maximum that the weights are taken against follows the largest score only
+    // where that has grown by more than 8 (in powers of 2): until then weights up to
+    // 2^8 serve as well, and the outputs need no rescaling.
+    if (__any((top - m) * a.scale_log2 > 8.0f)) {
+      const float m_new = fmaxf(m, top);
+      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= keep;
+    }
+    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float sum = 0.0f;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
+        sum += w;
+        if constexpr (!kCodes) s[tt][i] = w;
+        else s[tt][i] = masked && s[tt][i] == kNegInf ? kNegInf : w;  // V scales follow
+      }
+    l += sum;
+    if constexpr (kCodes) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(tile.v_scale + tt * 32 + i * 8 + half * 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float w = s[tt][4 * i + j];
+            s[tt][4 * i + j] = w == kNegInf ? 0.0f : w * x[j];
+          }
+        }
+    }
+    // O^T += V^T W^T.  The 16 tokens of a product are taken in the order in which a lane
+    // holds their weights: 4 half + (0..3), then 8 + 4 half + (0..3).
+    const uint32_t quad = lane & 15u;
+    const uint8_t* v_at = tile.v + (half * 4 + quad / 4) * kVP + ((lane >> 4) & 1u) * 32 +
+                          (quad & 3u) * 8;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = Mat<VM>::pack(s[u / 2][8 * (u & 1) + 2 * j], s[u / 2][8 * (u & 1) + 2 * j + 1]);
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 32; ++dt) {
+        const uint8_t* at = v_at + u * 16 * kVP + dt * 64;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(at + 8 * kVP));
+        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+        o[dt] = Mat<VM>::mul32(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+      }
+    }
+  }
+
+  __syncthreads();
+  if (lds.odd)
+    for (int32_t tok = begin; tok < end; ++tok) {
+      if (tok < my_begin || tok >= my_end) continue;
+      const int32_t t0 = tok & ~static_cast<int32_t>(kTileTokens - 1);
+      if (t0 >= all_begin && t0 + static_cast<int32_t>(kTileTokens) <= all_end) continue;
+      uint64_t at, scale_at;
+      const uint32_t page = page_of(pg, tok);
+      if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          float x[4] = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+          add_odd<Row, TYPE>(pg.v + at, dt * 32 + 8 * i + 4 * half, pg.dim, x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
+        }
+    }
+
+  l = sum32(l);
+  if (used == 1) {
+    many_store<Row, DP>(a, t, o, m, l);
+    return;
+  }
+  // This split's share for attend_many_join_kernel: 16 bytes a lane at a time.
+  const uint64_t slot = (static_cast<uint64_t>(unit) * a.many_splits + split) * pg.heads + head;
+  f32x4* part = reinterpret_cast<f32x4*>(a.many_o) + (slot * 4 + wave) * (DP / 8) * 64 + lane;
+#pragma unroll
+  for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      part[(dt * 4 + i) * 64] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
+                                      o[dt][4 * i + 3]};
+  reinterpret_cast<f32x2*>(a.many_ml)[(slot * 4 + wave) * 64 + lane] = f32x2{m, l};
+}
+
+// Joins the shares of split tiles: the same lanes hold the same rows and values.
+template <class Row, uint32_t DP>
+__global__ void __launch_bounds__(kManyThreads) attend_many_join_kernel(AttendParams a) {
+  const PagedView& pg = a.pages;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t head = blockIdx.x % pg.heads, unit = blockIdx.x / pg.heads;
+  ManyTile t;
+  if (!many_tile(a, unit, head, &t)) return;
+  int32_t begin = t.begin, end = t.end;
+  const uint32_t used = split_range(begin, end, 0, a.many_splits, a.many_piece);
+  if (used == 1) return;
+  auto slot = [&](uint32_t split) {
+    return ((static_cast<uint64_t>(unit) * a.many_splits + split) * pg.heads + head) * 4 + wave;
+  };
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.many_ml);
+  float m = kNegInf;
+  for (uint32_t s = 0; s < used; ++s) m = fmaxf(m, ml[slot(s) * 64 + lane][0]);
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+  float l = 0.0f;
+  for (uint32_t s = 0; s < used; ++s) {
+    const f32x2 x = ml[slot(s) * 64 + lane];
+    // A share without a maximum attended nothing, or only what is no number (l is NaN).
+    const float keep = x[0] == kNegInf ? (x[1] == 0.0f ? 0.0f : 1.0f)
+                                       : __builtin_amdgcn_exp2f((x[0] - m) * a.scale_log2);
+    l += x[1] * keep;
+    const f32x4* part = reinterpret_cast<const f32x4*>(a.many_o) + slot(s) * (DP / 8) * 64 + lane;
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const f32x4 y = part[(dt * 4 + i) * 64];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[dt][4 * i + j] += y[j] * keep;
+      }
+  }
+  many_store<Row, DP>(a, t, o, m, l);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: single tokens and short drafts, up to 16 rows of a KV head.  Bound by
+// reading the pages.  Each wave of a workgroup passes over tokens of its own, 32 at a
+// time, with no barrier: K goes from memory straight into the operand's registers
+// (lane: token lane % 16, 8 or 16 values), V through the wave's own part of LDS.  The
+// next 32 tokens are on their way meanwhile.  At the end the 4 waves join in LDS, and
+// the shares of a split sequence in attend_few_join_kernel.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kFewThreads = 256, kFewWaves = 4;
+constexpr uint32_t kFewTokens = 32;
+constexpr uint32_t few_v_pitch(uint32_t dp) { return 2 * dp + 32; }
+
+template <class Row, uint32_t TYPE, uint32_t DP>
+__global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
+attend_few_kernel(AttendParams a) {
+  constexpr bool kCodes = is_codes(TYPE);
+  using KM = Row;
+  using VM = typename std::conditional<kCodes, BF16, Row>::type;
+  constexpr uint32_t kPer = kCodes ? 16 : 8;
+  constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
+  constexpr uint32_t kCols = DP / kPer;
+  constexpr uint32_t kVLoads = (kFewTokens * kCols + 63) / 64;
+  constexpr uint32_t kVP = few_v_pitch(DP);
+  constexpr uint32_t kSteps = kKLoads * (kCodes ? 2 : 1);  // products of 32 values
+  struct WaveLds {
+    __attribute__((aligned(16))) uint8_t v[kFewTokens * kVP];
+  };
+  __shared__ WaveLds lds[kFewWaves];
+  __shared__ float join_m[kFewWaves][16], join_l[kFewWaves][16];
+  const PagedView& pg = a.pages;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t head = blockIdx.x % pg.heads;
+  const uint32_t rest = blockIdx.x / pg.heads;
+  const uint32_t split = rest % a.few_splits, seq = rest / a.few_splits;
+  const Seq sq = seq_of(a, seq);
+  const uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
+  if (rows == 0) return;
+  // More rows than a tile has come here only when the batch was said to have none such:
+  // they go one tile after another, unsplit.
+  uint32_t splits = a.few_splits;
+  if (rows > 16) {
+    if (a.many_units) return;  // attend_many_kernel's
+    splits = 1;
+  }
+  if (split >= splits) return;
+  const int32_t pos0 = sq.len - sq.rows;
+  const int32_t* table = a.block_table + seq * a.table_stride;
+  uint8_t* v_lds = lds[wave].v;
+
+  for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
+    const uint32_t row = row0 + col, last = min(row0 + 16, rows) - 1;
+    const bool valid = row < rows;
+    const int32_t pos = pos0 + static_cast<int32_t>(row / a.group);
+    const int32_t my_begin = row_begin(a, pos);
+    const int32_t my_end = valid ? row_end(a, sq.len, pos) : 0;
+    int32_t begin = row_begin(a, pos0 + static_cast<int32_t>(row0 / a.group)) &
+                    ~static_cast<int32_t>(kFewTokens - 1);
+    int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>(last / a.group));
+    const int32_t all_begin = row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
+    const int32_t all_end = row_end(a, sq.len, pos0 + static_cast<int32_t>(row0 / a.group));
+    const uint32_t used = split_range(begin, end, split, splits, a.few_piece);
+    if (split >= used) return;
+    const uint32_t token = row / a.group, g = row - token * a.group;
+    const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
+                                       static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
+                                          2;
+    u32x4 q[kSteps];
+#pragma unroll
+    for (uint32_t i = 0; i < kSteps; ++i)
+      q[i] = load_q8(q_row,
+                     kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
+                     valid);
+    f32x4 o[DP / 16];
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
+    float m = kNegInf, l = 0.0f;
+    bool odd = false;  // some tile attended in part holds V that is not finite
+
+    u32x4 kr[2][kKLoads], vr[kVLoads];
+    float k_scale[2], v_scale[2];  // of token 16 tt + col
+    uint32_t there = 0;            // bit 16 tt + col: that token's block exists
+    int32_t block[2];              // of the tokens to load next
+    auto load_blocks = [&](int32_t t0) {
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(col);
+        block[tt] = tok < end ? table[page_of(pg, tok)] : -1;
+      }
+    };
+    auto load = [&](int32_t t0) {
+      there = 0;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(col);
+        uint64_t at, scale_at;
+        const bool in = token_at(pg, block[tt], tok, page_of(pg, tok), head, &at, &scale_at);
+#pragma unroll
+        for (uint32_t i = 0; i < kKLoads; ++i) {
+          const uint32_t d = (i * 4 + quarter) * kPer;
+          kr[tt][i] = u32x4{0, 0, 0, 0};
+          if (in && d < pg.dim)
+            kr[tt][i] = *reinterpret_cast<const g_u32x4*>(pg.k + at + d * (kCodes ? 1 : 2));
+        }
+        k_scale[tt] = v_scale[tt] = 0.0f;
+        if constexpr (kCodes) {
+          if (in) {
+            k_scale[tt] = *reinterpret_cast<const g_f32*>(pg.k + scale_at);
+            v_scale[tt] = *reinterpret_cast<const g_f32*>(pg.v + scale_at);
+          }
+        }
+        there |= (static_cast<uint32_t>(__ballot(in)) & 0xffffu) << (16 * tt);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < kVLoads; ++i) {
+        const uint32_t c = lane + i * 64, j = c / kCols, d = c % kCols * kPer;
+        const int32_t tok = t0 + static_cast<int32_t>(j);
+        const int32_t b0 = __shfl(block[0], j & 15u), b1 = __shfl(block[1], j & 15u);
+        uint64_t at, scale_at;
+        vr[i] = u32x4{0, 0, 0, 0};
+        if (token_at(pg, j < 16 ? b0 : b1, tok, page_of(pg, tok), head, &at, &scale_at) &&
+            j < kFewTokens && d < pg.dim)
+          vr[i] = *reinterpret_cast<const g_u32x4*>(pg.v + at + d * (kCodes ? 1 : 2));
+      }
+    };
+
+    int32_t t0 = begin + static_cast<int32_t>(wave * kFewTokens);
+    constexpr int32_t kStep = kFewTokens * kFewWaves;
+    load_blocks(t0);
+    if (t0 < end) load(t0);
+    load_blocks(t0 + kStep);
+    for (; t0 < end; t0 += kStep) {
+      const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kFewTokens) > all_end;
+      // V into LDS.
+#pragma unroll
+      for (uint32_t i = 0; i < kVLoads; ++i) {
+        const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
+        const bool mine = kFewTokens * kCols % 64 == 0 || j < kFewTokens;
+        u32x4 v0 = vr[i], v1{0, 0, 0, 0};
+        if constexpr (kCodes) {
+          const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
+          const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
+          v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
+          v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
+        }
+        if (partial && TYPE != PF_KV_INT8) {
+          odd |= clear_odd<VM>(v0);
+          if constexpr (kCodes) odd |= clear_odd<VM>(v1);
+        }
+        if (mine) {
+          u32x4* vd = reinterpret_cast<u32x4*>(v_lds + j * kVP + cc * (kCodes ? 32 : 16));
+          vd[0] = v0;
+          if constexpr (kCodes) vd[1] = v1;
+        }
+      }
+      // S^T: this lane's row `col`, tokens 16 tt + 4 quarter + i.
+      f32x4 s[2];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        s[tt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t i = 0; i < kKLoads; ++i) {
+          if constexpr (kCodes) {
+            const u32x2 a0 = codes_to_16<KM, TYPE>(kr[tt][i][0]);
+            const u32x2 a1 = codes_to_16<KM, TYPE>(kr[tt][i][1]);
+            const u32x2 a2 = codes_to_16<KM, TYPE>(kr[tt][i][2]);
+            const u32x2 a3 = codes_to_16<KM, TYPE>(kr[tt][i][3]);
+            s[tt] = Mat<KM>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
+            s[tt] = Mat<KM>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
+          } else {
+            s[tt] = Mat<KM>::mul16(kr[tt][i], q[i], s[tt]);
+          }
+        }
+      }
+      float wv[2][4];
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kCodes) {
+            s[tt][i] *= __shfl(k_scale[tt], quarter * 4 + i);
+            wv[tt][i] = __shfl(v_scale[tt], quarter * 4 + i);
+          } else {
+            wv[tt][i] = 1.0f;
+          }
+        }
+      const bool masked = partial || there != 0xffffffffu;
+      if (masked) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(quarter) * 4 + i;
+            if (tok < my_begin || tok >= my_end || !(there >> (tt * 16 + quarter * 4 + i) & 1u)) {
+              s[tt][i] = kNegInf;
+              wv[tt][i] = 0.0f;
+            }
+          }
+      }
+      if (t0 + kStep < end) {
+        load(t0 + kStep);
+        load_blocks(t0 + 2 * kStep);
+      }
+      float top = kNegInf;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = max32(top);
+      if (__any((top - m) * a.scale_log2 > 8.0f)) {
+        const float m_new = fmaxf(m, top);
+        const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+        m = m_new;
+        l *= keep;
+#pragma unroll
+        for (uint32_t dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
+      }
+      const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
+          l += w;
+          wv[tt][i] *= w;
+        }
+      const u32x4 w{Mat<VM>::pack(wv[0][0], wv[0][1]), Mat<VM>::pack(wv[0][2], wv[0][3]),
+                    Mat<VM>::pack(wv[1][0], wv[1][1]), Mat<VM>::pack(wv[1][2], wv[1][3])};
+      // Every lane of the wave has stored its part of V before any reads another's.
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const uint8_t* v_at = v_lds + (quarter * 4 + col / 4) * kVP + (col & 3u) * 8;
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 16; ++dt) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_at + dt * 32));
+        const s16x4 hi =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_at + 16 * kVP + dt * 32));
+        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+        o[dt] = Mat<VM>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (__any(odd))
+      for (int32_t tok = begin; tok < end; ++tok) {
+        if ((static_cast<uint32_t>(tok - begin) / kFewTokens) % kFewWaves != wave) continue;
+        if (tok < my_begin || tok >= my_end) continue;
+        const int32_t t1 = tok & ~static_cast<int32_t>(kFewTokens - 1);
+        if (t1 >= all_begin && t1 + static_cast<int32_t>(kFewTokens) <= all_end) continue;
+        uint64_t at, scale_at;
+        const uint32_t page = page_of(pg, tok);
+        if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
+#pragma unroll
+        for (uint32_t dt = 0; dt < DP / 16; ++dt) {
+          float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
+          add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
+          o[dt] = f32x4{x[0], x[1], x[2], x[3]};
+        }
+      }
+
+    // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
+    // LDS (which V no longer needs), and the threads share the sums.
+    l += __shfl_xor(l, 16);
+    l = sum32(l);
+    float* mine = reinterpret_cast<float*>(lds[wave].v);
+    static_assert(sizeof(WaveLds) >= 16 * DP * sizeof(float), "a wave's outputs fit its LDS");
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 16; ++dt)
+      *reinterpret_cast<f32x4*>(mine + col * DP + dt * 16 + quarter * 4) = o[dt];
+    if (quarter == 0) {
+      join_m[wave][col] = m;
+      join_l[wave][col] = l;
+    }
+    __syncthreads();
+    const uint64_t slot = (static_cast<uint64_t>(seq) * a.few_splits + split) * pg.heads + head;
+    for (uint32_t i = tid; i < 16 * DP / 4; i += kFewThreads) {
+      const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
+      if (row0 + r >= rows) continue;
+      float top = kNegInf;
+#pragma unroll
+      for (uint32_t w = 0; w < kFewWaves; ++w) top = fmaxf(top, join_m[w][r]);
+      float sum = 0.0f;
+      f32x4 x{0, 0, 0, 0};
+#pragma unroll
+      for (uint32_t w = 0; w < kFewWaves; ++w) {
+        const float mw = join_m[w][r], lw = join_l[w][r];
+        const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
+                                         : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
+        sum += lw * keep;
+        const f32x4 y =
+            *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
+      }
+      if (used > 1) {
+        *reinterpret_cast<f32x4*>(a.few_o + (slot * 16 + r) * DP + d) = x;
+        if (d == 0) reinterpret_cast<f32x2*>(a.few_ml)[slot * 16 + r] = f32x2{top, sum};
+      } else {
+        const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+        const uint32_t rt = (row0 + r) / a.group, rg = row0 + r - rt * a.group;
+        const uint64_t at = sq.first + static_cast<uint64_t>(rt), qh = head * a.group + rg;
+        store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
+                        f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
+        if (a.lse && d == 0)
+          a.lse[at * a.q_heads + qh] =
+              sum == 0 ? kNegInf : top * a.scale_log2 * kLn2 + logf(sum);
+      }
+    }
+    __syncthreads();  // before the next tile of rows uses the LDS
+  }
+}
+
+// Joins the shares of split sequences: a workgroup a sequence and head, 4 values a thread.
+template <class Row, uint32_t DP>
+__global__ void __launch_bounds__(kFewThreads) attend_few_join_kernel(AttendParams a) {
+  const PagedView& pg = a.pages;
+  const uint32_t head = blockIdx.x % pg.heads, seq = blockIdx.x / pg.heads;
+  const Seq sq = seq_of(a, seq);
+  const uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
+  if (rows == 0 || rows > 16) return;
+  const int32_t pos0 = sq.len - sq.rows;
+  int32_t begin = row_begin(a, pos0) & ~static_cast<int32_t>(kFewTokens - 1);
+  int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>((rows - 1) / a.group));
+  const uint32_t used = split_range(begin, end, 0, a.few_splits, a.few_piece);
+  if (used == 1) return;
+  for (uint32_t i = threadIdx.x; i < rows * (DP / 4); i += kFewThreads) {
+    const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
+    auto slot = [&](uint32_t s) {
+      return ((static_cast<uint64_t>(seq) * a.few_splits + s) * pg.heads + head) * 16 + r;
+    };
+    const f32x2* ml = reinterpret_cast<const f32x2*>(a.few_ml);
+    float top = kNegInf;
+    for (uint32_t s = 0; s < used; ++s) top = fmaxf(top, ml[slot(s)][0]);
+    float sum = 0.0f;
+    f32x4 x{0, 0, 0, 0};
+    for (uint32_t s = 0; s < used; ++s) {
+      const f32x2 y = ml[slot(s)];
+      const float keep = y[0] == kNegInf ? (y[1] == 0.0f ? 0.0f : 1.0f)
+                                         : __builtin_amdgcn_exp2f((y[0] - top) * a.scale_log2);
+      sum += y[1] * keep;
+      const f32x4 z = *reinterpret_cast<const f32x4*>(a.few_o + slot(s) * DP + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += z[j] * keep;
+    }
+    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+    const uint32_t rt = r / a.group, rg = r - rt * a.group;
+    const uint64_t at = sq.first + static_cast<uint64_t>(rt), qh = head * a.group + rg;
+    store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
+                    f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
+    if (a.lse && d == 0)
+      a.lse[at * a.q_heads + qh] = sum == 0 ? kNegInf : top * a.scale_log2 * kLn2 + logf(sum);
+  }
+}
+
+template <class Row, uint32_t TYPE, uint32_t DP>
+hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
+  if (p.few_splits) {
+    const uint32_t units = p.num_seqs * p.pages.heads;
+    hipLaunchKernelGGL((attend_few_kernel<Row, TYPE, DP>), dim3(units * p.few_splits),
+                       dim3(kFewThreads), 0, stream, p);
+    if (p.few_splits > 1)
+      hipLaunchKernelGGL((attend_few_join_kernel<Row, DP>), dim3(units), dim3(kFewThreads), 0,
+                         stream, p);
+  }
+  if (p.many_units) {
+    const uint32_t units = p.many_units * p.pages.heads;
+    hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP>), dim3(units * p.many_splits),
+                       dim3(kManyThreads), 0, stream, p);
+    if (p.many_splits > 1)
+      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(units), dim3(kManyThreads), 0,
+                         stream, p);
+  }
+  return hipGetLastError();
+}
+
+template <class Row, uint32_t TYPE>
+hipError_t launch_dim(const AttendParams& p, hipStream_t stream) {
+  switch (padded_dim(p.pages.dim)) {
+    case 64: return launch_kernels<Row, TYPE, 64>(p, stream);
+    case 96: return launch_kernels<Row, TYPE, 96>(p, stream);
+    case 128: return launch_kernels<Row, TYPE, 128>(p, stream);
+    case 192: return launch_kernels<Row, TYPE, 192>(p, stream);
+    default: return launch_kernels<Row, TYPE, 256>(p, stream);
+  }
+}
+
+template <class Row>
+hipError_t launch_type(const AttendParams& p, hipStream_t stream) {
+  if (p.pages.type == PF_KV_E4M3) return launch_dim<Row, PF_KV_E4M3>(p, stream);
+  if (p.pages.type == PF_KV_INT8) return launch_dim<Row, PF_KV_INT8>(p, stream);
+  return launch_dim<Row, Row::kType>(p, stream);
+}
+
+}  // namespace
+}  // namespace pf

@@ -1,5 +1,6 @@
 // pf_paged.cpp — entry points of the paged-cache operators: argument checks, and
-// the launches (pf_paged.hip, pf_attend.hip).
+// the launches (pf_paged.hip, pf_attend_*.hip).
+#include <algorithm>
 #include <cmath>
 
 #include "pf_common.h"
@@ -218,8 +219,8 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   if (!std::isfinite(a->scale)) return invalid("the scale is not finite");
   if (a->num_seqs == 0 || a->num_rows == 0) return PF_OK;
   if (a->table_width == 0) return invalid("the block table has no entries");
-  if (static_cast<uint64_t>(a->table_width) * pv.block_size >= kMaxTokens)
-    return invalid("the block table spans 2^31 tokens or more");
+  if (static_cast<uint64_t>(a->table_width) * pv.block_size > kMaxTokens - kAttendSlack)
+    return invalid("the block table spans more than 2^31 - 65536 tokens");
   if (a->table_stride < a->table_width && a->num_seqs > 1)
     return invalid("rows of the block table overlap");
   if (a->num_seqs >= (1u << 24) || a->num_rows >= kMaxTokens / a->num_q_heads)
@@ -254,10 +255,20 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   p.num_seqs = a->num_seqs;
   p.table_width = a->table_width;
   // A window as long as the table hides nothing.
-  const uint32_t room = a->table_width * pv.block_size;
+  const uint32_t room = a->table_width * pv.block_size;  // checked above
   p.window = a->window >= room ? 0 : a->window;
   p.causal = a->causal != 0;
-  p.scale_log2 = static_cast<float>(a->scale * 1.4426950408889634);
+  p.scale_log2 = static_cast<float>(std::fabs(a->scale) * 1.4426950408889634);
+  // The kernels hide a score by -infinity, which a scale of 0 would turn into NaN; this
+  // one leaves every weight at 1 as 0 does.
+  if (p.scale_log2 < 1e-37f) p.scale_log2 = 1e-37f;
+  p.q_sign = a->scale < 0 ? 0x80008000u : 0;
+  p.aligned = aligned;
+  plan_attend(&p, a->max_query_len, a->max_seq_len, ws ? ws->data : 0, ws ? ws->bytes : 0);
+  const uint64_t grid =
+      std::max<uint64_t>(static_cast<uint64_t>(p.num_seqs) * p.few_splits,
+                         static_cast<uint64_t>(p.many_units) * p.many_splits) * pv.heads;
+  if (grid > 0x7fffffffull) return invalid("too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
   if (int rc = on.enter(s, pv.k)) return rc;
@@ -265,7 +276,7 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   PF_HIP(hipGetDevice(&dev));
   if (ws && ws->device != dev)
     return invalid(strf("the workspace is on device %d, the stream on device %d", ws->device, dev));
-  PF_HIP(launch_attend(p, a->q.type, s));
+  PF_HIP(a->q.type == PF_KV_BF16 ? launch_attend_bf16(p, s) : launch_attend_fp16(p, s));
   return PF_OK;
 }
 

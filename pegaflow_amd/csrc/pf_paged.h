@@ -1,5 +1,5 @@
 // pf_paged.h — the paged-cache operators' arguments, shared by their entry
-// points (pf_paged.cpp) and kernels (pf_paged.hip, pf_attend.hip).
+// points (pf_paged.cpp) and kernels (pf_paged.hip, pf_attend_*.hip).
 #pragma once
 
 #include <hip/hip_runtime_api.h>
@@ -50,8 +50,89 @@ struct AttendParams {
   uint32_t num_rows, q_heads, group, num_seqs, table_width;
   uint32_t window;  // 0: none
   uint32_t causal;
-  float scale_log2;  // score scale times log2(e)
+  float scale_log2;   // |score scale| times log2(e), above 0
+  uint32_t q_sign;    // flips the sign of two 16-bit values where the scale is negative
+  uint32_t aligned;   // q and out move by 16 bytes
+  // The launch (plan_attend): sequences of up to few_rows rows of a KV head go to the
+  // kernel for few, in few_splits shares of few_piece tokens (0: none do), the others
+  // in many_units tiles of rows and many_splits shares.
+  uint32_t few_rows, few_splits, few_piece;
+  uint32_t many_units, many_splits, many_piece;
+  float *few_o, *few_ml, *many_o, *many_ml;  // shares, in the workspace
 };
+
+constexpr uint32_t kFewRows = 16;        // of attend_few_kernel's tile
+constexpr uint32_t kManyRows = 128;      // of attend_many_kernel's
+constexpr uint32_t kAttendSlack = 1u << 16;  // tokens that a kernel's counting may run past the end
+
+// Head sizes that the kernels are built for.
+inline uint32_t padded_dim(uint32_t dim) {
+  return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+}
+
+// Shapes the launch of a batch whose longest query has `most_new` rows and longest
+// sequence `longest` tokens (bounds that may be loose, or wrong: every row is attended
+// whatever they say), joining in `bytes` of workspace at `ws`.
+inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, uint64_t ws,
+                        uint64_t bytes) {
+  constexpr uint64_t kCus = 256;
+  const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
+  const uint64_t room = static_cast<uint64_t>(p->table_width) * p->pages.block_size;
+  if (longest == 0 || longest > room) longest = room;
+  if (most_new == 0 || most_new > p->num_rows) most_new = p->num_rows;
+  if (p->window && p->window + most_new < longest) longest = p->window + most_new;
+  auto ceil_div = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+  const bool all_few = most_new * group <= kFewRows;
+  const bool any_few = all_few || (p->num_seqs > 1 && group <= kFewRows);
+  p->few_rows = any_few && !all_few ? kFewRows : 0;
+  p->few_splits = p->few_piece = p->many_units = p->many_splits = p->many_piece = 0;
+  uint64_t at = ws;
+  const uint64_t end = ws + bytes;
+  if (any_few) {
+    const uint64_t units = p->num_seqs * heads;
+    const uint64_t slot = kFewRows * (dim * 4 + 8);
+    const uint64_t want = ceil_div(kCus * 4, units);
+    uint64_t piece = ceil_div(ceil_div(longest, want), 128) * 128;
+    if (piece < 256) piece = 256;
+    uint64_t splits = ceil_div(longest, piece);
+    if (splits * units * slot > end - at) {
+      splits = (end - at) / (units * slot);
+      if (splits < 2) splits = 1;
+      piece = ceil_div(ceil_div(longest, splits), 128) * 128;
+    }
+    p->few_splits = static_cast<uint32_t>(splits);
+    p->few_piece = static_cast<uint32_t>(piece);
+    if (splits > 1) {
+      const uint64_t n = units * splits * kFewRows;
+      p->few_o = reinterpret_cast<float*>(at);
+      p->few_ml = reinterpret_cast<float*>(at + n * dim * 4);
+      at += n * (dim * 4 + 8);
+    }
+  }
+  if (!all_few) {
+    const uint64_t rows = p->num_rows * group;
+    const uint64_t seqs = p->num_seqs < p->num_rows ? p->num_seqs : p->num_rows;
+    const uint64_t tiles = rows / kManyRows + seqs, units = tiles * heads;
+    const uint64_t slot = kManyRows * (dim * 4 + 16);
+    const uint64_t want = units < kCus * 2 ? kCus * 2 / units : 1;
+    uint64_t piece = ceil_div(ceil_div(longest, want), 64) * 64;
+    if (piece < 256) piece = 256;
+    uint64_t splits = ceil_div(longest, piece);
+    if (splits * units * slot > end - at) {
+      splits = (end - at) / (units * slot);
+      if (splits < 2) splits = 1;
+      piece = ceil_div(ceil_div(longest, splits), 64) * 64;
+    }
+    p->many_units = static_cast<uint32_t>(tiles);
+    p->many_splits = static_cast<uint32_t>(splits);
+    p->many_piece = static_cast<uint32_t>(piece);
+    if (splits > 1) {
+      const uint64_t n = units * splits * kManyRows;
+      p->many_o = reinterpret_cast<float*>(at);
+      p->many_ml = reinterpret_cast<float*>(at + n * dim * 4);
+    }
+  }
+}
 
 hipError_t launch_kv_write(const PagedView& pages, const RowsView& k, const RowsView& v,
                            uint32_t row_type, const int64_t* slots, uint32_t n, bool aligned,
@@ -59,6 +140,7 @@ hipError_t launch_kv_write(const PagedView& pages, const RowsView& k, const Rows
 hipError_t launch_kv_read(const PagedView& pages, const RowsView& k, const RowsView& v,
                           uint32_t row_type, const int64_t* slots, uint32_t n, bool aligned,
                           hipStream_t stream);
-hipError_t launch_attend(const AttendParams& p, uint32_t row_type, hipStream_t stream);
+hipError_t launch_attend_bf16(const AttendParams& p, hipStream_t stream);
+hipError_t launch_attend_fp16(const AttendParams& p, hipStream_t stream);
 
 }  // namespace pf

@@ -133,7 +133,7 @@ ATTEND_REFUSALS = [
     (dict(scale=float("nan")), "not finite"),
     (dict(scale=float("inf")), "not finite"),
     (dict(table_width=0), "no entries"),
-    (dict(table_width=1 << 27), "2^31 tokens"),
+    (dict(table_width=(1 << 27) - 4095), "2^31 - 65536 tokens"),
     (dict(table_stride=3), "rows of the block table overlap"),
     (dict(num_rows=1 << 30), "too many rows"),
     (dict(out=rows(ts=128)), "out: rows overlap"),
