@@ -160,20 +160,31 @@ __device__ __forceinline__ void store_out4(uint64_t row, uint32_t d, const Atten
 }
 
 // V in a tile that some row attends only in part: a weight of 0 must not meet an
-// infinity or NaN, so those values are zero in LDS, and the tile's caller returns for
-// them at the end (add_odd).  Returns whether there were any.
-template <class VM>
+// infinity or NaN, so those values are taken as zero, and the tile's caller returns for
+// them at the end (add_odd).  Returns whether there were any among these 16 bytes.
+template <class Row, uint32_t TYPE>
 __device__ __forceinline__ bool clear_odd(u32x4& v) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) top = max(top, max(v[w] & 0x7fffu, (v[w] >> 16) & 0x7fffu));
-  if (top < VM::kInf) return false;
+  if constexpr (TYPE == PF_KV_INT8) return false;
+  bool odd = false;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if ((v[w] & 0x7fffu) >= VM::kInf) v[w] &= 0xffff0000u;
-    if (((v[w] >> 16) & 0x7fffu) >= VM::kInf) v[w] &= 0xffffu;
+    if constexpr (TYPE == PF_KV_E4M3) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        if (((v[w] >> i) & 0x7fu) == 0x7fu) {
+          v[w] &= ~(0xffu << i);
+          odd = true;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 16)
+        if (((v[w] >> i) & 0x7fffu) >= Row::kInf) {
+          v[w] &= ~(0xffffu << i);
+          odd = true;
+        }
+    }
   }
-  return true;
+  return odd;
 }
 
 // Adds the infinities and NaN among values d to d + 3 of V of the token at `at` (their
@@ -255,6 +266,7 @@ __device__ __forceinline__ bool token_at(const PagedView& p, int32_t block, uint
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kTileTokens = 64;
 constexpr uint32_t kManyThreads = 256;
+constexpr uint32_t kRing = 256;
 
 // Bytes from one token to the next in LDS.  K: 16-byte reads of 16 neighbouring tokens
 // fall into different banks.  V: a transposing read takes 64 bytes of each of 4 tokens.
@@ -269,15 +281,19 @@ template <uint32_t DP>
 struct ManyLds {
   // Two tiles in turn where two workgroups still fit the compute unit's 160 KB.
   static constexpr uint32_t kBuffers = DP <= 128 ? 2 : 1;
-  struct Tile {
-    __attribute__((aligned(16))) uint8_t k[kTileTokens * k_pitch(DP)];
-    __attribute__((aligned(16))) uint8_t v[kTileTokens * v_pitch(DP)];
-    __attribute__((aligned(16))) float k_scale[kTileTokens];
-    __attribute__((aligned(16))) float v_scale[kTileTokens];
-  } tile[kBuffers];
-  // Tokens of a tile whose block is missing, in turn over four tiles: a slot is cleared
-  // two tiles before its next use.
-  unsigned long long hole[4];
+  struct K {
+    __attribute__((aligned(16))) uint8_t data[kTileTokens * k_pitch(DP)];
+    __attribute__((aligned(16))) float k_scale[kTileTokens], v_scale[kTileTokens];
+  } k[kBuffers];
+  struct V {
+    __attribute__((aligned(16))) uint8_t data[kTileTokens * v_pitch(DP)];
+  } v[kBuffers];
+  // Where units of tokens lie in K's (or V's) pages, and their scales, for the tiles to
+  // come: a ring of two halves, each filled as the other is used up.  A unit is the tokens
+  // that surely share a block (AttendParams::unit_shift); one without a block has a place
+  // that may be read, and is not there.
+  uint64_t at[kRing], scale_at[kRing];
+  uint8_t there[kRing];
   uint32_t odd;  // some tile attended in part holds V that is not finite
 };
 
@@ -371,13 +387,15 @@ template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1)
 attend_many_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
-  using KM = Row;                                          // K as multiplied
+  using KM = Row;                                                 // K as multiplied
   using VM = typename std::conditional<kCodes, BF16, Row>::type;  // V and the weights
-  constexpr uint32_t kPer = kCodes ? 16 : 8;               // values of a 16-byte load
-  constexpr uint32_t kCols = DP / kPer;
-  constexpr uint32_t kLoads = (kTileTokens * kCols + kManyThreads - 1) / kManyThreads;
-  constexpr bool kWhole = kTileTokens * kCols % kManyThreads == 0;
+  constexpr uint32_t kPer = kCodes ? 16 : 8;                      // values of a 16-byte load
+  // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
+  constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
+  constexpr uint32_t kLoads = kTileTokens * kCols / kManyThreads;
+  constexpr uint32_t kLoadTokens = kManyThreads / kCols;  // of one load of the workgroup
   constexpr uint32_t kKP = k_pitch(DP), kVP = v_pitch(DP);
+  constexpr int32_t kStep = kTileTokens;
   using Lds = ManyLds<DP>;
   __shared__ Lds lds;
   const PagedView& pg = a.pages;
@@ -395,20 +413,19 @@ attend_many_kernel(AttendParams a) {
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, split, a.many_splits, a.many_piece);
   if (split >= used) return;
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
   const int32_t* table = a.block_table + t.seq * a.table_stride;
 
   // Tokens that every row of the workgroup attends, and this wave's and row's.
-  const uint32_t wave0 = t.row - (lane & 31u), group = a.group;
+  const uint32_t wave0 = __builtin_amdgcn_readfirstlane(t.row), group = a.group;
   const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + kTileRows, t.rows) - 1;
   const int32_t all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
   const int32_t all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
   const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
   const int32_t my_begin = row_begin(a, pos);
   const int32_t my_end = t.valid ? row_end(a, t.s.len, pos) : 0;
-  const bool wave_valid = wave0 < t.rows;
-  const uint32_t wave_last = min(wave0 + 32, t.rows) - 1;
-  const int32_t wave_end =
-      wave_valid ? row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(wave_last / group)) : 0;
+  const bool wave_rows = wave0 < t.rows;
 
   u32x4 q[DP / 16];
   const uint64_t q_row = row_address(a, a.q, t);
@@ -422,145 +439,170 @@ attend_many_kernel(AttendParams a) {
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
   float m = kNegInf, l = 0.0f;
 
-  // This thread's part of a tile: 16 bytes of kLoads tokens, and of 8-bit pages the K or
-  // V scale of one token (threads 0 to 127).
-  int32_t block[kLoads], s_block = 0;
+  // This thread's part of a tile: 16 bytes of tokens my_tok + kLoadTokens * i, values
+  // my_d and on, and of 8-bit pages the scales of token 16 * wave + lane (lanes 0 to 15).
+  const uint32_t my_tok = tid / kCols, my_d = (tid % kCols) * kPer;
+  const bool my_col = my_d < pg.dim;
+  const uint32_t shift = a.unit_shift, in_unit = (1u << shift) - 1, tile_units = kTileTokens >> shift;
+  // A load's tokens repeat their place in their unit after at most two loads.
+  constexpr uint32_t kOffsets = kLoadTokens < 16 ? 2 : 1;
+  uint32_t lane_at[kOffsets];
+#pragma unroll
+  for (uint32_t i = 0; i < kOffsets; ++i)
+    lane_at[i] = ((my_tok + i * kLoadTokens) & in_unit) * pg.token_bytes +
+                 (my_col ? my_d : 0) * (kCodes ? 1 : 2);
+  const uint32_t lane_scale = (lane & in_unit & 15u) * 4u;
   u32x4 kr[kLoads], vr[kLoads];
-  float sr = 0.0f;
-  auto token_of = [&](uint32_t i) { return (tid + i * kManyThreads) / kCols; };
-  auto col_of = [&](uint32_t i) { return (tid + i * kManyThreads) % kCols; };
-  auto load_blocks = [&](int32_t t0) {
-#pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) {
-      const int32_t tok = t0 + static_cast<int32_t>(token_of(i));
-      block[i] = tok < end ? table[page_of(pg, tok)] : -1;
-    }
-    if constexpr (kCodes) {
-      const int32_t tok = t0 + static_cast<int32_t>(tid & 63u);
-      s_block = tok < end && tid < 128 ? table[page_of(pg, tok)] : -1;
-    }
+  float k_sr = 0.0f, v_sr = 0.0f;
+  // The half of the ring that starts with tile n.
+  auto fill_ring = [&](uint32_t n) {
+    if (tid >= kRing / 2) return;
+    const uint32_t unit = n * tile_units + tid;
+    const int32_t tok = begin + static_cast<int32_t>(unit << shift);
+    const uint32_t page = page_of(pg, min(tok, end - 1));
+    const int32_t block = tok < end ? table[page] : -1;
+    uint64_t at, scale_at;
+    const bool in = token_at(pg, block, tok, page, head, &at, &scale_at);
+    lds.at[unit % kRing] = in ? at : 0;
+    if constexpr (kCodes) lds.scale_at[unit % kRing] = in ? scale_at : pg.scale_offset;
+    lds.there[unit % kRing] = in;
   };
-  auto load_tile = [&](int32_t t0) {
-#pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) {
-      const int32_t tok = t0 + static_cast<int32_t>(token_of(i));
-      const uint32_t d = col_of(i) * kPer;
-      uint64_t at, scale_at;
-      const bool in = token_at(pg, block[i], tok, page_of(pg, tok), head, &at, &scale_at);
-      kr[i] = u32x4{0, 0, 0, 0};
-      vr[i] = u32x4{0, 0, 0, 0};
-      if (tok < end && in && d < pg.dim && (kWhole || token_of(i) < kTileTokens)) {
-        at += d * (kCodes ? 1 : 2);
-        kr[i] = *reinterpret_cast<const g_u32x4*>(pg.k + at);
-        vr[i] = *reinterpret_cast<const g_u32x4*>(pg.v + at);
-      }
-    }
-    if constexpr (kCodes) {
-      const int32_t tok = t0 + static_cast<int32_t>(tid & 63u);
-      uint64_t at, scale_at;
-      const bool in = token_at(pg, s_block, tok, page_of(pg, tok), head, &at, &scale_at);
-      sr = 0.0f;
-      if (tid < 128 && tok < end && in)
-        sr = *reinterpret_cast<const g_f32*>((tid < 64 ? pg.k : pg.v) + scale_at);
-    }
+  auto unit_of = [&](uint32_t n, uint32_t tok) {
+    return (n * tile_units & (kRing - 1)) + (tok >> shift);
   };
-  // Into LDS.  `partial`: some row does not attend every token.
-  auto store_tile = [&](int32_t t0, uint32_t slot, bool partial, typename Lds::Tile& tile) {
+  auto load_k = [&](uint32_t n) {
 #pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) {
-      const uint32_t tok = token_of(i), col = col_of(i);
-      if (!kWhole && tok >= kTileTokens) continue;
-      if (t0 + static_cast<int32_t>(tok) < end && static_cast<uint32_t>(block[i]) >= pg.num_blocks)
-        atomicOr(&lds.hole[slot], 1ull << tok);
-      u32x4 v0, v1{0, 0, 0, 0};
-      if constexpr (kCodes) {
-        const u32x2 a0 = codes_to_16<KM, TYPE>(kr[i][0]), a1 = codes_to_16<KM, TYPE>(kr[i][1]);
-        const u32x2 a2 = codes_to_16<KM, TYPE>(kr[i][2]), a3 = codes_to_16<KM, TYPE>(kr[i][3]);
-        u32x4* kd = reinterpret_cast<u32x4*>(tile.k + tok * kKP + col * 32);
-        kd[0] = u32x4{a0[0], a0[1], a1[0], a1[1]};
-        kd[1] = u32x4{a2[0], a2[1], a3[0], a3[1]};
-        const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
-        const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
-        v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
-        v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
-      } else {
-        *reinterpret_cast<u32x4*>(tile.k + tok * kKP + col * 16) = kr[i];
-        v0 = vr[i];
-      }
-      if (partial && TYPE != PF_KV_INT8) {
-        bool odd = clear_odd<VM>(v0);
-        if constexpr (kCodes) odd |= clear_odd<VM>(v1);
-        if (odd) lds.odd = 1;
-      }
-      if constexpr (kCodes) {
-        u32x4* vd = reinterpret_cast<u32x4*>(tile.v + tok * kVP + col * 32);
-        vd[0] = v0;
-        vd[1] = v1;
-      } else {
-        *reinterpret_cast<u32x4*>(tile.v + tok * kVP + col * 16) = v0;
-      }
-    }
+    for (uint32_t i = 0; i < kLoads; ++i)
+      kr[i] = *reinterpret_cast<const g_u32x4*>(
+          pg.k + lds.at[unit_of(n, my_tok + i * kLoadTokens)] + lane_at[i % kOffsets]);
     if constexpr (kCodes)
-      if (tid < 128) (tid < 64 ? tile.k_scale : tile.v_scale)[tid & 63u] = sr;
+      if (lane < 16) {
+        const uint64_t at = lds.scale_at[unit_of(n, wave * 16 + lane)] + lane_scale;
+        k_sr = *reinterpret_cast<const g_f32*>(pg.k + at);
+        v_sr = *reinterpret_cast<const g_f32*>(pg.v + at);
+      }
   };
-
-  if (tid < 4) lds.hole[tid] = 0;
-  if (tid == 4) lds.odd = 0;
-  load_blocks(begin);
-  load_tile(begin);
-  __syncthreads();
-  uint32_t n = 0;
-  for (int32_t t0 = begin; t0 < end; t0 += kTileTokens, ++n) {
-    const uint32_t slot = n & 3u;
-    const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kTileTokens) > all_end;
-    typename Lds::Tile& tile = lds.tile[n % Lds::kBuffers];
-    if (Lds::kBuffers == 1 && n) __syncthreads();  // the tile before has been read
-    store_tile(t0, slot, partial, tile);
-    __syncthreads();
-    if (tid == 0) lds.hole[(slot + 2) & 3u] = 0;
-    const int32_t next = t0 + static_cast<int32_t>(kTileTokens);
-    if (next < end) {
-      load_blocks(next);
-      load_tile(next);
+  auto load_v = [&](uint32_t n) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i)
+      vr[i] = *reinterpret_cast<const g_u32x4*>(
+          pg.v + lds.at[unit_of(n, my_tok + i * kLoadTokens)] + lane_at[i % kOffsets]);
+  };
+  auto tokens_there = [&](uint32_t n) { return __ballot(lds.there[unit_of(n, lane)] != 0); };
+  // K into LDS.
+  auto store_k = [&](uint32_t n) {
+    typename Lds::K& tile = lds.k[n % Lds::kBuffers];
+    if (my_col)
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) {
+        u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kKP + my_d * 2);
+        if constexpr (kCodes) {
+          const u32x2 x0 = codes_to_16<KM, TYPE>(kr[i][0]), x1 = codes_to_16<KM, TYPE>(kr[i][1]);
+          const u32x2 x2 = codes_to_16<KM, TYPE>(kr[i][2]), x3 = codes_to_16<KM, TYPE>(kr[i][3]);
+          to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
+          to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
+        } else {
+          to[0] = kr[i];
+        }
+      }
+    if constexpr (kCodes)
+      if (lane < 16) {
+        tile.k_scale[wave * 16 + lane] = k_sr;
+        tile.v_scale[wave * 16 + lane] = v_sr;
+      }
+  };
+  // V of tile n into LDS; `masked`: some row does not attend every token; bit j of
+  // `there`: token j has a block.
+  auto store_v = [&](uint32_t n, bool masked, uint64_t there) {
+    typename Lds::V& tile = lds.v[n % Lds::kBuffers];
+    if (masked) {
+      bool odd = false;
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) {
+        const uint32_t tok = my_tok + i * kLoadTokens;
+        if (!(there >> tok & 1u) || begin + static_cast<int32_t>(n * kTileTokens + tok) >= end)
+          vr[i] = u32x4{0, 0, 0, 0};
+        odd |= clear_odd<Row, TYPE>(vr[i]);
+      }
+      if (odd && my_col) lds.odd = 1;
     }
-    if (t0 >= wave_end) continue;  // this wave's rows end before the tile
-
-    // S^T: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.
-    f32x16 s[2];
+    if (my_col)
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) {
+        u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kVP + my_d * 2);
+        if constexpr (kCodes) {
+          const u32x2 x0 = codes_to_16<VM, TYPE>(vr[i][0]), x1 = codes_to_16<VM, TYPE>(vr[i][1]);
+          const u32x2 x2 = codes_to_16<VM, TYPE>(vr[i][2]), x3 = codes_to_16<VM, TYPE>(vr[i][3]);
+          to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
+          to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
+        } else {
+          to[0] = vr[i];
+        }
+      }
+  };
+  // S^T of tile n: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.
+  f32x16 s[2];
+  auto scores = [&](uint32_t n) {
+    const uint8_t* at = lds.k[n % Lds::kBuffers].data + (lane & 31u) * kKP + half * 16;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[tt][i] = 0.0f;
-    const uint8_t* k_at = tile.k + (lane & 31u) * kKP + half * 16;
 #pragma unroll
     for (uint32_t kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
-        s[tt] = Mat<KM>::mul32(*reinterpret_cast<const u32x4*>(k_at + tt * 32 * kKP + kk * 32),
-                               q[kk], s[tt]);
+        s[tt] = Mat<KM>::mul32(*reinterpret_cast<const u32x4*>(at + tt * 32 * kKP + kk * 32), q[kk],
+                               s[tt]);
     if constexpr (kCodes) {
+      const float* scale = lds.k[n % Lds::kBuffers].k_scale + half * 4;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(tile.k_scale + tt * 32 + i * 8 + half * 4);
+          const f32x4 x = *reinterpret_cast<const f32x4*>(scale + tt * 32 + i * 8);
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[tt][4 * i + j] *= x[j];
         }
     }
-    const uint64_t hole = lds.hole[slot];
-    const bool masked = partial || hole;
+  };
+  // O^T += V^T W^T of 16 tokens of tile n, the weights w of its tokens 16 u and on.  They
+  // are taken in the order in which a lane holds their weights: 4 half + (0..3), then 8 +
+  // 4 half + (0..3).
+  const uint32_t quad = lane & 15u;
+  const uint32_t v_lane = (half * 4 + quad / 4) * kVP + ((lane >> 4) & 1u) * 32 + (quad & 3u) * 8;
+  auto add_v = [&](uint32_t n, int u, u32x4 w) {
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt) {
+      const uint8_t* from = lds.v[n % Lds::kBuffers].data + v_lane + u * 16 * kVP + dt * 64;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from + 8 * kVP));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      o[dt] = Mat<VM>::mul32(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+    }
+  };
+  // Tile n's scores and softmax.  Its product with V follows in the next step, under that
+  // tile's softmax: p are the weights of tile n - 1 at first, of tile n at the end.
+  u32x4 p[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) p[u] = u32x4{0, 0, 0, 0};
+  auto step = [&](int32_t t0, uint32_t n, bool masked, uint64_t hole) {
+    scores(n);
     if (masked) {
+      // Token 32 tt + 8 (i / 4) + i % 4 of this half's, against its row's limits.
+      const int32_t lo = my_begin - t0 - static_cast<int32_t>(4 * half);
+      const int32_t hi = my_end - t0 - static_cast<int32_t>(4 * half);
+      const uint64_t gone = hole >> (4 * half);
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const uint32_t j = tt * 32 + 8 * (i / 4) + 4 * half + i % 4;
-          const int32_t tok = t0 + static_cast<int32_t>(j);
-          if (tok < my_begin || tok >= my_end || (hole >> j & 1)) s[tt][i] = kNegInf;
+          const int32_t j = tt * 32 + 8 * (i / 4) + i % 4;
+          if (j < lo || j >= hi || (static_cast<uint32_t>(gone >> (32 * tt)) >> (j & 31) & 1u))
+            s[tt][i] = kNegInf;
         }
     }
-    float top = kNegInf;
+    float top = s[0][0];
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -569,69 +611,110 @@ attend_many_kernel(AttendParams a) {
     // The maximum that the weights are taken against follows the largest score only
     // where that has grown by more than 8 (in powers of 2): until then weights up to
     // 2^8 serve as well, and the outputs need no rescaling.
-    if (__any((top - m) * a.scale_log2 > 8.0f)) {
+    const bool grown = __any((top - m) * a.scale_log2 > 8.0f);
+    float keep = 1.0f;
+    if (grown) {
       const float m_new = fmaxf(m, top);
-      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+      keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
       m = m_new;
-      l *= keep;
+    }
+    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      add_v(n + 1, u, p[u]);
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float z = s[u / 2][8 * (u & 1) + i];
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z, a.scale_log2, base));
+        sum += x[i];
+      }
+      if constexpr (kCodes) {
+        const float* scale = lds.k[n % Lds::kBuffers].v_scale + u * 16 + half * 4;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(scale + g * 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[4 * g + j] *= y[j];
+        }
+        if (masked) {  // a hidden token's scale may be anything
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (s[u / 2][8 * (u & 1) + i] == kNegInf) x[i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[u][j] = Mat<VM>::pack(x[2 * j], x[2 * j + 1]);
+    }
+    // The weights before the branch, so that they are computed beside the products.
+    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (uint32_t i = 0; i < DP / 32 * 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // product
+      __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);  // exponentials
+      __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);    // vector
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+    }
+    l = l * keep + sum;
+    if (grown) {  // the outputs up to tile n - 1
 #pragma unroll
       for (uint32_t dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] *= keep;
     }
-    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
-    float sum = 0.0f;
+  };
+
+  if (tid == 0) lds.odd = 0;
+  // Values past the head's size, and V before the first tile, which meets weights of 0.
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+  for (uint32_t i = 0; i < kLoads; ++i)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
-        sum += w;
-        if constexpr (!kCodes) s[tt][i] = w;
-        else s[tt][i] = masked && s[tt][i] == kNegInf ? kNegInf : w;  // V scales follow
-      }
-    l += sum;
-    if constexpr (kCodes) {
+    for (uint32_t j = 0; j < kPer / 8; ++j) {
+      const uint32_t tok = my_tok + i * kLoadTokens;
+      if (my_d >= DP) continue;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(tile.v_scale + tt * 32 + i * 8 + half * 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float w = s[tt][4 * i + j];
-            s[tt][4 * i + j] = w == kNegInf ? 0.0f : w * x[j];
-          }
-        }
-    }
-    // O^T += V^T W^T.  The 16 tokens of a product are taken in the order in which a lane
-    // holds their weights: 4 half + (0..3), then 8 + 4 half + (0..3).
-    const uint32_t quad = lane & 15u;
-    const uint8_t* v_at = tile.v + (half * 4 + quad / 4) * kVP + ((lane >> 4) & 1u) * 32 +
-                          (quad & 3u) * 8;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      u32x4 w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = Mat<VM>::pack(s[u / 2][8 * (u & 1) + 2 * j], s[u / 2][8 * (u & 1) + 2 * j + 1]);
-#pragma unroll
-      for (uint32_t dt = 0; dt < DP / 32; ++dt) {
-        const uint8_t* at = v_at + u * 16 * kVP + dt * 64;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(at));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(at + 8 * kVP));
-        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-        o[dt] = Mat<VM>::mul32(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+      for (uint32_t b = 0; b < Lds::kBuffers; ++b) {
+        if (!my_col)
+          reinterpret_cast<u32x4*>(lds.k[b].data + tok * kKP + my_d * 2)[j] = u32x4{0, 0, 0, 0};
+        reinterpret_cast<u32x4*>(lds.v[b].data + tok * kVP + my_d * 2)[j] = u32x4{0, 0, 0, 0};
       }
     }
+  if (begin < end) {
+    fill_ring(0);
+    __syncthreads();
+    load_k(0);
+    uint64_t there = tokens_there(0), v_there = ~0ull;
+    bool v_masked = false;
+    uint32_t n = 0;
+    for (int32_t t0 = begin; t0 < end; t0 += kStep, ++n) {
+      const bool masked = t0 < all_begin || t0 + kStep > all_end || ~there;
+      if (Lds::kBuffers == 1) __syncthreads();  // the tiles before have been read
+      store_k(n);
+      if (n) store_v(n - 1, v_masked, v_there);
+      if ((n + 1) * tile_units % (kRing / 2) == 0) fill_ring(n + 1);
+      __syncthreads();
+      v_masked = masked;
+      v_there = there;
+      there = tokens_there(n + 1);
+      load_v(n);
+      load_k(n + 1);
+      if (wave_rows) step(t0, n, masked, ~v_there);
+    }
+    if (Lds::kBuffers == 1) __syncthreads();
+    store_v(n - 1, v_masked, v_there);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) add_v(n - 1, u, p[u]);
   }
 
   __syncthreads();
   if (lds.odd)
     for (int32_t tok = begin; tok < end; ++tok) {
       if (tok < my_begin || tok >= my_end) continue;
-      const int32_t t0 = tok & ~static_cast<int32_t>(kTileTokens - 1);
-      if (t0 >= all_begin && t0 + static_cast<int32_t>(kTileTokens) <= all_end) continue;
+      const int32_t t0 = tok & ~(kStep - 1);
+      if (t0 >= all_begin && t0 + kStep <= all_end) continue;
       uint64_t at, scale_at;
       const uint32_t page = page_of(pg, tok);
       if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
@@ -843,16 +926,13 @@ attend_few_kernel(AttendParams a) {
       for (uint32_t i = 0; i < kVLoads; ++i) {
         const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
         const bool mine = kFewTokens * kCols % 64 == 0 || j < kFewTokens;
+        if (partial) odd |= clear_odd<Row, TYPE>(vr[i]);
         u32x4 v0 = vr[i], v1{0, 0, 0, 0};
         if constexpr (kCodes) {
           const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
           const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
           v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
           v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
-        }
-        if (partial && TYPE != PF_KV_INT8) {
-          odd |= clear_odd<VM>(v0);
-          if constexpr (kCodes) odd |= clear_odd<VM>(v1);
         }
         if (mine) {
           u32x4* vd = reinterpret_cast<u32x4*>(v_lds + j * kVP + cc * (kCodes ? 32 : 16));

@@ -264,6 +264,7 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   if (p.scale_log2 < 1e-37f) p.scale_log2 = 1e-37f;
   p.q_sign = a->scale < 0 ? 0x80008000u : 0;
   p.aligned = aligned;
+  while (p.unit_shift < 4 && !(pv.block_size >> p.unit_shift & 1u)) ++p.unit_shift;
   plan_attend(&p, a->max_query_len, a->max_seq_len, ws ? ws->data : 0, ws ? ws->bytes : 0);
   const uint64_t grid =
       std::max<uint64_t>(static_cast<uint64_t>(p.num_seqs) * p.few_splits,

@@ -53,6 +53,7 @@ struct AttendParams {
   float scale_log2;   // |score scale| times log2(e), above 0
   uint32_t q_sign;    // flips the sign of two 16-bit values where the scale is negative
   uint32_t aligned;   // q and out move by 16 bytes
+  uint32_t unit_shift;  // 2^unit_shift aligned tokens, at most 16, share a block
   // The launch (plan_attend): sequences of up to few_rows rows of a KV head go to the
   // kernel for few, in few_splits shares of few_piece tokens (0: none do), the others
   // in many_units tiles of rows and many_splits shares.
