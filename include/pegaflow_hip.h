@@ -656,8 +656,10 @@ typedef struct pf_attend_args {
   uint32_t window;       /* 0: none */
   uint32_t causal;
   float scale;           /* of the scores */
-  uint32_t max_seq_len;  /* hints that shape the launch, not limits: the longest */
-  uint32_t max_query_len; /* sequence and query; 0: table_width * block_size, num_rows */
+  uint32_t max_seq_len;   /* the longest sequence, as a hint that shapes the launch */
+                          /* (0: table_width * block_size)                          */
+  uint32_t max_query_len; /* no sequence has more rows (0: num_rows); those that one */
+                          /* has beyond it may stay as they were                     */
 } pf_attend_args;
 
 /* Device memory in which calls with few rows and long sequences join the shares

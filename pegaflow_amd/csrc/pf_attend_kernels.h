@@ -25,7 +25,10 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "pf_paged_device.h"
+
 
 namespace pf {
 namespace {
@@ -165,26 +168,20 @@ __device__ __forceinline__ void store_out4(uint64_t row, uint32_t d, const Atten
 template <class Row, uint32_t TYPE>
 __device__ __forceinline__ bool clear_odd(u32x4& v) {
   if constexpr (TYPE == PF_KV_INT8) return false;
-  bool odd = false;
+  u32x4 odd;  // all ones in the values to clear
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    if constexpr (TYPE == PF_KV_E4M3) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        if (((v[w] >> i) & 0x7fu) == 0x7fu) {
-          v[w] &= ~(0xffu << i);
-          odd = true;
-        }
+    if constexpr (TYPE == PF_KV_E4M3) {  // NaN: 0x7f and a sign
+      const uint32_t top = ((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+      odd[w] = (top >> 7) * 0xffu;
     } else {
-#pragma unroll
-      for (int i = 0; i < 32; i += 16)
-        if (((v[w] >> i) & 0x7fffu) >= Row::kInf) {
-          v[w] &= ~(0xffffu << i);
-          odd = true;
-        }
+      const int32_t lo = static_cast<int32_t>(Row::kInf - 1 - (v[w] & 0x7fffu)) >> 31;
+      const int32_t hi = static_cast<int32_t>(Row::kInf - 1 - ((v[w] >> 16) & 0x7fffu)) >> 31;
+      odd[w] = (static_cast<uint32_t>(lo) & 0xffffu) | (static_cast<uint32_t>(hi) << 16);
     }
+    v[w] &= ~odd[w];
   }
-  return odd;
+  return (odd[0] | odd[1] | odd[2] | odd[3]) != 0;
 }
 
 // Adds the infinities and NaN among values d to d + 3 of V of the token at `at` (their
@@ -201,8 +198,8 @@ __device__ __forceinline__ void add_odd(uint64_t at, uint32_t d, uint32_t dim, f
     for (int i = 0; i < 4; ++i) v[i] = Row::to_float((x[i / 2] >> (16 * (i & 1))) & 0xffffu);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (!__builtin_isfinite(v[i])) o[i] += v[i];
+  for (int i = 0; i < 4; ++i)  // v - v is 0 or NaN
+    o[i] += v[i] - v[i] == 0.0f ? 0.0f : v[i];
 }
 
 // A sequence of the batch: its first row, its rows, its tokens.  Starts and lengths
@@ -216,6 +213,11 @@ __device__ __forceinline__ Seq seq_of(const AttendParams& a, uint32_t b) {
   const int32_t last = min(max(a.query_starts[b + 1], 0), total);
   const int32_t room = static_cast<int32_t>(a.table_width * a.pages.block_size);
   return {first, max(last - first, 0), min(max(a.seq_lens[b], 0), room)};
+}
+
+// The lowest n bits (none for n < 0, all for n > 63).
+__device__ __forceinline__ uint64_t bits_below(int32_t n) {
+  return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
 // Tokens that the row at position `pos` attends: [begin, end).
@@ -540,20 +542,35 @@ attend_many_kernel(AttendParams a) {
         }
       }
   };
-  // S^T of tile n: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.
+  // S^T of tile n: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.  The reads
+  // of one group of products are under way during the group before.
   f32x16 s[2];
-  auto scores = [&](uint32_t n) {
+  constexpr uint32_t kGroup = 2;  // steps of 16 values: 4 products
+  u32x4 kf[2][kGroup][2];
+  auto read_k = [&](uint32_t n, uint32_t g, u32x4 (&f)[kGroup][2]) {
     const uint8_t* at = lds.k[n % Lds::kBuffers].data + (lane & 31u) * kKP + half * 16;
+#pragma unroll
+    for (uint32_t j = 0; j < kGroup; ++j)
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+        f[j][tt] = *reinterpret_cast<const u32x4*>(at + tt * 32 * kKP + (g * kGroup + j) * 32);
+  };
+  auto scores = [&](uint32_t n) {
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[tt][i] = 0.0f;
 #pragma unroll
-    for (uint32_t kk = 0; kk < DP / 16; ++kk)
+    for (uint32_t g = 0; g < DP / 16 / kGroup; ++g) {
+      if (g + 1 < DP / 16 / kGroup) read_k(n, g + 1, kf[(g + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        s[tt] = Mat<KM>::mul32(*reinterpret_cast<const u32x4*>(at + tt * 32 * kKP + kk * 32), q[kk],
-                               s[tt]);
+      for (uint32_t j = 0; j < kGroup; ++j)
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+          s[tt] = Mat<KM>::mul32(kf[g & 1][j][tt], q[g * kGroup + j], s[tt]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (kCodes) {
       const float* scale = lds.k[n % Lds::kBuffers].k_scale + half * 4;
 #pragma unroll
@@ -566,20 +583,25 @@ attend_many_kernel(AttendParams a) {
         }
     }
   };
-  // O^T += V^T W^T of 16 tokens of tile n, the weights w of its tokens 16 u and on.  They
-  // are taken in the order in which a lane holds their weights: 4 half + (0..3), then 8 +
-  // 4 half + (0..3).
+  // V^T of 16 tokens of tile n, from 16 u on.  They are taken in the order in which a
+  // lane holds their weights: 4 half + (0..3), then 8 + 4 half + (0..3).
   const uint32_t quad = lane & 15u;
   const uint32_t v_lane = (half * 4 + quad / 4) * kVP + ((lane >> 4) & 1u) * 32 + (quad & 3u) * 8;
-  auto add_v = [&](uint32_t n, int u, u32x4 w) {
+  u32x4 vf[2][DP / 32];
+  auto read_v = [&](uint32_t n, int u, u32x4 (&f)[DP / 32]) {
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 32; ++dt) {
       const uint8_t* from = lds.v[n % Lds::kBuffers].data + v_lane + u * 16 * kVP + dt * 64;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from + 8 * kVP));
       const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-      o[dt] = Mat<VM>::mul32(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+      f[dt] = u32x4{x[0], x[1], y[0], y[1]};
     }
+  };
+  // O^T += V^T W^T.
+  auto add_v = [&](const u32x4 (&f)[DP / 32], u32x4 w) {
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt) o[dt] = Mat<VM>::mul32(f[dt], w, o[dt]);
   };
   // Tile n's scores and softmax.  Its product with V follows in the next step, under that
   // tile's softmax: p are the weights of tile n - 1 at first, of tile n at the end.
@@ -587,20 +609,28 @@ attend_many_kernel(AttendParams a) {
 #pragma unroll
   for (int u = 0; u < 4; ++u) p[u] = u32x4{0, 0, 0, 0};
   auto step = [&](int32_t t0, uint32_t n, bool masked, uint64_t hole) {
+    __builtin_amdgcn_s_setprio(1);  // ahead of the other workgroup's softmax
     scores(n);
+    __builtin_amdgcn_s_setprio(0);
+    read_v(n + 1, 0, vf[0]);  // the buffer of tile n - 1
     if (masked) {
-      // Token 32 tt + 8 (i / 4) + i % 4 of this half's, against its row's limits.
+      // Bit j of `seen`: this half's token j, of 64, is attended; its scores are tokens
+      // 32 tt + 8 (i / 4) + i % 4.
       const int32_t lo = my_begin - t0 - static_cast<int32_t>(4 * half);
       const int32_t hi = my_end - t0 - static_cast<int32_t>(4 * half);
-      const uint64_t gone = hole >> (4 * half);
+      const uint64_t seen = bits_below(hi) & ~bits_below(lo) & ~(hole >> (4 * half));
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+      for (int tt = 0; tt < 2; ++tt) {
+        const int32_t word = static_cast<int32_t>(seen >> (32 * tt));
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int32_t j = tt * 32 + 8 * (i / 4) + i % 4;
-          if (j < lo || j >= hi || (static_cast<uint32_t>(gone >> (32 * tt)) >> (j & 31) & 1u))
-            s[tt][i] = kNegInf;
+          const int b = 8 * (i / 4) + i % 4;
+          const uint32_t keep = static_cast<uint32_t>(word << (31 - b) >> 31);
+          const float x = s[tt][i];
+          s[tt][i] = __builtin_bit_cast(
+              float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
         }
+      }
     }
     float top = s[0][0];
 #pragma unroll
@@ -622,7 +652,9 @@ attend_many_kernel(AttendParams a) {
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      add_v(n + 1, u, p[u]);
+      if (u < 3) read_v(n + 1, u + 1, vf[(u + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      add_v(vf[u & 1], p[u]);
       float x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -646,16 +678,13 @@ attend_many_kernel(AttendParams a) {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) p[u][j] = Mat<VM>::pack(x[2 * j], x[2 * j + 1]);
-    }
-    // The weights before the branch, so that they are computed beside the products.
-    asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+      asm volatile("" : "+v"(p[u]), "+v"(sum));  // here, beside the products
 #pragma unroll
-    for (uint32_t i = 0; i < DP / 32 * 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // product
-      __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);  // exponentials
-      __builtin_amdgcn_sched_group_barrier(0x2, 6, 0);    // vector
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+      for (uint32_t i = 0; i < DP / 32; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
+        __builtin_amdgcn_sched_group_barrier(0x402, 8, 0);  // vector and exponentials
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     l = l * keep + sum;
     if (grown) {  // the outputs up to tile n - 1
@@ -695,6 +724,7 @@ attend_many_kernel(AttendParams a) {
       if (n) store_v(n - 1, v_masked, v_there);
       if ((n + 1) * tile_units % (kRing / 2) == 0) fill_ring(n + 1);
       __syncthreads();
+      read_k(n, 0, kf[0]);
       v_masked = masked;
       v_there = there;
       there = tokens_there(n + 1);
@@ -706,7 +736,10 @@ attend_many_kernel(AttendParams a) {
     store_v(n - 1, v_masked, v_there);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 4; ++u) add_v(n - 1, u, p[u]);
+    for (int u = 0; u < 4; ++u) {
+      read_v(n - 1, u, vf[u & 1]);
+      add_v(vf[u & 1], p[u]);
+    }
   }
 
   __syncthreads();
@@ -794,11 +827,24 @@ __global__ void __launch_bounds__(kManyThreads) attend_many_join_kernel(AttendPa
 // time, with no barrier: K goes from memory straight into the operand's registers
 // (lane: token lane % 16, 8 or 16 values), V through the wave's own part of LDS.  The
 // next 32 tokens are on their way meanwhile.  At the end the 4 waves join in LDS, and
-// the shares of a split sequence in attend_few_join_kernel.
+// the shares of a split sequence in the workgroup that finishes last.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kFewThreads = 256, kFewWaves = 4;
+constexpr uint32_t kFewWaves = 4, kFewThreads = kFewWaves * 64;
 constexpr uint32_t kFewTokens = 32;
 constexpr uint32_t few_v_pitch(uint32_t dp) { return 2 * dp + 32; }
+
+// Values d to d + 3 of an output row, o / l, and with the first the log-sum-exp.
+template <class Row>
+__device__ __forceinline__ void few_store(const AttendParams& a, const Seq& sq, uint32_t head,
+                                          uint32_t row, uint32_t d, f32x4 o, float m, float l) {
+  const float inv = l == 0 ? 0.0f : 1.0f / l;
+  const uint32_t token = row / a.group, g = row - token * a.group;
+  const uint64_t at = sq.first + static_cast<uint64_t>(token), qh = head * a.group + g;
+  store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
+                  f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv});
+  if (a.lse && d == 0)
+    a.lse[at * a.q_heads + qh] = l == 0 ? kNegInf : m * a.scale_log2 * kLn2 + logf(l);
+}
 
 template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
@@ -814,329 +860,414 @@ attend_few_kernel(AttendParams a) {
   constexpr uint32_t kSteps = kKLoads * (kCodes ? 2 : 1);  // products of 32 values
   struct WaveLds {
     __attribute__((aligned(16))) uint8_t v[kFewTokens * kVP];
+    // Of 32 tokens to load next: where they lie; of the tile at hand: its scales.
+    uint64_t at[kFewTokens];
+    __attribute__((aligned(16))) float k_scale[kFewTokens], v_scale[kFewTokens];
   };
   __shared__ WaveLds lds[kFewWaves];
   __shared__ float join_m[kFewWaves][16], join_l[kFewWaves][16];
+  __shared__ bool finished;
   const PagedView& pg = a.pages;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t head = blockIdx.x % pg.heads;
   const uint32_t rest = blockIdx.x / pg.heads;
   const uint32_t split = rest % a.few_splits, seq = rest / a.few_splits;
-  const Seq sq = seq_of(a, seq);
-  const uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
-  if (rows == 0) return;
-  // More rows than a tile has come here only when the batch was said to have none such:
-  // they go one tile after another, unsplit.
-  uint32_t splits = a.few_splits;
-  if (rows > 16) {
-    if (a.many_units) return;  // attend_many_kernel's
-    splits = 1;
-  }
-  if (split >= splits) return;
-  const int32_t pos0 = sq.len - sq.rows;
   const int32_t* table = a.block_table + seq * a.table_stride;
+  // Without a window a share starts at a token known from here on: a launch that is all
+  // latency asks for its first block beside the sequence's length (a token behind 10,000
+  // 18.8 -> 18.0 us; where shares wait for their turn it costs 2%).
+  const bool ask_early = !a.window && gridDim.x <= 512;
+  int32_t early_block = -1;
+  if (ask_early)
+    early_block = table[page_of(pg, min(split * a.few_piece + wave * kFewTokens + (lane & 31u),
+                                        a.table_width * pg.block_size - 1))];
+  const Seq sq = seq_of(a, seq);
+  uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
+  if (rows > kFewRows) {
+    if (a.many_units) return;  // attend_many_kernel's
+    rows = kFewRows;
+  }
+  if (rows > a.few_rows_most) rows = a.few_rows_most;  // more than the batch was said to have
+  if (rows == 0) return;
+  const int32_t pos0 = sq.len - sq.rows;
   uint8_t* v_lds = lds[wave].v;
 
-  for (uint32_t row0 = 0; row0 < rows; row0 += 16) {
-    const uint32_t row = row0 + col, last = min(row0 + 16, rows) - 1;
-    const bool valid = row < rows;
-    const int32_t pos = pos0 + static_cast<int32_t>(row / a.group);
-    const int32_t my_begin = row_begin(a, pos);
-    const int32_t my_end = valid ? row_end(a, sq.len, pos) : 0;
-    int32_t begin = row_begin(a, pos0 + static_cast<int32_t>(row0 / a.group)) &
-                    ~static_cast<int32_t>(kFewTokens - 1);
-    int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>(last / a.group));
-    const int32_t all_begin = row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
-    const int32_t all_end = row_end(a, sq.len, pos0 + static_cast<int32_t>(row0 / a.group));
-    const uint32_t used = split_range(begin, end, split, splits, a.few_piece);
-    if (split >= used) return;
-    const uint32_t token = row / a.group, g = row - token * a.group;
-    const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
-                                       static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
-                                          2;
-    u32x4 q[kSteps];
+  const uint32_t row = col, last = rows - 1;
+  const bool valid = row < rows;
+  const int32_t pos = pos0 + static_cast<int32_t>(row / a.group);
+  const int32_t my_begin = row_begin(a, pos);
+  const int32_t my_end = valid ? row_end(a, sq.len, pos) : 0;
+  int32_t begin = row_begin(a, pos0) &
+                  ~static_cast<int32_t>(kFewTokens - 1);
+  int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>(last / a.group));
+  const int32_t all_begin = row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
+  const int32_t all_end = row_end(a, sq.len, pos0);
+  const uint32_t used = split_range(begin, end, split, a.few_splits, a.few_piece);
+  if (split >= used) return;
+  const uint32_t token = row / a.group, g = row - token * a.group;
+  const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
+                                     static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
+                                        2;
+  u32x4 q[kSteps];
 #pragma unroll
-    for (uint32_t i = 0; i < kSteps; ++i)
-      q[i] = load_q8(q_row,
-                     kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
-                     valid);
-    f32x4 o[DP / 16];
+  for (uint32_t i = 0; i < kSteps; ++i)
+    q[i] = load_q8(q_row,
+                   kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
+                   valid);
+  f32x4 o[DP / 16];
 #pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
-    float m = kNegInf, l = 0.0f;
-    bool odd = false;  // some tile attended in part holds V that is not finite
+  for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
+  float m = kNegInf, l = 0.0f;
+  bool odd = false;  // some tile attended in part holds V that is not finite
 
-    u32x4 kr[2][kKLoads], vr[kVLoads];
-    float k_scale[2], v_scale[2];  // of token 16 tt + col
-    uint32_t there = 0;            // bit 16 tt + col: that token's block exists
-    int32_t block[2];              // of the tokens to load next
-    auto load_blocks = [&](int32_t t0) {
+  u32x4 kr[2][kKLoads], vr[kVLoads];
+  // Token t0 + lane of a tile, lanes 0 to 31: its block (of the tile to load next), its
+  // place and, once the tile is on its way, its scales.  A token past the end or
+  // without a block reads some other place: it is masked and its V zeroed.
+  int32_t block = -1;
+  float k_scale = 0.0f, v_scale = 0.0f;
+  uint32_t there = 0;  // bit j: token j of the tile has a block
+  auto load_block = [&](int32_t t0) {
+    const int32_t tok = t0 + static_cast<int32_t>(lane & 31u);
+    block = tok < end ? table[page_of(pg, tok)] : -1;
+  };
+  // d of this lane's part of K and V (some other value where there is none).
+  uint32_t k_at[kKLoads], v_at[kVLoads];
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(col);
-        block[tt] = tok < end ? table[page_of(pg, tok)] : -1;
+  for (uint32_t i = 0; i < kKLoads; ++i) {
+    const uint32_t d = (i * 4 + quarter) * kPer;
+    k_at[i] = (d < pg.dim ? d : 0) * (kCodes ? 1 : 2);
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kVLoads; ++i) {
+    const uint32_t d = (lane + i * 64) % kCols * kPer;
+    v_at[i] = (d < pg.dim ? d : 0) * (kCodes ? 1 : 2);
+  }
+  auto load = [&](int32_t t0) {
+    const int32_t tok = t0 + static_cast<int32_t>(lane & 31u);
+    uint64_t place, scale_place;
+    const bool in =
+        token_at(pg, block, tok, page_of(pg, tok), head, &place, &scale_place);
+    there = static_cast<uint32_t>(__ballot(in));
+    if (lane < 32) {
+      lds[wave].at[lane] = in ? place : 0;
+      if constexpr (kCodes) {
+        if (!in) scale_place = pg.scale_offset;
+        k_scale = *reinterpret_cast<const g_f32*>(pg.k + scale_place);
+        v_scale = *reinterpret_cast<const g_f32*>(pg.v + scale_place);
       }
-    };
-    auto load = [&](int32_t t0) {
-      there = 0;
+    }
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(col);
-        uint64_t at, scale_at;
-        const bool in = token_at(pg, block[tt], tok, page_of(pg, tok), head, &at, &scale_at);
+    for (int tt = 0; tt < 2; ++tt) {
+      const uint64_t at = pg.k + lds[wave].at[tt * 16 + col];
 #pragma unroll
-        for (uint32_t i = 0; i < kKLoads; ++i) {
-          const uint32_t d = (i * 4 + quarter) * kPer;
-          kr[tt][i] = u32x4{0, 0, 0, 0};
-          if (in && d < pg.dim)
-            kr[tt][i] = *reinterpret_cast<const g_u32x4*>(pg.k + at + d * (kCodes ? 1 : 2));
-        }
-        k_scale[tt] = v_scale[tt] = 0.0f;
-        if constexpr (kCodes) {
-          if (in) {
-            k_scale[tt] = *reinterpret_cast<const g_f32*>(pg.k + scale_at);
-            v_scale[tt] = *reinterpret_cast<const g_f32*>(pg.v + scale_at);
-          }
-        }
-        there |= (static_cast<uint32_t>(__ballot(in)) & 0xffffu) << (16 * tt);
-      }
+      for (uint32_t i = 0; i < kKLoads; ++i)
+        kr[tt][i] = *reinterpret_cast<const g_u32x4*>(at + k_at[i]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kVLoads; ++i)
+      vr[i] = *reinterpret_cast<const g_u32x4*>(
+          pg.v + lds[wave].at[(lane + i * 64) / kCols] + v_at[i]);
+  };
+
+  constexpr int32_t kStep = kFewTokens * kFewWaves;
+  auto tile = [&](int32_t t0) {
+    const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kFewTokens) > all_end;
+    const bool masked = partial || there != 0xffffffffu;
+    // V into LDS.
+    if (masked) {
 #pragma unroll
       for (uint32_t i = 0; i < kVLoads; ++i) {
-        const uint32_t c = lane + i * 64, j = c / kCols, d = c % kCols * kPer;
-        const int32_t tok = t0 + static_cast<int32_t>(j);
-        const int32_t b0 = __shfl(block[0], j & 15u), b1 = __shfl(block[1], j & 15u);
-        uint64_t at, scale_at;
-        vr[i] = u32x4{0, 0, 0, 0};
-        if (token_at(pg, j < 16 ? b0 : b1, tok, page_of(pg, tok), head, &at, &scale_at) &&
-            j < kFewTokens && d < pg.dim)
-          vr[i] = *reinterpret_cast<const g_u32x4*>(pg.v + at + d * (kCodes ? 1 : 2));
+        const uint32_t j = (lane + i * 64) / kCols;
+        if (!(there >> j & 1u)) vr[i] = u32x4{0, 0, 0, 0};
+        odd |= clear_odd<Row, TYPE>(vr[i]);
       }
-    };
-
-    int32_t t0 = begin + static_cast<int32_t>(wave * kFewTokens);
-    constexpr int32_t kStep = kFewTokens * kFewWaves;
-    load_blocks(t0);
-    if (t0 < end) load(t0);
-    load_blocks(t0 + kStep);
-    for (; t0 < end; t0 += kStep) {
-      const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kFewTokens) > all_end;
-      // V into LDS.
+    }
 #pragma unroll
-      for (uint32_t i = 0; i < kVLoads; ++i) {
-        const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
-        const bool mine = kFewTokens * kCols % 64 == 0 || j < kFewTokens;
-        if (partial) odd |= clear_odd<Row, TYPE>(vr[i]);
-        u32x4 v0 = vr[i], v1{0, 0, 0, 0};
+    for (uint32_t i = 0; i < kVLoads; ++i) {
+      const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
+      u32x4 v0 = vr[i], v1{0, 0, 0, 0};
+      if constexpr (kCodes) {
+        const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
+        const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
+        v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
+        v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
+      }
+      u32x4* vd = reinterpret_cast<u32x4*>(v_lds + j * kVP + cc * (kCodes ? 32 : 16));
+      vd[0] = v0;
+      if constexpr (kCodes) vd[1] = v1;
+    }
+    if constexpr (kCodes) {
+      if (lane < 32) {
+        lds[wave].k_scale[lane] = k_scale;
+        lds[wave].v_scale[lane] = v_scale;
+      }
+    }
+    if (pg.dim != DP) {  // values past the head's size
+#pragma unroll
+      for (uint32_t i = 0; i < kKLoads; ++i)
+        if ((i * 4 + quarter) * kPer >= pg.dim) kr[0][i] = kr[1][i] = u32x4{0, 0, 0, 0};
+    }
+    // S^T: this lane's row `col`, tokens 16 tt + 4 quarter + i.
+    f32x4 s[2];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      s[tt] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (uint32_t i = 0; i < kKLoads; ++i) {
         if constexpr (kCodes) {
-          const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
-          const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
-          v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
-          v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
-        }
-        if (mine) {
-          u32x4* vd = reinterpret_cast<u32x4*>(v_lds + j * kVP + cc * (kCodes ? 32 : 16));
-          vd[0] = v0;
-          if constexpr (kCodes) vd[1] = v1;
-        }
-      }
-      // S^T: this lane's row `col`, tokens 16 tt + 4 quarter + i.
-      f32x4 s[2];
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        s[tt] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (uint32_t i = 0; i < kKLoads; ++i) {
-          if constexpr (kCodes) {
-            const u32x2 a0 = codes_to_16<KM, TYPE>(kr[tt][i][0]);
-            const u32x2 a1 = codes_to_16<KM, TYPE>(kr[tt][i][1]);
-            const u32x2 a2 = codes_to_16<KM, TYPE>(kr[tt][i][2]);
-            const u32x2 a3 = codes_to_16<KM, TYPE>(kr[tt][i][3]);
-            s[tt] = Mat<KM>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
-            s[tt] = Mat<KM>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
-          } else {
-            s[tt] = Mat<KM>::mul16(kr[tt][i], q[i], s[tt]);
-          }
+          const u32x2 a0 = codes_to_16<KM, TYPE>(kr[tt][i][0]);
+          const u32x2 a1 = codes_to_16<KM, TYPE>(kr[tt][i][1]);
+          const u32x2 a2 = codes_to_16<KM, TYPE>(kr[tt][i][2]);
+          const u32x2 a3 = codes_to_16<KM, TYPE>(kr[tt][i][3]);
+          s[tt] = Mat<KM>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
+          s[tt] = Mat<KM>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
+        } else {
+          s[tt] = Mat<KM>::mul16(kr[tt][i], q[i], s[tt]);
         }
       }
-      float wv[2][4];
+    }
+    float wv[2][4];
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      f32x4 x{1, 1, 1, 1}, y{1, 1, 1, 1};
+      if constexpr (kCodes) {
+        x = *reinterpret_cast<const f32x4*>(lds[wave].k_scale + tt * 16 + quarter * 4);
+        y = *reinterpret_cast<const f32x4*>(lds[wave].v_scale + tt * 16 + quarter * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kCodes) s[tt][i] *= x[i];
+        wv[tt][i] = y[i];
+      }
+    }
+    const uint32_t seen_blocks = there;
+    if (t0 + kStep < end) {
+      load(t0 + kStep);
+      load_block(t0 + 2 * kStep);
+    }
+    if (masked) {
+      // Bit 16 tt + i: this lane's token 16 tt + 4 quarter + i is attended.
+      const int32_t at = t0 + static_cast<int32_t>(quarter) * 4;
+      const uint32_t seen =
+          static_cast<uint32_t>(bits_below(my_end - at) & ~bits_below(my_begin - at)) &
+          (seen_blocks >> (quarter * 4));
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (kCodes) {
-            s[tt][i] *= __shfl(k_scale[tt], quarter * 4 + i);
-            wv[tt][i] = __shfl(v_scale[tt], quarter * 4 + i);
-          } else {
-            wv[tt][i] = 1.0f;
-          }
+          const uint32_t keep =
+              static_cast<uint32_t>(static_cast<int32_t>(seen << (31 - tt * 16 - i)) >> 31);
+          const float x = s[tt][i], y = wv[tt][i];
+          s[tt][i] = __builtin_bit_cast(
+              float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
+          wv[tt][i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & keep);
         }
-      const bool masked = partial || there != 0xffffffffu;
-      if (masked) {
+    }
+    float top = kNegInf;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
+    for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int32_t tok = t0 + tt * 16 + static_cast<int32_t>(quarter) * 4 + i;
-            if (tok < my_begin || tok >= my_end || !(there >> (tt * 16 + quarter * 4 + i) & 1u)) {
-              s[tt][i] = kNegInf;
-              wv[tt][i] = 0.0f;
-            }
-          }
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = max32(top);
+    if (__any((top - m) * a.scale_log2 > 8.0f)) {
+      const float m_new = fmaxf(m, top);
+      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+      m = m_new;
+      l *= keep;
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
+    }
+    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
+        l += w;
+        wv[tt][i] *= w;
       }
-      if (t0 + kStep < end) {
-        load(t0 + kStep);
-        load_blocks(t0 + 2 * kStep);
-      }
-      float top = kNegInf;
+    const u32x4 w{Mat<VM>::pack(wv[0][0], wv[0][1]), Mat<VM>::pack(wv[0][2], wv[0][3]),
+                  Mat<VM>::pack(wv[1][0], wv[1][1]), Mat<VM>::pack(wv[1][2], wv[1][3])};
+    // Every lane of the wave has stored its part of V before any reads another's.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const uint8_t* v_from = v_lds + (quarter * 4 + col / 4) * kVP + (col & 3u) * 8;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = max32(top);
-      if (__any((top - m) * a.scale_log2 > 8.0f)) {
-        const float m_new = fmaxf(m, top);
-        const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
-        m = m_new;
-        l *= keep;
-#pragma unroll
-        for (uint32_t dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
-      }
-      const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
-          l += w;
-          wv[tt][i] *= w;
-        }
-      const u32x4 w{Mat<VM>::pack(wv[0][0], wv[0][1]), Mat<VM>::pack(wv[0][2], wv[0][3]),
-                    Mat<VM>::pack(wv[1][0], wv[1][1]), Mat<VM>::pack(wv[1][2], wv[1][3])};
-      // Every lane of the wave has stored its part of V before any reads another's.
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const uint8_t* v_at = v_lds + (quarter * 4 + col / 4) * kVP + (col & 3u) * 8;
+    for (uint32_t dt = 0; dt < DP / 16; ++dt) {
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_from + dt * 32));
+      const s16x4 hi =
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_from + 16 * kVP + dt * 32));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      o[dt] = Mat<VM>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  int32_t t0 = begin + static_cast<int32_t>(wave * kFewTokens);
+  if (t0 < end) {
+    if (ask_early)
+      block = t0 + static_cast<int32_t>(lane & 31u) < end ? early_block : -1;
+    else
+      load_block(t0);
+    load(t0);
+    load_block(t0 + kStep);
+  }
+  for (; t0 < end; t0 += kStep) tile(t0);
+  if (__any(odd))
+    for (int32_t tok = begin; tok < end; ++tok) {
+      if ((static_cast<uint32_t>(tok - begin) / kFewTokens) % kFewWaves != wave) continue;
+      if (tok < my_begin || tok >= my_end) continue;
+      const int32_t t1 = tok & ~static_cast<int32_t>(kFewTokens - 1);
+      if (t1 >= all_begin && t1 + static_cast<int32_t>(kFewTokens) <= all_end) continue;
+      uint64_t at, scale_at;
+      const uint32_t page = page_of(pg, tok);
+      if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
 #pragma unroll
       for (uint32_t dt = 0; dt < DP / 16; ++dt) {
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_at + dt * 32));
-        const s16x4 hi =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_at + 16 * kVP + dt * 32));
-        const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-        o[dt] = Mat<VM>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+        float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
+        add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
+        o[dt] = f32x4{x[0], x[1], x[2], x[3]};
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    if (__any(odd))
-      for (int32_t tok = begin; tok < end; ++tok) {
-        if ((static_cast<uint32_t>(tok - begin) / kFewTokens) % kFewWaves != wave) continue;
-        if (tok < my_begin || tok >= my_end) continue;
-        const int32_t t1 = tok & ~static_cast<int32_t>(kFewTokens - 1);
-        if (t1 >= all_begin && t1 + static_cast<int32_t>(kFewTokens) <= all_end) continue;
-        uint64_t at, scale_at;
-        const uint32_t page = page_of(pg, tok);
-        if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
-#pragma unroll
-        for (uint32_t dt = 0; dt < DP / 16; ++dt) {
-          float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
-          add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
-          o[dt] = f32x4{x[0], x[1], x[2], x[3]};
-        }
-      }
 
-    // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
-    // LDS (which V no longer needs), and the threads share the sums.
-    l += __shfl_xor(l, 16);
-    l = sum32(l);
-    float* mine = reinterpret_cast<float*>(lds[wave].v);
-    static_assert(sizeof(WaveLds) >= 16 * DP * sizeof(float), "a wave's outputs fit its LDS");
+  // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
+  // LDS (which V no longer needs), and the threads share the sums.
+  l += __shfl_xor(l, 16);
+  l = sum32(l);
+  float* mine = reinterpret_cast<float*>(lds[wave].v);
+  static_assert(sizeof(WaveLds) >= 16 * DP * sizeof(float), "a wave's outputs fit its LDS");
 #pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt)
-      *reinterpret_cast<f32x4*>(mine + col * DP + dt * 16 + quarter * 4) = o[dt];
-    if (quarter == 0) {
-      join_m[wave][col] = m;
-      join_l[wave][col] = l;
-    }
-    __syncthreads();
-    const uint64_t slot = (static_cast<uint64_t>(seq) * a.few_splits + split) * pg.heads + head;
-    for (uint32_t i = tid; i < 16 * DP / 4; i += kFewThreads) {
-      const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
-      if (row0 + r >= rows) continue;
-      float top = kNegInf;
-#pragma unroll
-      for (uint32_t w = 0; w < kFewWaves; ++w) top = fmaxf(top, join_m[w][r]);
-      float sum = 0.0f;
-      f32x4 x{0, 0, 0, 0};
-#pragma unroll
-      for (uint32_t w = 0; w < kFewWaves; ++w) {
-        const float mw = join_m[w][r], lw = join_l[w][r];
-        const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
-                                         : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
-        sum += lw * keep;
-        const f32x4 y =
-            *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
-      }
-      if (used > 1) {
-        *reinterpret_cast<f32x4*>(a.few_o + (slot * 16 + r) * DP + d) = x;
-        if (d == 0) reinterpret_cast<f32x2*>(a.few_ml)[slot * 16 + r] = f32x2{top, sum};
-      } else {
-        const float inv = sum == 0 ? 0.0f : 1.0f / sum;
-        const uint32_t rt = (row0 + r) / a.group, rg = row0 + r - rt * a.group;
-        const uint64_t at = sq.first + static_cast<uint64_t>(rt), qh = head * a.group + rg;
-        store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
-                        f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
-        if (a.lse && d == 0)
-          a.lse[at * a.q_heads + qh] =
-              sum == 0 ? kNegInf : top * a.scale_log2 * kLn2 + logf(sum);
-      }
-    }
-    __syncthreads();  // before the next tile of rows uses the LDS
+  for (uint32_t dt = 0; dt < DP / 16; ++dt)
+    *reinterpret_cast<f32x4*>(mine + col * DP + dt * 16 + quarter * 4) = o[dt];
+  if (quarter == 0) {
+    join_m[wave][col] = m;
+    join_l[wave][col] = l;
   }
-}
-
-// Joins the shares of split sequences: a workgroup a sequence and head, 4 values a thread.
-template <class Row, uint32_t DP>
-__global__ void __launch_bounds__(kFewThreads) attend_few_join_kernel(AttendParams a) {
-  const PagedView& pg = a.pages;
-  const uint32_t head = blockIdx.x % pg.heads, seq = blockIdx.x / pg.heads;
-  const Seq sq = seq_of(a, seq);
-  const uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
-  if (rows == 0 || rows > 16) return;
-  const int32_t pos0 = sq.len - sq.rows;
-  int32_t begin = row_begin(a, pos0) & ~static_cast<int32_t>(kFewTokens - 1);
-  int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>((rows - 1) / a.group));
-  const uint32_t used = split_range(begin, end, 0, a.few_splits, a.few_piece);
-  if (used == 1) return;
-  for (uint32_t i = threadIdx.x; i < rows * (DP / 4); i += kFewThreads) {
+  __syncthreads();
+  const uint64_t slot = (static_cast<uint64_t>(seq) * a.few_splits + split) * pg.heads + head;
+  const __amdgpu_buffer_rsrc_t share = __builtin_amdgcn_make_buffer_rsrc(
+      a.few_o + (used > 1 ? slot * a.few_rows_most * DP : 0), 0,
+      static_cast<int>(a.few_rows_most * DP * 4), 0x00027000);
+  for (uint32_t i = tid; i < 16 * DP / 4; i += kFewThreads) {
     const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
-    auto slot = [&](uint32_t s) {
-      return ((static_cast<uint64_t>(seq) * a.few_splits + s) * pg.heads + head) * 16 + r;
-    };
-    const f32x2* ml = reinterpret_cast<const f32x2*>(a.few_ml);
+    if (r >= rows) continue;
     float top = kNegInf;
-    for (uint32_t s = 0; s < used; ++s) top = fmaxf(top, ml[slot(s)][0]);
+#pragma unroll
+    for (uint32_t w = 0; w < kFewWaves; ++w) top = fmaxf(top, join_m[w][r]);
     float sum = 0.0f;
     f32x4 x{0, 0, 0, 0};
-    for (uint32_t s = 0; s < used; ++s) {
-      const f32x2 y = ml[slot(s)];
-      const float keep = y[0] == kNegInf ? (y[1] == 0.0f ? 0.0f : 1.0f)
-                                         : __builtin_amdgcn_exp2f((y[0] - top) * a.scale_log2);
-      sum += y[1] * keep;
-      const f32x4 z = *reinterpret_cast<const f32x4*>(a.few_o + slot(s) * DP + d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += z[j] * keep;
+    for (uint32_t w = 0; w < kFewWaves; ++w) {
+      const float mw = join_m[w][r], lw = join_l[w][r];
+      const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
+                                       : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
+      sum += lw * keep;
+      const f32x4 y =
+          *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
     }
-    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
-    const uint32_t rt = r / a.group, rg = r - rt * a.group;
-    const uint64_t at = sq.first + static_cast<uint64_t>(rt), qh = head * a.group + rg;
-    store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
-                    f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
-    if (a.lse && d == 0)
-      a.lse[at * a.q_heads + qh] = sum == 0 ? kNegInf : top * a.scale_log2 * kLn2 + logf(sum);
+    if (used > 1) {
+      // Written through the XCD's L2 (the sc1 policy of agent-scope stores, which the
+      // language offers for at most 8 bytes at a time).
+      constexpr int kSc1 = 16;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), share,
+                                             static_cast<int>((r * DP + d) * 4), 0, kSc1);
+      if (d == 0)
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.few_ml) + slot * a.few_rows_most + r,
+                           __builtin_bit_cast(uint64_t, f32x2{top, sum}), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      few_store<Row>(a, sq, head, r, d, x, top, sum);
+    }
+  }
+  if (used == 1) return;
+  // The split that finishes last joins them all, in order.  Shares go through the XCD's
+  // L2 to where every XCD sees them; a workgroup counts itself once its stores have been
+  // acknowledged, and the last one puts the count back to 0 for the next call.
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  uint32_t* count = a.few_count + (static_cast<uint64_t>(seq) * pg.heads + head) * kCountStride;
+  if (tid == 0) {
+    const uint32_t before =
+        __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before + 1 == used)
+      __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    finished = before + 1 == used;
+  }
+  __syncthreads();
+  if (!finished) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  const uint64_t slot0 = static_cast<uint64_t>(seq) * a.few_splits * pg.heads + head;
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.few_ml);
+  // Each share's factor exp(m - largest m), of every row, and the rows' sums.
+  static_assert(sizeof(lds) >= kFewMaxSplits * 64 + kFewThreads * 16, "factors and sums fit");
+  float* factor = reinterpret_cast<float*>(lds);  // [used][16]
+  for (uint32_t r = wave; r < rows; r += kFewWaves) {
+    float m_s = kNegInf, l_s = 0.0f;
+    float largest = kNegInf;
+    for (uint32_t s = lane; s < used; s += 64)
+      largest = fmaxf(largest, ml[(slot0 + s * pg.heads) * a.few_rows_most + r][0]);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) largest = fmaxf(largest, __shfl_xor(largest, step));
+    float sum = 0.0f;
+    for (uint32_t s = lane; s < used; s += 64) {
+      const f32x2 y = ml[(slot0 + s * pg.heads) * a.few_rows_most + r];
+      m_s = y[0];
+      l_s = y[1];
+      // A share without a maximum attended nothing, or only what is no number.
+      const float f = m_s == kNegInf ? (l_s == 0.0f ? 0.0f : 1.0f)
+                                     : __builtin_amdgcn_exp2f((m_s - largest) * a.scale_log2);
+      factor[s * 16 + r] = f;
+      sum += l_s * f;
+    }
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) sum += __shfl_xor(sum, step);
+    if (lane == 0) {
+      join_m[0][r] = largest;
+      join_l[0][r] = sum;
+    }
+  }
+  __syncthreads();
+  // 4 values an item; where there are fewer items than threads, groups of threads share
+  // the splits out and add up in LDS.
+  const uint32_t items = rows * (DP / 4);
+  uint32_t groups = 1;
+  while (groups * 2 * items <= kFewThreads) groups *= 2;
+  const uint32_t group = tid / items;
+  f32x4* sums = reinterpret_cast<f32x4*>(factor + used * 16);
+  for (uint32_t i0 = 0; i0 < items; i0 += kFewThreads) {
+    const uint32_t i = groups > 1 ? tid - group * items : i0 + tid;
+    const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
+    const bool mine = groups > 1 ? group < groups : i < items;
+    f32x4 x{0, 0, 0, 0};
+    if (mine) {
+      const float* part = a.few_o + (slot0 * a.few_rows_most + r) * DP + d;
+      const uint64_t stride = static_cast<uint64_t>(pg.heads) * a.few_rows_most * DP;
+      const uint32_t first = groups > 1 ? group : 0;
+#pragma unroll 8
+      for (uint32_t s = first; s < used; s += groups) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(part + s * stride);
+        const float f = factor[s * 16 + r];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += y[j] * f;
+      }
+    }
+    if (groups > 1) {
+      if (mine) sums[tid] = x;
+      __syncthreads();
+      if (group == 0)
+        for (uint32_t g = 1; g < groups; ++g) {
+          const f32x4 y = sums[g * items + i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] += y[j];
+        }
+    }
+    if (mine && group * (groups > 1) == 0)
+      few_store<Row>(a, sq, head, r, d, x, join_m[0][r], join_l[0][r]);
   }
 }
 
@@ -1146,9 +1277,6 @@ hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
     const uint32_t units = p.num_seqs * p.pages.heads;
     hipLaunchKernelGGL((attend_few_kernel<Row, TYPE, DP>), dim3(units * p.few_splits),
                        dim3(kFewThreads), 0, stream, p);
-    if (p.few_splits > 1)
-      hipLaunchKernelGGL((attend_few_join_kernel<Row, DP>), dim3(units), dim3(kFewThreads), 0,
-                         stream, p);
   }
   if (p.many_units) {
     const uint32_t units = p.many_units * p.pages.heads;

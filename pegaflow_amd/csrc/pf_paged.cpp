@@ -324,10 +324,15 @@ int pf_attend_workspace_create(int device, uint64_t bytes, pf_attend_workspace**
     const bool had = hipGetDevice(&prev) == hipSuccess;
     const int rc = pf_init(device);
     void* p = nullptr;
-    const hipError_t e = rc == PF_OK ? hipMalloc(&p, bytes) : hipSuccess;
+    hipError_t e = rc == PF_OK ? hipMalloc(&p, bytes) : hipSuccess;
+    if (p) {  // its counts start at 0
+      e = hipMemset(p, 0, pf::workspace_counts(bytes) * pf::kCountStride * 4);
+      if (e == hipSuccess) e = hipDeviceSynchronize();
+    }
+    if (e != hipSuccess && p) (void)hipFree(p);
     if (had && prev != device) (void)hipSetDevice(prev);
     if (rc != PF_OK) return rc;
-    if (e != hipSuccess) return pf::hip_fail(e, "hipMalloc(workspace)");
+    if (e != hipSuccess) return pf::hip_fail(e, "pf_attend_workspace_create");
     *out = new pf_attend_workspace{device, reinterpret_cast<uint64_t>(p), bytes};
     return PF_OK;
   });

@@ -55,20 +55,53 @@ struct AttendParams {
   uint32_t aligned;   // q and out move by 16 bytes
   uint32_t unit_shift;  // 2^unit_shift aligned tokens, at most 16, share a block
   // The launch (plan_attend): sequences of up to few_rows rows of a KV head go to the
-  // kernel for few, in few_splits shares of few_piece tokens (0: none do), the others
-  // in many_units tiles of rows and many_splits shares.
-  uint32_t few_rows, few_splits, few_piece;
+  // kernel for few, in few_splits shares of few_piece tokens (0: none do) of at most
+  // few_rows_most rows, the others in many_units tiles of rows and many_splits shares.
+  uint32_t few_rows, few_splits, few_piece, few_rows_most;
   uint32_t many_units, many_splits, many_piece;
   float *few_o, *few_ml, *many_o, *many_ml;  // shares, in the workspace
+  uint32_t* few_count;  // finished shares of each sequence and head, 0 between calls
 };
 
 constexpr uint32_t kFewRows = 16;        // of attend_few_kernel's tile
 constexpr uint32_t kManyRows = 128;      // of attend_many_kernel's
+constexpr uint32_t kFewMaxSplits = 192;
+// A count of finished shares has a 128-byte line of its own: adds to one line run one
+// after another.  The first kCounts of them (or a sixteenth of a small workspace) are at
+// the workspace's start.
+constexpr uint32_t kCountStride = 32;
+constexpr uint64_t kCounts = 8192;
+inline uint64_t workspace_counts(uint64_t bytes) {
+  const uint64_t n = bytes / 16 / (kCountStride * 4);
+  return n < kCounts ? n : kCounts;
+}
 constexpr uint32_t kAttendSlack = 1u << 16;  // tokens that a kernel's counting may run past the end
 
 // Head sizes that the kernels are built for.
 inline uint32_t padded_dim(uint32_t dim) {
   return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256;
+}
+
+// Tokens of a share of attend_few_kernel: `units` sequences and heads, the longest of
+// `longest` tokens.  (Measured with 128 values a head, 4 rows, in us.)
+//
+// The chip holds 512 of its workgroups at once, and a launch of a few more than that
+// takes twice as long: 384 units of up to 1,000 tokens whole 15.9, in two shares 24.4; 512
+// of 2,000 whole 55.6, in two 70.5; 128 of 4,000 in 2, 4 and 8 shares 56.0, 57.3 and 64.7.
+// Many launches' worth of shares, though, even out lengths that the host does not
+// know: 512 of up to 16,000 tokens, on average half, in shares of 1,024 tokens 216, of
+// 8,192 278.  Where units are few, a share of s tokens takes about 7.5 ns a token and
+// the join 280 ns a share, so shares of sqrt(37 * longest) are best: one sequence of
+// 10,000 tokens and 8 heads in shares of 256, 512, 1,024 and 2,048 takes 21.3, 17.6, 19.9
+// and 27.6; of 30,000 (8-bit) 37.5, 27.2, 22.3 and 26.2; of 3,000 13.3, 14.8, 18.5 and 22.4.
+inline uint64_t few_piece(uint64_t units, uint64_t longest) {
+  constexpr uint64_t kSlots = 512, kEven = 1024;
+  if (units * longest >= 4 * kSlots * kEven) return kEven;
+  const uint64_t most = units < kSlots ? kSlots / units : 1;
+  const uint64_t whole = (longest + most - 1) / most;
+  uint64_t piece = 128;
+  while (piece * piece < 37 * longest) piece += 128;
+  return piece > whole ? piece : whole;
 }
 
 // Shapes the launch of a batch whose longest query has `most_new` rows and longest
@@ -87,24 +120,25 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
   const bool any_few = all_few || (p->num_seqs > 1 && group <= kFewRows);
   p->few_rows = any_few && !all_few ? kFewRows : 0;
   p->few_splits = p->few_piece = p->many_units = p->many_splits = p->many_piece = 0;
-  uint64_t at = ws;
+  const uint64_t counts = workspace_counts(bytes);
+  uint64_t at = ws + counts * kCountStride * 4;
   const uint64_t end = ws + bytes;
+  p->few_count = reinterpret_cast<uint32_t*>(ws);
   if (any_few) {
     const uint64_t units = p->num_seqs * heads;
-    const uint64_t slot = kFewRows * (dim * 4 + 8);
-    const uint64_t want = ceil_div(kCus * 4, units);
-    uint64_t piece = ceil_div(ceil_div(longest, want), 128) * 128;
-    if (piece < 256) piece = 256;
+    p->few_rows_most = static_cast<uint32_t>(all_few ? most_new * group : kFewRows);
+    const uint64_t slot = p->few_rows_most * (dim * 4 + 8);
+    uint64_t piece = few_piece(units, longest);
     uint64_t splits = ceil_div(longest, piece);
-    if (splits * units * slot > end - at) {
-      splits = (end - at) / (units * slot);
-      if (splits < 2) splits = 1;
-      piece = ceil_div(ceil_div(longest, splits), 128) * 128;
-    }
+    if (splits > kFewMaxSplits) splits = kFewMaxSplits;
+    if (units > counts) splits = 1;
+    if (splits * units * slot > end - at) splits = (end - at) / (units * slot);
+    if (splits < 2) splits = 1;
+    piece = ceil_div(ceil_div(longest, splits), 128) * 128;
     p->few_splits = static_cast<uint32_t>(splits);
     p->few_piece = static_cast<uint32_t>(piece);
     if (splits > 1) {
-      const uint64_t n = units * splits * kFewRows;
+      const uint64_t n = units * splits * p->few_rows_most;
       p->few_o = reinterpret_cast<float*>(at);
       p->few_ml = reinterpret_cast<float*>(at + n * dim * 4);
       at += n * (dim * 4 + 8);

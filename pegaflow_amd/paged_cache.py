@@ -168,8 +168,9 @@ class PagedKVCache:
         ``seq_lens[b]`` tokens in all (int32), the new ones last and written already,
         in the blocks ``block_table[b]`` (int32).  ``window``: a row sees only so many
         tokens, itself included.  ``scale`` defaults to head_dim ** -0.5.  ``lse``, if
-        given, is an fp32 [rows, heads] tensor.  ``max_seq_len`` and ``max_query_len``
-        shape the launch; what they leave out is attended all the same.  Without a
+        given, is an fp32 [rows, heads] tensor.  ``max_seq_len``, the longest sequence, is
+        a hint that shapes the launch; ``max_query_len`` says that no sequence has more
+        rows, and those that one has beyond it may stay as they were.  Without a
         ``workspace`` no sequence is split, which is slow where few rows attend
         long sequences."""
         qr, n, heads = _rows(q, None, self.head_dim, "q")

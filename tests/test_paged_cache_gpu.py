@@ -316,9 +316,9 @@ def test_long_sequences_are_split_and_joined(gpu, workspace, form, group, new, c
     b.check(*b.run(workspace=small))
     small.close()
     b.check(*b.run(workspace=None))
-    # Hints that say too little, or far too much, change the launch and nothing else.
-    b.check(*b.run(workspace=workspace, max_seq_len=1, max_query_len=1))
+    # Bounds far too high, and a length hint that says too little, change the launch alone.
     b.check(*b.run(workspace=workspace, max_seq_len=1 << 20, max_query_len=1 << 20))
+    b.check(*b.run(workspace=workspace, max_seq_len=1))
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 1 << 31])
@@ -405,12 +405,29 @@ def test_lengths_beyond_the_table_are_cut(gpu, workspace):
 def test_query_starts_are_bounded(gpu, workspace):
     """Starts outside the rows, or out of order, read and write no row outside the call's."""
     b = Batch([5, 6, 7], [20, 30, 40], LLAMA, 4, seed=13)
+    n = len(b.q)
     for starts in ([-9, 5, 11, 4000], [2 ** 31 - 1, -2 ** 31, 0, 18], [18, 11, 5, 0]):
-        b.starts = np.array(starts, np.int32)
-        try:
-            b.run(workspace=workspace)
-        except AssertionError:
-            pass  # rows of no sequence keep what they held; only the bounds count here
+        # The values between the rows of a wider buffer, and 40 rows behind them.
+        q = device_rows(b.q, "fused")[0]
+        out, flat, view = device_rows(np.full((n + 40,) + b.q.shape[1:], 0x5a5a, np.uint16), "fused")
+        rows = DeviceArray(b.q.shape, "bf16", out.buffer, out._offset, out.stride())
+        b.dev.cache.attend(q, rows, device_array(b.table, "int32"), device_array(b.lens, "int32"),
+                           device_array(np.array(starts, np.int32), "int32"), workspace=workspace)
+        synchronize()
+        back = out.buffer.download().view(np.uint16)
+        got = np.lib.stride_tricks.as_strided(back, view.shape, view.strides)
+        view[:n] = got[:n]
+        assert np.array_equal(back, flat)
+
+
+def test_rows_beyond_the_longest_query(gpu, workspace):
+    """max_query_len bounds a sequence's rows: those beyond stay, or are attended."""
+    b = Batch([9, 1, 3], [700, 20, 30], LLAMA, 4, seed=23)
+    got, _ = b.run(workspace=workspace, max_query_len=1)
+    want, _ = b.run(workspace=workspace)
+    kept = (got == 0x5a5a).all((1, 2))
+    assert kept.sum() and not kept[[0, 9, 10]].any()
+    b.check(np.where(kept[:, None, None], want, got), None)
 
 
 @pytest.mark.parametrize("first_block", [0, 1])
