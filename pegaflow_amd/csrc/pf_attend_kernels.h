@@ -299,31 +299,41 @@ struct ManyLds {
   uint32_t odd;  // some tile attended in part holds V that is not finite
 };
 
-// The rows tile `index` of the batch (tiles of all sequences in order, of sequences
-// with more than `least` rows): its sequence and tile in it, false if there is none.
+// The rows tile `index` of the batch, of the sequences with more than `least` rows: its
+// sequence and tile in it, false if there is none.  Workgroups start in the order of their
+// index, so tiles that attend much come first: up to 64 sequences go by their length, and
+// a sequence's tiles from the last.  (Nine sequences of up to 700 new and 4,100 cached
+// tokens, in the order of the batch 347 us.)
 __device__ __forceinline__ bool find_tile(const AttendParams& a, uint32_t index, uint32_t tile_rows,
                                           uint32_t least, uint32_t* seq, uint32_t* tile) {
   const uint32_t lane = threadIdx.x & 63u;
   for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
     uint32_t tiles = 0;
+    int32_t len = -1;
     if (b0 + lane < a.num_seqs) {
-      const uint32_t rows = static_cast<uint32_t>(seq_of(a, b0 + lane).rows) * a.group;
+      const Seq s = seq_of(a, b0 + lane);
+      const uint32_t rows = static_cast<uint32_t>(s.rows) * a.group;
       if (rows > least) tiles = (rows + tile_rows - 1) / tile_rows;
+      len = s.len;
     }
-    uint32_t sum = tiles;  // of lanes 0 .. lane
-#pragma unroll
-    for (uint32_t step = 1; step < 64; step *= 2) {
-      const uint32_t x = __shfl_up(sum, step);
-      if (lane >= step) sum += x;
+    // Tiles before this lane's sequence, of the 64 at hand.
+    uint32_t before = 0;
+    const uint32_t count = min(a.num_seqs - b0, 64u);
+    for (uint32_t j = 0; j < count; ++j) {
+      const int32_t other = __builtin_amdgcn_readlane(len, j);
+      const uint32_t n = __builtin_amdgcn_readlane(tiles, j);
+      if (other > len || (other == len && j < lane)) before += n;
     }
-    const uint64_t past = __ballot(sum > index);
-    if (past) {
-      const int at = __builtin_ctzll(past);
+    const uint64_t here = __ballot(index >= before && index < before + tiles);
+    if (here) {
+      const int at = __builtin_ctzll(here);
       *seq = b0 + at;
-      *tile = index - __shfl(sum - tiles, at);
+      *tile = __builtin_amdgcn_readlane(before + tiles, at) - 1 - index;
       return true;
     }
-    index -= __shfl(sum, 63);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) tiles += __shfl_xor(static_cast<int>(tiles), step);
+    index -= tiles;
   }
   return false;
 }
@@ -337,7 +347,7 @@ struct ManyTile {
   bool valid;
 };
 __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, uint32_t head,
-                                          ManyTile* t) {
+                                          uint32_t wave, ManyTile* t) {
   uint32_t tile = 0;
   if (!find_tile(a, unit, kTileRows, a.few_rows, &t->seq, &tile)) return false;
   t->seq = __builtin_amdgcn_readfirstlane(t->seq);
@@ -350,7 +360,7 @@ __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, 
   t->begin = row_begin(a, t->pos0 + static_cast<int32_t>(row0 / a.group)) &
              ~static_cast<int32_t>(kTileTokens - 1);
   t->end = row_end(a, t->s.len, t->pos0 + static_cast<int32_t>(last / a.group));
-  t->row = row0 + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+  t->row = row0 + wave * 32 + (threadIdx.x & 31);
   t->valid = t->row < t->rows;
   return true;
 }
@@ -408,10 +418,9 @@ attend_many_kernel(AttendParams a) {
   const uint32_t head = blockIdx.x % pg.heads;
   const uint32_t rest = blockIdx.x / pg.heads;
   const uint32_t split = rest % a.many_splits;
-  // Later tiles of a sequence attend more tokens: they start first.
-  const uint32_t unit = a.many_units - 1 - rest / a.many_splits;
+  const uint32_t unit = rest / a.many_splits;
   ManyTile t;
-  if (!many_tile(a, unit, head, &t)) return;
+  if (!many_tile(a, unit, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, split, a.many_splits, a.many_piece);
   if (split >= used) return;
@@ -611,7 +620,7 @@ attend_many_kernel(AttendParams a) {
   auto step = [&](int32_t t0, uint32_t n, bool masked, uint64_t hole) {
     __builtin_amdgcn_s_setprio(1);  // ahead of the other workgroup's softmax
     scores(n);
-    __builtin_amdgcn_s_setprio(0);
+    //prio0
     read_v(n + 1, 0, vf[0]);  // the buffer of tile n - 1
     if (masked) {
       // Bit j of `seen`: this half's token j, of 64, is attended; its scores are tokens
@@ -686,6 +695,7 @@ attend_many_kernel(AttendParams a) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     l = l * keep + sum;
     if (grown) {  // the outputs up to tile n - 1
 #pragma unroll
@@ -779,14 +789,15 @@ attend_many_kernel(AttendParams a) {
   reinterpret_cast<f32x2*>(a.many_ml)[(slot * 4 + wave) * 64 + lane] = f32x2{m, l};
 }
 
-// Joins the shares of split tiles: the same lanes hold the same rows and values.
+// Joins the shares of split tiles, a workgroup each wave's rows: the same lanes hold the
+// same rows and values.
 template <class Row, uint32_t DP>
-__global__ void __launch_bounds__(kManyThreads) attend_many_join_kernel(AttendParams a) {
+__global__ void __launch_bounds__(64) attend_many_join_kernel(AttendParams a) {
   const PagedView& pg = a.pages;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t head = blockIdx.x % pg.heads, unit = blockIdx.x / pg.heads;
+  const uint32_t lane = threadIdx.x, wave = blockIdx.x & 3u;
+  const uint32_t head = (blockIdx.x >> 2) % pg.heads, unit = (blockIdx.x >> 2) / pg.heads;
   ManyTile t;
-  if (!many_tile(a, unit, head, &t)) return;
+  if (!many_tile(a, unit, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, 0, a.many_splits, a.many_piece);
   if (used == 1) return;
@@ -795,6 +806,7 @@ __global__ void __launch_bounds__(kManyThreads) attend_many_join_kernel(AttendPa
   };
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.many_ml);
   float m = kNegInf;
+#pragma unroll 4
   for (uint32_t s = 0; s < used; ++s) m = fmaxf(m, ml[slot(s) * 64 + lane][0]);
   f32x16 o[DP / 32];
 #pragma unroll
@@ -802,21 +814,30 @@ __global__ void __launch_bounds__(kManyThreads) attend_many_join_kernel(AttendPa
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
   float l = 0.0f;
-  for (uint32_t s = 0; s < used; ++s) {
+  // The loads of a share are under way while the share before is added.
+  f32x4 y[2][DP / 8];
+  auto load = [&](uint32_t s, f32x4 (&to)[DP / 8]) {
+    const f32x4* part = reinterpret_cast<const f32x4*>(a.many_o) + slot(s) * (DP / 8) * 64 + lane;
+#pragma unroll
+    for (uint32_t i = 0; i < DP / 8; ++i) to[i] = part[i * 64];
+  };
+  auto add = [&](uint32_t s, const f32x4 (&from)[DP / 8]) {
     const f32x2 x = ml[slot(s) * 64 + lane];
     // A share without a maximum attended nothing, or only what is no number (l is NaN).
     const float keep = x[0] == kNegInf ? (x[1] == 0.0f ? 0.0f : 1.0f)
                                        : __builtin_amdgcn_exp2f((x[0] - m) * a.scale_log2);
     l += x[1] * keep;
-    const f32x4* part = reinterpret_cast<const f32x4*>(a.many_o) + slot(s) * (DP / 8) * 64 + lane;
 #pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt)
+    for (uint32_t i = 0; i < DP / 8; ++i)
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const f32x4 y = part[(dt * 4 + i) * 64];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[dt][4 * i + j] += y[j] * keep;
-      }
+      for (int j = 0; j < 4; ++j) o[i / 4][4 * (i % 4) + j] += from[i][j] * keep;
+  };
+  load(0, y[0]);
+  for (uint32_t s = 0; s < used; s += 2) {
+    if (s + 1 < used) load(s + 1, y[1]);
+    add(s, y[0]);
+    if (s + 2 < used) load(s + 2, y[0]);
+    if (s + 1 < used) add(s + 1, y[1]);
   }
   many_store<Row, DP>(a, t, o, m, l);
 }
@@ -1283,7 +1304,7 @@ hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
     hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP>), dim3(units * p.many_splits),
                        dim3(kManyThreads), 0, stream, p);
     if (p.many_splits > 1)
-      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(units), dim3(kManyThreads), 0,
+      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(units * 4), dim3(64), 0,
                          stream, p);
   }
   return hipGetLastError();
