@@ -615,9 +615,9 @@ typedef struct pf_kv_rows {
  * padding and written nowhere.  The slots of one call are distinct: of rows
  * given the same slot, parts of each may stay.
  *
- * 8-bit pages: scale = max|x| / 448 (E4M3) or / 127 (INT8) over the head_dim
- * values of a token and head, code = x / scale rounded to nearest, ties to even,
- * both in fp32.  Zeros have scale 0; values with an infinity or NaN among them
+ * 8-bit pages: scale = max|x| * (1 / 448) (E4M3) or * (1 / 127) (INT8) over the
+ * head_dim values of a token and head, code = x / scale rounded to nearest, ties to
+ * even; the inverse, the scale and the quotient are each rounded to fp32.  Zeros have scale 0; values with an infinity or NaN among them
  * have scale NaN and codes 0, and read back as NaN. */
 int pf_kv_write(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* v,
                 uint64_t slots, uint64_t num_rows, pf_stream stream);
@@ -640,7 +640,7 @@ int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* 
  * stay as they were.  A length beyond the table is cut to it.
  *
  * Scores, softmax statistics and sums are held in fp32; the weights are rounded
- * to 16 bits (those of FP16 rows, else BF16) for the product with V. */
+ * to 16 bits, the type of the rows, for the product with V. */
 typedef struct pf_attend_args {
   pf_kv_rows q;          /* [num_rows, num_q_heads, head_dim] */
   pf_kv_rows out;        /* the same shape and type; may not overlap q */

@@ -55,7 +55,7 @@ def encode(x, kind):
     m = np.abs(x).max(-1)
     ok = np.isfinite(x).all(-1)
     with np.errstate(all="ignore"):
-        s = (m / np.float32(LARGEST[kind])).astype(np.float32)
+        s = (m * (np.float32(1) / np.float32(LARGEST[kind]))).astype(np.float32)
         q = np.where(s[..., None] > 0, x / s[..., None], np.float32(0)).astype(np.float32)
         q = np.where(ok[..., None], q, np.float32(0))
     codes = to_e4m3(q) if kind == "e4m3" else np.rint(q).astype(np.int8).view(np.uint8)
@@ -140,7 +140,9 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
     32-bit sum of dim products is off by (dim + 4) half-steps of sum |q k| scale at most, the
     weight's exponential by that and 2^-21; l and o are sums of n terms, each addition off by
     half a step (n in all; also those of a join), l's errors counted again in the quotient.
-    A weight under fp16's normal range is off by 2^-25 of the largest weight instead."""
+    A weight under fp16's normal range is off by 2^-25 of the largest weight instead; one
+    that carries the scale of a code by 2^-25 of 2^6 times the largest such scale or less,
+    so its products by 2^-31 of that scale times the code."""
     n, q_heads, dim = q.shape
     group = q_heads // pages.heads
     out = np.zeros((n, q_heads, dim))
@@ -157,6 +159,7 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
         there = (block >= 0) & (block < pages.num_blocks)
         slots = np.where(there, block, 0).astype(np.int64) * bs + t % bs
         kv = pages.get(slots)[0]
+        v_scale = pages.scales()[1, slots // bs, slots % bs] if pages.kind in LARGEST else None
         for r in range(a, e):
             p = length - (e - a) + (r - a)
             see = there & ((t <= p) if causal else True)
@@ -179,6 +182,12 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
                 bound[r, h] = size * (HALF_STEP[weights or rows] + off) + (
                     HALF_STEP[rows] * np.abs(out[r, h]) + 2.0 ** -24)
                 if (weights or rows) == "fp16":
-                    bound[r, h] += 2.0 ** -25 * np.abs(v).sum(0) / l
+                    least = 2.0 ** -25 * np.abs(v).sum(0)
+                    if v_scale is not None:
+                        s = v_scale[see, h // group].astype(np.float64)[:, None]
+                        with np.errstate(all="ignore"):
+                            codes = np.divide(np.abs(v), s, out=np.zeros_like(v), where=s > 0)
+                            least = 2.0 ** -31 * s.max() * codes.sum(0)
+                    bound[r, h] += least / l
                 lse_bound[r, h] = dz + 2.0 ** -21 + (len(z) + 8) * u + 2.0 ** -22 * abs(lse[r, h])
     return out, lse, bound, lse_bound

@@ -17,9 +17,9 @@
 // lanes, and the weights are already where the second product reads them.  That product
 // reads V^T from LDS with the transposing 16-bit loads.
 //
-// Weights are rounded to 16 bits for the product with V (bf16, or fp16 for 16-bit
-// pages of fp16 rows): the matrix core takes no more, and the rounding, at most half a
-// step of each weight, is of the size of the output's own.  Scores, maxima, sums and
+// Weights are rounded to the rows' 16 bits for the product with V: the matrix core takes
+// no more, and the rounding, at most half a step of each weight, is of the size of the
+// output's own.  Scores, maxima, sums and
 // outputs stay in fp32 until the end.
 #pragma once
 
@@ -160,6 +160,30 @@ __device__ __forceinline__ void store_out4(uint64_t row, uint32_t d, const Atten
     p[2] = static_cast<uint16_t>(v[1]);
     p[3] = static_cast<uint16_t>(v[1] >> 16);
   }
+}
+
+// fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
+// may be anything that 32 bits hold, so all weights of a row, its sum l and its outputs
+// carry a power of two, 2^lift, until the end: with the largest scale that the row has
+// attended s 2^lift is at most 2^7, and w, which lags its maximum by at most 2^8, makes
+// 2^15 of it.  A product is then a normal number down to 2^-20 of the largest scale, and
+// off by 2^-31 of that below.  (bf16 weights need none of it, but are off by up to 2^-8
+// where the outputs hold 2^-11.)
+constexpr float kLiftRoom = 7.0f, kLiftStart = 64.0f, kLiftNone = -100.0f;
+// Lowers `lift` (kLiftStart before the first token; kLiftNone for no row) to suit scales
+// up to `big` (or 2^66, so that the factor is a normal number: values as large as that
+// are infinite in fp16), and returns the factor that the row's sums take.  Other rows of
+// the wave have lifts of their own: `limit` is the largest scale that suits them all.
+__device__ __forceinline__ float lower_lift(float big, float* lift, float* limit) {
+  const float room =
+      kLiftRoom - static_cast<float>(__builtin_amdgcn_frexp_expf(fminf(big, 0x1p66f)));
+  const float old = *lift;
+  if (big > 0.0f) *lift = fminf(old, room);
+  float most = *lift;
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
+  *limit = __builtin_amdgcn_exp2f(kLiftRoom - most);
+  return __builtin_amdgcn_exp2f(*lift - old);
 }
 
 // V in a tile that some row attends only in part: a weight of 0 must not meet an
@@ -399,9 +423,8 @@ template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1)
 attend_many_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
-  using KM = Row;                                                 // K as multiplied
-  using VM = typename std::conditional<kCodes, BF16, Row>::type;  // V and the weights
-  constexpr uint32_t kPer = kCodes ? 16 : 8;                      // values of a 16-byte load
+  constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
+  constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
   // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
   constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
   constexpr uint32_t kLoads = kTileTokens * kCols / kManyThreads;
@@ -449,6 +472,7 @@ attend_many_kernel(AttendParams a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
   float m = kNegInf, l = 0.0f;
+  float lift = t.valid ? kLiftStart : kLiftNone, lift_limit = 0.0f;  // kLift
 
   // This thread's part of a tile: 16 bytes of tokens my_tok + kLoadTokens * i, values
   // my_d and on, and of 8-bit pages the scales of token 16 * wave + lane (lanes 0 to 15).
@@ -508,8 +532,8 @@ attend_many_kernel(AttendParams a) {
       for (uint32_t i = 0; i < kLoads; ++i) {
         u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kKP + my_d * 2);
         if constexpr (kCodes) {
-          const u32x2 x0 = codes_to_16<KM, TYPE>(kr[i][0]), x1 = codes_to_16<KM, TYPE>(kr[i][1]);
-          const u32x2 x2 = codes_to_16<KM, TYPE>(kr[i][2]), x3 = codes_to_16<KM, TYPE>(kr[i][3]);
+          const u32x2 x0 = codes_to_16<Row, TYPE>(kr[i][0]), x1 = codes_to_16<Row, TYPE>(kr[i][1]);
+          const u32x2 x2 = codes_to_16<Row, TYPE>(kr[i][2]), x3 = codes_to_16<Row, TYPE>(kr[i][3]);
           to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
           to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
         } else {
@@ -542,8 +566,8 @@ attend_many_kernel(AttendParams a) {
       for (uint32_t i = 0; i < kLoads; ++i) {
         u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kVP + my_d * 2);
         if constexpr (kCodes) {
-          const u32x2 x0 = codes_to_16<VM, TYPE>(vr[i][0]), x1 = codes_to_16<VM, TYPE>(vr[i][1]);
-          const u32x2 x2 = codes_to_16<VM, TYPE>(vr[i][2]), x3 = codes_to_16<VM, TYPE>(vr[i][3]);
+          const u32x2 x0 = codes_to_16<Row, TYPE>(vr[i][0]), x1 = codes_to_16<Row, TYPE>(vr[i][1]);
+          const u32x2 x2 = codes_to_16<Row, TYPE>(vr[i][2]), x3 = codes_to_16<Row, TYPE>(vr[i][3]);
           to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
           to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
         } else {
@@ -577,7 +601,7 @@ attend_many_kernel(AttendParams a) {
       for (uint32_t j = 0; j < kGroup; ++j)
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
-          s[tt] = Mat<KM>::mul32(kf[g & 1][j][tt], q[g * kGroup + j], s[tt]);
+          s[tt] = Mat<Row>::mul32(kf[g & 1][j][tt], q[g * kGroup + j], s[tt]);
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (kCodes) {
@@ -610,7 +634,7 @@ attend_many_kernel(AttendParams a) {
   // O^T += V^T W^T.
   auto add_v = [&](const u32x4 (&f)[DP / 32], u32x4 w) {
 #pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt) o[dt] = Mat<VM>::mul32(f[dt], w, o[dt]);
+    for (uint32_t dt = 0; dt < DP / 32; ++dt) o[dt] = Mat<Row>::mul32(f[dt], w, o[dt]);
   };
   // Tile n's scores and softmax.  Its product with V follows in the next step, under that
   // tile's softmax: p are the weights of tile n - 1 at first, of tile n at the end.
@@ -650,14 +674,30 @@ attend_many_kernel(AttendParams a) {
     // The maximum that the weights are taken against follows the largest score only
     // where that has grown by more than 8 (in powers of 2): until then weights up to
     // 2^8 serve as well, and the outputs need no rescaling.
-    const bool grown = __any((top - m) * a.scale_log2 > 8.0f);
+    bool grown = __any((top - m) * a.scale_log2 > 8.0f);
     float keep = 1.0f;
     if (grown) {
       const float m_new = fmaxf(m, top);
       keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
       m = m_new;
     }
-    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    if constexpr (kLift) {
+      const float* scale = lds.k[n % Lds::kBuffers].v_scale;
+      if (__any(scale[lane] > lift_limit)) {  // a scale that some row may not have room for
+        float big = 0.0f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float y = scale[32 * tt + 8 * (i / 4) + 4 * half + i % 4];
+            big = fmaxf(big, s[tt][i] == kNegInf ? 0.0f : y);
+          }
+        keep *= lower_lift(max32(big), &lift, &lift_limit);
+        grown = true;
+      }
+      base += lift;
+    }
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -686,7 +726,7 @@ attend_many_kernel(AttendParams a) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[u][j] = Mat<VM>::pack(x[2 * j], x[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) p[u][j] = Mat<Row>::pack(x[2 * j], x[2 * j + 1]);
       asm volatile("" : "+v"(p[u]), "+v"(sum));  // here, beside the products
 #pragma unroll
       for (uint32_t i = 0; i < DP / 32; ++i) {
@@ -752,6 +792,14 @@ attend_many_kernel(AttendParams a) {
     }
   }
 
+  if constexpr (kLift) {
+    const float down = __builtin_amdgcn_exp2f(-lift);
+    l *= down;
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= down;
+  }
   __syncthreads();
   if (lds.odd)
     for (int32_t tok = begin; tok < end; ++tok) {
@@ -871,8 +919,7 @@ template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
 attend_few_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
-  using KM = Row;
-  using VM = typename std::conditional<kCodes, BF16, Row>::type;
+  constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr uint32_t kPer = kCodes ? 16 : 8;
   constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
   constexpr uint32_t kCols = DP / kPer;
@@ -941,6 +988,7 @@ attend_few_kernel(AttendParams a) {
   for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
   float m = kNegInf, l = 0.0f;
   bool odd = false;  // some tile attended in part holds V that is not finite
+  float lift = valid ? kLiftStart : kLiftNone, lift_limit = 0.0f;  // kLift
 
   u32x4 kr[2][kKLoads], vr[kVLoads];
   // Token t0 + lane of a tile, lanes 0 to 31: its block (of the tile to load next), its
@@ -1010,8 +1058,8 @@ attend_few_kernel(AttendParams a) {
       const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
       u32x4 v0 = vr[i], v1{0, 0, 0, 0};
       if constexpr (kCodes) {
-        const u32x2 b0 = codes_to_16<VM, TYPE>(vr[i][0]), b1 = codes_to_16<VM, TYPE>(vr[i][1]);
-        const u32x2 b2 = codes_to_16<VM, TYPE>(vr[i][2]), b3 = codes_to_16<VM, TYPE>(vr[i][3]);
+        const u32x2 b0 = codes_to_16<Row, TYPE>(vr[i][0]), b1 = codes_to_16<Row, TYPE>(vr[i][1]);
+        const u32x2 b2 = codes_to_16<Row, TYPE>(vr[i][2]), b3 = codes_to_16<Row, TYPE>(vr[i][3]);
         v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
         v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
       }
@@ -1038,14 +1086,14 @@ attend_few_kernel(AttendParams a) {
 #pragma unroll
       for (uint32_t i = 0; i < kKLoads; ++i) {
         if constexpr (kCodes) {
-          const u32x2 a0 = codes_to_16<KM, TYPE>(kr[tt][i][0]);
-          const u32x2 a1 = codes_to_16<KM, TYPE>(kr[tt][i][1]);
-          const u32x2 a2 = codes_to_16<KM, TYPE>(kr[tt][i][2]);
-          const u32x2 a3 = codes_to_16<KM, TYPE>(kr[tt][i][3]);
-          s[tt] = Mat<KM>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
-          s[tt] = Mat<KM>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
+          const u32x2 a0 = codes_to_16<Row, TYPE>(kr[tt][i][0]);
+          const u32x2 a1 = codes_to_16<Row, TYPE>(kr[tt][i][1]);
+          const u32x2 a2 = codes_to_16<Row, TYPE>(kr[tt][i][2]);
+          const u32x2 a3 = codes_to_16<Row, TYPE>(kr[tt][i][3]);
+          s[tt] = Mat<Row>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
+          s[tt] = Mat<Row>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
         } else {
-          s[tt] = Mat<KM>::mul16(kr[tt][i], q[i], s[tt]);
+          s[tt] = Mat<Row>::mul16(kr[tt][i], q[i], s[tt]);
         }
       }
     }
@@ -1064,6 +1112,7 @@ attend_few_kernel(AttendParams a) {
       }
     }
     const uint32_t seen_blocks = there;
+    const bool lower = kLift && __any(v_scale > lift_limit);
     if (t0 + kStep < end) {
       load(t0 + kStep);
       load_block(t0 + 2 * kStep);
@@ -1103,7 +1152,24 @@ attend_few_kernel(AttendParams a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
     }
-    const float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    if constexpr (kLift) {
+      if (lower) {  // a scale that some row may not have room for; hidden ones are 0 here
+        float big = 0.0f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) big = fmaxf(big, wv[tt][i]);
+        big = fmaxf(big, __shfl_xor(big, 16));
+        const float keep = lower_lift(max32(big), &lift, &lift_limit);
+        l *= keep;
+#pragma unroll
+        for (uint32_t dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
+      }
+      base += lift;
+    }
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -1112,8 +1178,8 @@ attend_few_kernel(AttendParams a) {
         l += w;
         wv[tt][i] *= w;
       }
-    const u32x4 w{Mat<VM>::pack(wv[0][0], wv[0][1]), Mat<VM>::pack(wv[0][2], wv[0][3]),
-                  Mat<VM>::pack(wv[1][0], wv[1][1]), Mat<VM>::pack(wv[1][2], wv[1][3])};
+    const u32x4 w{Mat<Row>::pack(wv[0][0], wv[0][1]), Mat<Row>::pack(wv[0][2], wv[0][3]),
+                  Mat<Row>::pack(wv[1][0], wv[1][1]), Mat<Row>::pack(wv[1][2], wv[1][3])};
     // Every lane of the wave has stored its part of V before any reads another's.
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const uint8_t* v_from = v_lds + (quarter * 4 + col / 4) * kVP + (col & 3u) * 8;
@@ -1123,7 +1189,7 @@ attend_few_kernel(AttendParams a) {
       const s16x4 hi =
           __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_from + 16 * kVP + dt * 32));
       const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-      o[dt] = Mat<VM>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
+      o[dt] = Mat<Row>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
@@ -1137,6 +1203,14 @@ attend_few_kernel(AttendParams a) {
     load_block(t0 + kStep);
   }
   for (; t0 < end; t0 += kStep) tile(t0);
+  if constexpr (kLift) {
+    const float down = __builtin_amdgcn_exp2f(-lift);
+    l *= down;
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dt][i] *= down;
+  }
   if (__any(odd))
     for (int32_t tok = begin; tok < end; ++tok) {
       if ((static_cast<uint32_t>(tok - begin) / kFewTokens) % kFewWaves != wave) continue;

@@ -2,11 +2,12 @@
 // back, at 16 bits or as 8-bit codes with one scale for each token and head.
 //
 // Row x (one token, one head, `dim` values) is held as codes c and scale s:
-//   s = max|x| / L (L = 448 for e4m3, 127 for int8),  c = round(x / s),
-// both divisions in 32 bits, rounded to nearest, ties to even.  A row of zeros has
+//   s = max|x| * (1 / L) (L = 448 for e4m3, 127 for int8),  c = round(x / s),
+// 1 / L, the product and the quotient each rounded to 32 bits, to nearest, ties to even:
+// s is off by an ulp at most, and costs one multiplication.  A row of zeros has
 // s = 0 and codes 0.  A row with an infinity or NaN has s = NaN and codes 0, so it
-// reads back as NaN throughout.  |x| / s exceeds L at most by the roundings of s and
-// of the quotient: by a factor under 1 + 2^-8 even where s is subnormal (the
+// reads back as NaN throughout.  |x| / s exceeds L at most by the roundings of 1 / L, s
+// and the quotient: by a factor under 1 + 2^-8 even where s is subnormal (the
 // smallest max|x| is 2^-133, which leaves s 7 bits), and both conversions round
 // such a quotient back to L, so nothing is clamped.
 //
@@ -165,8 +166,8 @@ kv_write_kernel(PagedView p, RowsView k, RowsView v, const int64_t* __restrict__
         pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2, word));
       }
       const uint32_t m = group_max<LANES>(umax(pair[0], pair[1]));
-      constexpr float kLargest = TYPE == PF_KV_E4M3 ? 448.0f : 127.0f;
-      float s = Row::to_float(m) / kLargest;
+      constexpr float kInverse = 1.0f / (TYPE == PF_KV_E4M3 ? 448.0f : 127.0f);
+      float s = Row::to_float(m) * kInverse;
       u32x2 c{0, 0};
       if (m >= Row::kInf)
         s = __builtin_nanf("");

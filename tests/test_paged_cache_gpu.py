@@ -247,10 +247,9 @@ class Batch:
         return got[front:front + n], got_lse[front:front + n]
 
     def check(self, got, lse, causal=True, window=0, scale=None, **kw):
-        codes = self.kind in oracle.LARGEST
         out, want_lse, bound, lse_bound = oracle.attend(
             self.pages, self.q, self.rows, self.table, self.lens, self.starts,
-            scale or self.scale, causal, window, "bf16" if codes else self.rows)
+            scale or self.scale, causal, window)
         x = oracle.from_bits(got, self.rows).astype(np.float64)
         assert np.array_equal(np.isnan(x), np.isnan(out))
         fine = np.isfinite(out)
@@ -368,6 +367,28 @@ def test_values_that_are_not_finite(gpu, workspace, form, group, new, cached):
             b.pages.values()[kv, block, off, 0, 3] = bad[b.rows]
     b.dev.upload()
     b.check(*b.run(workspace=workspace))
+
+
+@pytest.mark.parametrize("sizes", ["growing", "falling", "mixed", "late"])
+@pytest.mark.parametrize("form,group", [(FORMS[4], 5), (FORMS[5], 1), (FORMS[2], 4),
+                                        (("int8", "fp16", 2, 128, 16, False), 4)], ids=str)
+@pytest.mark.parametrize("new,cached", [((1, 1), (2000, 40)), ((150, 30, 1), (40, 300, 7))],
+                         ids=str)
+def test_scales_of_all_sizes(gpu, workspace, form, group, sizes, new, cached):
+    """V's scales over 27 powers of two: rows that attend only small ones keep their precision
+    beside rows that attend large ones."""
+    b = Batch(new, cached, form, group, seed=14)
+    bs, rng = b.pages.block_size, np.random.default_rng(15)
+    for i, n in enumerate(b.lens):
+        t = np.arange(n)
+        size = {"growing": -20 + 27 * t / n, "falling": 7 - 27 * t / n,
+                "mixed": rng.uniform(-20, 7, n), "late": np.where(t < n - 9, -12, 7)}[sizes]
+        scale = np.exp2(size)[:, None] * rng.uniform(0.5, 1, (n, b.pages.heads))
+        scale[(t % 50 < 3) & (t % 100 < 50)] = 0
+        b.pages.scales()[1, b.table[i][t // bs], t % bs] = scale
+    b.dev.upload()
+    for w in (None, workspace):
+        b.check(*b.run(workspace=w))
 
 
 @pytest.mark.parametrize("form,group", [(LLAMA, 4), (FORMS[2], 4), (FORMS[1], 1)], ids=str)
