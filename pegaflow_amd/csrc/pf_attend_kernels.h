@@ -25,7 +25,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
+#include <utility>
 
 #include "pf_paged_device.h"
 
@@ -160,6 +160,18 @@ __device__ __forceinline__ void store_out4(uint64_t row, uint32_t d, const Atten
     p[2] = static_cast<uint16_t>(v[1]);
     p[3] = static_cast<uint16_t>(v[1] >> 16);
   }
+}
+
+// Lane N of this lane's 16, an operand of the instruction that uses it.
+template <int N>
+__device__ __forceinline__ float of16(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x150 + N, 0xf, 0xf, true));
+}
+// x[i] *= lane FIRST + i of these 16's y.
+template <int FIRST, int... I>
+__device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequence<int, I...>) {
+  ((x[I] *= of16<FIRST + I>(y)), ...);
 }
 
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
@@ -588,7 +600,16 @@ attend_many_kernel(AttendParams a) {
       for (int tt = 0; tt < 2; ++tt)
         f[j][tt] = *reinterpret_cast<const u32x4*>(at + tt * 32 * kKP + (g * kGroup + j) * 32);
   };
+  // Scales of the tile: lane i of 16 holds that of this half's token i, and 32 tt on.
+  float ks[2], vs[2];
+  const uint32_t my_scale = 8 * ((lane & 15u) / 4) + 4 * half + (lane & 3u);
   auto scores = [&](uint32_t n) {
+    if constexpr (kCodes)
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+        ks[tt] = lds.k[n % Lds::kBuffers].k_scale[32 * tt + my_scale];
+        vs[tt] = lds.k[n % Lds::kBuffers].v_scale[32 * tt + my_scale];
+      }
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -605,15 +626,15 @@ attend_many_kernel(AttendParams a) {
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (kCodes) {
-      const float* scale = lds.k[n % Lds::kBuffers].k_scale + half * 4;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+      for (int tt = 0; tt < 2; ++tt) {
+        float x[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4*>(scale + tt * 32 + i * 8);
+        for (int i = 0; i < 16; ++i) x[i] = s[tt][i];
+        scale_by<0>(x, ks[tt], std::make_integer_sequence<int, 16>());
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[tt][4 * i + j] *= x[j];
-        }
+        for (int i = 0; i < 16; ++i) s[tt][i] = x[i];
+      }
     }
   };
   // V^T of 16 tokens of tile n, from 16 u on.  They are taken in the order in which a
@@ -683,16 +704,14 @@ attend_many_kernel(AttendParams a) {
     }
     float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
     if constexpr (kLift) {
-      const float* scale = lds.k[n % Lds::kBuffers].v_scale;
-      if (__any(scale[lane] > lift_limit)) {  // a scale that some row may not have room for
+      if (__any(fmaxf(vs[0], vs[1]) > lift_limit)) {  // some row may not have room for it
+        const float* scale = lds.k[n % Lds::kBuffers].v_scale + 4 * half;
         float big = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float y = scale[32 * tt + 8 * (i / 4) + 4 * half + i % 4];
-            big = fmaxf(big, s[tt][i] == kNegInf ? 0.0f : y);
-          }
+          for (int i = 0; i < 16; ++i)
+            big = fmaxf(big, s[tt][i] == kNegInf ? 0.0f : scale[32 * tt + 8 * (i / 4) + i % 4]);
         keep *= lower_lift(max32(big), &lift, &lift_limit);
         grown = true;
       }
@@ -712,13 +731,10 @@ attend_many_kernel(AttendParams a) {
         sum += x[i];
       }
       if constexpr (kCodes) {
-        const float* scale = lds.k[n % Lds::kBuffers].v_scale + u * 16 + half * 4;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(scale + g * 8);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[4 * g + j] *= y[j];
-        }
+        if (u & 1)
+          scale_by<8>(x, vs[u / 2], std::make_integer_sequence<int, 8>());
+        else
+          scale_by<0>(x, vs[u / 2], std::make_integer_sequence<int, 8>());
         if (masked) {  // a hidden token's scale may be anything
 #pragma unroll
           for (int i = 0; i < 8; ++i)
