@@ -131,10 +131,11 @@ def _put(pages, which, b, t, x):
     view[:, b, t] = x
 
 
-def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, weights=None):
+def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, weights=None,
+           every=1):
     """(out, lse, bound, lse bound) in 64 bits of query bits [n, heads, dim]: bound is how far each output
     of a kernel may be off that holds scores, statistics and sums in 32 bits, rounds each weight
-    to ``weights`` and the output to ``rows``.
+    to ``weights`` and the output to ``rows``.  Only every ``every``-th row is computed.
 
     A weight's rounding and the errors below scale with A = sum w |v| / sum w.  A score's
     32-bit sum of dim products is off by (dim + 4) half-steps of sum |q k| scale at most, the
@@ -160,7 +161,7 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
         slots = np.where(there, block, 0).astype(np.int64) * bs + t % bs
         kv = pages.get(slots)[0]
         v_scale = pages.scales()[1, slots // bs, slots % bs] if pages.kind in LARGEST else None
-        for r in range(a, e):
+        for r in range(a + -a % every, e, every):
             p = length - (e - a) + (r - a)
             see = there & ((t <= p) if causal else True)
             if window:

@@ -452,12 +452,16 @@ attend_many_kernel(AttendParams a) {
   // Heads of one tile are neighbours: with 8 of them each has an XCD's L2 for its pages.
   const uint32_t head = blockIdx.x % pg.heads;
   const uint32_t rest = blockIdx.x / pg.heads;
-  const uint32_t split = rest % a.many_splits;
-  const uint32_t unit = rest / a.many_splits;
+  uint32_t unit = rest, split = 0, splits = 1;
+  if (rest >= a.many_whole) {
+    splits = a.many_splits;
+    split = (rest - a.many_whole) % splits;
+    unit = a.many_whole + (rest - a.many_whole) / splits;
+  }
   ManyTile t;
   if (!many_tile(a, unit, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
-  const uint32_t used = split_range(begin, end, split, a.many_splits, a.many_piece);
+  const uint32_t used = split_range(begin, end, split, splits, a.many_piece);
   if (split >= used) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
@@ -842,7 +846,7 @@ attend_many_kernel(AttendParams a) {
     return;
   }
   // This split's share for attend_many_join_kernel: 16 bytes a lane at a time.
-  const uint64_t slot = (static_cast<uint64_t>(unit) * a.many_splits + split) * pg.heads + head;
+  const uint64_t slot = (rest - a.many_whole) * static_cast<uint64_t>(pg.heads) + head;
   f32x4* part = reinterpret_cast<f32x4*>(a.many_o) + (slot * 4 + wave) * (DP / 8) * 64 + lane;
 #pragma unroll
   for (uint32_t dt = 0; dt < DP / 32; ++dt)
@@ -859,14 +863,14 @@ template <class Row, uint32_t DP>
 __global__ void __launch_bounds__(64) attend_many_join_kernel(AttendParams a) {
   const PagedView& pg = a.pages;
   const uint32_t lane = threadIdx.x, wave = blockIdx.x & 3u;
-  const uint32_t head = (blockIdx.x >> 2) % pg.heads, unit = (blockIdx.x >> 2) / pg.heads;
+  const uint32_t head = (blockIdx.x >> 2) % pg.heads, left = (blockIdx.x >> 2) / pg.heads;
   ManyTile t;
-  if (!many_tile(a, unit, head, wave, &t)) return;
+  if (!many_tile(a, a.many_whole + left, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, 0, a.many_splits, a.many_piece);
   if (used == 1) return;
   auto slot = [&](uint32_t split) {
-    return ((static_cast<uint64_t>(unit) * a.many_splits + split) * pg.heads + head) * 4 + wave;
+    return ((static_cast<uint64_t>(left) * a.many_splits + split) * pg.heads + head) * 4 + wave;
   };
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.many_ml);
   float m = kNegInf;
@@ -1390,12 +1394,13 @@ hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
                        dim3(kFewThreads), 0, stream, p);
   }
   if (p.many_units) {
-    const uint32_t units = p.many_units * p.pages.heads;
-    hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP>), dim3(units * p.many_splits),
+    const uint32_t left = p.many_units - p.many_whole;
+    hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP>),
+                       dim3((p.many_whole + left * p.many_splits) * p.pages.heads),
                        dim3(kManyThreads), 0, stream, p);
-    if (p.many_splits > 1)
-      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(units * 4), dim3(64), 0,
-                         stream, p);
+    if (left)
+      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(left * p.pages.heads * 4),
+                         dim3(64), 0, stream, p);
   }
   return hipGetLastError();
 }

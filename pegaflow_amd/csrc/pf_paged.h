@@ -56,9 +56,10 @@ struct AttendParams {
   uint32_t unit_shift;  // 2^unit_shift aligned tokens, at most 16, share a block
   // The launch (plan_attend): sequences of up to few_rows rows of a KV head go to the
   // kernel for few, in few_splits shares of few_piece tokens (0: none do) of at most
-  // few_rows_most rows, the others in many_units tiles of rows and many_splits shares.
+  // few_rows_most rows, the others in many_units tiles of rows, of which those from
+  // many_whole on go in many_splits shares of many_piece tokens.
   uint32_t few_rows, few_splits, few_piece, few_rows_most;
-  uint32_t many_units, many_splits, many_piece;
+  uint32_t many_units, many_whole, many_splits, many_piece;
   float *few_o, *few_ml, *many_o, *many_ml;  // shares, in the workspace
   uint32_t* few_count;  // finished shares of each sequence and head, 0 between calls
 };
@@ -119,7 +120,8 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
   const bool all_few = most_new * group <= kFewRows;
   const bool any_few = all_few || (p->num_seqs > 1 && group <= kFewRows);
   p->few_rows = any_few && !all_few ? kFewRows : 0;
-  p->few_splits = p->few_piece = p->many_units = p->many_splits = p->many_piece = 0;
+  p->few_splits = p->few_piece = 0;
+  p->many_units = p->many_whole = p->many_splits = p->many_piece = 0;
   const uint64_t counts = workspace_counts(bytes);
   uint64_t at = ws + counts * kCountStride * 4;
   const uint64_t end = ws + bytes;
@@ -147,9 +149,20 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
   if (!all_few) {
     const uint64_t rows = p->num_rows * group;
     const uint64_t seqs = p->num_seqs < p->num_rows ? p->num_seqs : p->num_rows;
-    const uint64_t tiles = rows / kManyRows + seqs, units = tiles * heads;
+    const uint64_t tiles = seqs > 1 ? rows / kManyRows + seqs : ceil_div(rows, kManyRows);
+    // The tiles that fill the chip, once or more, are passed over whole; those left over
+    // are split among the workgroups that it holds at once, where they are long enough for
+    // their join: the last tiles are those of the first rows, which attend little more than
+    // what is cached.  2,100 rows of 32 heads behind 30,000 tokens take 1,156 us, whole
+    // 1,627 (2,048 rows: 1,095); behind 4,000 216 and 251, 2,000 148 and 151, 1,000 107
+    // and 99; seven times 300 behind 10,000 435 and 595.
+    constexpr uint64_t kSplitCached = 2048;
+    const uint64_t slots = kCus * (dim <= 128 ? 2 : 1);
+    uint64_t whole = tiles * heads / slots * slots / heads;
+    if (whole && longest < most_new + kSplitCached) whole = tiles;
+    const uint64_t units = (tiles - whole) * heads;
     const uint64_t slot = kManyRows * (dim * 4 + 16);
-    const uint64_t want = units < kCus * 2 ? kCus * 2 / units : 1;
+    const uint64_t want = units && units < slots ? slots / units : 1;
     uint64_t piece = ceil_div(ceil_div(longest, want), 64) * 64;
     if (piece < 256) piece = 256;
     uint64_t splits = ceil_div(longest, piece);
@@ -158,6 +171,8 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
       if (splits < 2) splits = 1;
       piece = ceil_div(ceil_div(longest, splits), 64) * 64;
     }
+    if (splits == 1) whole = tiles;
+    p->many_whole = static_cast<uint32_t>(whole);
     p->many_units = static_cast<uint32_t>(tiles);
     p->many_splits = static_cast<uint32_t>(splits);
     p->many_piece = static_cast<uint32_t>(piece);

@@ -246,11 +246,12 @@ class Batch:
         assert (got_lse[:front] == 77).all() and (got_lse[front + n:] == 77).all()
         return got[front:front + n], got_lse[front:front + n]
 
-    def check(self, got, lse, causal=True, window=0, scale=None, **kw):
-        out, want_lse, bound, lse_bound = oracle.attend(
+    def check(self, got, lse, causal=True, window=0, scale=None, every=1, **kw):
+        out, want_lse, bound, lse_bound = (x[::every] for x in oracle.attend(
             self.pages, self.q, self.rows, self.table, self.lens, self.starts,
-            scale or self.scale, causal, window)
-        x = oracle.from_bits(got, self.rows).astype(np.float64)
+            scale or self.scale, causal, window, every=every))
+        x = oracle.from_bits(got, self.rows).astype(np.float64)[::every]
+        lse = None if lse is None else lse[::every]
         assert np.array_equal(np.isnan(x), np.isnan(out))
         fine = np.isfinite(out)
         off = np.abs(x - out)[fine] / np.maximum(bound[fine], 1e-300)
@@ -318,6 +319,28 @@ def test_long_sequences_are_split_and_joined(gpu, workspace, form, group, new, c
     # Bounds far too high, and a length hint that says too little, change the launch alone.
     b.check(*b.run(workspace=workspace, max_seq_len=1 << 20, max_query_len=1 << 20))
     b.check(*b.run(workspace=workspace, max_seq_len=1))
+
+
+@pytest.mark.parametrize("form,group,new,cached", [
+    (("bf16", "bf16", 64, 16, 16, False), 1, (1030,), (2300,)),
+    (("int8", "fp16", 32, 208, 16, True), 2, (70, 500, 1), (2900, 2500, 2600))], ids=str)
+def test_tiles_left_over_are_split(gpu, workspace, form, group, new, cached):
+    """A few tiles of rows more than the chip holds at once: the last ones in shares, and
+    whole without a workspace."""
+    b = Batch(new, cached, form, group, seed=17)
+    for w in (workspace, None):
+        b.check(*b.run(workspace=w, tail=1), every=37)
+
+
+@pytest.mark.parametrize("form,group,new,cached", [
+    (("bf16", "bf16", 64, 16, 16, False), 1, (1030,), (2300,)),
+    (("int8", "fp16", 32, 208, 16, True), 2, (70, 500, 1), (2900, 2500, 2600))], ids=str)
+def test_tiles_left_over_are_split(gpu, workspace, form, group, new, cached):
+    """A few tiles of rows more than the chip holds at once: the last ones in shares, and
+    whole without a workspace."""
+    b = Batch(new, cached, form, group, seed=17)
+    for w in (workspace, None):
+        b.check(*b.run(workspace=w, tail=1), every=37)
 
 
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 1 << 31])
