@@ -8,7 +8,9 @@ import numpy as np
 import pytest
 
 from oracle import paged as oracle
-from pegaflow_amd.paged_cache import AttentionWorkspace, PagedKVCache
+from pegaflow_amd.engine import PegaEngine
+from pegaflow_amd.load_state import PyLoadState
+from pegaflow_amd.paged_cache import AttentionWorkspace, PagedKVCache, segment_bytes
 from pegaflow_amd.runtime import DeviceArray, DeviceBuffer, Stream, synchronize
 from pegaflow_amd.transfer import KVCacheRegistration
 
@@ -598,3 +600,79 @@ def test_scale_defaults_to_the_head_size(gpu, workspace):
     got = b.run(workspace=workspace)
     same = b.run(workspace=workspace, scale=1 / math.sqrt(128))
     assert np.array_equal(got[0], same[0])
+
+
+@pytest.mark.parametrize("kind,rows,head_major", [("e4m3", "bf16", False), ("int8", "fp16", True),
+                                                  ("bf16", "bf16", False)])
+def test_saved_blocks_answer_as_before(gpu, workspace, kind, rows, head_major):
+    """A serving step's life: a prompt's K and V written and attended, its full blocks saved by
+    hash, the pages given to others, the blocks loaded elsewhere, and the next tokens written
+    and attended behind them, with the bits that the pages would have given in place."""
+    heads, dim, bs, nb, group, layers = 2, 64, 16, 40, 4, 2
+    prompt, steps = 150, 12
+    full = prompt // bs
+    rng = np.random.default_rng(30)
+    seg = segment_bytes(bs, heads, dim, kind)
+    engine = PegaEngine(pool_size=64 << 20)
+    bufs, caches, names = [], [], [f"layer.{i}" for i in range(layers)]
+    for name in names:
+        buf = DeviceBuffer(2 * nb * seg)
+        buf.fill_random(len(bufs) + 1)
+        engine.register_context_layer("inst", "ns", 0, name, buf.ptr, buf.nbytes, nb, seg,
+                                      nb * seg, 2, 0, 1, layers)
+        reg = KVCacheRegistration.create(buf.ptr, buf.nbytes, nb, seg, nb * seg, 2)
+        bufs.append(buf)
+        caches.append(PagedKVCache(reg, bs, heads, dim, kind, head_major=head_major))
+    hashes = [bytes([i]) * 32 for i in range(full)]
+
+    def run(cache, table, first, k, v, q):
+        """Writes tokens `first` on and attends them; the outputs' bits."""
+        n = len(k)
+        t = np.arange(first, first + n)
+        slots = device_array((table[t // bs].astype(np.int64) * bs + t % bs), "int64")
+        cache.write(device_rows(k, rows=rows)[0], device_rows(v, rows=rows)[0], slots)
+        out = device_rows(np.zeros_like(q), rows=rows)[0]
+        cache.attend(device_rows(q, rows=rows)[0], out, device_array(table[None], "int32"),
+                     device_array(np.array([first + n], np.int32), "int32"),
+                     device_array(np.array([0, n], np.int32), "int32"), workspace=workspace,
+                     max_seq_len=first + n, max_query_len=n)
+        synchronize()
+        return out.download().view(np.uint16).reshape(q.shape)
+
+    old = rng.permutation(nb)[:20].astype(np.int32)
+    data = [[values(rng, (prompt + steps, h, dim), rows) for h in (heads, heads, heads * group)]
+            for _ in names]
+    for cache, (k, v, q) in zip(caches, data):
+        host = oracle.Pages(nb, bs, heads, dim, kind, head_major, rows)
+        t = np.arange(prompt)
+        host.set(old[t // bs].astype(np.int64) * bs + t % bs, k[:prompt], v[:prompt])
+        got = run(cache, old, 0, k[:prompt], v[:prompt], q[:prompt])
+        want, _, bound, _ = oracle.attend(host, q[:prompt], rows, old[None], [prompt], [0, prompt],
+                                          dim ** -0.5, every=11)
+        x = oracle.from_bits(got, rows).astype(np.float64)
+        assert (np.abs(x - want) <= bound)[::11].all()
+    engine.batch_save_kv_blocks("inst", 0, 0, [(n, [int(b) for b in old[:full]], hashes)
+                                               for n in names])
+    assert engine.count_prefix_hit_blocks("inst", hashes) == full
+    # What the next tokens answer with the blocks in place.
+    kept = [[run(cache, old, prompt + i, k[prompt + i:][:1], v[prompt + i:][:1],
+                 q[prompt + i:][:1]) for i in range(steps)]
+            for cache, (k, v, q) in zip(caches, data)]
+    for buf in bufs:  # other requests' tokens, of any bits
+        buf.fill_random(99)
+    new = rng.permutation(nb)[:20].astype(np.int32)
+    state = PyLoadState(num_layers=layers)
+    engine.batch_load_kv_blocks("inst", 0, 0, state.shm_name(), names,
+                                [int(b) for b in new[:full]], hashes)
+    for i in range(layers):
+        assert state.wait_for_layer(i, 60.0)
+    for cache, (k, v, q), want in zip(caches, data, kept):
+        # The block that was not full is computed again.
+        run(cache, new, full * bs, k[full * bs:prompt], v[full * bs:prompt], q[full * bs:prompt])
+        for i in range(steps):
+            got = run(cache, new, prompt + i, k[prompt + i:][:1], v[prompt + i:][:1],
+                      q[prompt + i:][:1])
+            assert np.array_equal(got, want[i])
+    engine.close()
+    for buf in bufs:
+        buf.close()
