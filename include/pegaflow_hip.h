@@ -617,8 +617,9 @@ typedef struct pf_kv_rows {
  *
  * 8-bit pages: scale = max|x| * (1 / 448) (E4M3) or * (1 / 127) (INT8) over the
  * head_dim values of a token and head, code = x / scale rounded to nearest, ties to
- * even; the inverse, the scale and the quotient are each rounded to fp32.  Zeros have scale 0; values with an infinity or NaN among them
- * have scale NaN and codes 0, and read back as NaN. */
+ * even; the inverse, the scale and the quotient are each rounded to fp32.  Zeros have
+ * scale 0; values with an infinity or NaN among them have scale NaN and codes 0, and
+ * read back as NaN. */
 int pf_kv_write(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* v,
                 uint64_t slots, uint64_t num_rows, pf_stream stream);
 /* The reverse: the values at slots[i] into row i of k and v, code * scale rounded

@@ -216,7 +216,8 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   if (a->num_q_heads == 0 || a->num_q_heads % pv.heads)
     return invalid(strf("%u query heads are no multiple of %u KV heads", a->num_q_heads, pv.heads));
   if (a->window && !a->causal) return invalid("a window needs causal attention");
-  if (!std::isfinite(a->scale)) return invalid("the scale is not finite");
+  p.scale_log2 = static_cast<float>(std::fabs(a->scale) * 1.4426950408889634);
+  if (!std::isfinite(p.scale_log2)) return invalid("the scale is not finite");
   if (a->num_seqs == 0 || a->num_rows == 0) return PF_OK;
   if (a->table_width == 0) return invalid("the block table has no entries");
   if (static_cast<uint64_t>(a->table_width) * pv.block_size > kMaxTokens - kAttendSlack)
@@ -258,7 +259,6 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   const uint32_t room = a->table_width * pv.block_size;  // checked above
   p.window = a->window >= room ? 0 : a->window;
   p.causal = a->causal != 0;
-  p.scale_log2 = static_cast<float>(std::fabs(a->scale) * 1.4426950408889634);
   // The kernels hide a score by -infinity, which a scale of 0 would turn into NaN; this
   // one leaves every weight at 1 as 0 does.
   if (p.scale_log2 < 1e-37f) p.scale_log2 = 1e-37f;

@@ -132,6 +132,7 @@ ATTEND_REFUSALS = [
     (dict(window=5, causal=0), "a window needs causal"),
     (dict(scale=float("nan")), "not finite"),
     (dict(scale=float("inf")), "not finite"),
+    (dict(scale=-3e38), "not finite"),
     (dict(table_width=0), "no entries"),
     (dict(table_width=(1 << 27) - 4095), "2^31 - 65536 tokens"),
     (dict(table_stride=3), "rows of the block table overlap"),
