@@ -290,18 +290,22 @@ __device__ __forceinline__ bool token_at(const PagedView& p, int32_t block, uint
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup of 4 waves takes 128 rows, 32 a wave, and 64 tokens at a
-// time.  K and V of those tokens go through registers into LDS, converted to 16 bits,
-// under the previous tile's products; each wave then multiplies its rows with them.
+// Many rows: a workgroup of 4 waves takes 128 rows, or of 8 waves 256, 32 a wave, and 64
+// tokens at a time.  K and V of those tokens go through registers into LDS, converted to
+// 16 bits, under the previous tile's products; each wave then multiplies its rows with
+// them.
 //
 // Bound by the matrix cores and, close behind, by the softmax on the vector units: 64
 // tokens x 32 rows take a wave 32 products of 32 cycles at head size 128, and 2,048
-// weights 32 times (multiply-add, exponential, maximum, sum, rounding).  Two workgroups
-// share a compute unit so that one's products run under the other's softmax.
+// weights 32 times (multiply-add, exponential, maximum, sum, rounding).  Two waves share
+// each vector unit, of two workgroups or one, so that one's products run under the
+// other's softmax.  Under such load the clock falls from 2.4 to 1.7-1.9 GHz.
+//
+// 8,192 new tokens (bf16, 32 heads of 128 on 8) take 532 us, 1,030 TFLOP/s where a large
+// product of matrices reaches 1,240; 578 in tiles of 128 rows, which load and store K and
+// V twice as often (without that work 484).  2,048 behind 30,000: 963.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kTileTokens = 64;
-constexpr uint32_t kManyThreads = 256;
 constexpr uint32_t kRing = 256;
 
 // Bytes from one token to the next in LDS.  K: 16-byte reads of 16 neighbouring tokens
@@ -380,16 +384,17 @@ struct ManyTile {
   int32_t pos0;                   // position of the sequence's first new token
   bool valid;
 };
+template <uint32_t ROWS>
 __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, uint32_t head,
                                           uint32_t wave, ManyTile* t) {
   uint32_t tile = 0;
-  if (!find_tile(a, unit, kTileRows, a.few_rows, &t->seq, &tile)) return false;
+  if (!find_tile(a, unit, ROWS, a.few_rows, &t->seq, &tile)) return false;
   t->seq = __builtin_amdgcn_readfirstlane(t->seq);
   tile = __builtin_amdgcn_readfirstlane(tile);
   t->s = seq_of(a, t->seq);
   t->head = head;
   t->rows = static_cast<uint32_t>(t->s.rows) * a.group;
-  const uint32_t row0 = tile * kTileRows, last = min(row0 + kTileRows, t->rows) - 1;
+  const uint32_t row0 = tile * ROWS, last = min(row0 + ROWS, t->rows) - 1;
   t->pos0 = t->s.len - t->s.rows;
   t->begin = row_begin(a, t->pos0 + static_cast<int32_t>(row0 / a.group)) &
              ~static_cast<int32_t>(kTileTokens - 1);
@@ -429,16 +434,19 @@ __device__ __forceinline__ void many_store(const AttendParams& a, const ManyTile
   }
 }
 
-template <class Row, uint32_t TYPE, uint32_t DP>
-__global__ void __launch_bounds__(kManyThreads, DP <= 128 ? 2 : 1)
+template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
+__global__ void __launch_bounds__(2 * ROWS, DP <= 128 ? 2 : 1)
 attend_many_kernel(AttendParams a) {
+  constexpr uint32_t kThreads = 2 * ROWS, kWaves = ROWS / 32;
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
   // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
   constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
-  constexpr uint32_t kLoads = kTileTokens * kCols / kManyThreads;
-  constexpr uint32_t kLoadTokens = kManyThreads / kCols;  // of one load of the workgroup
+  // Tokens of one load of the workgroup, whose threads may be more than a tile needs: then
+  // its halves load and store the same.
+  constexpr uint32_t kLoadTokens = kThreads / kCols < kTileTokens ? kThreads / kCols : kTileTokens;
+  constexpr uint32_t kLoads = kTileTokens / kLoadTokens;
   constexpr uint32_t kKP = k_pitch(DP), kVP = v_pitch(DP);
   constexpr int32_t kStep = kTileTokens;
   using Lds = ManyLds<DP>;
@@ -457,7 +465,7 @@ attend_many_kernel(AttendParams a) {
     unit = a.many_whole + (rest - a.many_whole) / splits;
   }
   ManyTile t;
-  if (!many_tile(a, unit, head, wave, &t)) return;
+  if (!many_tile<ROWS>(a, unit, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, split, splits, a.many_piece);
   if (split >= used) return;
@@ -467,7 +475,7 @@ attend_many_kernel(AttendParams a) {
 
   // Tokens that every row of the workgroup attends, and this wave's and row's.
   const uint32_t wave0 = __builtin_amdgcn_readfirstlane(t.row), group = a.group;
-  const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + kTileRows, t.rows) - 1;
+  const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + ROWS, t.rows) - 1;
   const int32_t all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
   const int32_t all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
   const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
@@ -489,8 +497,9 @@ attend_many_kernel(AttendParams a) {
   float lift = t.valid ? kLiftStart : kLiftNone, lift_limit = 0.0f;  // kLift
 
   // This thread's part of a tile: 16 bytes of tokens my_tok + kLoadTokens * i, values
-  // my_d and on, and of 8-bit pages the scales of token 16 * wave + lane (lanes 0 to 15).
-  const uint32_t my_tok = tid / kCols, my_d = (tid % kCols) * kPer;
+  // my_d and on, and of 8-bit pages the scales of token 16 * wave + lane (lanes 0 to 15 of
+  // the first 4 waves).
+  const uint32_t my_tok = tid / kCols % kTileTokens, my_d = (tid % kCols) * kPer;
   const bool my_col = my_d < pg.dim;
   const uint32_t shift = a.unit_shift, in_unit = (1u << shift) - 1, tile_units = kTileTokens >> shift;
   // A load's tokens repeat their place in their unit after at most two loads.
@@ -525,7 +534,7 @@ attend_many_kernel(AttendParams a) {
       kr[i] = *reinterpret_cast<const g_u32x4*>(
           pg.k + lds.at[unit_of(n, my_tok + i * kLoadTokens)] + lane_at[i % kOffsets]);
     if constexpr (kCodes)
-      if (lane < 16) {
+      if (lane < 16 && wave < 4) {
         const uint64_t at = lds.scale_at[unit_of(n, wave * 16 + lane)] + lane_scale;
         k_sr = *reinterpret_cast<const g_f32*>(pg.k + at);
         v_sr = *reinterpret_cast<const g_f32*>(pg.v + at);
@@ -555,7 +564,7 @@ attend_many_kernel(AttendParams a) {
         }
       }
     if constexpr (kCodes)
-      if (lane < 16) {
+      if (lane < 16 && wave < 4) {
         tile.k_scale[wave * 16 + lane] = k_sr;
         tile.v_scale[wave * 16 + lane] = v_sr;
       }
@@ -845,30 +854,31 @@ attend_many_kernel(AttendParams a) {
   }
   // This split's share for attend_many_join_kernel: 16 bytes a lane at a time.
   const uint64_t slot = (rest - a.many_whole) * static_cast<uint64_t>(pg.heads) + head;
-  f32x4* part = reinterpret_cast<f32x4*>(a.many_o) + (slot * 4 + wave) * (DP / 8) * 64 + lane;
+  f32x4* part = reinterpret_cast<f32x4*>(a.many_o) + (slot * kWaves + wave) * (DP / 8) * 64 + lane;
 #pragma unroll
   for (uint32_t dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
       part[(dt * 4 + i) * 64] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
                                       o[dt][4 * i + 3]};
-  reinterpret_cast<f32x2*>(a.many_ml)[(slot * 4 + wave) * 64 + lane] = f32x2{m, l};
+  reinterpret_cast<f32x2*>(a.many_ml)[(slot * kWaves + wave) * 64 + lane] = f32x2{m, l};
 }
 
 // Joins the shares of split tiles, a workgroup each wave's rows: the same lanes hold the
 // same rows and values.
-template <class Row, uint32_t DP>
+template <class Row, uint32_t DP, uint32_t ROWS>
 __global__ void __launch_bounds__(64) attend_many_join_kernel(AttendParams a) {
+  constexpr uint32_t kWaves = ROWS / 32;
   const PagedView& pg = a.pages;
-  const uint32_t lane = threadIdx.x, wave = blockIdx.x & 3u;
-  const uint32_t head = (blockIdx.x >> 2) % pg.heads, left = (blockIdx.x >> 2) / pg.heads;
+  const uint32_t lane = threadIdx.x, wave = blockIdx.x % kWaves;
+  const uint32_t head = blockIdx.x / kWaves % pg.heads, left = blockIdx.x / kWaves / pg.heads;
   ManyTile t;
-  if (!many_tile(a, a.many_whole + left, head, wave, &t)) return;
+  if (!many_tile<ROWS>(a, a.many_whole + left, head, wave, &t)) return;
   int32_t begin = t.begin, end = t.end;
   const uint32_t used = split_range(begin, end, 0, a.many_splits, a.many_piece);
   if (used == 1) return;
   auto slot = [&](uint32_t split) {
-    return ((static_cast<uint64_t>(left) * a.many_splits + split) * pg.heads + head) * 4 + wave;
+    return ((static_cast<uint64_t>(left) * a.many_splits + split) * pg.heads + head) * kWaves + wave;
   };
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.many_ml);
   float m = kNegInf;
@@ -1390,6 +1400,17 @@ attend_few_kernel(AttendParams a) {
   }
 }
 
+template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
+void launch_many(const AttendParams& p, hipStream_t stream) {
+  const uint32_t left = p.many_units - p.many_whole;
+  hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP, ROWS>),
+                     dim3((p.many_whole + left * p.many_splits) * p.pages.heads), dim3(2 * ROWS), 0,
+                     stream, p);
+  if (left)
+    hipLaunchKernelGGL((attend_many_join_kernel<Row, DP, ROWS>),
+                       dim3(left * p.pages.heads * (ROWS / 32)), dim3(64), 0, stream, p);
+}
+
 template <class Row, uint32_t TYPE, uint32_t DP>
 hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
   if (p.few_splits) {
@@ -1398,13 +1419,14 @@ hipError_t launch_kernels(const AttendParams& p, hipStream_t stream) {
                        dim3(kFewThreads), 0, stream, p);
   }
   if (p.many_units) {
-    const uint32_t left = p.many_units - p.many_whole;
-    hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP>),
-                       dim3((p.many_whole + left * p.many_splits) * p.pages.heads),
-                       dim3(kManyThreads), 0, stream, p);
-    if (left)
-      hipLaunchKernelGGL((attend_many_join_kernel<Row, DP>), dim3(left * p.pages.heads * 4),
-                         dim3(64), 0, stream, p);
+    if constexpr (DP <= kWideMaxDim) {
+      if (p.many_rows == kWideRows)
+        launch_many<Row, TYPE, DP, kWideRows>(p, stream);
+      else
+        launch_many<Row, TYPE, DP, kManyRows>(p, stream);
+    } else {
+      launch_many<Row, TYPE, DP, kManyRows>(p, stream);
+    }
   }
   return hipGetLastError();
 }

@@ -269,7 +269,7 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   const uint64_t left = p.many_units - p.many_whole;
   const uint64_t grid =
       std::max<uint64_t>(static_cast<uint64_t>(p.num_seqs) * p.few_splits,
-                         std::max(p.many_whole + left * p.many_splits, left * 4)) * pv.heads;
+                         std::max(p.many_whole + left * p.many_splits, left * p.many_rows / 32)) * pv.heads;
   if (grid > 0x7fffffffull) return invalid("too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;

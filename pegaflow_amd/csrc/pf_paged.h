@@ -56,16 +56,18 @@ struct AttendParams {
   uint32_t unit_shift;  // 2^unit_shift aligned tokens, at most 16, share a block
   // The launch (plan_attend): sequences of up to few_rows rows of a KV head go to the
   // kernel for few, in few_splits shares of few_piece tokens (0: none do) of at most
-  // few_rows_most rows, the others in many_units tiles of rows, of which those from
-  // many_whole on go in many_splits shares of many_piece tokens.
+  // few_rows_most rows, the others in many_units tiles of many_rows rows, of which those
+  // from many_whole on go in many_splits shares of many_piece tokens.
   uint32_t few_rows, few_splits, few_piece, few_rows_most;
-  uint32_t many_units, many_whole, many_splits, many_piece;
+  uint32_t many_units, many_rows, many_whole, many_splits, many_piece;
   float *few_o, *few_ml, *many_o, *many_ml;  // shares, in the workspace
   uint32_t* few_count;  // finished shares of each sequence and head, 0 between calls
 };
 
 constexpr uint32_t kFewRows = 16;        // of attend_few_kernel's tile
-constexpr uint32_t kManyRows = 128;      // of attend_many_kernel's
+constexpr uint32_t kManyRows = 128;      // of attend_many_kernel's, or where rows are many
+constexpr uint32_t kWideRows = 256;      // and heads have up to kWideMaxDim values
+constexpr uint32_t kWideMaxDim = 128;
 constexpr uint32_t kFewMaxSplits = 192;
 // A count of finished shares has a 128-byte line of its own: adds to one line run one
 // after another.  The first kCounts of them (or a sixteenth of a small workspace) are at
@@ -103,6 +105,23 @@ inline uint64_t few_piece(uint64_t units, uint64_t longest) {
   uint64_t piece = 128;
   while (piece * piece < 37 * longest) piece += 128;
   return piece > whole ? piece : whole;
+}
+
+// Whether attend_many_kernel's tiles are of kWideRows rows: half the loads and writes to
+// LDS for a product, but one workgroup a compute unit, so that lengths even out less.
+// (Measured with 8 heads of 128 and a group of 4, in us, wide and not.)
+//
+// A sequence alone, from 512 rows and 4,096 tokens on: 8,192 new tokens 532 and 578, 130
+// behind 4,000 34.0 and 34.6; 2,000 new ones 66 and 62, 300 22 and 19.  Several, where the
+// chip is filled twice or more: 9 of up to 701 behind 4,100 (int8) 297 and 312, 16 of 480
+// behind 4,000 245 and 268, 8 of 960 (e4m3) 342 and 335; below that 8 of 240 behind 10,000
+// 324 and 288.
+inline bool wide_tiles(uint64_t seqs, uint64_t rows, uint64_t heads, uint64_t dim,
+                       uint64_t longest) {
+  constexpr uint64_t kLong = 4096, kUnits = 512;
+  if (dim > kWideMaxDim || longest < kLong) return false;
+  return seqs == 1 ? rows >= 2 * kWideRows
+                   : rows >= kWideRows * seqs && rows / kWideRows * heads >= kUnits;
 }
 
 // Shapes the launch of a batch whose longest query has `most_new` rows and longest
@@ -149,7 +168,8 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
   if (!all_few) {
     const uint64_t rows = p->num_rows * group;
     const uint64_t seqs = p->num_seqs < p->num_rows ? p->num_seqs : p->num_rows;
-    const uint64_t tiles = seqs > 1 ? rows / kManyRows + seqs : ceil_div(rows, kManyRows);
+    const uint64_t many = wide_tiles(seqs, rows, heads, dim, longest) ? kWideRows : kManyRows;
+    const uint64_t tiles = seqs > 1 ? rows / many + seqs : ceil_div(rows, many);
     // The tiles that fill the chip, once or more, are passed over whole; those left over
     // are split among the workgroups that it holds at once, where they are long enough for
     // their join: the last tiles are those of the first rows, which attend little more than
@@ -157,11 +177,11 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
     // 1,627 (2,048 rows: 1,095); behind 4,000 216 and 251, 2,000 148 and 151, 1,000 107
     // and 99; seven times 300 behind 10,000 435 and 595.
     constexpr uint64_t kSplitCached = 2048;
-    const uint64_t slots = kCus * (dim <= 128 ? 2 : 1);
+    const uint64_t slots = kCus * (dim <= 128 && many == kManyRows ? 2 : 1);
     uint64_t whole = tiles * heads / slots * slots / heads;
     if (whole && longest < most_new + kSplitCached) whole = tiles;
     const uint64_t units = (tiles - whole) * heads;
-    const uint64_t slot = kManyRows * (dim * 4 + 16);
+    const uint64_t slot = many * (dim * 4 + 16);
     const uint64_t want = units && units < slots ? slots / units : 1;
     uint64_t piece = ceil_div(ceil_div(longest, want), 64) * 64;
     if (piece < 256) piece = 256;
@@ -172,12 +192,13 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
       piece = ceil_div(ceil_div(longest, splits), 64) * 64;
     }
     if (splits == 1) whole = tiles;
+    p->many_rows = static_cast<uint32_t>(many);
     p->many_whole = static_cast<uint32_t>(whole);
     p->many_units = static_cast<uint32_t>(tiles);
     p->many_splits = static_cast<uint32_t>(splits);
     p->many_piece = static_cast<uint32_t>(piece);
     if (splits > 1) {
-      const uint64_t n = units * splits * kManyRows;
+      const uint64_t n = units * splits * many;
       p->many_o = reinterpret_cast<float*>(at);
       p->many_ml = reinterpret_cast<float*>(at + n * dim * 4);
     }

@@ -57,7 +57,7 @@ void any_batch() {
     const uint64_t n = std::min(left, i % 2 ? bound : pick(1, bound));
     left -= n;
     if (n * p.group > p.few_rows && p.many_units)
-      tiles += (n * p.group + kManyRows - 1) / kManyRows;
+      tiles += (n * p.group + p.many_rows - 1) / p.many_rows;
     else if (n * p.group <= kFewRows)
       ++few;
     else
@@ -81,9 +81,9 @@ void any_batch() {
     const uint64_t shares = static_cast<uint64_t>(p.many_units - p.many_whole) * p.pages.heads *
                             p.many_splits;
     EXPECT(reinterpret_cast<uint64_t>(p.many_o) == at && at % 16 == 0);
-    EXPECT(reinterpret_cast<uint64_t>(p.many_ml) == at + shares * kManyRows * dim * 4);
+    EXPECT(reinterpret_cast<uint64_t>(p.many_ml) == at + shares * p.many_rows * dim * 4);
     // A wave's 64 lanes each hold a maximum and a sum: two lanes a row.
-    EXPECT(at + shares * kManyRows * (dim * 4 + 16) <= ws + bytes);
+    EXPECT(at + shares * p.many_rows * (dim * 4 + 16) <= ws + bytes);
     EXPECT(p.many_piece % 64 == 0 && p.many_piece >= 64);
   }
   if (!bytes) EXPECT(p.few_splits <= 1 && p.many_whole == p.many_units);
@@ -91,24 +91,26 @@ void any_batch() {
 
 void rules() {
   const uint64_t ws = 1ull << 40, bytes = 64ull << 20;
-  AttendParams p = batch(1, 500, 8, 128, 4, 10500);  // 128 workgroups: four shares each
+  AttendParams p = batch(1, 500, 8, 128, 4, 10500);  // 64 workgroups: four shares each
   plan_attend(&p, 500, 10500, ws, bytes);
-  EXPECT(p.many_units == 16 && p.many_whole == 0 && p.many_splits == 4);
-  p = batch(1, 2048, 8, 128, 4, 32048);  // 512: whole
+  EXPECT(p.many_rows == 256 && p.many_units == 8 && p.many_whole == 0 && p.many_splits == 4);
+  p = batch(1, 2048, 8, 128, 4, 32048);  // 256: whole
   plan_attend(&p, 2048, 32048, ws, bytes);
-  EXPECT(p.many_units == 64 && p.many_whole == 64);
-  p = batch(1, 2100, 8, 128, 4, 32100);  // 16 more: split among as many
+  EXPECT(p.many_units == 32 && p.many_whole == 32);
+  p = batch(1, 2100, 8, 128, 4, 32100);  // 8 more: split among as many
   plan_attend(&p, 2100, 32100, ws, bytes);
-  EXPECT(p.many_units == 66 && p.many_whole == 64 && p.many_splits == 32);
-  p = batch(1, 2100, 8, 128, 4, 3100);  // not worth a join
+  EXPECT(p.many_units == 33 && p.many_whole == 32 && p.many_splits == 32);
+  p = batch(1, 2100, 8, 128, 4, 3100);  // shorter: narrow tiles, not worth a join
   plan_attend(&p, 2100, 3100, ws, bytes);
-  EXPECT(p.many_whole == 66);
+  EXPECT(p.many_rows == 128 && p.many_units == 66 && p.many_whole == 66);
   p = batch(1, 2100, 8, 128, 4, 32100);  // no workspace
   plan_attend(&p, 2100, 32100, 0, 0);
-  EXPECT(p.many_whole == 66);
+  EXPECT(p.many_whole == 33);
   p = batch(1, 1100, 8, 256, 4, 9100);  // one workgroup a compute unit
   plan_attend(&p, 1100, 9100, ws, bytes);
-  EXPECT(p.many_units == 35 && p.many_whole == 32 && p.many_splits > 1);
+  EXPECT(p.many_rows == 128 && p.many_units == 35 && p.many_whole == 32 && p.many_splits > 1);
+  EXPECT(wide_tiles(16, 16384, 8, 128, 4500) && !wide_tiles(16, 16383, 8, 128, 4500));
+  EXPECT(!wide_tiles(65, 16384, 64, 128, 4500) && wide_tiles(64, 16384, 64, 128, 4500));
   EXPECT(few_piece(8, 10001) < 1024 && few_piece(384, 1000) == 1000);
 }
 

@@ -345,6 +345,31 @@ def test_tiles_left_over_are_split(gpu, workspace, form, group, new, cached):
         b.check(*b.run(workspace=w, tail=1), every=37)
 
 
+@pytest.mark.parametrize("options", [{}, {"window": 3990}, {"causal": False}], ids=str)
+@pytest.mark.parametrize("form,group", [
+    (LLAMA, 4), (FORMS[2], 4), (FORMS[4], 5), (FORMS[5], 1), (FORMS[1], 1), (FORMS[8], 2),
+    (("e4m3", "bf16", 2, 64, 16, False), 1), (("int8", "fp16", 2, 48, 16, False), 3)], ids=str)
+def test_wide_tiles(gpu, workspace, form, group, options):
+    """Many rows of a long sequence, in tiles of 256: full ones and one of a few rows."""
+    b = Batch([530 // group + 1], [4000], form, group, seed=18, holes=True)
+    for w in (workspace, None):
+        b.check(*b.run(workspace=w, tail=2, **options), every=23, **options)
+
+
+def test_wide_tiles_of_several_sequences(gpu, workspace):
+    """Wide tiles beside a single token and a short chunk, the last ones in shares."""
+    form = ("fp16", "fp16", 64, 16, 16, False)
+    b = Batch([1500, 1, 700, 9], [4200, 3000, 2900, 2800], form, 1, seed=19)
+    for w in (workspace, None):
+        b.check(*b.run(workspace=w, front=1), every=41)
+    b = Batch([1500, 620], [4200, 2900], form, 1, seed=20)
+    bs = b.pages.block_size
+    for t, kv, bad in ((4300, 1, NAN16), (5000, 1, INF16), (5600, 0, NAN16)):
+        b.pages.values()[kv, b.table[0][t // bs], t % bs, :, 3] = bad["fp16"]
+    b.dev.upload()
+    b.check(*b.run(workspace=workspace), every=41)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 1 << 31])
 @pytest.mark.parametrize("form,group", [(LLAMA, 4), (FORMS[4], 5)], ids=str)
 def test_window(gpu, workspace, form, group, window):
