@@ -927,10 +927,12 @@ __global__ void __launch_bounds__(64) attend_many_join_kernel(AttendParams a) {
 // the shares of a split sequence in the workgroup that finishes last.
 //
 // 64 sequences of up to 16,000 e4m3 tokens (8 heads of 128, 1.03 GB) take 227 us, 4.5
-// TB/s where a large copy moves 5.2.  Smaller batches are latency: 32 sequences behind
-// 1,000 fp16 tokens (12 heads of 64) 16 us, of which each 32 tokens of a wave take 1.2;
-// one behind 10,000 (8 heads of 128) 17.5, 12.6 of them the pass and 5 the join.  Eight
-// waves a workgroup, or tokens under way two tiles ahead (16.1 -> 17.5), gained nothing.
+// TB/s where a large copy moves 5.2.  32 sequences behind 1,000 fp16 tokens (12 heads of
+// 64, 57 MB) take 16, of which the memory works some 10 and the rest is the start, the
+// first loads and the end; one behind 10,000 (8 heads of 128, 41 MB) 16, 12.8 of them the
+// pass and 3.2 the join (4.5 where a share's values were not asked for before its factor
+// was known).  Eight waves a workgroup, or tokens under way two tiles ahead (16.1 ->
+// 17.5), gained nothing.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kFewWaves = 4, kFewThreads = kFewWaves * 64;
 constexpr uint32_t kFewTokens = 32;
@@ -978,7 +980,7 @@ attend_few_kernel(AttendParams a) {
   const int32_t* table = a.block_table + seq * a.table_stride;
   // Without a window a share starts at a token known from here on: a launch that is all
   // latency asks for its first block beside the sequence's length (a token behind 10,000
-  // 18.8 -> 18.0 us; where shares wait for their turn it costs 2%).
+  // gains 0.8 us; where shares wait for their turn it costs 2%).
   const bool ask_early = !a.window && gridDim.x <= 512;
   int32_t early_block = -1;
   if (ask_early)
@@ -1332,41 +1334,61 @@ attend_few_kernel(AttendParams a) {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   const uint64_t slot0 = static_cast<uint64_t>(seq) * a.few_splits * pg.heads + head;
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.few_ml);
-  // Each share's factor exp(m - largest m), of every row, and the rows' sums.
-  static_assert(sizeof(lds) >= kFewMaxSplits * 64 + kFewThreads * 16, "factors and sums fit");
-  float* factor = reinterpret_cast<float*>(lds);  // [used][16]
-  for (uint32_t r = wave; r < rows; r += kFewWaves) {
-    float m_s = kNegInf, l_s = 0.0f;
-    float largest = kNegInf;
-    for (uint32_t s = lane; s < used; s += 64)
-      largest = fmaxf(largest, ml[(slot0 + s * pg.heads) * a.few_rows_most + r][0]);
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) largest = fmaxf(largest, __shfl_xor(largest, step));
-    float sum = 0.0f;
-    for (uint32_t s = lane; s < used; s += 64) {
-      const f32x2 y = ml[(slot0 + s * pg.heads) * a.few_rows_most + r];
-      m_s = y[0];
-      l_s = y[1];
-      // A share without a maximum attended nothing, or only what is no number.
-      const float f = m_s == kNegInf ? (l_s == 0.0f ? 0.0f : 1.0f)
-                                     : __builtin_amdgcn_exp2f((m_s - largest) * a.scale_log2);
-      factor[s * 16 + r] = f;
-      sum += l_s * f;
-    }
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) sum += __shfl_xor(sum, step);
-    if (lane == 0) {
-      join_m[0][r] = largest;
-      join_l[0][r] = sum;
-    }
-  }
-  __syncthreads();
   // 4 values an item; where there are fewer items than threads, groups of threads share
   // the splits out and add up in LDS.
   const uint32_t items = rows * (DP / 4);
   uint32_t groups = 1;
   while (groups * 2 * items <= kFewThreads) groups *= 2;
   const uint32_t group = tid / items;
+  const uint64_t stride = static_cast<uint64_t>(pg.heads) * a.few_rows_most * DP;
+  const uint32_t first = groups > 1 ? group : 0;
+  auto part = [&](uint32_t i, uint32_t s) {
+    return *reinterpret_cast<const f32x4*>(a.few_o + (slot0 * a.few_rows_most + i / (DP / 4)) * DP +
+                                           i % (DP / 4) * 4 + s * stride);
+  };
+  // The first shares' values are under way while their factors are computed.
+  constexpr uint32_t kAhead = 8;
+  const uint32_t item = groups > 1 ? tid - group * items : tid;
+  f32x4 ahead[kAhead];
+#pragma unroll
+  for (uint32_t j = 0; j < kAhead; ++j)
+    if (group < groups && item < items && first + j * groups < used)
+      ahead[j] = part(item, first + j * groups);
+  // Each share's factor exp(m - largest m), of every row, and the rows' sums.
+  static_assert(sizeof(lds) >= kFewMaxSplits * 64 + kFewThreads * 16, "factors and sums fit");
+  float* factor = reinterpret_cast<float*>(lds);  // [used][16]
+  for (uint32_t r = wave; r < rows; r += kFewWaves) {
+    constexpr uint32_t kEach = kFewMaxSplits / 64;
+    f32x2 y[kEach];
+    float largest = kNegInf;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+      const uint32_t s = lane + j * 64;
+      y[j] = f32x2{kNegInf, 0.0f};
+      if (s < used) y[j] = ml[(slot0 + s * pg.heads) * a.few_rows_most + r];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) largest = fmaxf(largest, y[j][0]);
+    // Lanes from `used` on hold nothing.
+    for (uint32_t step = 1; step < 64 && step < used; step *= 2)
+      largest = fmaxf(largest, __shfl_xor(largest, step));
+    float sum = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+      // A share without a maximum attended nothing, or only what is no number.
+      const float f = y[j][0] == kNegInf
+                          ? (y[j][1] == 0.0f ? 0.0f : 1.0f)
+                          : __builtin_amdgcn_exp2f((y[j][0] - largest) * a.scale_log2);
+      if (lane + j * 64 < used) factor[(lane + j * 64) * 16 + r] = f;
+      sum += y[j][1] * f;
+    }
+    for (uint32_t step = 1; step < 64 && step < used; step *= 2) sum += __shfl_xor(sum, step);
+    if (lane == 0) {
+      join_m[0][r] = largest;
+      join_l[0][r] = sum;
+    }
+  }
+  __syncthreads();
   f32x4* sums = reinterpret_cast<f32x4*>(factor + used * 16);
   for (uint32_t i0 = 0; i0 < items; i0 += kFewThreads) {
     const uint32_t i = groups > 1 ? tid - group * items : i0 + tid;
@@ -1374,16 +1396,18 @@ attend_few_kernel(AttendParams a) {
     const bool mine = groups > 1 ? group < groups : i < items;
     f32x4 x{0, 0, 0, 0};
     if (mine) {
-      const float* part = a.few_o + (slot0 * a.few_rows_most + r) * DP + d;
-      const uint64_t stride = static_cast<uint64_t>(pg.heads) * a.few_rows_most * DP;
-      const uint32_t first = groups > 1 ? group : 0;
-#pragma unroll 8
-      for (uint32_t s = first; s < used; s += groups) {
-        const f32x4 y = *reinterpret_cast<const f32x4*>(part + s * stride);
+      auto add = [&](uint32_t s, f32x4 y) {
         const float f = factor[s * 16 + r];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] += y[j] * f;
-      }
+      };
+      uint32_t s = first;
+      if (i0 == 0)
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j, s += groups)
+          if (s < used) add(s, ahead[j]);
+#pragma unroll 8
+      for (; s < used; s += groups) add(s, part(i, s));
     }
     if (groups > 1) {
       if (mine) sums[tid] = x;

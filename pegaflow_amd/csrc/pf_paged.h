@@ -89,14 +89,15 @@ inline uint32_t padded_dim(uint32_t dim) {
 // `longest` tokens.  (Measured with 128 values a head, 4 rows, in us.)
 //
 // The chip holds 512 of its workgroups at once, and a launch of a few more than that
-// takes twice as long: 384 units of up to 1,000 tokens whole 15.9, in two shares 24.4; 512
-// of 2,000 whole 55.6, in two 70.5; 128 of 4,000 in 2, 4 and 8 shares 56.0, 57.3 and 64.7.
+// takes twice as long: 384 units of 1,000 tokens whole 45.0, in two shares 55.2; 512 of
+// 2,000 whole 97.3, in two 108.3; 128 of 4,000 in 2, 4 and 8 shares 55.4, 56.5 and 59.8.
 // Many launches' worth of shares, though, even out lengths that the host does not
-// know: 512 of up to 16,000 tokens, on average half, in shares of 1,024 tokens 216, of
-// 8,192 278.  Where units are few, a share of s tokens takes about 7.5 ns a token and
-// the join 280 ns a share, so shares of sqrt(37 * longest) are best: one sequence of
-// 10,000 tokens and 8 heads in shares of 256, 512, 1,024 and 2,048 takes 21.3, 17.6, 19.9
-// and 27.6; of 30,000 (8-bit) 37.5, 27.2, 22.3 and 26.2; of 3,000 13.3, 14.8, 18.5 and 22.4.
+// know: 512 of up to 16,000 tokens, on average half, in shares of 1,024 tokens 226, of
+// 8,192 277.  Where units are few, a share of s tokens takes about 7.5 ns a token and
+// the join 200 to 280 ns a share, so shares of sqrt(37 * longest) are best: one sequence
+// of 10,000 tokens and 8 heads in shares of 256, 512, 1,024 and 2,048 takes 20.5, 16.1,
+// 18.7 and 27.1; of 30,000 (8-bit) 36.7, 26.0, 20.9 and 24.1; of 3,000 12.0, 14.2, 18.1
+// and 22.4.
 inline uint64_t few_piece(uint64_t units, uint64_t longest) {
   constexpr uint64_t kSlots = 512, kEven = 1024;
   if (units * longest >= 4 * kSlots * kEven) return kEven;
