@@ -51,20 +51,25 @@ def _row_type(dtype) -> int:
 
 def _rows(x, heads: int | None, dim: int, what: str):
     """(KVRows, tokens, heads) of a [tokens, heads, head_dim] tensor."""
-    shape, stride = x.shape, x.stride()
+    shape = x.shape
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} is [tokens, {heads or 'heads'}, {dim}], got {tuple(shape)}")
-    if stride[2] != 1:
-        raise ValueError(f"{what}: the values of a row are not neighbours (stride {stride[2]})")
-    return (KVRows(x.data_ptr(), stride[0], stride[1], _row_type(x.dtype), 0), shape[0], shape[1])
+    by_token, by_head, by_value = x.stride()
+    if by_value != 1:
+        raise ValueError(f"{what}: the values of a row are not neighbours (stride {by_value})")
+    t = _row_types.get(x.dtype) or _row_type(x.dtype)
+    return KVRows(x.data_ptr(), by_token, by_head, t), shape[0], shape[1]
 
 
-_INDEX = {"torch.int32": "int32", "torch.int64": "int64", "int32": "int32", "int64": "int64"}
+_index_types: dict = {}  # a tensor's dtype -> its name
 
 
 def _index(x, dims: int, dtype: str, what: str):
     shape = x.shape
-    if len(shape) != dims or _INDEX.get(str(x.dtype)) != dtype:
+    name = _index_types.get(x.dtype)
+    if name is None:
+        name = _index_types[x.dtype] = _name(x.dtype)
+    if len(shape) != dims or name != dtype:
         raise ValueError(f"{what} is a {dims}-dimensional {dtype} tensor, got "
                          f"{tuple(shape)} of {x.dtype}")
     if shape[-1] > 1 and x.stride()[-1] != 1:
