@@ -267,9 +267,10 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   while (p.unit_shift < 4 && !(pv.block_size >> p.unit_shift & 1u)) ++p.unit_shift;
   plan_attend(&p, a->max_query_len, a->max_seq_len, ws ? ws->data : 0, ws ? ws->bytes : 0);
   const uint64_t left = p.many_units - p.many_whole;
-  const uint64_t grid =
-      std::max<uint64_t>(static_cast<uint64_t>(p.num_seqs) * p.few_splits,
-                         std::max(p.many_whole + left * p.many_splits, left * p.many_rows / 32)) * pv.heads;
+  const uint64_t grid = std::max({static_cast<uint64_t>(p.num_seqs) * p.few_splits,
+                                  p.many_whole + left * p.many_splits,
+                                  left * (p.many_rows / 32) * (padded_dim(pv.dim) / 32)}) *
+                        pv.heads;
   if (grid > 0x7fffffffull) return invalid("too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
