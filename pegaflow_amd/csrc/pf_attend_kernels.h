@@ -870,20 +870,28 @@ attend_many_kernel(AttendParams a) {
   reinterpret_cast<f32x2*>(a.many_ml)[(slot * kWaves + wave) * 64 + lane] = f32x2{m, l};
 }
 
-// Joins the shares of split tiles.  A workgroup takes 32 rows and 32 values of each, in the
-// lanes that held them; its 4 waves go through the shares in turn, and join in LDS.  (One
-// wave for the rows' whole outputs: 20 rows of 32 heads behind 10,000 tokens, 40 shares of
-// 256, took 48.7 us, now 27.4.)
+// Joins the shares of split tiles.  A wave takes 32 rows and 32 values of each, in the
+// lanes that held them.  Of more than kJoinFew shares (TURNS) the 4 waves of a workgroup
+// take turns and join in LDS: 20 rows of 32 heads behind 2,000 tokens, in 8 shares, 17.8
+// us and otherwise 22.2; behind 10,000, in 40, 27.3 (48.7 where a wave joined the rows'
+// whole outputs).  Of few shares each wave takes other values, in a quarter of the
+// workgroups: 500 rows behind 10,000, in 4 shares, 9.1 us of this kernel and otherwise 10.7.
 constexpr uint32_t kJoinThreads = 256;
-template <class Row, uint32_t DP, uint32_t ROWS>
+constexpr uint32_t kJoinFew = 4;
+// Workgroups of 32 rows.
+constexpr uint32_t join_parts(uint32_t dp, bool turns) {
+  return turns ? dp / 32 : (dp / 32 + 3) / 4;
+}
+template <class Row, uint32_t DP, uint32_t ROWS, bool TURNS>
 __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendParams a) {
-  constexpr uint32_t kWaves = ROWS / 32, kParts = DP / 32, kStep = kJoinThreads / 64;
-  __shared__ f32x4 join_o[kStep][4][64];
-  __shared__ f32x2 join_ml[kStep][64];
+  constexpr uint32_t kWaves = ROWS / 32, kJoinWaves = kJoinThreads / 64;
+  __shared__ f32x4 join_o[kJoinWaves][4][64];
+  __shared__ f32x2 join_ml[kJoinWaves][64];
   const PagedView& pg = a.pages;
   const uint32_t lane = threadIdx.x & 63u, mine = threadIdx.x >> 6, half = lane >> 5;
-  const uint32_t dt = blockIdx.x % kParts, wave = blockIdx.x / kParts % kWaves;
-  const uint32_t rest = blockIdx.x / kParts / kWaves;
+  constexpr uint32_t kParts = join_parts(DP, TURNS), kStep = TURNS ? kJoinWaves : 1;
+  const uint32_t dt = TURNS ? blockIdx.x % kParts : blockIdx.x % kParts * kJoinWaves + mine;
+  const uint32_t wave = blockIdx.x / kParts % kWaves, rest = blockIdx.x / kParts / kWaves;
   const uint32_t head = rest % pg.heads, left = rest / pg.heads;
   ManyTile t;
   if (!many_tile<ROWS>(a, a.many_whole + left, head, wave, &t)) return;
@@ -896,9 +904,11 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
   };
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.many_ml) + lane;
   const f32x4* part = reinterpret_cast<const f32x4*>(a.many_o) + dt * 4 * 64 + lane;
+  if (!TURNS && dt >= DP / 32) return;
+  const uint32_t first = TURNS ? mine : 0;
   float m = kNegInf, l = 0.0f;
 #pragma unroll 4
-  for (uint32_t s = mine; s < used; s += kStep) m = fmaxf(m, ml[slot(s) * 64][0]);
+  for (uint32_t s = first; s < used; s += kStep) m = fmaxf(m, ml[slot(s) * 64][0]);
   // A share without a maximum attended nothing, or only what is no number (l is NaN).
   auto factor = [&](f32x2 x, float top) {
     return x[0] == kNegInf ? (x[1] == 0.0f ? 0.0f : 1.0f)
@@ -908,7 +918,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = f32x4{0, 0, 0, 0};
 #pragma unroll 4
-  for (uint32_t s = mine; s < used; s += kStep) {
+  for (uint32_t s = first; s < used; s += kStep) {
     const f32x2 x = ml[slot(s) * 64];
     const float keep = factor(x, m);
     l += x[1] * keep;
@@ -919,16 +929,28 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
       for (int j = 0; j < 4; ++j) o[i][j] += y[j] * keep;
     }
   }
+  auto store = [&](uint32_t i, f32x4 x, float sum) {
+    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+    store_out4<Row>(row_address(a, a.out, t), dt * 32 + 8 * i + 4 * half, a,
+                    f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
+  };
+  if constexpr (!TURNS) {
+    if (!t.valid) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store(i, o[i], l);
+    if (dt == 0) many_lse(a, t, m, l);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) join_o[mine][i][lane] = o[i];
   join_ml[mine][lane] = f32x2{m, l};
   __syncthreads();
   float top = kNegInf, sum = 0.0f;
 #pragma unroll
-  for (uint32_t w = 0; w < kStep; ++w) top = fmaxf(top, join_ml[w][lane][0]);
+  for (uint32_t w = 0; w < kJoinWaves; ++w) top = fmaxf(top, join_ml[w][lane][0]);
   f32x4 x{0, 0, 0, 0};
 #pragma unroll
-  for (uint32_t w = 0; w < kStep; ++w) {
+  for (uint32_t w = 0; w < kJoinWaves; ++w) {
     const f32x2 y = join_ml[w][lane];
     const float keep = factor(y, top);
     sum += y[1] * keep;
@@ -936,9 +958,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
     for (int j = 0; j < 4; ++j) x[j] += join_o[w][mine][lane][j] * keep;
   }
   if (!t.valid) return;
-  const float inv = sum == 0 ? 0.0f : 1.0f / sum;
-  store_out4<Row>(row_address(a, a.out, t), dt * 32 + 8 * mine + 4 * half, a,
-                  f32x4{x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv});
+  store(mine, x, sum);
   if (dt == 0 && mine == 0) many_lse(a, t, top, sum);
 }
 
@@ -1454,10 +1474,13 @@ void launch_many(const AttendParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((attend_many_kernel<Row, TYPE, DP, ROWS>),
                      dim3((p.many_whole + left * p.many_splits) * p.pages.heads), dim3(2 * ROWS), 0,
                      stream, p);
-  if (left)
-    hipLaunchKernelGGL((attend_many_join_kernel<Row, DP, ROWS>),
-                       dim3(left * p.pages.heads * (ROWS / 32) * (DP / 32)), dim3(kJoinThreads),
-                       0, stream, p);
+  if (!left) return;
+  const bool turns = p.many_splits > kJoinFew;
+  const dim3 grid(left * p.pages.heads * (ROWS / 32) * join_parts(DP, turns)), block(kJoinThreads);
+  if (turns)
+    hipLaunchKernelGGL((attend_many_join_kernel<Row, DP, ROWS, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((attend_many_join_kernel<Row, DP, ROWS, false>), grid, block, 0, stream, p);
 }
 
 template <class Row, uint32_t TYPE, uint32_t DP>
