@@ -174,10 +174,11 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
     // The tiles that fill the chip, once or more, are passed over whole; those left over
     // are split among the workgroups that it holds at once, where they are long enough for
     // their join: the last tiles are those of the first rows, which attend little more than
-    // what is cached.  2,100 rows of 32 heads behind 30,000 tokens take 1,156 us, whole
-    // 1,627 (2,048 rows: 1,095); behind 4,000 216 and 251, 2,000 148 and 151, 1,000 107
-    // and 99; seven times 300 behind 10,000 435 and 595.
-    constexpr uint64_t kSplitCached = 2048;
+    // what is cached.  2,100 rows of 32 heads behind 30,000 tokens took 1,156 us, whole
+    // 1,627 (2,048 rows: 1,095); behind 4,000 216 and 251, 1,500 122 and 122, 1,000 106 and
+    // 100; seven times 300 (8-bit) behind 10,000 435 and 595, 1,900 115 and 140; 2,500
+    // behind 1,900 176 and 169.
+    constexpr uint64_t kSplitCached = 1536;
     const uint64_t slots = kCus * (dim <= 128 && many == kManyRows ? 2 : 1);
     uint64_t whole = tiles * heads / slots * slots / heads;
     if (whole && longest < most_new + kSplitCached) whole = tiles;
