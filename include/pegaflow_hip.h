@@ -641,7 +641,8 @@ int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* 
  * stay as they were.  A length beyond the table is cut to it.
  *
  * Scores, softmax statistics and sums are held in fp32; the weights are rounded
- * to 16 bits, the type of the rows, for the product with V. */
+ * to 16 bits, the type of the rows, for the product with V (to twice as many where a
+ * sequence has at most 16 rows of a KV head). */
 typedef struct pf_attend_args {
   pf_kv_rows q;          /* [num_rows, num_q_heads, head_dim] */
   pf_kv_rows out;        /* the same shape and type; may not overlap q */

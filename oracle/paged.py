@@ -132,10 +132,11 @@ def _put(pages, which, b, t, x):
 
 
 def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, weights=None,
-           every=1):
+           every=1, fine=()):
     """(out, lse, bound, lse bound) in 64 bits of query bits [n, heads, dim]: bound is how far each output
     of a kernel may be off that holds scores, statistics and sums in 32 bits, rounds each weight
     to ``weights`` and the output to ``rows``.  Only every ``every``-th row is computed.
+    Of the sequences in ``fine`` a weight is two such numbers, the second the rounding of the first.
 
     A weight's rounding and the errors below scale with A = sum w |v| / sum w.  A score's
     32-bit sum of dim products is off by (dim + 4) half-steps of sum |q k| scale at most, the
@@ -180,7 +181,8 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
                     lse[r, h] = m + np.log(l)
                     size = (w @ np.abs(v)) / l
                 off = 2 * dz + 2.0 ** -20 + 2 * (len(z) + 8) * u
-                bound[r, h] = size * (HALF_STEP[weights or rows] + off) + (
+                step = HALF_STEP[weights or rows] ** (2 if i in fine else 1)
+                bound[r, h] = size * (step + off) + (
                     HALF_STEP[rows] * np.abs(out[r, h]) + 2.0 ** -24)
                 if (weights or rows) == "fp16":
                     least = 2.0 ** -25 * np.abs(v).sum(0)

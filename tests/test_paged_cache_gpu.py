@@ -251,7 +251,8 @@ class Batch:
     def check(self, got, lse, causal=True, window=0, scale=None, every=1, **kw):
         out, want_lse, bound, lse_bound = (x[::every] for x in oracle.attend(
             self.pages, self.q, self.rows, self.table, self.lens, self.starts,
-            scale or self.scale, causal, window, every=every))
+            scale or self.scale, causal, window, every=every,
+            fine=np.flatnonzero(np.diff(self.starts) * self.group <= 16)))
         x = oracle.from_bits(got, self.rows).astype(np.float64)[::every]
         lse = None if lse is None else lse[::every]
         assert np.array_equal(np.isnan(x), np.isnan(out))
