@@ -37,10 +37,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) uint8_t l_u8;
-typedef __attribute__((address_space(3))) u32x4 l_u32x4;
 typedef __attribute__((address_space(3))) s16x4 l_s16x4;
-typedef __attribute__((address_space(3))) f32x4 l_f32x4;
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_inff();
@@ -688,7 +685,6 @@ attend_many_kernel(AttendParams a) {
   auto step = [&](int32_t t0, uint32_t n, bool masked, uint64_t hole) {
     __builtin_amdgcn_s_setprio(1);  // ahead of the other workgroup's softmax
     scores(n);
-    //prio0
     read_v(n + 1, 0, vf[0]);  // the buffer of tile n - 1
     if (masked) {
       // Bit j of `seen`: this half's token j, of 64, is attended; its scores are tokens
