@@ -200,9 +200,10 @@ __device__ __forceinline__ float lower_lift(float big, float* lift, float* limit
   return __builtin_amdgcn_exp2f(*lift - old);
 }
 
-// V in a tile that some row attends only in part: a weight of 0 must not meet an
-// infinity or NaN, so those values are taken as zero, and the tile's caller returns for
-// them at the end (add_odd).  Returns whether there were any among these 16 bytes.
+// V in a tile that some row attends only in part, or that has tokens without a block: a
+// weight of 0 must not meet an infinity or NaN, so those values are taken as zero, and the
+// tile's caller returns for them at the end (add_odd).  Returns whether there were any among
+// these 16 bytes.
 template <class Row, uint32_t TYPE>
 __device__ __forceinline__ bool clear_odd(u32x4& v) {
   if constexpr (TYPE == PF_KV_INT8) return false;
@@ -291,6 +292,25 @@ __device__ __forceinline__ bool token_at(const PagedView& p, int32_t block, uint
   *at = base + off * p.token_bytes + h * p.head_bytes;
   *scale_at = base + p.scale_offset + (h * p.block_size + off) * 4u;
   return static_cast<uint32_t>(block) < p.num_blocks;
+}
+
+// The tokens t0 to t0 + 63 under `end` that have a block and hold V that is not finite, as
+// bits: each lane looks at one.
+template <class Row, uint32_t TYPE>
+__device__ __forceinline__ uint64_t odd_tokens(const PagedView& p, const int32_t* table,
+                                               uint32_t head, int32_t t0, int32_t end) {
+  const int32_t tok = t0 + static_cast<int32_t>(threadIdx.x & 63u);
+  bool odd = false;
+  if (tok < end) {
+    uint64_t at, scale_at;
+    const uint32_t page = page_of(p, tok);
+    if (token_at(p, table[page], tok, page, head, &at, &scale_at))
+      for (uint32_t d = 0; d < p.dim * (is_codes(TYPE) ? 1 : 2); d += 16) {
+        u32x4 v = *reinterpret_cast<const g_u32x4*>(p.v + at + d);
+        odd |= clear_odd<Row, TYPE>(v);
+      }
+  }
+  return __ballot(odd);
 }
 
 // ---------------------------------------------------------------------------
@@ -836,24 +856,26 @@ attend_many_kernel(AttendParams a) {
       for (int i = 0; i < 16; ++i) o[dt][i] *= down;
   }
   __syncthreads();
-  if (lds.odd)
-    for (int32_t tok = begin; tok < end; ++tok) {
-      if (tok < my_begin || tok >= my_end) continue;
-      const int32_t t0 = tok & ~(kStep - 1);
-      if (t0 >= all_begin && t0 + kStep <= all_end) continue;
-      uint64_t at, scale_at;
-      const uint32_t page = page_of(pg, tok);
-      if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
+  // Those of every tile: where none was cleared the products have them already, and once
+  // more changes nothing.
+  if (TYPE != PF_KV_INT8 && lds.odd)
+    for (int32_t t0 = begin; t0 < end; t0 += kStep)
+      for (uint64_t left = odd_tokens<Row, TYPE>(pg, table, head, t0, end); left; left &= left - 1) {
+        const int32_t tok = t0 + __builtin_ctzll(left);
+        if (tok < my_begin || tok >= my_end) continue;
+        uint64_t at, scale_at;
+        const uint32_t page = page_of(pg, tok);
+        token_at(pg, table[page], tok, page, head, &at, &scale_at);
 #pragma unroll
-      for (uint32_t dt = 0; dt < DP / 32; ++dt)
+        for (uint32_t dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          float x[4] = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
-          add_odd<Row, TYPE>(pg.v + at, dt * 32 + 8 * i + 4 * half, pg.dim, x);
+          for (uint32_t i = 0; i < 4; ++i) {
+            float x[4] = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+            add_odd<Row, TYPE>(pg.v + at, dt * 32 + 8 * i + 4 * half, pg.dim, x);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
-        }
-    }
+            for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
+          }
+      }
 
   l = sum32(l);
   if (used == 1) {
@@ -1311,22 +1333,24 @@ attend_few_kernel(AttendParams a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[dt][i] *= down;
   }
-  if (__any(odd))
-    for (int32_t tok = begin; tok < end; ++tok) {
-      if ((static_cast<uint32_t>(tok - begin) / kFewTokens) % kFewWaves != wave) continue;
-      if (tok < my_begin || tok >= my_end) continue;
-      const int32_t t1 = tok & ~static_cast<int32_t>(kFewTokens - 1);
-      if (t1 >= all_begin && t1 + static_cast<int32_t>(kFewTokens) <= all_end) continue;
-      uint64_t at, scale_at;
-      const uint32_t page = page_of(pg, tok);
-      if (!token_at(pg, table[page], tok, page, head, &at, &scale_at)) continue;
+  // Those of all of this wave's tiles, as in attend_many_kernel.
+  if (TYPE != PF_KV_INT8 && __any(odd))
+    for (int32_t t1 = begin + static_cast<int32_t>(wave * kFewTokens); t1 < end; t1 += kStep)
+      for (uint64_t left = odd_tokens<Row, TYPE>(
+               pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
+           left; left &= left - 1) {
+        const int32_t tok = t1 + __builtin_ctzll(left);
+        if (tok < my_begin || tok >= my_end) continue;
+        uint64_t at, scale_at;
+        const uint32_t page = page_of(pg, tok);
+        token_at(pg, table[page], tok, page, head, &at, &scale_at);
 #pragma unroll
-      for (uint32_t dt = 0; dt < DP / 16; ++dt) {
-        float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
-        add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
-        o[dt] = f32x4{x[0], x[1], x[2], x[3]};
+        for (uint32_t dt = 0; dt < DP / 16; ++dt) {
+          float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
+          add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
+          o[dt] = f32x4{x[0], x[1], x[2], x[3]};
+        }
       }
-    }
 
   // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
   // LDS (which V no longer needs), and the threads share the sums.
