@@ -241,6 +241,36 @@ __device__ __forceinline__ void add_odd(uint64_t at, uint32_t d, uint32_t dim, f
     o[i] += v[i] - v[i] == 0.0f ? 0.0f : v[i];
 }
 
+// An output that is NaN while its row's sum is a number met an infinity in V: times a weight
+// that 16 bits hold as 0, times the two halves of a weight, of different signs or one of them
+// 0, or with one of the other sign.  Only the values themselves tell which: the output is set to
+// kLost, those values are added (odd_tokens, add_odd), and where none was it is NaN again.
+constexpr float kLost = 3.402823466e38f;
+template <int N, uint32_t COUNT, class V>
+__device__ __forceinline__ bool any_nan(const V (&o)[COUNT]) {
+  // Their sum, by 4 chains: also where two infinities meet, which costs a look in vain.
+  float sum[4] = {o[0][0], o[0][1], o[0][2], o[0][3]};
+#pragma unroll
+  for (uint32_t i = 4; i < COUNT * N; ++i) sum[i % 4] += o[i / N][i % N];
+  return __builtin_isunordered(sum[0] + sum[1], sum[2] + sum[3]);
+}
+template <int N, class V>
+__device__ __forceinline__ void lose_nan(V& o) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = o[i] != o[i] ? kLost : o[i];
+}
+template <int N, class V>
+__device__ __forceinline__ void restore_nan(V& o) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = o[i] == kLost ? __builtin_nanf("") : o[i];
+}
+
+// exp2(x), x <= 0, as the factor of a share in a join: never 0, which an infinity would not
+// survive (and too small to show in a number).
+__device__ __forceinline__ float share_factor(float x) {
+  return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f);
+}
+
 // A sequence of the batch: its first row, its rows, its tokens.  Starts and lengths
 // come from device memory and are bounded here.
 struct Seq {
@@ -856,9 +886,13 @@ attend_many_kernel(AttendParams a) {
       for (int i = 0; i < 16; ++i) o[dt][i] *= down;
   }
   __syncthreads();
+  bool odd = TYPE != PF_KV_INT8 && lds.odd;
+  if constexpr (!kCodes) odd |= __any(t.valid & (l == l) & any_nan<16>(o));
   // Those of every tile: where none was cleared the products have them already, and once
   // more changes nothing.
-  if (TYPE != PF_KV_INT8 && lds.odd)
+  if (__builtin_expect(odd, 0)) {
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt) lose_nan<16>(o[dt]);
     for (int32_t t0 = begin; t0 < end; t0 += kStep)
       for (uint64_t left = odd_tokens<Row, TYPE>(pg, table, head, t0, end); left; left &= left - 1) {
         const int32_t tok = t0 + __builtin_ctzll(left);
@@ -876,6 +910,9 @@ attend_many_kernel(AttendParams a) {
             for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
           }
       }
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt) restore_nan<16>(o[dt]);
+  }
 
   l = sum32(l);
   if (used == 1) {
@@ -937,7 +974,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
   // A share without a maximum attended nothing, or only what is no number (l is NaN).
   auto factor = [&](f32x2 x, float top) {
     return x[0] == kNegInf ? (x[1] == 0.0f ? 0.0f : 1.0f)
-                           : __builtin_amdgcn_exp2f((x[0] - top) * a.scale_log2);
+                           : share_factor((x[0] - top) * a.scale_log2);
   };
   f32x4 o[4];
 #pragma unroll
@@ -1334,7 +1371,10 @@ attend_few_kernel(AttendParams a) {
       for (int i = 0; i < 4; ++i) o[dt][i] *= down;
   }
   // Those of all of this wave's tiles, as in attend_many_kernel.
-  if (TYPE != PF_KV_INT8 && __any(odd))
+  if constexpr (!kCodes) odd |= valid & (l == l) & any_nan<4>(o);
+  if (TYPE != PF_KV_INT8 && __builtin_expect(__any(odd), 0)) {
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 16; ++dt) lose_nan<4>(o[dt]);
     for (int32_t t1 = begin + static_cast<int32_t>(wave * kFewTokens); t1 < end; t1 += kStep)
       for (uint64_t left = odd_tokens<Row, TYPE>(
                pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
@@ -1351,6 +1391,9 @@ attend_few_kernel(AttendParams a) {
           o[dt] = f32x4{x[0], x[1], x[2], x[3]};
         }
       }
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 16; ++dt) restore_nan<4>(o[dt]);
+  }
 
   // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
   // LDS (which V no longer needs), and the threads share the sums.
@@ -1382,7 +1425,7 @@ attend_few_kernel(AttendParams a) {
     for (uint32_t w = 0; w < kFewWaves; ++w) {
       const float mw = join_m[w][r], lw = join_l[w][r];
       const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
-                                       : __builtin_amdgcn_exp2f((mw - top) * a.scale_log2);
+                                       : share_factor((mw - top) * a.scale_log2);
       sum += lw * keep;
       const f32x4 y =
           *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
@@ -1466,7 +1509,7 @@ attend_few_kernel(AttendParams a) {
       // A share without a maximum attended nothing, or only what is no number.
       const float f = y[j][0] == kNegInf
                           ? (y[j][1] == 0.0f ? 0.0f : 1.0f)
-                          : __builtin_amdgcn_exp2f((y[j][0] - largest) * a.scale_log2);
+                          : share_factor((y[j][0] - largest) * a.scale_log2);
       if (lane + j * 64 < used) factor[(lane + j * 64) * 16 + r] = f;
       sum += y[j][1] * f;
     }

@@ -49,3 +49,22 @@ def test_beside_missing_blocks(gpu, workspace, form, group, new, cached):
     b.dev.upload()
     for w in (None, workspace):
         check(b, *b.run(workspace=w))
+
+
+@pytest.mark.parametrize("sharp", [1.0, 20.0, 60.0])
+@pytest.mark.parametrize("form,group", [(LLAMA, 4), (FORMS[1], 1), (FP16_80, 3)], ids=str)
+@pytest.mark.parametrize("new,cached", [((1, 1), (400, 390)), ((100, 30), (400, 350)),
+                                        ((3,), (3000,)), ((40,), (3000,))], ids=str)
+def test_infinities_keep_their_sign(gpu, workspace, form, group, new, cached, sharp):
+    """In tiles that every row attends whole: an infinity stays one however small its weight is,
+    and only two of both signs, or a NaN, make NaN."""
+    b = Batch(new, cached, form, group, seed=41, sharp=sharp)
+    inf, minus = INF16[b.rows], INF16[b.rows] | 0x8000
+    for i in range(len(new)):
+        for token, d, bits in ((40, 0, inf), (75, 1, minus), (41, 2, inf), (300, 2, inf),
+                               (42, 3, inf), (290, 3, minus), (220, 4, NAN16[b.rows]),
+                               (43, 17, minus)):
+            put(b, i, token, 0, d, bits)
+    b.dev.upload()
+    for w in (None, workspace):
+        check(b, *b.run(workspace=w))
