@@ -142,9 +142,10 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
     32-bit sum of dim products is off by (dim + 4) half-steps of sum |q k| scale at most, the
     weight's exponential by that and 2^-21; l and o are sums of n terms, each addition off by
     half a step (n in all; also those of a join), l's errors counted again in the quotient.
-    A weight under fp16's normal range is off by 2^-25 of the largest weight instead; one
-    that carries the scale of a code by 2^-25 of 2^6 times the largest such scale or less,
-    so its products by 2^-31 of that scale times the code."""
+    A weight under fp16's normal range is off by half its smallest step instead, 2^-25, where
+    2^12 stands for the largest weight: by 2^-37 of that; one that carries the scale of a code by
+    2^-25 of 2^6 times the largest such scale or less, so its products by 2^-31 of that scale
+    times the code."""
     n, q_heads, dim = q.shape
     group = q_heads // pages.heads
     out = np.zeros((n, q_heads, dim))
@@ -185,7 +186,7 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
                 bound[r, h] = size * (step + off) + (
                     HALF_STEP[rows] * np.abs(out[r, h]) + 2.0 ** -24)
                 if (weights or rows) == "fp16":
-                    least = 2.0 ** -25 * np.abs(v).sum(0)
+                    least = 2.0 ** -37 * np.abs(v).sum(0)
                     if v_scale is not None:
                         s = v_scale[see, h // group].astype(np.float64)[:, None]
                         with np.errstate(all="ignore"):

@@ -176,6 +176,22 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
   ((x[I] *= of16<FIRST + I>(y)), ...);
 }
 
+// fp16 weights over 16-bit pages are held as 2^12 times what they are, l and the outputs with
+// them: fp16's smallest step is 2^-24, and a weight off by half of it is then off by 2^-37 of
+// its row's largest, so that many small ones keep their sum.  (Held as they are, all under
+// 2^-25 were lost, of 30,000 tokens that far under one the whole output.)  The maximum may lag by
+// 2^3 only, not 2^8, for 2^15 to be the largest.  A lag of 2 and of 1, with a bit more room
+// each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
+constexpr float kFixedLift = 12.0f, kFixedLag = 3.0f;
+
+// The log-sum-exp of a row of maximum m, in units of the raw scores, and sum l.
+template <class Row>
+__device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, float l) {
+  if (l == 0) return kNegInf;
+  const bool lifted = Row::kType == PF_KV_FP16 && !is_codes(a.pages.type);
+  return m * a.scale_log2 * kLn2 + (logf(l) - (lifted ? kFixedLift * kLn2 : 0.0f));
+}
+
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
 // may be anything that 32 bits hold, so all weights of a row, its sum l and its outputs
 // carry a power of two, 2^lift, until the end: with the largest scale that the row has
@@ -466,13 +482,14 @@ __device__ __forceinline__ uint64_t row_address(const AttendParams& a, const Row
                       2;
 }
 
-// The log-sum-exp of this lane's row, where asked for; m is in units of the raw scores.
+// The log-sum-exp of this lane's row, where asked for.
+template <class Row>
 __device__ __forceinline__ void many_lse(const AttendParams& a, const ManyTile& t, float m,
                                          float l) {
   if (!a.lse || !t.valid || (threadIdx.x & 32)) return;
   const uint32_t token = t.row / a.group, g = t.row - token * a.group;
   a.lse[(t.s.first + static_cast<uint64_t>(token)) * a.q_heads + t.head * a.group + g] =
-      l == 0 ? kNegInf : m * a.scale_log2 * kLn2 + logf(l);
+      log_sum_exp<Row>(a, m, l);
 }
 
 // Outputs of this lane's row, o / l, and its log-sum-exp.
@@ -490,7 +507,7 @@ __device__ __forceinline__ void many_store(const AttendParams& a, const ManyTile
       store_out4<Row>(row, dt * 32 + 8 * i + 4 * half, a,
                       f32x4{o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv,
                             o[dt][4 * i + 3] * inv});
-  many_lse(a, t, m, l);
+  many_lse<Row>(a, t, m, l);
 }
 
 template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
@@ -499,6 +516,7 @@ attend_many_kernel(AttendParams a) {
   constexpr uint32_t kThreads = 2 * ROWS, kWaves = ROWS / 32;
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
+  constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
   constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
   // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
   constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
@@ -762,9 +780,9 @@ attend_many_kernel(AttendParams a) {
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tt][i]);
     top = max32(top);
     // The maximum that the weights are taken against follows the largest score only
-    // where that has grown by more than 8 (in powers of 2): until then weights up to
-    // 2^8 serve as well, and the outputs need no rescaling.
-    bool grown = __any((top - m) * a.scale_log2 > 8.0f);
+    // where that has grown by more than 8 (in powers of 2; kFixedLag under a fixed lift): until
+    // then weights up to 2^8 serve as well, and the outputs need no rescaling.
+    bool grown = __any((top - m) * a.scale_log2 > (kFixed ? kFixedLag : 8.0f));
     float keep = 1.0f;
     if (grown) {
       const float m_new = fmaxf(m, top);
@@ -786,6 +804,7 @@ attend_many_kernel(AttendParams a) {
       }
       base += lift;
     }
+    if constexpr (kFixed) base += kFixedLift;
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -1000,7 +1019,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
     if (!t.valid) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) store(i, o[i], l);
-    if (dt == 0) many_lse(a, t, m, l);
+    if (dt == 0) many_lse<Row>(a, t, m, l);
     return;
   }
 #pragma unroll
@@ -1021,7 +1040,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
   }
   if (!t.valid) return;
   store(mine, x, sum);
-  if (dt == 0 && mine == 0) many_lse(a, t, top, sum);
+  if (dt == 0 && mine == 0) many_lse<Row>(a, t, top, sum);
 }
 
 // ---------------------------------------------------------------------------
@@ -1053,8 +1072,7 @@ __device__ __forceinline__ void few_store(const AttendParams& a, const Seq& sq, 
   const uint64_t at = sq.first + static_cast<uint64_t>(token), qh = head * a.group + g;
   store_out4<Row>(a.out.data + (at * a.out.token_stride + qh * a.out.head_stride) * 2, d, a,
                   f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv});
-  if (a.lse && d == 0)
-    a.lse[at * a.q_heads + qh] = l == 0 ? kNegInf : m * a.scale_log2 * kLn2 + logf(l);
+  if (a.lse && d == 0) a.lse[at * a.q_heads + qh] = log_sum_exp<Row>(a, m, l);
 }
 
 template <class Row, uint32_t TYPE, uint32_t DP>
@@ -1062,6 +1080,7 @@ __global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
 attend_few_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
+  constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
   constexpr uint32_t kPer = kCodes ? 16 : 8;
   constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
   constexpr uint32_t kCols = DP / kPer;
@@ -1284,7 +1303,7 @@ attend_few_kernel(AttendParams a) {
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = max32(top);
-    if (__any((top - m) * a.scale_log2 > 8.0f)) {
+    if (__any((top - m) * a.scale_log2 > (kFixed ? kFixedLag : 8.0f))) {
       const float m_new = fmaxf(m, top);
       const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
       m = m_new;
@@ -1312,6 +1331,7 @@ attend_few_kernel(AttendParams a) {
       }
       base += lift;
     }
+    if constexpr (kFixed) base += kFixedLift;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
