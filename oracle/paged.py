@@ -144,7 +144,7 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
     half a step (n in all; also those of a join), l's errors counted again in the quotient.
     A weight under fp16's normal range is off by half its smallest step instead, 2^-25, where
     2^12 stands for the largest weight: by 2^-37 of that; one that carries the scale of a code by
-    2^-25 of 2^6 times the largest such scale or less, so its products by 2^-31 of that scale
+    2^-25 where the largest such scale is 2^11 or more, so its products by 2^-36 of that scale
     times the code."""
     n, q_heads, dim = q.shape
     group = q_heads // pages.heads
@@ -191,7 +191,7 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
                         s = v_scale[see, h // group].astype(np.float64)[:, None]
                         with np.errstate(all="ignore"):
                             codes = np.divide(np.abs(v), s, out=np.zeros_like(v), where=s > 0)
-                            least = 2.0 ** -31 * s.max() * codes.sum(0)
+                            least = 2.0 ** -36 * s.max() * codes.sum(0)
                     bound[r, h] += least / l
                 lse_bound[r, h] = dz + 2.0 ** -21 + (len(z) + 8) * u + 2.0 ** -22 * abs(lse[r, h])
     return out, lse, bound, lse_bound

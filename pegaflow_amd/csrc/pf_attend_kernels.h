@@ -182,37 +182,37 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
 // 2^-25 were lost, of 30,000 tokens that far under one the whole output.)  The maximum may lag by
 // 2^3 only, not 2^8, for 2^15 to be the largest.  A lag of 2 and of 1, with a bit more room
 // each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
-constexpr float kFixedLift = 12.0f, kFixedLag = 3.0f;
+constexpr float kFp16Room = 12.0f, kFp16Lag = 3.0f;
 
 // The log-sum-exp of a row of maximum m, in units of the raw scores, and sum l.
 template <class Row>
 __device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, float l) {
   if (l == 0) return kNegInf;
   const bool lifted = Row::kType == PF_KV_FP16 && !is_codes(a.pages.type);
-  return m * a.scale_log2 * kLn2 + (logf(l) - (lifted ? kFixedLift * kLn2 : 0.0f));
+  return m * a.scale_log2 * kLn2 + (logf(l) - (lifted ? kFp16Room * kLn2 : 0.0f));
 }
 
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
 // may be anything that 32 bits hold, so all weights of a row, its sum l and its outputs
 // carry a power of two, 2^lift, until the end: with the largest scale that the row has
-// attended s 2^lift is at most 2^7, and w, which lags its maximum by at most 2^8, makes
-// 2^15 of it.  A product is then a normal number down to 2^-20 of the largest scale, and
-// off by 2^-31 of that below.  (bf16 weights need none of it, but are off by up to 2^-8
+// attended s 2^lift is at most 2^12, and w, which lags its maximum by at most 2^3, makes
+// 2^15 of it.  A product is then a normal number down to 2^-25 of the largest scale, and
+// off by 2^-36 of that below.  (bf16 weights need none of it, but are off by up to 2^-8
 // where the outputs hold 2^-11.)
-constexpr float kLiftRoom = 7.0f, kLiftStart = 64.0f, kLiftNone = -100.0f;
+constexpr float kLiftStart = 64.0f, kLiftNone = -100.0f;
 // Lowers `lift` (kLiftStart before the first token; kLiftNone for no row) to suit scales
 // up to `big` (or 2^66, so that the factor is a normal number: values as large as that
 // are infinite in fp16), and returns the factor that the row's sums take.  Other rows of
 // the wave have lifts of their own: `limit` is the largest scale that suits them all.
 __device__ __forceinline__ float lower_lift(float big, float* lift, float* limit) {
   const float room =
-      kLiftRoom - static_cast<float>(__builtin_amdgcn_frexp_expf(fminf(big, 0x1p66f)));
+      kFp16Room - static_cast<float>(__builtin_amdgcn_frexp_expf(fminf(big, 0x1p66f)));
   const float old = *lift;
   if (big > 0.0f) *lift = fminf(old, room);
   float most = *lift;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) most = fmaxf(most, __shfl_xor(most, step));
-  *limit = __builtin_amdgcn_exp2f(kLiftRoom - most);
+  *limit = __builtin_amdgcn_exp2f(kFp16Room - most);
   return __builtin_amdgcn_exp2f(*lift - old);
 }
 
@@ -517,6 +517,7 @@ attend_many_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
+  constexpr float kLag = Row::kType == PF_KV_FP16 ? kFp16Lag : 8.0f;
   constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
   // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
   constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
@@ -780,9 +781,9 @@ attend_many_kernel(AttendParams a) {
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tt][i]);
     top = max32(top);
     // The maximum that the weights are taken against follows the largest score only
-    // where that has grown by more than 8 (in powers of 2; kFixedLag under a fixed lift): until
-    // then weights up to 2^8 serve as well, and the outputs need no rescaling.
-    bool grown = __any((top - m) * a.scale_log2 > (kFixed ? kFixedLag : 8.0f));
+    // where that has grown by more than 2^8 (2^3 in fp16): until then weights up to that serve
+    // as well, and the outputs need no rescaling.
+    bool grown = __any((top - m) * a.scale_log2 > kLag);
     float keep = 1.0f;
     if (grown) {
       const float m_new = fmaxf(m, top);
@@ -804,7 +805,7 @@ attend_many_kernel(AttendParams a) {
       }
       base += lift;
     }
-    if constexpr (kFixed) base += kFixedLift;
+    if constexpr (kFixed) base += kFp16Room;
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -1081,6 +1082,7 @@ attend_few_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
+  constexpr float kLag = Row::kType == PF_KV_FP16 ? kFp16Lag : 8.0f;
   constexpr uint32_t kPer = kCodes ? 16 : 8;
   constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
   constexpr uint32_t kCols = DP / kPer;
@@ -1303,7 +1305,7 @@ attend_few_kernel(AttendParams a) {
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = max32(top);
-    if (__any((top - m) * a.scale_log2 > (kFixed ? kFixedLag : 8.0f))) {
+    if (__any((top - m) * a.scale_log2 > kLag)) {
       const float m_new = fmaxf(m, top);
       const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
       m = m_new;
@@ -1331,7 +1333,7 @@ attend_few_kernel(AttendParams a) {
       }
       base += lift;
     }
-    if constexpr (kFixed) base += kFixedLift;
+    if constexpr (kFixed) base += kFp16Room;
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
 #pragma unroll

@@ -10,14 +10,15 @@ from test_paged_cache_gpu import Batch, workspace  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("rows", ["fp16", "bf16"])
+@pytest.mark.parametrize("kind,rows", [("fp16", "fp16"), ("bf16", "bf16"), ("e4m3", "fp16"),
+                                       ("int8", "fp16")])
 @pytest.mark.parametrize("new,cached", [((1,), (30000,)), ((3,), (30000,)), ((40,), (30000,)),
                                         ((1, 40), (5000, 20000))], ids=str)
-def test_one_token_takes_most_of_the_weight(gpu, workspace, rows, new, cached):
+def test_one_token_takes_most_of_the_weight(gpu, workspace, kind, rows, new, cached):
     """A token whose V is 0 lies 15 to 20 above all others in natural units: the outputs are
     the others' share, some 1e-3 and less."""
     dim = 64
-    b = Batch(new, cached, (rows, rows, 1, dim, 16, False), 1, seed=50)
+    b = Batch(new, cached, (kind, rows, 1, dim, 16, False), 1, seed=50)
     rng = np.random.default_rng(51)
     u = rng.choice([-1.0, 1.0], dim)  # q . k of a row below: its gap
     gaps = rng.uniform(15, 20, len(b.q))
