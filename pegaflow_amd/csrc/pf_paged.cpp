@@ -179,10 +179,10 @@ int move_rows(bool write, const pf_kv_pages* pages, const pf_kv_rows* k, const p
   if (int rc = view_pages(pages, ranges, &pv)) return rc;
   if (!k || !v) return invalid("null rows");
   if (k->type != v->type) return invalid("K and V rows differ in type");
-  if (!write && k->data == v->data) return invalid("K and V rows overlap");
   if (is_row_type(pv.type) && is_row_type(k->type) && pv.type != k->type)
     return invalid("16-bit pages hold the rows' own type");
   if (n == 0) return PF_OK;
+  if (!write && k->data == v->data) return invalid("K and V rows overlap");
   if (n >= kMaxTokens) return invalid("too many rows");
   RowsView kv, vv;
   bool aligned = true;
