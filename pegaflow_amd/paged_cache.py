@@ -29,6 +29,7 @@ KV_TYPES = {"bf16": _lib.KV_BF16, "fp16": _lib.KV_FP16, "e4m3": _lib.KV_E4M3,
 _ROW_NAMES = {"bf16": _lib.KV_BF16, "bfloat16": _lib.KV_BF16, "fp16": _lib.KV_FP16,
               "float16": _lib.KV_FP16}
 _row_types: dict = {}  # a tensor's dtype -> PF_KV_*
+_MOST = 2 ** 32 - 1  # of a 32-bit field, which ctypes fills with a number's low bits
 
 
 def lib():
@@ -81,6 +82,9 @@ def segment_bytes(block_size: int, num_kv_heads: int, head_dim: int, kv_type: st
     """Bytes of K (or V) of one block: the values, the scales of 8-bit types, padded
     to 16 (pf_kv_segment_bytes).  A KV-first layer of such blocks is a
     [2, num_blocks, segment_bytes] uint8 tensor."""
+    for n in (block_size, num_kv_heads, head_dim):
+        if not 0 <= n <= _MOST:
+            raise ValueError(f"pages of {block_size} tokens, {num_kv_heads} heads of {head_dim}")
     out = ctypes.c_uint64()
     check(lib().pf_kv_segment_bytes(block_size, num_kv_heads, head_dim, _kv_type(kv_type),
                                     ctypes.byref(out)), "segment_bytes")
@@ -200,9 +204,9 @@ class PagedKVCache:
                 raise ValueError("lse is not contiguous")
             lse_at = lse.data_ptr()
         args = AttendArgs(qr, outr, n, table, block_table.stride()[0], lens, starts, lse_at, heads,
-                          seqs, width, window, causal,
-                          1 / math.sqrt(self.head_dim) if scale is None else scale, max_seq_len,
-                          max_query_len)
+                          seqs, width, min(window, _MOST), causal,
+                          1 / math.sqrt(self.head_dim) if scale is None else scale,
+                          min(max_seq_len, _MOST), min(max_query_len, _MOST))
         check(lib().pf_kv_attend(self._ref, ctypes.byref(args),
                                  workspace.handle if workspace is not None else None,
                                  stream.handle if stream is not None else None), "attend")

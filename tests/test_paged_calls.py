@@ -23,3 +23,53 @@ def test_empty_torch_tensors_do_nothing():
     c = cache()
     c.write(k, v, slots)
     c.read(slots, k, v)
+
+
+class Tensor:
+    """A tensor's face without memory."""
+
+    def __init__(self, shape, dtype):
+        self.shape, self.dtype = shape, dtype
+
+    def stride(self):
+        out = [1]
+        for n in reversed(self.shape[1:]):
+            out.insert(0, out[0] * n)
+        return tuple(out)
+
+    def data_ptr(self):
+        return BASE
+
+
+@pytest.mark.parametrize("value", [0, 7, (1 << 32) - 1, 1 << 32, (1 << 32) + 5, (1 << 63) - 1])
+def test_bounds_past_32_bits_bound_nothing(monkeypatch, value):
+    """A window, a length or a number of rows that 32 bits do not hold is not cut to some other."""
+    from pegaflow_amd import paged_cache
+
+    class Library:
+        def pf_kv_attend(self, pages, args, workspace, stream):
+            seen.append(args._obj)
+            return 0
+
+    seen = []
+    c = cache()
+    monkeypatch.setattr(paged_cache, "lib", Library)
+    c.attend(Tensor((5, 4, 64), "bf16"), Tensor((5, 4, 64), "bf16"), Tensor((2, 4), "int32"),
+             Tensor((2,), "int32"), Tensor((3,), "int32"), window=value, max_seq_len=value,
+             max_query_len=value)
+    a, = seen
+    want = min(value, (1 << 32) - 1)
+    assert (a.window, a.max_seq_len, a.max_query_len) == (want, want, want)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_sizes_past_32_bits_are_refused(at):
+    for value in ((1 << 32) + 16, -16):
+        sizes = [16, 2, 64]
+        sizes[at] = value
+        with pytest.raises(ValueError):
+            segment_bytes(*sizes, "bf16")
+        seg = segment_bytes(16, 2, 64, "bf16")
+        reg = KVCacheRegistration.create(BASE, 20 * seg, 10, seg, 10 * seg, 2)
+        with pytest.raises(ValueError):
+            PagedKVCache(reg, *sizes, "bf16")
