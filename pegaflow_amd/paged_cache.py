@@ -9,8 +9,8 @@ other layer, at half the bytes.
 
 Tensors are torch's, or anything with their ``data_ptr()``, ``shape``,
 ``stride()`` and ``dtype`` (``runtime.DeviceArray``).  Calls are asynchronous on
-``stream`` (None: the current device's null stream, torch's default) and may be
-captured into a graph.  The reference has no counterpart: its blocks are filled and
+``stream`` (None: torch's current stream for torch's tensors, the current device's
+null stream for others) and may be captured into a graph.  The reference has no counterpart: its blocks are filled and
 read by the inference engine.
 """
 
@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
 
 from . import _lib
 from ._lib import AttendArgs, KVPages, KVRows, check
@@ -76,6 +77,19 @@ def _index(x, dims: int, dtype: str, what: str):
     if shape[-1] > 1 and x.stride()[-1] != 1:
         raise ValueError(f"{what}: its last dimension is not contiguous")
     return x.data_ptr()
+
+
+def _stream(stream: Stream | None, x):
+    """The handle of ``stream``, or else of the stream on which torch queues what it does
+    with its tensor ``x``."""
+    if stream is not None:
+        return stream.handle
+    torch = sys.modules.get("torch")
+    if torch is None or not isinstance(x, torch.Tensor) or not x.is_cuda:
+        return None
+    # current_stream() takes 1 to 2 us for its object, this 0.1.
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(x.get_device()) if raw else torch.cuda.current_stream(x.device).cuda_stream
 
 
 def segment_bytes(block_size: int, num_kv_heads: int, head_dim: int, kv_type: str) -> int:
@@ -152,8 +166,7 @@ class PagedKVCache:
         at = _index(slots, 1, "int64", "slots")
         if n != m or slots.shape[0] != n:
             raise ValueError(f"{n} rows of k, {m} of v and {slots.shape[0]} slots")
-        check(fn(self._ref, ctypes.byref(kr), ctypes.byref(vr), at, n,
-                 stream.handle if stream is not None else None), what)
+        check(fn(self._ref, ctypes.byref(kr), ctypes.byref(vr), at, n, _stream(stream, k)), what)
 
     def write(self, k, v, slots, stream: Stream | None = None) -> None:
         """Rows of ``k`` and ``v`` [tokens, kv_heads, head_dim] into ``slots`` (int64,
@@ -209,7 +222,7 @@ class PagedKVCache:
                           min(max_seq_len, _MOST), min(max_query_len, _MOST))
         check(lib().pf_kv_attend(self._ref, ctypes.byref(args),
                                  workspace.handle if workspace is not None else None,
-                                 stream.handle if stream is not None else None), "attend")
+                                 _stream(stream, q)), "attend")
 
 
 __all__ = ["KV_TYPES", "AttentionWorkspace", "PagedKVCache", "segment_bytes"]

@@ -73,3 +73,41 @@ def test_sizes_past_32_bits_are_refused(at):
         reg = KVCacheRegistration.create(BASE, 20 * seg, 10, seg, 10 * seg, 2)
         with pytest.raises(ValueError):
             PagedKVCache(reg, *sizes, "bf16")
+
+
+def test_torch_tensors_run_on_torchs_current_stream(monkeypatch):
+    """Without a stream of the caller's, calls follow what torch has queued on their tensors."""
+    torch = pytest.importorskip("torch")
+    from pegaflow_amd import paged_cache
+    from pegaflow_amd.runtime import Stream
+
+    class OnDevice1(torch.Tensor):
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+
+    def tensor(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype).as_subclass(OnDevice1)
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: seen.append(args[-1]) or 0
+
+    seen = []
+    c = cache()
+    monkeypatch.setattr(paged_cache, "lib", Library)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0x1230 + device,
+                        raising=False)
+    k, q = tensor(5, 2, 64), tensor(5, 4, 64)
+    slots = tensor(5, dtype=torch.int64)
+    batch = [tensor(*s, dtype=torch.int32) for s in ((2, 4), (2,), (3,))]
+    for stream, want in ((None, 0x1231), (Stream(0x77, owned=False), 0x77)):
+        c.write(k, k, slots, stream=stream)
+        c.read(slots, k, k, stream=stream)
+        c.attend(q, q, *batch, stream=stream)
+        assert seen == [want] * 3
+        seen.clear()
+    face = Tensor((5, 2, 64), "bf16")
+    c.write(face, face, Tensor((5,), "int64"))
+    assert seen == [None]
