@@ -566,8 +566,8 @@ int pf_host_wait_word(const uint64_t* word, uint64_t value, uint64_t timeout_us,
 /* Rows are [tokens, heads, head_dim] tensors of 16-bit values; a slot is     */
 /* block * block_size + position in the block.  Every call is asynchronous on */
 /* the caller's stream (NULL: the current device's null stream), allocates    */
-/* nothing and may be captured into a graph.  Tensors must lie on the stream's */
-/* device.                                                                    */
+/* nothing and may be captured into a graph.  Tensors that lie on another      */
+/* device than the stream are refused.                                        */
 /* ------------------------------------------------------------------------ */
 /* What rows and pages hold.  Rows are BF16 or FP16; pages the same type as    */
 /* the rows, or 8-bit codes with an fp32 scale for each token and head.        */

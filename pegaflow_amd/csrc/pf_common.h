@@ -245,11 +245,19 @@ class RangeCache {
   bool check(uint64_t addr, uint64_t len);
   // check, with the bounds of the allocation.
   bool find(uint64_t addr, uint64_t len, uint64_t* begin, uint64_t* end);
+  // Device of the allocation that the last successful check found, -1 for pinned memory
+  // and memory of other processes.
+  int device() const { return last_.device; }
 
  private:
+  struct Allocation {
+    uint64_t begin = 0, end = 0;
+    int device = -1;
+  };
   bool contains(uint64_t addr, uint64_t len);
-  std::vector<std::pair<uint64_t, uint64_t>> ok_;  // [begin, end)
-  uint64_t last_b_ = 0, last_e_ = 0;
+  void found(uint64_t begin, uint64_t end, int device);
+  std::vector<Allocation> ok_;
+  Allocation last_;
 };
 
 // Whether this process's runtime exports interprocess events: 1 yes, 0 no

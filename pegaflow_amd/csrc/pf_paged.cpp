@@ -40,18 +40,36 @@ int segment_bytes(uint32_t block_size, uint32_t heads, uint32_t dim, uint32_t ty
 }
 
 // The ranges that a call's kernels touch: each inside one device or pinned
-// allocation, checked after everything else that the arguments say.
+// allocation, checked after everything else that the arguments say, and on the stream's
+// device (a kernel that reads another device's memory faults).
 class Ranges {
  public:
-  void add(const char* what, uint64_t addr, uint64_t bytes) { list_[n_++] = {what, addr, bytes}; }
-  int check() const {
+  void add(const char* what, uint64_t addr, uint64_t bytes) { list_[n_++] = {what, addr, bytes, -1}; }
+  int check() {
     RangeCache cache;
-    for (int i = 0; i < n_; ++i)
+    for (int i = 0; i < n_; ++i) {
       if (!cache.check(list_[i].addr, list_[i].bytes))
         return invalid(strf("%s: range [0x%llx, +%llu) is not inside one device or pinned "
                             "allocation",
                             list_[i].what, (unsigned long long)list_[i].addr,
                             (unsigned long long)list_[i].bytes));
+      list_[i].device = cache.device();
+    }
+    return PF_OK;
+  }
+  int check_device(int device) const {
+    for (int i = 0; i < n_; ++i) {
+      int at = list_[i].device;
+      if (at < 0) {  // pinned, which every device reads, or another process's
+        hipPointerAttribute_t attr;
+        PF_HIP(hipPointerGetAttributes(&attr, reinterpret_cast<void*>(list_[i].addr)));
+        if (attr.type != hipMemoryTypeDevice) continue;
+        at = attr.device;
+      }
+      if (at != device)
+        return invalid(
+            strf("%s: on device %d, the stream on device %d", list_[i].what, at, device));
+    }
     return PF_OK;
   }
 
@@ -59,6 +77,7 @@ class Ranges {
   struct {
     const char* what;
     uint64_t addr, bytes;
+    int device;
   } list_[8];
   int n_ = 0;
 };
@@ -141,21 +160,18 @@ int add_array(const char* what, uint64_t addr, uint64_t bytes, uint64_t align, R
   return PF_OK;
 }
 
-// Makes the stream's device current while a call launches.  The pages' device
-// must be the stream's (the null stream's is the current one).
+// Makes the stream's device current while a call launches (the null stream's is the
+// current one).  Every range must be there.
 class OnDevice {
  public:
-  int enter(hipStream_t stream, uint64_t pages) {
+  int enter(hipStream_t stream, const Ranges& ranges) {
     int dev = 0;
     PF_HIP(hipGetDevice(&prev_));
     if (stream)
       PF_HIP(hipStreamGetDevice(stream, &dev));
     else
       dev = prev_;
-    hipPointerAttribute_t attr;
-    PF_HIP(hipPointerGetAttributes(&attr, reinterpret_cast<void*>(pages)));
-    if (attr.type == hipMemoryTypeDevice && attr.device != dev)
-      return invalid(strf("the pages are on device %d, the stream on device %d", attr.device, dev));
+    if (int rc = ranges.check_device(dev)) return rc;
     if (dev != prev_) {
       PF_HIP(hipSetDevice(dev));
       moved_ = true;
@@ -194,7 +210,7 @@ int move_rows(bool write, const pf_kv_pages* pages, const pf_kv_rows* k, const p
   if (int rc = ranges.check()) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
-  if (int rc = on.enter(s, pv.k)) return rc;
+  if (int rc = on.enter(s, ranges)) return rc;
   const int64_t* at = reinterpret_cast<const int64_t*>(slots);
   const uint32_t rows = static_cast<uint32_t>(n);
   PF_HIP(write ? launch_kv_write(pv, kv, vv, k->type, at, rows, aligned, s)
@@ -274,7 +290,7 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   if (grid > 0x7fffffffull) return invalid("too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
-  if (int rc = on.enter(s, pv.k)) return rc;
+  if (int rc = on.enter(s, ranges)) return rc;
   int dev = 0;
   PF_HIP(hipGetDevice(&dev));
   if (ws && ws->device != dev)

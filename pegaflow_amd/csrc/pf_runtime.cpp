@@ -68,14 +68,18 @@ static bool ipc_lookup(uint64_t addr, uint64_t len, uint64_t* base, uint64_t* en
 bool RangeCache::contains(uint64_t a, uint64_t len) {
   const uint64_t e = a + len;
   if (e < a) return false;
-  if (a >= last_b_ && e <= last_e_ && last_e_ > last_b_) return true;
+  if (a >= last_.begin && e <= last_.end && last_.end > last_.begin) return true;
   for (auto& r : ok_)
-    if (a >= r.first && e <= r.second) {
-      last_b_ = r.first;
-      last_e_ = r.second;
+    if (a >= r.begin && e <= r.end) {
+      last_ = r;
       return true;
     }
   return false;
+}
+
+void RangeCache::found(uint64_t begin, uint64_t end, int device) {
+  last_ = {begin, end, device};
+  ok_.push_back(last_);
 }
 
 bool RangeCache::check(uint64_t a, uint64_t len) {
@@ -83,9 +87,7 @@ bool RangeCache::check(uint64_t a, uint64_t len) {
   if (contains(a, len)) return true;
   uint64_t b = 0, e = 0;
   if (pinned_lookup(a, len, &b, &e) || ipc_lookup(a, len, &b, &e)) {
-    ok_.push_back({b, e});
-    last_b_ = b;
-    last_e_ = e;
+    found(b, e, -1);
     return true;
   }
   hipPointerAttribute_t attr;
@@ -105,16 +107,14 @@ bool RangeCache::check(uint64_t a, uint64_t len) {
   b = reinterpret_cast<uint64_t>(base);
   e = b + size;
   if (a < b || a + len > e) return false;
-  ok_.push_back({b, e});
-  last_b_ = b;
-  last_e_ = e;
+  found(b, e, attr.device);
   return true;
 }
 
 bool RangeCache::find(uint64_t a, uint64_t len, uint64_t* begin, uint64_t* end) {
   if (!check(a, len)) return false;
-  *begin = last_b_;
-  *end = last_e_;
+  *begin = last_.begin;
+  *end = last_.end;
   return true;
 }
 
