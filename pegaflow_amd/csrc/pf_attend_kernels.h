@@ -182,14 +182,14 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
 // 2^-25 were lost, of 30,000 tokens that far under one the whole output.)  The maximum may lag by
 // 2^3 only, not 2^8, for 2^15 to be the largest.  A lag of 2 and of 1, with a bit more room
 // each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
-constexpr float kFp16Room = 12.0f, kFp16Lag = 3.0f;
+constexpr float kFp16Room = 12.0f, kFp16Down = 0x1p-12f, kFp16Lag = 3.0f;
 
 // The log-sum-exp of a row of maximum m, in units of the raw scores, and sum l.
 template <class Row>
 __device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, float l) {
   if (l == 0) return kNegInf;
-  const bool lifted = Row::kType == PF_KV_FP16 && !is_codes(a.pages.type);
-  return m * a.scale_log2 * kLn2 + (logf(l) - (lifted ? kFp16Room * kLn2 : 0.0f));
+  if (Row::kType == PF_KV_FP16 && !is_codes(a.pages.type)) l *= kFp16Down;
+  return m * a.scale_log2 * kLn2 + logf(l);
 }
 
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
