@@ -913,8 +913,9 @@ attend_many_kernel(AttendParams a) {
   if (__builtin_expect(odd, 0)) {
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 32; ++dt) lose_nan<16>(o[dt]);
-    for (int32_t t0 = begin; t0 < end; t0 += kStep)
-      for (uint64_t left = odd_tokens<Row, TYPE>(pg, table, head, t0, end); left; left &= left - 1) {
+    for (int32_t t0 = begin; t0 < end; t0 += kStep) {
+      const uint64_t tokens = odd_tokens<Row, TYPE>(pg, table, head, t0, end);
+      for (uint64_t left = tokens; left; left &= left - 1) {
         const int32_t tok = t0 + __builtin_ctzll(left);
         if (tok < my_begin || tok >= my_end) continue;
         uint64_t at, scale_at;
@@ -930,6 +931,15 @@ attend_many_kernel(AttendParams a) {
             for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
           }
       }
+      if (!tokens) continue;
+      bool settled = true;  // NaN throughout, which nothing changes
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+          settled &= o[dt][i] != o[dt][i] || dt * 32 + 8 * (i / 4) + 4 * half >= pg.dim;
+      if (!__any(t.valid && !settled)) break;
+    }
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 32; ++dt) restore_nan<16>(o[dt]);
   }
@@ -1397,10 +1407,10 @@ attend_few_kernel(AttendParams a) {
   if (TYPE != PF_KV_INT8 && __builtin_expect(__any(odd), 0)) {
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 16; ++dt) lose_nan<4>(o[dt]);
-    for (int32_t t1 = begin + static_cast<int32_t>(wave * kFewTokens); t1 < end; t1 += kStep)
-      for (uint64_t left = odd_tokens<Row, TYPE>(
-               pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
-           left; left &= left - 1) {
+    for (int32_t t1 = begin + static_cast<int32_t>(wave * kFewTokens); t1 < end; t1 += kStep) {
+      const uint64_t tokens = odd_tokens<Row, TYPE>(
+          pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
+      for (uint64_t left = tokens; left; left &= left - 1) {
         const int32_t tok = t1 + __builtin_ctzll(left);
         if (tok < my_begin || tok >= my_end) continue;
         uint64_t at, scale_at;
@@ -1413,6 +1423,15 @@ attend_few_kernel(AttendParams a) {
           o[dt] = f32x4{x[0], x[1], x[2], x[3]};
         }
       }
+      if (!tokens) continue;
+      bool settled = true;
+#pragma unroll
+      for (uint32_t dt = 0; dt < DP / 16; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          settled &= o[dt][i] != o[dt][i] || dt * 16 + quarter * 4 >= pg.dim;
+      if (!__any(valid && !settled)) break;
+    }
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 16; ++dt) restore_nan<4>(o[dt]);
   }

@@ -68,3 +68,19 @@ def test_infinities_keep_their_sign(gpu, workspace, form, group, new, cached, sh
     b.dev.upload()
     for w in (None, workspace):
         check(b, *b.run(workspace=w))
+
+
+@pytest.mark.parametrize("bad", ["inf", "nan"])
+@pytest.mark.parametrize("form,group", [(LLAMA, 4), (FORMS[2], 4), (FP16_80, 3)], ids=str)
+@pytest.mark.parametrize("new,cached", [((1, 1), (400, 390)), ((100, 30), (400, 350))], ids=str)
+def test_nothing_but_such_values(gpu, workspace, form, group, new, cached, bad):
+    """Every value of V from a token on, in every head but the last."""
+    b = Batch(new, cached, form, group, seed=42)
+    codes = b.kind in oracle.LARGEST
+    bits = E4M3_NAN if codes else INF16[b.rows] if bad == "inf" else NAN16[b.rows]
+    for i, n in enumerate(b.lens):
+        for token in range(150, int(n)):
+            put(b, i, token, slice(0, b.pages.heads - 1), slice(None), bits)
+    b.dev.upload()
+    for w in (None, workspace):
+        check(b, *b.run(workspace=w))
