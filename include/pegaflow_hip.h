@@ -642,7 +642,8 @@ int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* 
  *
  * Scores, softmax statistics and sums are held in fp32; the weights are rounded
  * to 16 bits, the type of the rows, for the product with V (to twice as many where a
- * sequence has at most 16 rows of a KV head). */
+ * sequence has at most 16 rows of a KV head; fp16 weights, however small, to 2^-36 of the
+ * largest at least). */
 typedef struct pf_attend_args {
   pf_kv_rows q;          /* [num_rows, num_q_heads, head_dim] */
   pf_kv_rows out;        /* the same shape and type; may not overlap q */

@@ -18,8 +18,9 @@
 // reads V^T from LDS with the transposing 16-bit loads.
 //
 // Weights are rounded to the rows' 16 bits for the product with V: the matrix core takes
-// no more, and the rounding, at most half a step of each weight, is of the size of the
-// output's own.  (Of few rows the rest of each weight is multiplied as well.)  Scores, maxima, sums and outputs stay in fp32 until the end.
+// no more, and the rounding, at most half a step of each weight (of fp16 weights 2^-37 of the
+// largest at least), is of the size of the output's own.  (Of few rows the rest of each weight
+// is multiplied as well.)  Scores, maxima, sums and outputs stay in fp32 until the end.
 #pragma once
 
 #include <hip/hip_runtime.h>

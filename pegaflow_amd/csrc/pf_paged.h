@@ -126,8 +126,9 @@ inline bool wide_tiles(uint64_t seqs, uint64_t rows, uint64_t heads, uint64_t di
 }
 
 // Shapes the launch of a batch whose longest query has `most_new` rows and longest
-// sequence `longest` tokens (bounds that may be loose, or wrong: every row is attended
-// whatever they say), joining in `bytes` of workspace at `ws`.
+// sequence `longest` tokens, joining in `bytes` of workspace at `ws`.  `longest` may be wrong:
+// every row is attended whatever it says.  `most_new` may be loose but not too small: rows
+// that a sequence has beyond it may stay as they were.
 inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, uint64_t ws,
                         uint64_t bytes) {
   constexpr uint64_t kCus = 256;
