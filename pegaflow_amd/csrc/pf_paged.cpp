@@ -62,8 +62,10 @@ class Ranges {
       int at = list_[i].device;
       if (at < 0) {  // pinned, which every device reads, or another process's
         hipPointerAttribute_t attr;
-        PF_HIP(hipPointerGetAttributes(&attr, reinterpret_cast<void*>(list_[i].addr)));
-        if (attr.type != hipMemoryTypeDevice) continue;
+        const hipError_t e =
+            hipPointerGetAttributes(&attr, reinterpret_cast<void*>(list_[i].addr));
+        if (e != hipSuccess) (void)hipGetLastError();  // clear the probe's error
+        if (e != hipSuccess || attr.type != hipMemoryTypeDevice) continue;
         at = attr.device;
       }
       if (at != device)
