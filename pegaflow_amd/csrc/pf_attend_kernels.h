@@ -185,12 +185,16 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
 // each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
 constexpr float kFp16Room = 12.0f, kFp16Down = 0x1p-12f, kFp16Lag = 3.0f;
 
-// The log-sum-exp of a row of maximum m, in units of the raw scores, and sum l.
+// A row's maximum m is held as a power of two: of its largest score in base 2 the whole part,
+// so that weights are exp2(score - m) with one rounding, a lift adds to m exactly, and sums are
+// rescaled and joined by whole powers of two.
+
+// The log-sum-exp of a row of maximum m and sum l.
 template <class Row>
 __device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, float l) {
   if (l == 0) return kNegInf;
   if (Row::kType == PF_KV_FP16 && !is_codes(a.pages.type)) l *= kFp16Down;
-  return m * a.scale_log2 * kLn2 + logf(l);
+  return m * kLn2 + logf(l);
 }
 
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
@@ -199,8 +203,10 @@ __device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, flo
 // attended s 2^lift is at most 2^12, and w, which lags its maximum by at most 2^3, makes
 // 2^15 of it.  A product is then a normal number down to 2^-25 of the largest scale, and
 // off by 2^-36 of that below.  (bf16 weights need none of it, but are off by up to 2^-8
-// where the outputs hold 2^-11.)
-constexpr float kLiftStart = 64.0f, kLiftNone = -100.0f;
+// where the outputs hold 2^-11.)  A lift stops at 2^28: products with scales under 2^-16 are
+// then off by up to 2^-53, of which fp16 outputs show nothing, and exponents, which it is part
+// of, stay under 32 and are off by 2^-20 at most, of which a log-sum-exp would show more.
+constexpr float kLiftStart = 28.0f, kLiftNone = -100.0f;
 // Lowers `lift` (kLiftStart before the first token; kLiftNone for no row) to suit scales
 // up to `big` (or 2^66, so that the factor is a normal number: values as large as that
 // are infinite in fp16), and returns the factor that the row's sums take.  Other rows of
@@ -784,14 +790,15 @@ attend_many_kernel(AttendParams a) {
     // The maximum that the weights are taken against follows the largest score only
     // where that has grown by more than 2^8 (2^3 in fp16): until then weights up to that serve
     // as well, and the outputs need no rescaling.
-    bool grown = __any((top - m) * a.scale_log2 > kLag);
+    top *= a.scale_log2;
+    bool grown = __any(top - m > kLag);
     float keep = 1.0f;
     if (grown) {
-      const float m_new = fmaxf(m, top);
-      keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+      const float m_new = fmaxf(m, floorf(top));
+      keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
     }
-    float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float base = m == kNegInf ? 0.0f : -m;
     if constexpr (kLift) {
       if (__any(fmaxf(vs[0], vs[1]) > lift_limit)) {  // some row may not have room for it
         const float* scale = lds.k[n % Lds::kBuffers].v_scale + 4 * half;
@@ -1005,7 +1012,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
   // A share without a maximum attended nothing, or only what is no number (l is NaN).
   auto factor = [&](f32x2 x, float top) {
     return x[0] == kNegInf ? (x[1] == 0.0f ? 0.0f : 1.0f)
-                           : share_factor((x[0] - top) * a.scale_log2);
+                           : share_factor(x[0] - top);
   };
   f32x4 o[4];
 #pragma unroll
@@ -1316,9 +1323,10 @@ attend_few_kernel(AttendParams a) {
       for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = max32(top);
-    if (__any((top - m) * a.scale_log2 > kLag)) {
-      const float m_new = fmaxf(m, top);
-      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f((m - m_new) * a.scale_log2);
+    top *= a.scale_log2;
+    if (__any(top - m > kLag)) {
+      const float m_new = fmaxf(m, floorf(top));
+      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= keep;
 #pragma unroll
@@ -1326,7 +1334,7 @@ attend_few_kernel(AttendParams a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
     }
-    float base = m == kNegInf ? 0.0f : -m * a.scale_log2;
+    float base = m == kNegInf ? 0.0f : -m;
     if constexpr (kLift) {
       if (lower) {  // a scale that some row may not have room for; hidden ones are 0 here
         float big = 0.0f;
@@ -1467,7 +1475,7 @@ attend_few_kernel(AttendParams a) {
     for (uint32_t w = 0; w < kFewWaves; ++w) {
       const float mw = join_m[w][r], lw = join_l[w][r];
       const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
-                                       : share_factor((mw - top) * a.scale_log2);
+                                       : share_factor(mw - top);
       sum += lw * keep;
       const f32x4 y =
           *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
@@ -1551,7 +1559,7 @@ attend_few_kernel(AttendParams a) {
       // A share without a maximum attended nothing, or only what is no number.
       const float f = y[j][0] == kNegInf
                           ? (y[j][1] == 0.0f ? 0.0f : 1.0f)
-                          : share_factor((y[j][0] - largest) * a.scale_log2);
+                          : share_factor(y[j][0] - largest);
       if (lane + j * 64 < used) factor[(lane + j * 64) * 16 + r] = f;
       sum += y[j][1] * f;
     }

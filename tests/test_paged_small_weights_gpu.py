@@ -36,3 +36,17 @@ def test_one_token_takes_most_of_the_weight(gpu, workspace, kind, rows, new, cac
     b.dev.upload()
     for w in (None, workspace):
         b.check(*b.run(workspace=w))
+
+
+@pytest.mark.parametrize("kind,rows", [("e4m3", "fp16"), ("int8", "fp16"), ("int8", "bf16"),
+                                       ("fp16", "fp16")])
+@pytest.mark.parametrize("new,cached", [((4,) * 90, (20,) * 90), ((300,), (0,))], ids=str)
+def test_log_sum_exps_beside_small_values(gpu, workspace, kind, rows, new, cached):
+    """V of 2^-60 does not show in the statistics of the scores."""
+    b = Batch(new, cached, (kind, rows, 2, 16, 16, False), 2, seed=52, sharp=0.01)
+    if kind in oracle.LARGEST:
+        held = b.pages.scales()[1]
+        held[np.isfinite(held)] = 2.0 ** -60
+    b.dev.upload()
+    for window in (1, 2, 3, 5):
+        b.check(*b.run(workspace=workspace, window=window), window=window)
