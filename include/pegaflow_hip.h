@@ -641,9 +641,10 @@ int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* 
  * stay as they were.  A length beyond the table is cut to it.
  *
  * Scores, softmax statistics and sums are held in fp32; the weights are rounded
- * to 16 bits, the type of the rows, for the product with V (to twice as many where a
- * sequence has at most 16 rows of a KV head; fp16 weights, however small, to 2^-36 of the
- * largest at least). */
+ * to 16 bits, the type of the rows, for the product with V (fp16 weights, however small, to
+ * 2^-36 of the largest at least).  They are rounded to twice as many where a sequence has at
+ * most 16 rows of a KV head, in a batch of several sequences or where max_query_len (or
+ * num_rows) says so. */
 typedef struct pf_attend_args {
   pf_kv_rows q;          /* [num_rows, num_q_heads, head_dim] */
   pf_kv_rows out;        /* the same shape and type; may not overlap q */
