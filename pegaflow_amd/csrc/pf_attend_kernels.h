@@ -185,9 +185,11 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
 // each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
 constexpr float kFp16Room = 12.0f, kFp16Down = 0x1p-12f, kFp16Lag = 3.0f;
 
-// A row's maximum m is held as a power of two: of its largest score in base 2 the whole part,
-// so that weights are exp2(score - m) with one rounding, a lift adds to m exactly, and sums are
-// rescaled and joined by whole powers of two.
+// A row's maximum m is held in base 2, as its weights exp2(score - m) are taken.  Under a lift
+// of its own it is the whole part only: the lift then adds to it exactly, and the weight meets a
+// scale before it is rounded anyway.  Elsewhere the largest weight is 1 (or the lift), which 16
+// bits hold: with the whole part there as well 8,192 new bf16 tokens were off by 0.0023, not
+// 0.0020.
 
 // The log-sum-exp of a row of maximum m and sum l.
 template <class Row>
@@ -794,7 +796,7 @@ attend_many_kernel(AttendParams a) {
     bool grown = __any(top - m > kLag);
     float keep = 1.0f;
     if (grown) {
-      const float m_new = fmaxf(m, floorf(top));
+      const float m_new = fmaxf(m, kLift ? floorf(top) : top);
       keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
     }
@@ -1325,7 +1327,7 @@ attend_few_kernel(AttendParams a) {
     top = max32(top);
     top *= a.scale_log2;
     if (__any(top - m > kLag)) {
-      const float m_new = fmaxf(m, floorf(top));
+      const float m_new = fmaxf(m, kLift ? floorf(top) : top);
       const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
       l *= keep;
