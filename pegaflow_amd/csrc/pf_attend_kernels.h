@@ -177,19 +177,30 @@ __device__ __forceinline__ void scale_by(float* x, float y, std::integer_sequenc
   ((x[I] *= of16<FIRST + I>(y)), ...);
 }
 
+// The maximum that a row's weights are taken against follows its largest score only where that
+// has grown by more than 2^lag: until then weights up to that serve as well, and sums and
+// outputs need no rescaling.  But the largest weight is 1, which 16 bits hold, only where it
+// has followed: 2,000 new bf16 tokens are off by 0.0021 against 64 bits with a lag of 2^3 as of
+// 2^8, but where scores are six times as large by 0.0017 and 0.0019.  Prompts of 8,192 tokens
+// take 547 and 545 us, and 554 with a lag of 2^1.  Rescaling heads of 256 takes more: 2,000
+// behind 2,000 170 and 163, so that bf16 heads of more than 128 keep 2^8 (fp16 ones, whose
+// weights need the room, 173 and 163).
+template <class Row, uint32_t DP>
+constexpr float lag() {
+  return Row::kType == PF_KV_FP16 || DP <= 128 ? 3.0f : 8.0f;
+}
+
 // fp16 weights over 16-bit pages are held as 2^12 times what they are, l and the outputs with
 // them: fp16's smallest step is 2^-24, and a weight off by half of it is then off by 2^-37 of
 // its row's largest, so that many small ones keep their sum.  (Held as they are, all under
-// 2^-25 were lost, of 30,000 tokens that far under one the whole output.)  The maximum may lag by
-// 2^3 only, not 2^8, for 2^15 to be the largest.  A lag of 2 and of 1, with a bit more room
-// each, took 0.5% and 1% longer at prompts of 8,192 tokens; one of 3 or 4 nothing.
-constexpr float kFp16Room = 12.0f, kFp16Down = 0x1p-12f, kFp16Lag = 3.0f;
+// 2^-25 were lost, of 30,000 tokens that far under one the whole output.)  With its lag
+// none is over 2^15.
+constexpr float kFp16Room = 12.0f, kFp16Down = 0x1p-12f;
 
 // A row's maximum m is held in base 2, as its weights exp2(score - m) are taken.  Under a lift
 // of its own it is the whole part only: the lift then adds to it exactly, and the weight meets a
 // scale before it is rounded anyway.  Elsewhere the largest weight is 1 (or the lift), which 16
-// bits hold: with the whole part there as well 8,192 new bf16 tokens were off by 0.0023, not
-// 0.0020.
+// bits hold: with the whole part there as well 2,000 new bf16 tokens were off by 0.0023.
 
 // The log-sum-exp of a row of maximum m and sum l.
 template <class Row>
@@ -202,12 +213,12 @@ __device__ __forceinline__ float log_sum_exp(const AttendParams& a, float m, flo
 // fp16 weights over codes.  A weight meets a code as w s, s the scale of V's token, and s
 // may be anything that 32 bits hold, so all weights of a row, its sum l and its outputs
 // carry a power of two, 2^lift, until the end: with the largest scale that the row has
-// attended s 2^lift is at most 2^12, and w, which lags its maximum by at most 2^3, makes
-// 2^15 of it.  A product is then a normal number down to 2^-25 of the largest scale, and
-// off by 2^-36 of that below.  (bf16 weights need none of it, but are off by up to 2^-8
-// where the outputs hold 2^-11.)  A lift stops at 2^28: products with scales under 2^-16 are
-// then off by up to 2^-53, of which fp16 outputs show nothing, and exponents, which it is part
-// of, stay under 32 and are off by 2^-20 at most, of which a log-sum-exp would show more.
+// attended s 2^lift is at most 2^12, and w, at most 2^3, makes 2^15 of it.  A product is then a
+// normal number down to 2^-25 of the largest scale, and off by 2^-36 of that below.  (bf16
+// weights need none of it, but are off by up to 2^-8 where the outputs hold 2^-11.)  A lift
+// stops at 2^28: products with scales under 2^-16 are then off by up to 2^-53, of which fp16
+// outputs show nothing, and exponents, which it is part of, stay under 32 and are off by 2^-20
+// at most, of which a log-sum-exp would show more.
 constexpr float kLiftStart = 28.0f, kLiftNone = -100.0f;
 // Lowers `lift` (kLiftStart before the first token; kLiftNone for no row) to suit scales
 // up to `big` (or 2^66, so that the factor is a normal number: values as large as that
@@ -526,7 +537,6 @@ attend_many_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
-  constexpr float kLag = Row::kType == PF_KV_FP16 ? kFp16Lag : 8.0f;
   constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
   // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
   constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
@@ -789,11 +799,8 @@ attend_many_kernel(AttendParams a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tt][i]);
     top = max32(top);
-    // The maximum that the weights are taken against follows the largest score only
-    // where that has grown by more than 2^8 (2^3 in fp16): until then weights up to that serve
-    // as well, and the outputs need no rescaling.
     top *= a.scale_log2;
-    bool grown = __any(top - m > kLag);
+    bool grown = __any(top - m > lag<Row, DP>());
     float keep = 1.0f;
     if (grown) {
       const float m_new = fmaxf(m, kLift ? floorf(top) : top);
@@ -1102,7 +1109,6 @@ attend_few_kernel(AttendParams a) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
-  constexpr float kLag = Row::kType == PF_KV_FP16 ? kFp16Lag : 8.0f;
   constexpr uint32_t kPer = kCodes ? 16 : 8;
   constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
   constexpr uint32_t kCols = DP / kPer;
@@ -1326,7 +1332,7 @@ attend_few_kernel(AttendParams a) {
     top = fmaxf(top, __shfl_xor(top, 16));
     top = max32(top);
     top *= a.scale_log2;
-    if (__any(top - m > kLag)) {
+    if (__any(top - m > lag<Row, DP>())) {
       const float m_new = fmaxf(m, kLift ? floorf(top) : top);
       const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
       m = m_new;
