@@ -79,17 +79,32 @@ def _index(x, dims: int, dtype: str, what: str):
     return x.data_ptr()
 
 
+_current_streams: dict = {}  # a tensor's type -> its device's current stream, or None
+
+
+def _current_stream(kind: type):
+    """What gives the handle of a device's current stream, for tensors of torch's."""
+    torch = sys.modules.get("torch")
+    if torch is None or not issubclass(kind, torch.Tensor):
+        return None
+    # current_stream() takes 1 to 2 us for its object, the other 0.1.
+    return getattr(torch._C, "_cuda_getCurrentRawStream",
+                   lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream(stream: Stream | None, x):
     """The handle of ``stream``, or else of the stream on which torch queues what it does
     with its tensor ``x``."""
     if stream is not None:
         return stream.handle
-    torch = sys.modules.get("torch")
-    if torch is None or not isinstance(x, torch.Tensor) or not x.is_cuda:
+    kind = type(x)
+    if kind not in _current_streams:
+        _current_streams[kind] = _current_stream(kind)
+    current = _current_streams[kind]
+    if current is None:
         return None
-    # current_stream() takes 1 to 2 us for its object, this 0.1.
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(x.get_device()) if raw else torch.cuda.current_stream(x.device).cuda_stream
+    device = x.get_device()
+    return current(device) if device >= 0 else None
 
 
 def segment_bytes(block_size: int, num_kv_heads: int, head_dim: int, kv_type: str) -> int:
