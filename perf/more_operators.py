@@ -426,14 +426,13 @@ def _run_fork(c, s):
         parents, new = s["parents"].long(), s["new_blocks"].long()
         s["out_table"].copy_(s["table"][parents])
         page = s["lens"][parents].long() // c["block_size"]
-        part = s["lens"][parents] % c["block_size"] > 0  # a full block stays shared
         child = torch.arange(len(parents), device="cuda")
-        last = s["out_table"][child, page]
-        s["out_table"][child, page] = torch.where(part, s["new_blocks"], last)
-        # Of a child without a part-filled block the block is copied onto itself.
-        new = torch.where(part, new, last.long())
+        last = s["out_table"][child, page].long()
+        s["out_table"][child, page] = s["new_blocks"]
+        # A parent that ends with its block leaves nothing to copy.
+        last = torch.where(s["lens"][parents] % c["block_size"] > 0, last, new)
         for layer in s["segments"]:
-            layer[:, new] = layer[:, last.long()]
+            layer[:, new] = layer[:, last]
     return {"segments": s["segments"].view(torch.int32), "table": s["out_table"]}
 
 
