@@ -627,6 +627,98 @@ int pf_kv_write(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows*
 int pf_kv_read(const pf_kv_pages* pages, const pf_kv_rows* k, const pf_kv_rows* v,
                uint64_t slots, uint64_t num_rows, pf_stream stream);
 
+/* Rotary positions.  Pair i, (a, b), of a head of the token at position p becomes
+ *   (factor (a cos t - b sin t), factor (b cos t + a sin t)),  t = p frequencies[i]
+ * radians.  The pairs are values i and i + num_pairs (HALF) or 2 i and 2 i + 1
+ * (INTERLEAVED) of a head; values from 2 num_pairs on pass as they are.  The
+ * angle is off by less than 2^-29 turns for |p| < 2^32 and |frequency| <= 2 pi; the rest is fp32.
+ * frequencies: host memory, any finite numbers (a scaling for long contexts is one of
+ * frequencies and factor). */
+enum { PF_ROTARY_HALF = 1, PF_ROTARY_INTERLEAVED = 2 };
+typedef struct pf_rotary pf_rotary;
+int pf_rotary_create(int device, const double* frequencies, uint32_t num_pairs,
+                     uint32_t layout, float factor, pf_rotary** out);
+/* Waits for the device.  No call, or graph that holds one, may run afterwards. */
+int pf_rotary_destroy(pf_rotary* rotary);
+/* Rows of x [num_rows, num_heads, head_dim], turned to positions[i] (int64, device), into
+ * out, of the same type; out may be x itself (address and strides) and else may not overlap
+ * it.  head_dim is a multiple of 16 up to PF_KV_MAX_HEAD_DIM. */
+int pf_rotary_rotate(const pf_rotary* rotary, const pf_kv_rows* x, const pf_kv_rows* out,
+                     uint64_t positions, uint64_t num_rows, uint32_t num_heads,
+                     uint32_t head_dim, pf_stream stream);
+/* pf_rotary_rotate of q into q_out and pf_kv_write of k, turned, and v in one pass: k meets
+ * its one rounding (to the pages' 16 bits, or to a code of a scale of the turned values) as it
+ * is written.  A row of a padding slot is written nowhere, its query is turned all the same.
+ * num_q_heads 0: no queries (q and q_out may be null). */
+int pf_kv_write_rotated(const pf_kv_pages* pages, const pf_rotary* rotary, const pf_kv_rows* q,
+                        const pf_kv_rows* q_out, uint32_t num_q_heads, const pf_kv_rows* k,
+                        const pf_kv_rows* v, uint64_t positions, uint64_t slots,
+                        uint64_t num_rows, pf_stream stream);
+
+/* All layers of a cache, of pages of one shape, for the calls below that move blocks or
+ * tokens within them, each layer alike.  The layers lie on `device` (or in pinned memory) and
+ * are borrowed: no call, or graph that holds one, may run after one of them has been freed. */
+typedef struct pf_kv_layers pf_kv_layers;
+int pf_kv_layers_create(int device, const pf_kv_pages* layers, uint32_t num_layers,
+                        pf_kv_layers** out);
+/* Waits for the device. */
+int pf_kv_layers_destroy(pf_kv_layers* layers);
+
+/* Copies block from_blocks[i] to block to_blocks[i] (int32 [num_blocks], device), K and V, in
+ * every layer.  A pair with a block that is negative or past the last one is padding.  No
+ * block is copied to twice, and none that is copied to is copied from. */
+int pf_kv_copy_blocks(const pf_kv_layers* layers, uint64_t from_blocks, uint64_t to_blocks,
+                      uint64_t num_blocks, pf_stream stream);
+
+/* Forks sequences: child i is sequence parents[i] of a block table, with a block of its own
+ * for its next token.  Row i of out_table becomes the parent's row with entry seq_lens[parent]
+ * / block_size replaced by new_blocks[i]; where the parent has filled part of the block that
+ * stood there, that block is copied to new_blocks[i] in every layer.  The full blocks before
+ * it are shared.  new_blocks[i] negative or past the last block: the row is the parent's as
+ * it is (one child may go on in its parent's block).  parents[i] outside the table: padding, the
+ * row stays as it was.  out_table does not overlap the table; new blocks are distinct, and no
+ * parent's. */
+typedef struct pf_fork_args {
+  uint64_t block_table;  /* int32 [num_seqs, table_width], device */
+  uint64_t table_stride; /* entries from one sequence to the next */
+  uint64_t seq_lens;     /* int32 [num_seqs], device */
+  uint64_t parents;      /* int32 [num_children], device */
+  uint64_t new_blocks;   /* int32 [num_children], device */
+  uint64_t out_table;    /* int32 [num_children, table_width], device */
+  uint64_t out_stride;
+  uint32_t num_seqs;
+  uint32_t table_width;
+  uint32_t num_children;
+  uint32_t reserved;
+} pf_fork_args;
+int pf_kv_fork(const pf_kv_layers* layers, const pf_fork_args* args, pf_stream stream);
+
+/* Moves the kept tokens of sequences together, in every layer: token kept[kept_starts[b] + j]
+ * of sequence b (a position, in its row of block_table) goes to position first[b] + j of its
+ * row of out_table, bit by bit, scales included.  A sequence's kept positions ascend strictly.
+ *
+ * In place, with out_table the block_table itself: no token may move up (kept position j is
+ * first[b] + j or more), and sequences whose tokens move share no block.  To other blocks: none
+ * that a token goes to holds one that is read.  Tokens at positions outside a table's row, or
+ * in blocks that are negative or past the last one, do not move. */
+typedef struct pf_compact_args {
+  uint64_t block_table; /* int32 [num_seqs, table_width], device */
+  uint64_t table_stride;
+  uint64_t out_table;   /* of the same shape, device; block_table: in place */
+  uint64_t out_stride;
+  uint64_t kept;        /* int32 [num_kept], device */
+  uint64_t num_kept;
+  uint64_t kept_starts; /* int32 [num_seqs + 1], device */
+  uint64_t first;       /* int32 [num_seqs], device, or 0: every sequence from 0 on */
+  uint64_t out_lens;    /* int32 [num_seqs], device, or 0: receives first + kept tokens */
+  uint32_t num_seqs;
+  uint32_t table_width;
+  uint32_t max_kept;    /* most kept tokens of a sequence, as a hint that shapes the launch */
+                        /* (0: num_kept)                                                    */
+  uint32_t reserved;
+} pf_compact_args;
+int pf_kv_compact(const pf_kv_layers* layers, const pf_compact_args* args, pf_stream stream);
+
 /* Attention of new tokens over the pages.
  *
  * The batch's num_rows query rows are those of num_seqs sequences one after

@@ -195,3 +195,30 @@ def attend(pages, q, rows, table, lens, starts, scale, causal=True, window=0, we
                     bound[r, h] += least / l
                 lse_bound[r, h] = dz + 2.0 ** -21 + (len(z) + 8) * u + 2.0 ** -22 * abs(lse[r, h])
     return out, lse, bound, lse_bound
+
+
+def rotate(x, positions, frequencies, layout, factor=1.0):
+    """Rows [n, heads, dim] turned to their positions, in 64 bits (angles in the 64 bits of a
+    long double's fraction), and how far a kernel may be off that takes angles to 2^-29 turns
+    and the rest in 32 bits, before its result is rounded.
+
+    The angle's part is 2 pi 2^-29 < 2^-26; sine and cosine are off by 2^-23 (their sums, three
+    roundings of at most half a step of 1, 2^-25 each, of z twice), times the factor a half-step
+    more; two products and a sum round by a half-step, 2^-24, of each product: less than
+    2^-22 (|a| + |b|) |factor| in all; twice that is allowed."""
+    x = np.asarray(x, np.float64)
+    pairs = len(frequencies)
+    angle = np.asarray(positions, np.longdouble)[:, None] * np.asarray(frequencies, np.longdouble)
+    turn = 2 * np.longdouble("3.14159265358979323846264338327950288")
+    angle = np.asarray(angle - np.floor(angle / turn) * turn, np.float64)[:, None]
+    c, s = np.cos(angle) * factor, np.sin(angle) * factor
+    if layout == "half":
+        first, second = slice(0, pairs), slice(pairs, 2 * pairs)
+    else:
+        first, second = slice(0, 2 * pairs, 2), slice(1, 2 * pairs, 2)
+    a, b = x[..., first], x[..., second]
+    out, bound = x.copy(), np.zeros_like(x)
+    with np.errstate(invalid="ignore"):
+        out[..., first], out[..., second] = a * c - b * s, b * c + a * s
+        bound[..., first] = bound[..., second] = 2.0 ** -21 * (np.abs(a) + np.abs(b)) * abs(factor)
+    return out, bound

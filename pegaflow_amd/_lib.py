@@ -176,6 +176,7 @@ class LayerWords(ctypes.Structure):
 # values.
 KV_BF16, KV_FP16, KV_E4M3, KV_INT8 = 1, 2, 3, 4
 KV_TOKEN_MAJOR, KV_HEAD_MAJOR = 0, 1
+ROTARY_HALF, ROTARY_INTERLEAVED = 1, 2
 KV_MAX_HEAD_DIM = 256
 ATTEND_WORKSPACE_DEFAULT = 64 << 20
 
@@ -227,6 +228,24 @@ class AttendArgs(ctypes.Structure):
         ("max_seq_len", ctypes.c_uint32),
         ("max_query_len", ctypes.c_uint32),
     ]
+
+
+class ForkArgs(ctypes.Structure):
+    """pf_fork_args — children of sequences, with blocks of their own."""
+
+    _fields_ = [(n, ctypes.c_uint64) for n in (
+        "block_table", "table_stride", "seq_lens", "parents", "new_blocks", "out_table",
+        "out_stride")] + [(n, ctypes.c_uint32) for n in (
+            "num_seqs", "table_width", "num_children", "reserved")]
+
+
+class CompactArgs(ctypes.Structure):
+    """pf_compact_args — kept tokens of sequences, and where they go."""
+
+    _fields_ = [(n, ctypes.c_uint64) for n in (
+        "block_table", "table_stride", "out_table", "out_stride", "kept", "num_kept",
+        "kept_starts", "first", "out_lens")] + [(n, ctypes.c_uint32) for n in (
+            "num_seqs", "table_width", "max_kept", "reserved")]
 
 
 class SaveLayer(ctypes.Structure):
@@ -351,6 +370,19 @@ SIGNATURES = {
                           ctypes.POINTER(KVRows), u64, u64, vp]),
     "pf_kv_read": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(KVRows),
                          ctypes.POINTER(KVRows), u64, u64, vp]),
+    "pf_rotary_create": (i32, [i32, ctypes.POINTER(ctypes.c_double), u32, u32, ctypes.c_float,
+                               pvp]),
+    "pf_rotary_destroy": (i32, [vp]),
+    "pf_rotary_rotate": (i32, [vp, ctypes.POINTER(KVRows), ctypes.POINTER(KVRows), u64, u64, u32,
+                               u32, vp]),
+    "pf_kv_write_rotated": (i32, [ctypes.POINTER(KVPages), vp, ctypes.POINTER(KVRows),
+                                  ctypes.POINTER(KVRows), u32, ctypes.POINTER(KVRows),
+                                  ctypes.POINTER(KVRows), u64, u64, u64, vp]),
+    "pf_kv_layers_create": (i32, [i32, ctypes.POINTER(KVPages), u32, pvp]),
+    "pf_kv_layers_destroy": (i32, [vp]),
+    "pf_kv_copy_blocks": (i32, [vp, u64, u64, u64, vp]),
+    "pf_kv_fork": (i32, [vp, ctypes.POINTER(ForkArgs), vp]),
+    "pf_kv_compact": (i32, [vp, ctypes.POINTER(CompactArgs), vp]),
     "pf_attend_workspace_create": (i32, [i32, u64, pvp]),
     "pf_attend_workspace_destroy": (i32, [vp]),
     "pf_kv_attend": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(AttendArgs), vp, vp]),

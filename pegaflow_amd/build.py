@@ -28,6 +28,10 @@ SOURCES = [
     "pf_transfer.cpp",
     "pf_paged.cpp",
     "pf_paged.hip",
+    "pf_rotary.cpp",
+    "pf_rotary.hip",
+    "pf_pages.cpp",
+    "pf_pages.hip",
     "pf_attend_bf16.hip",
     "pf_attend_fp16.hip",
     "pf_load_state.cpp",

@@ -33,97 +33,16 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kHeads = 2;  // heads of a workgroup: independent loads in flight
 
-// 8 values of a row as 4 words.
-template <bool ALIGNED>
-__device__ __forceinline__ u32x4 load_row8(uint64_t at) {
-  if constexpr (ALIGNED) return *reinterpret_cast<const g_u32x4*>(at);
-  const g_u16* p = reinterpret_cast<const g_u16*>(at);
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
-  return v;
-}
-
-template <bool ALIGNED>
-__device__ __forceinline__ void store_row8(uint64_t at, u32x4 v) {
-  if constexpr (ALIGNED) {
-    *reinterpret_cast<g_u32x4*>(at) = v;
-  } else {
-    g_u16* p = reinterpret_cast<g_u16*>(at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      p[2 * i] = static_cast<uint16_t>(v[i]);
-      p[2 * i + 1] = static_cast<uint16_t>(v[i] >> 16);
-    }
-  }
-}
-
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-
-// The largest x of a group of LANES aligned lanes, in all of them.  Within 16 lanes by
-// cross-lane operands of the vector instructions, which cost no trip through LDS.
-template <uint32_t LANES>
-__device__ __forceinline__ uint32_t group_max(uint32_t x) {
-  constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e;  // lanes 1 0 3 2 and 2 3 0 1 of each four
-  constexpr int kMirror8 = 0x141, kMirror16 = 0x140;
-  x = umax(x, __builtin_amdgcn_mov_dpp(x, kSwap1, 0xf, 0xf, true));
-  x = umax(x, __builtin_amdgcn_mov_dpp(x, kSwap2, 0xf, 0xf, true));
-  x = umax(x, __builtin_amdgcn_mov_dpp(x, kMirror8, 0xf, 0xf, true));
-  if constexpr (LANES >= 16) x = umax(x, __builtin_amdgcn_mov_dpp(x, kMirror16, 0xf, 0xf, true));
-  if constexpr (LANES >= 32) x = umax(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), 16)));
-  return x;
-}
-
 // The 8 values of this lane as codes of scale s (s > 0).
-//
-// The quotients are IEEE divisions, at 5 operations each instead of the compiler's 10
-// or so: with y = 1 / s rounded to nearest, q = x y, and twice q += y (x - q s), each
-// step one fused operation.  The first correction leaves q within an ulp, and the second
-// then gives x / s rounded to nearest (Markstein's theorem), provided that x - q s is
-// exact, which it is where its last bit, 2^-24 x or more, is not below 2^-149.  With s >=
-// 2^-100 that holds for every x that does not round to code 0 anyway (|x| >= 2^-11 s);
-// rows smaller than that are divided.
 template <class Row, uint32_t TYPE>
-__device__ __forceinline__ u32x2 encode(u32x4 x, float s) {
+__device__ __forceinline__ u32x2 encode_row8(u32x4 x, float s) {
   float q[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     q[2 * i] = Row::to_float(x[i] & 0xffffu);
     q[2 * i + 1] = Row::to_float(x[i] >> 16);
   }
-  if (s >= 0x1p-100f) {
-    const float y = 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = q[i];
-      float z = v * y;
-      z = __builtin_fmaf(__builtin_fmaf(-z, s, v), y, z);
-      z = __builtin_fmaf(__builtin_fmaf(-z, s, v), y, z);
-      q[i] = __builtin_copysignf(z, v);  // also of 0
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] /= s;
-  }
-  u32x2 c;
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    if constexpr (TYPE == PF_KV_E4M3) {
-      int v = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * w], q[4 * w + 1], 0, false);
-      c[w] = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * w + 2], q[4 * w + 3], v, true);
-    } else {
-      // Added to 1.5 * 2^23 a quotient is rounded to an integer, ties to even, and the
-      // sum's low byte is its code.
-      uint32_t v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(uint32_t, q[4 * w + i] + 12582912.0f);
-      const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u);
-      const uint32_t hi = __builtin_amdgcn_perm(v[3], v[2], 0x04000c0cu);
-      c[w] = lo | hi;
-    }
-  }
-  return c;
+  return encode<TYPE>(q, s);
 }
 
 // Workgroup b: tokens (b / (2 * head_groups)) * groups + group, K or V, kHeads heads.
@@ -171,13 +90,12 @@ kv_write_kernel(PagedView p, RowsView k, RowsView v, const int64_t* __restrict__
         pair = __builtin_elementwise_max(pair, __builtin_bit_cast(u16x2, word));
       }
       const uint32_t m = group_max<LANES>(umax(pair[0], pair[1]));
-      constexpr float kInverse = 1.0f / (TYPE == PF_KV_E4M3 ? 448.0f : 127.0f);
-      float s = Row::to_float(m) * kInverse;
+      float s = Row::to_float(m) * kInverseLargest<TYPE>;
       u32x2 c{0, 0};
       if (m >= Row::kInf)
         s = __builtin_nanf("");
       else if (m)
-        c = encode<Row, TYPE>(x[i], s);
+        c = encode_row8<Row, TYPE>(x[i], s);
       if (mine) *reinterpret_cast<g_u32x2*>(at + d) = c;
       if (lane == 0)
         *reinterpret_cast<g_f32*>(segment + p.scale_offset + (h * p.block_size + token) * 4ull) = s;

@@ -3,9 +3,12 @@ that the transfer path saves and restores.
 
 ``PagedKVCache`` describes a layer's blocks as pages; ``write`` puts new tokens' K
 and V into them (at 16 bits, or as 8-bit codes with a scale for each token and
-head), ``read`` gives them back, ``attend`` attends new tokens over them.  An 8-bit
-layer keeps its scales inside its blocks, so it is saved and restored like any
-other layer, at half the bytes.
+head), ``write_rotated`` does so as it turns queries and keys to their positions
+(``RotaryPositions``), ``read`` gives them back, ``attend`` attends new tokens over
+them.  An 8-bit layer keeps its scales inside its blocks, so it is saved and restored
+like any other layer, at half the bytes.  ``PagedLayers`` moves blocks and tokens
+within all layers at once: forks of sequences, copies of blocks, kept tokens moved
+together.
 
 Tensors are torch's, or anything with their ``data_ptr()``, ``shape``,
 ``stride()`` and ``dtype`` (``runtime.DeviceArray``).  Calls are asynchronous on
@@ -21,7 +24,7 @@ import math
 import sys
 
 from . import _lib
-from ._lib import AttendArgs, KVPages, KVRows, check
+from ._lib import AttendArgs, CompactArgs, ForkArgs, KVPages, KVRows, check
 from .runtime import Stream
 from .transfer import KVCacheRegistration
 
@@ -126,6 +129,149 @@ def _kv_type(name: str) -> int:
     return KV_TYPES[name]
 
 
+def _most(what: str, n: int) -> int:
+    """A hint or bound that a 32-bit field holds."""
+    if n < 0:
+        raise ValueError(f"{what} is not negative")
+    return min(n, _MOST)
+
+
+def _wavelengths(rotary_dim: int, base: float, scaling: dict | None):
+    """(radians a position of each pair, factor of turned values) of a named scaling."""
+    if not base > 0:
+        raise ValueError(f"base {base}")
+    pairs = range(rotary_dim // 2)
+    s = dict(scaling or {"type": "none"})
+    kind = s.pop("type", None)
+    takes = {"none": (), "linear": ("factor",), "ntk": ("factor",),
+             "llama3": ("factor", "original_max_position", "low_freq_factor", "high_freq_factor"),
+             "yarn": ("factor", "original_max_position", "beta_fast", "beta_slow",
+                      "attention_factor")}
+    if kind not in takes:
+        raise ValueError(f"unknown scaling {kind!r} (one of {', '.join(takes)})")
+    needed = set(takes[kind][:2])
+    if set(s) - set(takes[kind]) or needed - set(s):
+        raise ValueError(f"scaling {kind!r} takes {', '.join(takes[kind])}, got {', '.join(s)}")
+    by = float(s.get("factor", 1.0))
+    if not by > 0 or not float(s.get("original_max_position", 1)) > 0:
+        raise ValueError("scaling: factor and original_max_position are above 0")
+    if kind == "ntk" and rotary_dim > 2:
+        base = base * by ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-2 * i / rotary_dim) for i in pairs]
+    if kind == "linear":
+        return [x / by for x in f], 1.0
+    if kind == "llama3":
+        # By the turns that a pair makes over the original context: many, and it stays; few,
+        # and it is stretched; in between a mean of both.
+        low, high = float(s.get("low_freq_factor", 1.0)), float(s.get("high_freq_factor", 4.0))
+        if not high > low:
+            raise ValueError("scaling: high_freq_factor is above low_freq_factor")
+        out = []
+        for x in f:
+            turns = s["original_max_position"] * x / (2 * math.pi)
+            keep = min(max((turns - low) / (high - low), 0.0), 1.0)
+            out.append(keep * x + (1 - keep) * x / by)
+        return out, 1.0
+    if kind == "yarn":
+        # As above, along the index of the pair, between those that make beta_fast and
+        # beta_slow turns.
+        fast, slow = float(s.get("beta_fast", 32.0)), float(s.get("beta_slow", 1.0))
+        if not fast > slow > 0 or not base > 1:
+            raise ValueError("scaling: beta_fast is above beta_slow, beta_slow above 0, base above 1")
+
+        def index(turns):
+            return (rotary_dim * math.log(s["original_max_position"] / (turns * 2 * math.pi))
+                    / (2 * math.log(base)))
+
+        low = max(math.floor(index(fast)), 0)
+        high = min(math.ceil(index(slow)), rotary_dim - 1)
+        width = high - low if high != low else 0.001
+        out = []
+        for i, x in enumerate(f):
+            stretch = min(max((i - low) / width, 0.0), 1.0)
+            out.append(stretch * x / by + (1 - stretch) * x)
+        factor = s.get("attention_factor")
+        if factor is None:
+            factor = 0.1 * math.log(by) + 1.0 if by > 1 else 1.0
+        return out, float(factor)
+    return f, 1.0
+
+
+class RotaryPositions:
+    """The angles by which a model turns queries and keys to their positions (pf_rotary).
+
+    The first ``rotary_dim`` values of a head are turned, in pairs: ``layout`` "half" pairs
+    values i and i + rotary_dim / 2, "interleaved" 2 i and 2 i + 1.  Pair i turns by
+    ``base`` ** (-2 i / rotary_dim) radians a position, for contexts beyond the trained
+    ones by less, as ``scaling`` says:
+
+    * {"type": "linear", "factor": s}: all s times slower;
+    * {"type": "ntk", "factor": s}: base * s ** (rotary_dim / (rotary_dim - 2));
+    * {"type": "llama3", "factor": s, "original_max_position": n}: s times slower where a
+      pair turns once or less over n positions, as before where four times or more
+      ("low_freq_factor" 1, "high_freq_factor" 4);
+    * {"type": "yarn", "factor": s, "original_max_position": n}: the same along the index,
+      between 32 turns and one ("beta_fast", "beta_slow"), turned values 0.1 ln s + 1
+      times as large ("attention_factor").
+
+    Or ``frequencies`` are the radians a position of each pair, and ``factor`` that of turned
+    values.  No angle loses precision at far positions.  It lives on ``device``, one for all
+    layers; close it after the last call, or graph, that uses it."""
+
+    def __init__(self, rotary_dim: int, *, base: float = 10000.0, layout: str = "half",
+                 scaling: dict | None = None, frequencies=None, factor: float | None = None,
+                 device: int = 0):
+        self.handle = None
+        if rotary_dim < 2 or rotary_dim % 2:
+            raise ValueError(f"rotary_dim {rotary_dim} is not an even number from 2 on")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"unknown layout {layout!r} (half or interleaved)")
+        if frequencies is None:
+            if factor is not None:
+                raise ValueError("a factor goes with frequencies")
+            frequencies, factor = _wavelengths(rotary_dim, base, scaling)
+        elif scaling is not None:
+            raise ValueError("either frequencies or a scaling")
+        self.frequencies = [float(x) for x in frequencies]
+        self.factor = 1.0 if factor is None else float(factor)
+        if len(self.frequencies) != rotary_dim // 2:
+            raise ValueError(f"{len(self.frequencies)} frequencies of {rotary_dim // 2} pairs")
+        self.rotary_dim = rotary_dim
+        self.layout = layout
+        h = ctypes.c_void_p()
+        check(lib().pf_rotary_create(
+            device, (ctypes.c_double * len(self.frequencies))(*self.frequencies),
+            len(self.frequencies),
+            _lib.ROTARY_HALF if layout == "half" else _lib.ROTARY_INTERLEAVED, self.factor,
+            ctypes.byref(h)), "pf_rotary_create")
+        self.handle = h.value
+
+    def rotate(self, x, out, positions, stream: Stream | None = None) -> None:
+        """Rows of ``x`` [tokens, heads, head_dim], turned to ``positions`` (int64), into
+        ``out``, the same shape and type, which may be ``x`` itself (pf_rotary_rotate)."""
+        dim = x.shape[-1]
+        xr, n, heads = _rows(x, None, dim, "x")
+        outr, m, _ = _rows(out, heads, dim, "out")
+        at = _index(positions, 1, "int64", "positions")
+        if n != m or positions.shape[0] != n:
+            raise ValueError(f"{n} rows of x, {m} of out and {positions.shape[0]} positions")
+        if n >= 2 ** 31 or heads > _MOST or dim > _MOST:
+            raise ValueError(f"rows [{n}, {heads}, {dim}] are too many")
+        check(lib().pf_rotary_rotate(self.handle, ctypes.byref(xr), ctypes.byref(outr), at, n,
+                                     heads, dim, _stream(stream, x)), "rotate")
+
+    def close(self) -> None:
+        if self.handle:
+            lib().pf_rotary_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class AttentionWorkspace:
     """Device memory in which ``attend`` joins the shares of split sequences
     (pf_attend_workspace).  Calls that share one must be ordered: one workspace a
@@ -189,6 +335,35 @@ class PagedKVCache:
         last block, is padding and written nowhere (pf_kv_write)."""
         self._move(lib().pf_kv_write, "paged write", k, v, slots, stream)
 
+    def write_rotated(self, q, q_out, k, v, positions, slots, rotary: RotaryPositions,
+                      stream: Stream | None = None) -> None:
+        """Queries ``q`` [tokens, heads, head_dim], turned to their ``positions`` (int64),
+        into ``q_out`` (which may be ``q`` itself), and rows of ``k``, turned, and of ``v`` into
+        ``slots``, as ``write`` does (pf_kv_write_rotated).  A turned key is rounded once, to
+        what the pages hold.  Without queries ``q`` and ``q_out`` are None."""
+        kr, n, _ = _rows(k, self.num_kv_heads, self.head_dim, "k")
+        vr, m, _ = _rows(v, self.num_kv_heads, self.head_dim, "v")
+        at = _index(slots, 1, "int64", "slots")
+        places = _index(positions, 1, "int64", "positions")
+        if n != m or slots.shape[0] != n or positions.shape[0] != n:
+            raise ValueError(f"{n} rows of k, {m} of v, {positions.shape[0]} positions and "
+                             f"{slots.shape[0]} slots")
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out go together")
+        q_ref = out_ref = None
+        heads = 0
+        if q is not None:
+            qr, m, heads = _rows(q, None, self.head_dim, "q")
+            outr, m_out, _ = _rows(q_out, heads, self.head_dim, "q_out")
+            if m != n or m_out != n:
+                raise ValueError(f"{n} rows of k, {m} of q and {m_out} of q_out")
+            if heads > _MOST:
+                raise ValueError(f"{heads} heads are too many")
+            q_ref, out_ref = ctypes.byref(qr), ctypes.byref(outr)
+        check(lib().pf_kv_write_rotated(self._ref, rotary.handle, q_ref, out_ref, heads,
+                                        ctypes.byref(kr), ctypes.byref(vr), places, at, n,
+                                        _stream(stream, k)), "write_rotated")
+
     def read(self, slots, k, v, stream: Stream | None = None) -> None:
         """The values at ``slots`` into rows of ``k`` and ``v``; rows of padding slots
         are left as they were (pf_kv_read)."""
@@ -240,4 +415,105 @@ class PagedKVCache:
                                  _stream(stream, q)), "attend")
 
 
-__all__ = ["KV_TYPES", "AttentionWorkspace", "PagedKVCache", "segment_bytes"]
+class PagedLayers:
+    """All layers of a cache, ``PagedKVCache`` of one shape, for what moves blocks and tokens
+    within them, each layer alike (pf_kv_layers).  The layers' memory is borrowed; close it
+    after the last call, or graph, that uses it."""
+
+    def __init__(self, caches, device: int = 0):
+        self.handle = None
+        self.caches = list(caches)
+        if not self.caches:
+            raise ValueError("no layers")
+        h = ctypes.c_void_p()
+        pages = (KVPages * len(self.caches))(*[c._pages for c in self.caches])
+        check(lib().pf_kv_layers_create(device, pages, len(self.caches), ctypes.byref(h)),
+              "pf_kv_layers_create")
+        self.handle = h.value
+
+    def copy_blocks(self, from_blocks, to_blocks, stream: Stream | None = None) -> None:
+        """Block ``from_blocks[i]`` over block ``to_blocks[i]`` (int32), K and V, in every layer
+        (pf_kv_copy_blocks).  A block that does not exist makes its pair padding."""
+        src = _index(from_blocks, 1, "int32", "from_blocks")
+        dst = _index(to_blocks, 1, "int32", "to_blocks")
+        n = from_blocks.shape[0]
+        if to_blocks.shape[0] != n:
+            raise ValueError(f"{n} blocks to copy and {to_blocks.shape[0]} to copy to")
+        check(lib().pf_kv_copy_blocks(self.handle, src, dst, n, _stream(stream, from_blocks)),
+              "copy_blocks")
+
+    def fork(self, block_table, seq_lens, parents, new_blocks, out_table,
+             stream: Stream | None = None) -> None:
+        """Child i of sequence ``parents[i]`` (int32) gets row i of ``out_table``: its parent's
+        row of ``block_table``, with ``new_blocks[i]`` (int32) for its next token, into which
+        the parent's part-filled block, if any, is copied in every layer (pf_kv_fork).  A
+        negative new block leaves the row as the parent's; a parent that does not exist leaves
+        the child's row as it was."""
+        table = _index(block_table, 2, "int32", "block_table")
+        lens = _index(seq_lens, 1, "int32", "seq_lens")
+        who = _index(parents, 1, "int32", "parents")
+        new = _index(new_blocks, 1, "int32", "new_blocks")
+        out = _index(out_table, 2, "int32", "out_table")
+        seqs, width = block_table.shape
+        n = parents.shape[0]
+        if seq_lens.shape[0] != seqs or new_blocks.shape[0] != n or \
+                tuple(out_table.shape) != (n, width):
+            raise ValueError(f"{seqs} block tables of {width}, {seq_lens.shape[0]} lengths, {n} "
+                             f"parents, {new_blocks.shape[0]} new blocks and an out_table of "
+                             f"{tuple(out_table.shape)}")
+        if max(seqs, width, n) > _MOST:
+            raise ValueError("too many sequences")
+        args = ForkArgs(table, block_table.stride()[0], lens, who, new, out,
+                        out_table.stride()[0], seqs, width, n, 0)
+        check(lib().pf_kv_fork(self.handle, ctypes.byref(args), _stream(stream, block_table)),
+              "fork")
+
+    def compact(self, block_table, kept, kept_starts, *, first=None, out_table=None,
+                out_lens=None, max_kept: int = 0, stream: Stream | None = None) -> None:
+        """Moves the kept tokens of sequences together, in every layer (pf_kv_compact).
+
+        Sequence b keeps the tokens at positions ``kept[kept_starts[b]]`` to
+        ``kept[kept_starts[b + 1] - 1]`` (int32, ascending); they go to positions ``first[b]``
+        (int32; None: 0) and on of its row of ``out_table``, by default in place of what
+        ``block_table`` holds there.  In place no token may move up; other blocks that tokens
+        go to may not be among those that are read.  ``out_lens`` (int32), if given, receives
+        first + kept tokens; ``max_kept``, the most of a sequence, is a hint that shapes the
+        launch."""
+        table = _index(block_table, 2, "int32", "block_table")
+        at = _index(kept, 1, "int32", "kept")
+        starts = _index(kept_starts, 1, "int32", "kept_starts")
+        seqs, width = block_table.shape
+        if out_table is None:
+            out_table = block_table
+        out = _index(out_table, 2, "int32", "out_table")
+        if tuple(out_table.shape) != (seqs, width) or kept_starts.shape[0] != seqs + 1:
+            raise ValueError(f"block tables [{seqs}, {width}], an out_table of "
+                             f"{tuple(out_table.shape)} and {kept_starts.shape[0]} starts of kept "
+                             "tokens (one more than sequences)")
+        optional = []
+        for x, what in ((first, "first"), (out_lens, "out_lens")):
+            optional.append(0 if x is None else _index(x, 1, "int32", what))
+            if x is not None and x.shape[0] != seqs:
+                raise ValueError(f"{seqs} sequences and {x.shape[0]} of {what}")
+        if max(seqs, width) > _MOST:
+            raise ValueError("too many sequences")
+        args = CompactArgs(table, block_table.stride()[0], out, out_table.stride()[0], at,
+                           kept.shape[0], starts, optional[0], optional[1], seqs, width,
+                           _most("max_kept", max_kept), 0)
+        check(lib().pf_kv_compact(self.handle, ctypes.byref(args), _stream(stream, block_table)),
+              "compact")
+
+    def close(self) -> None:
+        if self.handle:
+            lib().pf_kv_layers_destroy(self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+__all__ = ["KV_TYPES", "AttentionWorkspace", "PagedKVCache", "PagedLayers", "RotaryPositions",
+           "segment_bytes"]
