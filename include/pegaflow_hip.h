@@ -770,6 +770,32 @@ int pf_attend_workspace_destroy(pf_attend_workspace* workspace);
 int pf_kv_attend(const pf_kv_pages* pages, const pf_attend_args* args,
                  pf_attend_workspace* workspace, pf_stream stream);
 
+/* Groups of neighbouring sequences that share their first tokens: those of group g, from
+ * group_starts[g] to group_starts[g+1] (ascending), hold the first shared_lens[g] tokens in the
+ * same blocks, the first of their rows of the block table.  Sequences before the first group and
+ * behind the last one share nothing. */
+typedef struct pf_shared_args {
+  uint64_t group_starts;   /* int32 [num_groups + 1], device */
+  uint64_t shared_lens;    /* int32 [num_groups], device */
+  uint32_t num_groups;
+  uint32_t max_shared_len; /* the longest shared length, and the most tokens that a sequence */
+  uint32_t max_own_len;    /* has behind its shared ones, new ones included: hints that shape */
+                           /* the launch (0: unknown)                                         */
+  uint32_t reserved;
+} pf_shared_args;
+/* pf_kv_attend, to the same definition, with the tokens that a group shares passed over once for
+ * all its sequences.  That takes a workspace with room for two shares or more of each row
+ * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
+ * 192, 256), a max_query_len that is not 0 and of at most 64 rows a KV head, and no window; any
+ * other call runs as pf_kv_attend.  New tokens are not shared: a group whose shared_lens
+ * reaches into those of one of its sequences (or past its end) is cut to what all have cached.
+ * args->max_seq_len is used where the hints of `shared` are not both given.  The weights of shared
+ * tokens are rounded once, those of a sequence's own to twice as many bits.  No bits change from
+ * call to call. */
+int pf_kv_attend_shared(const pf_kv_pages* pages, const pf_attend_args* args,
+                        const pf_shared_args* shared, pf_attend_workspace* workspace,
+                        pf_stream stream);
+
 /* ------------------------------------------------------------------------ */
 /* Synthetic data and verification kernels (benchmarks and parity tests).     */
 /* ------------------------------------------------------------------------ */

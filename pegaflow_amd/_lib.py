@@ -230,6 +230,19 @@ class AttendArgs(ctypes.Structure):
     ]
 
 
+class SharedArgs(ctypes.Structure):
+    """pf_shared_args — groups of sequences that share their first tokens."""
+
+    _fields_ = [
+        ("group_starts", ctypes.c_uint64),
+        ("shared_lens", ctypes.c_uint64),
+        ("num_groups", ctypes.c_uint32),
+        ("max_shared_len", ctypes.c_uint32),
+        ("max_own_len", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
 class ForkArgs(ctypes.Structure):
     """pf_fork_args — children of sequences, with blocks of their own."""
 
@@ -386,6 +399,8 @@ SIGNATURES = {
     "pf_attend_workspace_create": (i32, [i32, u64, pvp]),
     "pf_attend_workspace_destroy": (i32, [vp]),
     "pf_kv_attend": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(AttendArgs), vp, vp]),
+    "pf_kv_attend_shared": (i32, [ctypes.POINTER(KVPages), ctypes.POINTER(AttendArgs),
+                                  ctypes.POINTER(SharedArgs), vp, vp]),
     "pf_fill_random": (i32, [u64, u64, u64, u64, vp]),
     "pf_verify_random": (i32, [u64, u64, u64, u64, pu64]),
     "pf_verify_random_chunks": (i32, [pu64, pu64, u64, u64, u64, pu64]),

@@ -34,6 +34,8 @@ SOURCES = [
     "pf_pages.hip",
     "pf_attend_bf16.hip",
     "pf_attend_fp16.hip",
+    "pf_shared_bf16.hip",
+    "pf_shared_fp16.hip",
     "pf_load_state.cpp",
     "pf_engine.cpp",
     "pf_disk.cpp",
@@ -82,7 +84,7 @@ def build(verbose: bool = False) -> str:
 
     # The attention kernels take the longest: first.
     sources = sorted((s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))),
-                     key=lambda s: not s.startswith("pf_attend_"))
+                     key=lambda s: not s.startswith(("pf_attend_", "pf_shared_")))
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
         objs = list(pool.map(compile_one, sources))
     tmp = LIB + ".tmp"

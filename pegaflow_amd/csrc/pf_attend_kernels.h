@@ -494,6 +494,105 @@ __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, 
   return true;
 }
 
+// A group of sequences that share their first tokens: the first one that has rows, whose
+// blocks hold these, the rows of all, and the tokens that every row attends.  The whole wave
+// calls.
+struct Group {
+  uint32_t seq;
+  int32_t first, rows, shared;
+};
+// Starts of the group's sequences, bounded as in seq_of.
+__device__ __forceinline__ int32_t group_start(const AttendParams& a, uint32_t g) {
+  return min(max(a.group_starts[g], 0), static_cast<int32_t>(a.num_seqs));
+}
+__device__ __forceinline__ int32_t row_start(const AttendParams& a, uint32_t b) {
+  return min(max(a.query_starts[b], 0), static_cast<int32_t>(a.num_rows));
+}
+__device__ __forceinline__ Group group_of(const AttendParams& a, uint32_t g) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const int32_t first = group_start(a, g), last = max(group_start(a, g + 1), first);
+  const int32_t room = static_cast<int32_t>(a.table_width * a.pages.block_size);
+  Group out{0, row_start(a, first), 0, min(max(a.shared_lens[g], 0), room)};
+  out.rows = max(row_start(a, last) - out.first, 0);
+  bool found = false;
+  for (int32_t b0 = first; b0 < last; b0 += 64) {
+    const int32_t b = b0 + static_cast<int32_t>(lane);
+    int32_t most = 0x7fffffff;
+    if (b < last) {
+      const Seq s = seq_of(a, b);
+      if (s.rows) most = max(a.causal ? s.len - s.rows : s.len, 0);
+    }
+    const uint64_t with_rows = __ballot(most != 0x7fffffff);
+    if (with_rows && !found) {
+      out.seq = b0 + __builtin_ctzll(with_rows);
+      found = true;
+    }
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) most = min(most, __shfl_xor(most, step));
+    out.shared = min(out.shared, most);
+  }
+  out.seq = __builtin_amdgcn_readfirstlane(out.seq);
+  out.shared = __builtin_amdgcn_readfirstlane(out.shared);
+  return out;
+}
+
+// Tile `index` of the groups' rows, false if there is none or its group shares nothing.
+template <uint32_t ROWS>
+__device__ __forceinline__ bool shared_tile(const AttendParams& a, uint32_t index, uint32_t head,
+                                            uint32_t wave, ManyTile* t) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t g0 = 0; g0 < a.num_groups; g0 += 64) {
+    uint32_t tiles = 0;
+    if (g0 + lane < a.num_groups) {
+      const int32_t first = group_start(a, g0 + lane);
+      const int32_t last = max(group_start(a, g0 + lane + 1), first);
+      const uint32_t rows = static_cast<uint32_t>(max(row_start(a, last) - row_start(a, first), 0));
+      tiles = (rows * a.group + ROWS - 1) / ROWS;
+    }
+    uint32_t before = 0;
+    const uint32_t count = min(a.num_groups - g0, 64u);
+    for (uint32_t j = 0; j < count; ++j) {
+      const uint32_t n = __builtin_amdgcn_readlane(tiles, j);
+      if (index < before + n) {
+        const Group group = group_of(a, g0 + j);
+        if (group.shared == 0) return false;
+        const uint32_t row0 = (index - before) * ROWS;
+        t->seq = group.seq;
+        t->head = head;
+        t->s = {group.first, group.rows, group.shared};
+        t->rows = static_cast<uint32_t>(group.rows) * a.group;
+        t->row = row0 + wave * 32 + (lane & 31u);
+        t->begin = 0;
+        t->end = group.shared;
+        t->pos0 = 0;
+        t->valid = t->row < t->rows;
+        return true;
+      }
+      before += n;
+    }
+    index -= before;
+  }
+  return false;
+}
+
+// The group of sequence `seq`, and how many tokens it shares there (0 of none).
+__device__ __forceinline__ int32_t shared_of(const AttendParams& a, int32_t seq) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t g0 = 0; g0 < a.num_groups; g0 += 64) {
+    const uint32_t g = g0 + lane;
+    const uint64_t in =
+        __ballot(g < a.num_groups && group_start(a, g) <= seq && seq < group_start(a, g + 1));
+    if (in) return group_of(a, g0 + __builtin_ctzll(in)).shared;
+  }
+  return 0;
+}
+
+// A share of one row and query head, as an index to their outputs, and maxima and sums.
+__device__ __forceinline__ uint64_t share_at(const AttendParams& a, uint32_t share, uint32_t row,
+                                             uint32_t q_head) {
+  return (static_cast<uint64_t>(share) * a.num_rows + row) * a.q_heads + q_head;
+}
+
 __device__ __forceinline__ uint64_t row_address(const AttendParams& a, const RowsView& v,
                                                 const ManyTile& t) {
   const uint32_t token = t.row / a.group, g = t.row - token * a.group;
@@ -530,9 +629,11 @@ __device__ __forceinline__ void many_store(const AttendParams& a, const ManyTile
   many_lse<Row>(a, t, m, l);
 }
 
-template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
-__global__ void __launch_bounds__(2 * ROWS, DP <= 128 ? 2 : 1)
-attend_many_kernel(AttendParams a) {
+// Workgroup `index` of attend_many_kernel, or (SHARED) of attend_shared_kernel's tiles of the
+// tokens that groups of sequences share.
+template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS, bool SHARED>
+__device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& lds,
+                                            uint32_t index) {
   constexpr uint32_t kThreads = 2 * ROWS, kWaves = ROWS / 32;
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
@@ -547,24 +648,31 @@ attend_many_kernel(AttendParams a) {
   constexpr uint32_t kKP = k_pitch(DP), kVP = v_pitch(DP);
   constexpr int32_t kStep = kTileTokens;
   using Lds = ManyLds<DP>;
-  __shared__ Lds lds;
   const PagedView& pg = a.pages;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, half = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // Heads of one tile are neighbours: with 8 of them each has an XCD's L2 for its pages.
-  const uint32_t head = blockIdx.x % pg.heads;
-  const uint32_t rest = blockIdx.x / pg.heads;
+  const uint32_t head = index % pg.heads;
+  const uint32_t rest = index / pg.heads;
   uint32_t unit = rest, split = 0, splits = 1;
-  if (rest >= a.many_whole) {
-    splits = a.many_splits;
-    split = (rest - a.many_whole) % splits;
-    unit = a.many_whole + (rest - a.many_whole) / splits;
-  }
   ManyTile t;
-  if (!many_tile<ROWS>(a, unit, head, wave, &t)) return;
+  if constexpr (SHARED) {
+    splits = a.prefix_splits;
+    split = rest % splits;
+    unit = rest / splits;
+    if (!shared_tile<ROWS>(a, unit, head, wave, &t)) return;
+  } else {
+    if (rest >= a.many_whole) {
+      splits = a.many_splits;
+      split = (rest - a.many_whole) % splits;
+      unit = a.many_whole + (rest - a.many_whole) / splits;
+    }
+    if (!many_tile<ROWS>(a, unit, head, wave, &t)) return;
+  }
   int32_t begin = t.begin, end = t.end;
-  const uint32_t used = split_range(begin, end, split, splits, a.many_piece);
+  const uint32_t used =
+      split_range(begin, end, split, splits, SHARED ? a.prefix_piece : a.many_piece);
   if (split >= used) return;
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
@@ -573,11 +681,18 @@ attend_many_kernel(AttendParams a) {
   // Tokens that every row of the workgroup attends, and this wave's and row's.
   const uint32_t wave0 = __builtin_amdgcn_readfirstlane(t.row), group = a.group;
   const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + ROWS, t.rows) - 1;
-  const int32_t all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
-  const int32_t all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
-  const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
-  const int32_t my_begin = row_begin(a, pos);
-  const int32_t my_end = t.valid ? row_end(a, t.s.len, pos) : 0;
+  int32_t all_begin, all_end, my_begin, my_end;
+  if constexpr (SHARED) {  // every row attends them all
+    all_begin = my_begin = 0;
+    all_end = t.end;
+    my_end = t.valid ? t.end : 0;
+  } else {
+    all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
+    all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
+    const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
+    my_begin = row_begin(a, pos);
+    my_end = t.valid ? row_end(a, t.s.len, pos) : 0;
+  }
   const bool wave_rows = wave0 < t.rows;
 
   u32x4 q[DP / 16];
@@ -962,6 +1077,20 @@ attend_many_kernel(AttendParams a) {
   }
 
   l = sum32(l);
+  if constexpr (SHARED) {
+    if (!t.valid) return;
+    const uint32_t token = t.row / group, g = t.row - token * group;
+    const uint64_t at = share_at(a, split, t.s.first + token, head * group + g);
+    f32x4* part = reinterpret_cast<f32x4*>(a.share_o + at * DP) + half;
+#pragma unroll
+    for (uint32_t dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        part[dt * 8 + 2 * i] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
+                                     o[dt][4 * i + 3]};
+    if (half == 0) reinterpret_cast<f32x2*>(a.share_ml)[at] = f32x2{m, l};
+    return;
+  }
   if (used == 1) {
     many_store<Row, DP>(a, t, o, m, l);
     return;
@@ -977,6 +1106,13 @@ attend_many_kernel(AttendParams a) {
       part[(dt * 4 + i) * 64] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
                                       o[dt][4 * i + 3]};
   reinterpret_cast<f32x2*>(a.many_ml)[(slot * kWaves + wave) * 64 + lane] = f32x2{m, l};
+}
+
+template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
+__global__ void __launch_bounds__(2 * ROWS, DP <= 128 ? 2 : 1)
+attend_many_kernel(AttendParams a) {
+  __shared__ ManyLds<DP> lds;
+  attend_many<Row, TYPE, DP, ROWS, false>(a, lds, blockIdx.x);
 }
 
 // Joins the shares of split tiles.  A wave takes 32 rows and 32 values of each, in the
@@ -1103,9 +1239,23 @@ __device__ __forceinline__ void few_store(const AttendParams& a, const Seq& sq, 
   if (a.lse && d == 0) a.lse[at * a.q_heads + qh] = log_sum_exp<Row>(a, m, l);
 }
 
-template <class Row, uint32_t TYPE, uint32_t DP>
-__global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
-attend_few_kernel(AttendParams a) {
+template <uint32_t DP>
+struct FewLds {
+  struct Wave {
+    __attribute__((aligned(16))) uint8_t v[kFewTokens * few_v_pitch(DP)];
+    // Of 32 tokens to load next: where they lie; of the tile at hand: its scales.
+    uint64_t at[kFewTokens];
+    __attribute__((aligned(16))) float k_scale[kFewTokens], v_scale[kFewTokens];
+  } wave[kFewWaves];
+  float join_m[kFewWaves][16], join_l[kFewWaves][16];
+  bool finished;
+};
+
+// Workgroup `index` of attend_few_kernel, or (SHARED) of attend_shared_kernel's tiles of the
+// tokens that a sequence has to itself, 16 rows each.
+template <class Row, uint32_t TYPE, uint32_t DP, bool SHARED>
+__device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& mem,
+                                           uint32_t index) {
   constexpr bool kCodes = is_codes(TYPE);
   constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
   constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
@@ -1115,52 +1265,57 @@ attend_few_kernel(AttendParams a) {
   constexpr uint32_t kVLoads = (kFewTokens * kCols + 63) / 64;
   constexpr uint32_t kVP = few_v_pitch(DP);
   constexpr uint32_t kSteps = kKLoads * (kCodes ? 2 : 1);  // products of 32 values
-  struct WaveLds {
-    __attribute__((aligned(16))) uint8_t v[kFewTokens * kVP];
-    // Of 32 tokens to load next: where they lie; of the tile at hand: its scales.
-    uint64_t at[kFewTokens];
-    __attribute__((aligned(16))) float k_scale[kFewTokens], v_scale[kFewTokens];
-  };
-  __shared__ WaveLds lds[kFewWaves];
-  __shared__ float join_m[kFewWaves][16], join_l[kFewWaves][16];
-  __shared__ bool finished;
+  using WaveLds = typename FewLds<DP>::Wave;
+  WaveLds (&lds)[kFewWaves] = mem.wave;
+  float (&join_m)[kFewWaves][16] = mem.join_m, (&join_l)[kFewWaves][16] = mem.join_l;
+  bool& finished = mem.finished;
   const PagedView& pg = a.pages;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t head = blockIdx.x % pg.heads;
-  const uint32_t rest = blockIdx.x / pg.heads;
-  const uint32_t split = rest % a.few_splits, seq = rest / a.few_splits;
+  const uint32_t head = index % pg.heads;
+  const uint32_t rest = index / pg.heads;
+  const uint32_t splits = SHARED ? a.own_splits : a.few_splits, split = rest % splits;
+  const uint32_t seq = SHARED ? rest / splits / a.own_tiles : rest / splits;
+  const uint32_t row0 = SHARED ? rest / splits % a.own_tiles * kFewRows : 0;
   const int32_t* table = a.block_table + seq * a.table_stride;
   // Without a window a share starts at a token known from here on: a launch that is all
   // latency asks for its first block beside the sequence's length (a token behind 10,000
   // gains 0.8 us; where shares wait for their turn it costs 2%).
-  const bool ask_early = !a.window && gridDim.x <= 512;
+  const bool ask_early = !SHARED && !a.window && gridDim.x <= 512;
   int32_t early_block = -1;
   if (ask_early)
     early_block = table[page_of(pg, min(split * a.few_piece + wave * kFewTokens + (lane & 31u),
                                         a.table_width * pg.block_size - 1))];
   const Seq sq = seq_of(a, seq);
   uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
-  if (rows > kFewRows) {
-    if (a.many_units) return;  // attend_many_kernel's
-    rows = kFewRows;
+  int32_t shared = 0;
+  if constexpr (SHARED) {
+    if (rows <= row0) return;
+    rows = min(rows - row0, kFewRows);
+    shared = shared_of(a, static_cast<int32_t>(seq));
+  } else {
+    if (rows > kFewRows) {
+      if (a.many_units) return;  // attend_many_kernel's
+      rows = kFewRows;
+    }
+    if (rows > a.few_rows_most) rows = a.few_rows_most;  // more than the batch was said to have
+    if (rows == 0) return;
   }
-  if (rows > a.few_rows_most) rows = a.few_rows_most;  // more than the batch was said to have
-  if (rows == 0) return;
   const int32_t pos0 = sq.len - sq.rows;
   uint8_t* v_lds = lds[wave].v;
 
-  const uint32_t row = col, last = rows - 1;
-  const bool valid = row < rows;
+  const uint32_t row = row0 + col, last = row0 + rows - 1;
+  const bool valid = col < rows;
   const int32_t pos = pos0 + static_cast<int32_t>(row / a.group);
-  const int32_t my_begin = row_begin(a, pos);
+  const int32_t my_begin = SHARED ? shared : row_begin(a, pos);
   const int32_t my_end = valid ? row_end(a, sq.len, pos) : 0;
-  int32_t begin = row_begin(a, pos0) &
-                  ~static_cast<int32_t>(kFewTokens - 1);
+  int32_t begin = SHARED ? shared : row_begin(a, pos0) & ~static_cast<int32_t>(kFewTokens - 1);
   int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>(last / a.group));
-  const int32_t all_begin = row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
-  const int32_t all_end = row_end(a, sq.len, pos0);
-  const uint32_t used = split_range(begin, end, split, a.few_splits, a.few_piece);
+  const int32_t all_begin =
+      SHARED ? shared : row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
+  const int32_t all_end = row_end(a, sq.len, pos0 + static_cast<int32_t>(row0 / a.group));
+  const uint32_t used =
+      split_range(begin, end, split, splits, SHARED ? a.own_piece : a.few_piece);
   if (split >= used) return;
   const uint32_t token = row / a.group, g = row - token * a.group;
   const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
@@ -1469,7 +1624,7 @@ attend_few_kernel(AttendParams a) {
   __syncthreads();
   const uint64_t slot = (static_cast<uint64_t>(seq) * a.few_splits + split) * pg.heads + head;
   const __amdgpu_buffer_rsrc_t share = __builtin_amdgcn_make_buffer_rsrc(
-      a.few_o + (used > 1 ? slot * a.few_rows_most * DP : 0), 0,
+      a.few_o + (!SHARED && used > 1 ? slot * a.few_rows_most * DP : 0), 0,
       static_cast<int>(a.few_rows_most * DP * 4), 0x00027000);
   for (uint32_t i = tid; i < 16 * DP / 4; i += kFewThreads) {
     const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
@@ -1490,6 +1645,13 @@ attend_few_kernel(AttendParams a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
     }
+    if constexpr (SHARED) {
+      const uint32_t tok = (row0 + r) / a.group, qh = head * a.group + (row0 + r) - tok * a.group;
+      const uint64_t at = share_at(a, a.prefix_splits + split, sq.first + tok, qh);
+      *reinterpret_cast<f32x4*>(a.share_o + at * DP + d) = x;
+      if (d == 0) reinterpret_cast<f32x2*>(a.share_ml)[at] = f32x2{top, sum};
+      continue;
+    }
     if (used > 1) {
       // Written through the XCD's L2 (the sc1 policy of agent-scope stores, which the
       // language offers for at most 8 bytes at a time).
@@ -1504,7 +1666,7 @@ attend_few_kernel(AttendParams a) {
       few_store<Row>(a, sq, head, r, d, x, top, sum);
     }
   }
-  if (used == 1) return;
+  if (SHARED || used == 1) return;
   // The split that finishes last joins them all, in order.  Shares go through the XCD's
   // L2 to where every XCD sees them; a workgroup counts itself once its stores have been
   // acknowledged, and the last one puts the count back to 0 for the next call.
@@ -1611,6 +1773,13 @@ attend_few_kernel(AttendParams a) {
     if (mine && group * (groups > 1) == 0)
       few_store<Row>(a, sq, head, r, d, x, join_m[0][r], join_l[0][r]);
   }
+}
+
+template <class Row, uint32_t TYPE, uint32_t DP>
+__global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
+attend_few_kernel(AttendParams a) {
+  __shared__ FewLds<DP> lds;
+  attend_few<Row, TYPE, DP, false>(a, lds, blockIdx.x);
 }
 
 template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>

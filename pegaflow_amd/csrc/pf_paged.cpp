@@ -1,5 +1,5 @@
 // pf_paged.cpp — entry points of the paged-cache operators: argument checks, and
-// the launches (pf_paged.hip, pf_attend_*.hip).
+// the launches (pf_paged.hip, pf_attend_*.hip, pf_shared_*.hip).
 #include <algorithm>
 #include <cmath>
 
@@ -45,8 +45,9 @@ int move_rows(bool write, const pf_kv_pages* pages, const pf_kv_rows* k, const p
   return PF_OK;
 }
 
-int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspace* ws,
-           pf_stream stream) {
+// `shared`: the groups of sequences that share their first tokens, or null.
+int attend(const pf_kv_pages* pages, const pf_attend_args* a, const pf_shared_args* shared,
+           pf_attend_workspace* ws, pf_stream stream) {
   Ranges ranges;
   AttendParams p{};
   if (int rc = view_pages(pages, ranges, &p.pages)) return rc;
@@ -87,6 +88,16 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
     return rc;
   if (a->lse)
     if (int rc = add_array("lse", a->lse, a->num_rows * a->num_q_heads * 4, 4, ranges)) return rc;
+  const uint32_t groups = shared ? shared->num_groups : 0;
+  if (groups) {
+    if (groups >= (1u << 24)) return invalid("too many groups");
+    if (int rc = add_array("group_starts", shared->group_starts, (groups + 1ull) * 4, 4, ranges))
+      return rc;
+    if (int rc = add_array("shared_lens", shared->shared_lens, groups * 4ull, 4, ranges)) return rc;
+    p.group_starts = reinterpret_cast<const int32_t*>(shared->group_starts);
+    p.shared_lens = reinterpret_cast<const int32_t*>(shared->shared_lens);
+    p.num_groups = groups;
+  }
   if (int rc = ranges.check()) return rc;
   p.block_table = reinterpret_cast<const int32_t*>(a->block_table);
   p.table_stride = a->table_stride;
@@ -108,12 +119,23 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   p.q_sign = a->scale < 0 ? 0x80008000u : 0;
   p.aligned = aligned;
   while (p.unit_shift < 4 && !(pv.block_size >> p.unit_shift & 1u)) ++p.unit_shift;
-  plan_attend(&p, a->max_query_len, a->max_seq_len, ws ? ws->data : 0, ws ? ws->bytes : 0);
-  const uint64_t left = p.many_units - p.many_whole;
-  const uint64_t grid = std::max({static_cast<uint64_t>(p.num_seqs) * p.few_splits,
-                                  p.many_whole + left * p.many_splits,
-                                  left * (p.many_rows / 32) * (padded_dim(pv.dim) / 32)}) *
-                        pv.heads;
+  const uint64_t work = ws ? ws->data : 0, bytes = ws ? ws->bytes : 0;
+  const bool joined = groups && plan_shared(&p, a->max_query_len, shared->max_shared_len,
+                                            shared->max_own_len, work, bytes);
+  uint64_t grid = 0;
+  if (joined) {
+    grid = std::max(shared_grid(p), shared_join_grid(p));
+  } else {
+    uint64_t longest = a->max_seq_len;
+    if (shared && shared->max_shared_len && shared->max_own_len)
+      longest = static_cast<uint64_t>(shared->max_shared_len) + shared->max_own_len;
+    plan_attend(&p, a->max_query_len, longest, work, bytes);
+    const uint64_t left = p.many_units - p.many_whole;
+    grid = std::max({static_cast<uint64_t>(p.num_seqs) * p.few_splits,
+                     p.many_whole + left * p.many_splits,
+                     left * (p.many_rows / 32) * (padded_dim(pv.dim) / 32)}) *
+           pv.heads;
+  }
   if (grid > 0x7fffffffull) return invalid("too many rows");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
@@ -122,7 +144,10 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, pf_attend_workspac
   PF_HIP(hipGetDevice(&dev));
   if (ws && ws->device != dev)
     return invalid(strf("the workspace is on device %d, the stream on device %d", ws->device, dev));
-  PF_HIP(a->q.type == PF_KV_BF16 ? launch_attend_bf16(p, s) : launch_attend_fp16(p, s));
+  if (joined)
+    PF_HIP(a->q.type == PF_KV_BF16 ? launch_shared_bf16(p, s) : launch_shared_fp16(p, s));
+  else
+    PF_HIP(a->q.type == PF_KV_BF16 ? launch_attend_bf16(p, s) : launch_attend_fp16(p, s));
   return PF_OK;
 }
 
@@ -184,7 +209,16 @@ int pf_attend_workspace_destroy(pf_attend_workspace* workspace) {
 
 int pf_kv_attend(const pf_kv_pages* pages, const pf_attend_args* args,
                  pf_attend_workspace* workspace, pf_stream stream) {
-  return pf::guarded([&] { return pf::attend(pages, args, workspace, stream); });
+  return pf::guarded([&] { return pf::attend(pages, args, nullptr, workspace, stream); });
+}
+
+int pf_kv_attend_shared(const pf_kv_pages* pages, const pf_attend_args* args,
+                        const pf_shared_args* shared, pf_attend_workspace* workspace,
+                        pf_stream stream) {
+  return pf::guarded([&]() -> int {
+    if (!shared) return pf::invalid("null groups");
+    return pf::attend(pages, args, shared, workspace, stream);
+  });
 }
 
 }  // extern "C"

@@ -62,6 +62,17 @@ struct AttendParams {
   uint32_t many_units, many_rows, many_whole, many_splits, many_piece;
   float *few_o, *few_ml, *many_o, *many_ml;  // shares, in the workspace
   uint32_t* few_count;  // finished shares of each sequence and head, 0 between calls
+  // Groups of sequences that share their first tokens (attend_shared_kernel; num_groups 0:
+  // none do).  Group g has the sequences group_starts[g] to group_starts[g + 1].
+  const int32_t* group_starts;
+  const int32_t* shared_lens;
+  uint32_t num_groups;
+  // The launch (plan_shared): the groups' rows go in prefix_units tiles of kManyRows over the
+  // shared tokens, in prefix_splits shares of prefix_piece tokens, each sequence's in own_tiles
+  // tiles of kFewRows over its own, in own_splits shares of own_piece.  Every row and query head
+  // then has prefix_splits + own_splits places for shares.
+  uint32_t prefix_units, prefix_splits, prefix_piece, own_tiles, own_splits, own_piece;
+  float *share_o, *share_ml;  // in the workspace
 };
 
 constexpr uint32_t kFewRows = 16;        // of attend_few_kernel's tile
@@ -208,6 +219,67 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
   }
 }
 
+// Rows of a sequence and KV head up to which shared tokens are passed over once for a group: a
+// sequence with more fills tiles of its own, and reads them seldom enough.
+constexpr uint32_t kSharedRows = 64;
+constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
+
+// Shapes the launch of a batch whose groups share up to `most_shared` tokens, whose sequences
+// have up to `most_own` more and `most_new` rows, joining in `bytes` of workspace at `ws`.  Like
+// plan_attend's, lengths may be wrong and rows too few.  False where the batch is better off, or
+// has to be, attended by plan_attend's kernels.
+inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared,
+                        uint64_t most_own, uint64_t ws, uint64_t bytes) {
+  const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
+  const uint64_t room = static_cast<uint64_t>(p->table_width) * p->pages.block_size;
+  if (most_shared == 0 || most_shared > room) most_shared = room;
+  if (most_own == 0 || most_own > room) most_own = room;
+  if (most_new == 0 || most_new > p->num_rows) most_new = p->num_rows;
+  auto ceil_div = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
+  if (p->num_groups == 0 || p->num_seqs < 2 || p->window || most_new * group > kSharedRows)
+    return false;
+  p->own_tiles = static_cast<uint32_t>(ceil_div(most_new * group, kFewRows));
+  const uint64_t groups = p->num_groups < p->num_rows ? p->num_groups : p->num_rows;
+  const uint64_t tiles = p->num_rows * group / kManyRows + groups;
+  p->prefix_units = static_cast<uint32_t>(tiles);
+  constexpr uint64_t kPrefix = 256;  // workgroups
+  uint64_t splits = kPrefix / (tiles * heads);
+  if (splits < 1) splits = 1;
+  if (splits > kSharedMaxSplits) splits = kSharedMaxSplits;
+  uint64_t piece = ceil_div(ceil_div(most_shared, splits), 64) * 64;
+  if (piece < 256) piece = 256;
+  splits = ceil_div(most_shared, piece);
+  uint64_t own_piece = few_piece(p->num_seqs * p->own_tiles * heads, most_own);
+  uint64_t own_splits = ceil_div(most_own, own_piece);
+  if (own_splits > kSharedMaxSplits) own_splits = kSharedMaxSplits;
+  const uint64_t share = p->num_rows * p->q_heads * (dim * 4 + 8);
+  const uint64_t counts = workspace_counts(bytes) * kCountStride * 4;
+  const uint64_t most = (bytes - counts) / share;
+  if (most < 2) return false;
+  if (own_splits > most / 2) own_splits = most / 2;
+  if (splits > most - own_splits) splits = most - own_splits;
+  piece = ceil_div(ceil_div(most_shared, splits), 64) * 64;
+  own_piece = ceil_div(ceil_div(most_own, own_splits), 128) * 128;
+  p->prefix_splits = static_cast<uint32_t>(splits);
+  p->prefix_piece = static_cast<uint32_t>(piece);
+  p->own_splits = static_cast<uint32_t>(own_splits);
+  p->own_piece = static_cast<uint32_t>(own_piece);
+  p->share_o = reinterpret_cast<float*>(ws + counts);
+  p->share_ml = reinterpret_cast<float*>(ws + counts + (splits + own_splits) * p->num_rows *
+                                                           p->q_heads * dim * 4);
+  return true;
+}
+inline uint64_t shared_grid(const AttendParams& p) {
+  return (static_cast<uint64_t>(p.prefix_units) * p.prefix_splits +
+          static_cast<uint64_t>(p.num_seqs) * p.own_tiles * p.own_splits) *
+         p.pages.heads;
+}
+// Heads of a workgroup of attend_shared_join_kernel, one a wave.
+constexpr uint32_t kJoinHeads = 4;
+inline uint64_t shared_join_grid(const AttendParams& p) {
+  return static_cast<uint64_t>(p.num_rows) * ((p.q_heads + kJoinHeads - 1) / kJoinHeads);
+}
+
 hipError_t launch_kv_write(const PagedView& pages, const RowsView& k, const RowsView& v,
                            uint32_t row_type, const int64_t* slots, uint32_t n, bool aligned,
                            hipStream_t stream);
@@ -216,5 +288,7 @@ hipError_t launch_kv_read(const PagedView& pages, const RowsView& k, const RowsV
                           hipStream_t stream);
 hipError_t launch_attend_bf16(const AttendParams& p, hipStream_t stream);
 hipError_t launch_attend_fp16(const AttendParams& p, hipStream_t stream);
+hipError_t launch_shared_bf16(const AttendParams& p, hipStream_t stream);
+hipError_t launch_shared_fp16(const AttendParams& p, hipStream_t stream);
 
 }  // namespace pf

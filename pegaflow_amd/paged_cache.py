@@ -24,7 +24,7 @@ import math
 import sys
 
 from . import _lib
-from ._lib import AttendArgs, CompactArgs, ForkArgs, KVPages, KVRows, check
+from ._lib import AttendArgs, CompactArgs, ForkArgs, KVPages, KVRows, SharedArgs, check
 from .runtime import Stream
 from .transfer import KVCacheRegistration
 
@@ -385,6 +385,44 @@ class PagedKVCache:
         rows, and those that one has beyond it may stay as they were.  Without a
         ``workspace`` no sequence is split, which is slow where few rows attend
         long sequences."""
+        args = self._attend_args(q, out, block_table, seq_lens, query_starts, scale, causal,
+                                 window, lse, max_seq_len, max_query_len)
+        check(lib().pf_kv_attend(self._ref, ctypes.byref(args),
+                                 workspace.handle if workspace is not None else None,
+                                 _stream(stream, q)), "attend")
+
+    def attend_shared(self, q, out, block_table, seq_lens, query_starts, group_starts, shared_lens,
+                      *, scale: float | None = None, causal: bool = True, lse=None,
+                      max_shared_len: int = 0, max_own_len: int = 0, max_query_len: int = 0,
+                      workspace: AttentionWorkspace | None = None,
+                      stream: Stream | None = None) -> None:
+        """``attend`` of a batch in which groups of sequences share their first tokens, which
+        are passed over once for all of a group (pf_kv_attend_shared).
+
+        The sequences of group g are ``group_starts[g]`` to ``group_starts[g + 1]`` (int32);
+        the first entries of their rows of ``block_table`` are the same blocks, in which their
+        first ``shared_lens[g]`` tokens lie (int32; none of them new).  Others share nothing.
+        ``max_shared_len`` and ``max_own_len``, the most tokens that a group shares and that a
+        sequence has behind these, are hints that shape the launch.  Sharing takes a
+        ``workspace`` and a ``max_query_len`` (at most 64 rows a KV head); without, the call
+        runs as ``attend``."""
+        starts = _index(group_starts, 1, "int32", "group_starts")
+        lens = _index(shared_lens, 1, "int32", "shared_lens")
+        groups = shared_lens.shape[0]
+        if group_starts.shape[0] != groups + 1:
+            raise ValueError(f"{groups} shared lengths and {group_starts.shape[0]} group starts "
+                             "(one more than groups)")
+        args = self._attend_args(q, out, block_table, seq_lens, query_starts, scale, causal, 0,
+                                 lse, 0, max_query_len)
+        shared = SharedArgs(starts, lens, min(groups, _MOST),
+                            _most("max_shared_len", max_shared_len),
+                            _most("max_own_len", max_own_len), 0)
+        check(lib().pf_kv_attend_shared(self._ref, ctypes.byref(args), ctypes.byref(shared),
+                                        workspace.handle if workspace is not None else None,
+                                        _stream(stream, q)), "attend_shared")
+
+    def _attend_args(self, q, out, block_table, seq_lens, query_starts, scale, causal, window, lse,
+                     max_seq_len, max_query_len) -> AttendArgs:
         qr, n, heads = _rows(q, None, self.head_dim, "q")
         outr, m, out_heads = _rows(out, heads, self.head_dim, "out")
         if n != m:
@@ -406,13 +444,11 @@ class PagedKVCache:
             if n and heads and (stride[1] != 1 and heads > 1 or stride[0] != heads and n > 1):
                 raise ValueError("lse is not contiguous")
             lse_at = lse.data_ptr()
-        args = AttendArgs(qr, outr, n, table, block_table.stride()[0], lens, starts, lse_at, heads,
+        return AttendArgs(qr, outr, n, table, block_table.stride()[0], lens, starts, lse_at, heads,
                           seqs, width, min(window, _MOST), causal,
                           1 / math.sqrt(self.head_dim) if scale is None else scale,
                           min(max_seq_len, _MOST), min(max_query_len, _MOST))
-        check(lib().pf_kv_attend(self._ref, ctypes.byref(args),
-                                 workspace.handle if workspace is not None else None,
-                                 _stream(stream, q)), "attend")
+
 
 
 class PagedLayers:
