@@ -787,8 +787,8 @@ typedef struct pf_shared_args {
  * all its sequences.  That takes a workspace with room for two shares or more of each row
  * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
  * 192, 256), a max_query_len that is not 0 and of at most 64 rows a KV head, and no window; any
- * other call runs as pf_kv_attend.  New tokens are not shared: a group whose shared_lens
- * reaches into those of one of its sequences (or past its end) is cut to what all have cached.
+ * other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a sequence
+ * takes as many as it has cached (in front of its new ones).
  * args->max_seq_len is used where the hints of `shared` are not both given.  The weights of shared
  * tokens are rounded once, those of a sequence's own to twice as many bits.  No bits change from
  * call to call. */

@@ -494,97 +494,133 @@ __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, 
   return true;
 }
 
-// A group of sequences that share their first tokens: the first one that has rows, whose
-// blocks hold these, the rows of all, and the tokens that every row attends.  The whole wave
-// calls.
-struct Group {
-  uint32_t seq;
-  int32_t first, rows, shared;
-};
-// Starts of the group's sequences, bounded as in seq_of.
+// Groups of sequences that share their first tokens.  Starts are bounded as in seq_of.
 __device__ __forceinline__ int32_t group_start(const AttendParams& a, uint32_t g) {
   return min(max(a.group_starts[g], 0), static_cast<int32_t>(a.num_seqs));
 }
 __device__ __forceinline__ int32_t row_start(const AttendParams& a, uint32_t b) {
   return min(max(a.query_starts[b], 0), static_cast<int32_t>(a.num_rows));
 }
-__device__ __forceinline__ Group group_of(const AttendParams& a, uint32_t g) {
-  const uint32_t lane = threadIdx.x & 63u;
-  const int32_t first = group_start(a, g), last = max(group_start(a, g + 1), first);
-  const int32_t room = static_cast<int32_t>(a.table_width * a.pages.block_size);
-  Group out{0, row_start(a, first), 0, min(max(a.shared_lens[g], 0), room)};
-  out.rows = max(row_start(a, last) - out.first, 0);
-  bool found = false;
-  for (int32_t b0 = first; b0 < last; b0 += 64) {
-    const int32_t b = b0 + static_cast<int32_t>(lane);
-    int32_t most = 0x7fffffff;
-    if (b < last) {
-      const Seq s = seq_of(a, b);
-      if (s.rows) most = max(a.causal ? s.len - s.rows : s.len, 0);
-    }
-    const uint64_t with_rows = __ballot(most != 0x7fffffff);
-    if (with_rows && !found) {
-      out.seq = b0 + __builtin_ctzll(with_rows);
-      found = true;
-    }
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) most = min(most, __shfl_xor(most, step));
-    out.shared = min(out.shared, most);
-  }
-  out.seq = __builtin_amdgcn_readfirstlane(out.seq);
-  out.shared = __builtin_amdgcn_readfirstlane(out.shared);
-  return out;
+// Tokens that all rows of a sequence attend, if it shares them: none of its new ones.
+__device__ __forceinline__ int32_t cached_of(const AttendParams& a, const Seq& s) {
+  return max(a.causal ? s.len - s.rows : s.len, 0);
 }
-
-// Tile `index` of the groups' rows, false if there is none or its group shares nothing.
-template <uint32_t ROWS>
-__device__ __forceinline__ bool shared_tile(const AttendParams& a, uint32_t index, uint32_t head,
-                                            uint32_t wave, ManyTile* t) {
+// How many tokens sequence `seq` shares: its group's, of those that it has cached.  The whole
+// wave calls.
+__device__ __forceinline__ int32_t shared_of(const AttendParams& a, int32_t seq, const Seq& s) {
   const uint32_t lane = threadIdx.x & 63u;
   for (uint32_t g0 = 0; g0 < a.num_groups; g0 += 64) {
+    const uint32_t g = g0 + lane;
+    int32_t shared = 0;
+    bool mine = false;
+    if (g < a.num_groups) {
+      shared = a.shared_lens[g];
+      mine = group_start(a, g) <= seq && seq < group_start(a, g + 1);
+    }
+    const uint64_t in = __ballot(mine);
+    if (in) {
+      shared = __builtin_amdgcn_readlane(shared, __builtin_ctzll(in));
+      return min(max(shared, 0), cached_of(a, s));
+    }
+  }
+  return 0;
+}
+
+// Tile `index` of the rows of group `g`: those of its sequences one after another.  A row
+// attends as many of the shared tokens, `my_end`, as its sequence has cached, all rows at least
+// `all_end`; the tile passes over those that any sequence has, in that one's blocks.
+template <uint32_t ROWS>
+__device__ __forceinline__ bool group_tile(const AttendParams& a, uint32_t g, uint32_t index,
+                                           uint32_t wave, ManyTile* t, int32_t* all_end,
+                                           int32_t* my_end) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const int32_t first = group_start(a, g), last = max(group_start(a, g + 1), first);
+  const int32_t first_row = row_start(a, first);
+  const int32_t room = static_cast<int32_t>(a.table_width * a.pages.block_size);
+  int32_t shared = min(max(a.shared_lens[g], 0), room);
+  t->rows = static_cast<uint32_t>(max(row_start(a, last) - first_row, 0)) * a.group;
+  t->s = {first_row, 0, 0};
+  t->row = index * ROWS + wave * 32 + (lane & 31u);
+  t->valid = t->row < t->rows;
+  const int32_t token = first_row + static_cast<int32_t>(t->row / a.group);
+  constexpr int32_t kNone = 0x7fffffff;
+  constexpr uint32_t kChunks = 4;  // of 64 sequences, whose loads are under way together
+  int32_t least = kNone, most = -1, mine = 0;
+  for (int32_t b0 = first; b0 < last; b0 += 64 * kChunks) {
+    int32_t start[kChunks], cached[kChunks], end[kChunks];
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      const int32_t b = b0 + static_cast<int32_t>(c * 64 + lane);
+      start[c] = kNone;
+      cached[c] = end[c] = -1;
+      if (b < last) {
+        const Seq s = seq_of(a, b);
+        start[c] = s.first;
+        end[c] = s.first + s.rows;
+        if (s.rows) cached[c] = cached_of(a, s);
+      }
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < kChunks; ++c) {
+      if (b0 + static_cast<int32_t>(c * 64) >= last) break;
+      int32_t lo = cached[c] < 0 ? kNone : cached[c], hi = cached[c];
+#pragma unroll
+      for (int step = 1; step < 64; step *= 2) {
+        lo = min(lo, __shfl_xor(lo, step));
+        hi = max(hi, __shfl_xor(hi, step));
+      }
+      least = min(least, lo);
+      if (hi > most) {
+        most = hi;
+        t->seq = b0 + c * 64 + __builtin_ctzll(__ballot(cached[c] == hi));
+      }
+      // The last sequence that starts at this lane's token or before: starts ascend.
+      int at = 0;
+#pragma unroll
+      for (int step = 32; step; step /= 2) {
+        const int32_t then = __shfl(start[c], at + step);
+        at += then <= token ? step : 0;
+      }
+      // All lanes read before any decides: a lane reads nothing of one that does not take part.
+      const int32_t from = __shfl(start[c], at), to = __shfl(end[c], at);
+      const int32_t has = __shfl(cached[c], at);
+      mine = from <= token && token < to ? has : mine;
+    }
+  }
+  shared = min(shared, most);
+  if (shared <= 0) return false;
+  t->seq = __builtin_amdgcn_readfirstlane(t->seq);
+  t->begin = 0;
+  t->end = shared;
+  *all_end = __builtin_amdgcn_readfirstlane(min(shared, least));
+  *my_end = t->valid ? min(shared, mine) : 0;
+  return true;
+}
+
+// Tile `index` of all groups' rows, false if there is none or its group shares nothing.
+template <uint32_t ROWS>
+__device__ __forceinline__ bool shared_tile(const AttendParams& a, uint32_t index, uint32_t head,
+                                            uint32_t wave, ManyTile* t, int32_t* all_end,
+                                            int32_t* my_end) {
+  const uint32_t lane = threadIdx.x & 63u;
+  t->head = head;
+  t->pos0 = 0;
+  for (uint32_t g0 = 0; g0 < a.num_groups; g0 += 64) {
     uint32_t tiles = 0;
-    if (g0 + lane < a.num_groups) {
+    const uint32_t count = min(a.num_groups - g0, 64u);
+    if (lane < count) {
       const int32_t first = group_start(a, g0 + lane);
       const int32_t last = max(group_start(a, g0 + lane + 1), first);
       const uint32_t rows = static_cast<uint32_t>(max(row_start(a, last) - row_start(a, first), 0));
       tiles = (rows * a.group + ROWS - 1) / ROWS;
     }
-    uint32_t before = 0;
-    const uint32_t count = min(a.num_groups - g0, 64u);
     for (uint32_t j = 0; j < count; ++j) {
       const uint32_t n = __builtin_amdgcn_readlane(tiles, j);
-      if (index < before + n) {
-        const Group group = group_of(a, g0 + j);
-        if (group.shared == 0) return false;
-        const uint32_t row0 = (index - before) * ROWS;
-        t->seq = group.seq;
-        t->head = head;
-        t->s = {group.first, group.rows, group.shared};
-        t->rows = static_cast<uint32_t>(group.rows) * a.group;
-        t->row = row0 + wave * 32 + (lane & 31u);
-        t->begin = 0;
-        t->end = group.shared;
-        t->pos0 = 0;
-        t->valid = t->row < t->rows;
-        return true;
-      }
-      before += n;
+      if (index < n) return group_tile<ROWS>(a, g0 + j, index, wave, t, all_end, my_end);
+      index -= n;
     }
-    index -= before;
   }
   return false;
-}
-
-// The group of sequence `seq`, and how many tokens it shares there (0 of none).
-__device__ __forceinline__ int32_t shared_of(const AttendParams& a, int32_t seq) {
-  const uint32_t lane = threadIdx.x & 63u;
-  for (uint32_t g0 = 0; g0 < a.num_groups; g0 += 64) {
-    const uint32_t g = g0 + lane;
-    const uint64_t in =
-        __ballot(g < a.num_groups && group_start(a, g) <= seq && seq < group_start(a, g + 1));
-    if (in) return group_of(a, g0 + __builtin_ctzll(in)).shared;
-  }
-  return 0;
 }
 
 // A share of one row and query head, as an index to their outputs, and maxima and sums.
@@ -657,11 +693,12 @@ __device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& 
   const uint32_t rest = index / pg.heads;
   uint32_t unit = rest, split = 0, splits = 1;
   ManyTile t;
+  int32_t all_begin, all_end, my_begin, my_end;
   if constexpr (SHARED) {
     splits = a.prefix_splits;
     split = rest % splits;
     unit = rest / splits;
-    if (!shared_tile<ROWS>(a, unit, head, wave, &t)) return;
+    if (!shared_tile<ROWS>(a, unit, head, wave, &t, &all_end, &my_end)) return;
   } else {
     if (rest >= a.many_whole) {
       splits = a.many_splits;
@@ -681,11 +718,8 @@ __device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& 
   // Tokens that every row of the workgroup attends, and this wave's and row's.
   const uint32_t wave0 = __builtin_amdgcn_readfirstlane(t.row), group = a.group;
   const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + ROWS, t.rows) - 1;
-  int32_t all_begin, all_end, my_begin, my_end;
-  if constexpr (SHARED) {  // every row attends them all
+  if constexpr (SHARED) {
     all_begin = my_begin = 0;
-    all_end = t.end;
-    my_end = t.valid ? t.end : 0;
   } else {
     all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
     all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
@@ -1223,7 +1257,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_many_join_kernel(AttendPa
 // was known).  Eight waves a workgroup, or tokens under way two tiles ahead (16.1 ->
 // 17.5), gained nothing.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kFewWaves = 4, kFewThreads = kFewWaves * 64;
+constexpr uint32_t kFewThreads = kFewWaves * 64;
 constexpr uint32_t kFewTokens = 32;
 constexpr uint32_t few_v_pitch(uint32_t dp) { return 2 * dp + 32; }
 
@@ -1252,7 +1286,7 @@ struct FewLds {
 };
 
 // Workgroup `index` of attend_few_kernel, or (SHARED) of attend_shared_kernel's tiles of the
-// tokens that a sequence has to itself, 16 rows each.
+// tokens that a sequence has to itself, 16 rows each, of which each takes own_waves waves.
 template <class Row, uint32_t TYPE, uint32_t DP, bool SHARED>
 __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& mem,
                                            uint32_t index) {
@@ -1272,8 +1306,18 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   const PagedView& pg = a.pages;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t head = index % pg.heads;
-  const uint32_t rest = index / pg.heads;
+  // The waves that share a unit: this one's place among them, and the first.
+  const uint32_t waves = SHARED ? a.own_waves : kFewWaves;
+  const uint32_t turn = SHARED ? wave % waves : wave, wave0 = wave - turn;
+  bool active = true;  // SHARED: of a unit without a share, whose waves only meet the others
+  uint32_t unit = index;
+  if constexpr (SHARED) {
+    unit = index * (kFewWaves / waves) + wave / waves;
+    active = unit < a.num_seqs * a.own_tiles * a.own_splits * pg.heads;
+    if (!active) unit = 0;
+  }
+  const uint32_t head = unit % pg.heads;
+  const uint32_t rest = unit / pg.heads;
   const uint32_t splits = SHARED ? a.own_splits : a.few_splits, split = rest % splits;
   const uint32_t seq = SHARED ? rest / splits / a.own_tiles : rest / splits;
   const uint32_t row0 = SHARED ? rest / splits % a.own_tiles * kFewRows : 0;
@@ -1290,9 +1334,9 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
   int32_t shared = 0;
   if constexpr (SHARED) {
-    if (rows <= row0) return;
-    rows = min(rows - row0, kFewRows);
-    shared = shared_of(a, static_cast<int32_t>(seq));
+    active = active && rows > row0;
+    rows = active ? min(rows - row0, kFewRows) : 1;
+    shared = shared_of(a, static_cast<int32_t>(seq), sq);
   } else {
     if (rows > kFewRows) {
       if (a.many_units) return;  // attend_many_kernel's
@@ -1314,9 +1358,27 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   const int32_t all_begin =
       SHARED ? shared : row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
   const int32_t all_end = row_end(a, sq.len, pos0 + static_cast<int32_t>(row0 / a.group));
-  const uint32_t used =
-      split_range(begin, end, split, splits, SHARED ? a.own_piece : a.few_piece);
-  if (split >= used) return;
+  uint32_t used = 0;
+  if constexpr (SHARED) {
+    // Shares are those of the sequence, and the same for all its tiles.
+    const int32_t tile_end = end;
+    end = row_end(a, sq.len, pos0 + sq.rows - 1);
+    used = split_range(begin, end, split, splits, a.own_piece);
+    end = min(end, tile_end);
+    active = active && split < used;
+    // The join is told how many there are of each kind, 0 of a row beyond the tiles.
+    if (active && head == 0 && split == 0 && row0 == 0 && turn == 0) {
+      int32_t b = 0, e = shared;
+      const uint32_t prefix = shared ? split_range(b, e, 0, a.prefix_splits, a.prefix_piece) : 0;
+      for (uint32_t i = lane; i < static_cast<uint32_t>(sq.rows); i += 64)
+        a.share_info[sq.first + i] =
+            (i + 1) * a.group <= a.own_tiles * kFewRows ? prefix | used << 8 : 0;
+    }
+    if (!active) end = begin;
+  } else {
+    used = split_range(begin, end, split, splits, a.few_piece);
+    if (split >= used) return;
+  }
   const uint32_t token = row / a.group, g = row - token * a.group;
   const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
                                      static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
@@ -1326,7 +1388,7 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   for (uint32_t i = 0; i < kSteps; ++i)
     q[i] = load_q8(q_row,
                    kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
-                   valid);
+                   valid && active);
   f32x4 o[DP / 16];
 #pragma unroll
   for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
@@ -1384,7 +1446,7 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
           pg.v + lds[wave].at[(lane + i * 64) / kCols] + v_at[i]);
   };
 
-  constexpr int32_t kStep = kFewTokens * kFewWaves;
+  const int32_t kStep = static_cast<int32_t>(kFewTokens * waves);
   auto tile = [&](int32_t t0) {
     const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kFewTokens) > all_end;
     const bool masked = partial || there != 0xffffffffu;
@@ -1556,7 +1618,7 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  int32_t t0 = begin + static_cast<int32_t>(wave * kFewTokens);
+  int32_t t0 = begin + static_cast<int32_t>(turn * kFewTokens);
   if (t0 < end) {
     if (ask_early)
       block = t0 + static_cast<int32_t>(lane & 31u) < end ? early_block : -1;
@@ -1579,7 +1641,7 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   if (TYPE != PF_KV_INT8 && __builtin_expect(__any(odd), 0)) {
 #pragma unroll
     for (uint32_t dt = 0; dt < DP / 16; ++dt) lose_nan<4>(o[dt]);
-    for (int32_t t1 = begin + static_cast<int32_t>(wave * kFewTokens); t1 < end; t1 += kStep) {
+    for (int32_t t1 = begin + static_cast<int32_t>(turn * kFewTokens); t1 < end; t1 += kStep) {
       const uint64_t tokens = odd_tokens<Row, TYPE>(
           pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
       for (uint64_t left = tokens; left; left &= left - 1) {
@@ -1626,22 +1688,25 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
   const __amdgpu_buffer_rsrc_t share = __builtin_amdgcn_make_buffer_rsrc(
       a.few_o + (!SHARED && used > 1 ? slot * a.few_rows_most * DP : 0), 0,
       static_cast<int>(a.few_rows_most * DP * 4), 0x00027000);
-  for (uint32_t i = tid; i < 16 * DP / 4; i += kFewThreads) {
+  if (!active) return;
+  for (uint32_t i = tid - wave0 * 64; i < 16 * DP / 4; i += waves * 64) {
     const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
     if (r >= rows) continue;
     float top = kNegInf;
 #pragma unroll
-    for (uint32_t w = 0; w < kFewWaves; ++w) top = fmaxf(top, join_m[w][r]);
+    for (uint32_t w = 0; w < kFewWaves; ++w)
+      if (w < waves) top = fmaxf(top, join_m[wave0 + w][r]);
     float sum = 0.0f;
     f32x4 x{0, 0, 0, 0};
 #pragma unroll
     for (uint32_t w = 0; w < kFewWaves; ++w) {
-      const float mw = join_m[w][r], lw = join_l[w][r];
+      if (w >= waves) break;
+      const float mw = join_m[wave0 + w][r], lw = join_l[wave0 + w][r];
       const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
                                        : share_factor(mw - top);
       sum += lw * keep;
-      const f32x4 y =
-          *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w].v) + r * DP + d);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(
+          reinterpret_cast<const float*>(lds[wave0 + w].v) + r * DP + d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
     }

@@ -34,10 +34,11 @@ attend_shared_kernel(AttendParams a) {
 }
 
 // Joins the shares of a row: a wave to a query head, 4 values a lane, shares in turn where a
-// head's values take part of a wave only.
+// head's values take part of a wave only.  Everything that a wave reads is asked for at once, also
+// the places of shares that turn out to be none: one wait instead of three.
 template <class Row, uint32_t DP>
 __global__ void __launch_bounds__(kJoinHeads * 64) attend_shared_join_kernel(AttendParams a) {
-  constexpr uint32_t kLanes = DP / 4, kTurns = 64 / kLanes;
+  constexpr uint32_t kLanes = DP / 4, kTurns = 64 / kLanes, kFlight = 8;
   static_assert(2 * kSharedMaxSplits <= 64, "a lane for each share");
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t per_row = (a.q_heads + kJoinHeads - 1) / kJoinHeads;
@@ -45,38 +46,26 @@ __global__ void __launch_bounds__(kJoinHeads * 64) attend_shared_join_kernel(Att
   const uint32_t q_head = __builtin_amdgcn_readfirstlane(blockIdx.x % per_row * kJoinHeads +
                                                          (threadIdx.x >> 6));
   if (q_head >= a.q_heads) return;
-  // The row's sequence.
-  uint32_t seq = a.num_seqs;
-  for (uint32_t b0 = 0; b0 < a.num_seqs; b0 += 64) {
-    const uint32_t b = b0 + lane;
-    const uint64_t in = __ballot(b < a.num_seqs && a.query_starts[b] <= static_cast<int32_t>(row) &&
-                                 static_cast<int32_t>(row) < a.query_starts[b + 1]);
-    if (in) {
-      seq = b0 + __builtin_ctzll(in);
-      break;
-    }
-  }
-  if (seq == a.num_seqs) return;  // of none: stays as it was
-  const Seq sq = seq_of(a, seq);
-  const uint32_t head = q_head / a.group;
-  const uint32_t in_seq = (row - static_cast<uint32_t>(sq.first)) * a.group + q_head - head * a.group;
-  const uint32_t tile = in_seq / kFewRows;
-  if (tile >= a.own_tiles) return;  // more rows than the batch was said to have
-  const int32_t shared = shared_of(a, static_cast<int32_t>(seq));
-  int32_t begin = 0, end = shared;
-  const uint32_t prefix =
-      shared ? split_range(begin, end, 0, a.prefix_splits, a.prefix_piece) : 0;
-  // Of its tile, as attend_few counts them.
-  const uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
-  const uint32_t last = min((tile + 1) * kFewRows, rows) - 1;
-  begin = shared;
-  end = row_end(a, sq.len, sq.len - sq.rows + static_cast<int32_t>(last / a.group));
-  const uint32_t used = prefix + split_range(begin, end, 0, a.own_splits, a.own_piece);
-  auto share = [&](uint32_t i) {
-    return share_at(a, i < prefix ? i : a.prefix_splits + i - prefix, row, q_head);
-  };
+  const uint32_t turn = lane / kLanes, d = lane % kLanes * 4;
+  const uint32_t places = a.prefix_splits + a.own_splits;
   f32x2 ml{kNegInf, 0.0f};
-  if (lane < used) ml = reinterpret_cast<const f32x2*>(a.share_ml)[share(lane)];
+  if (lane < places) ml = reinterpret_cast<const f32x2*>(a.share_ml)[share_at(a, lane, row, q_head)];
+  auto part = [&](uint32_t i) {
+    f32x4 x{0, 0, 0, 0};
+    if (turn < kTurns && i < places)
+      x = *reinterpret_cast<const f32x4*>(a.share_o + share_at(a, i, row, q_head) * DP + d);
+    return x;
+  };
+  f32x4 x[kFlight];
+#pragma unroll
+  for (uint32_t j = 0; j < kFlight; ++j) x[j] = part(j * kTurns + turn);
+  const uint32_t info = a.share_info[row];
+  const int32_t first = row_start(a, 0), last = row_start(a, a.num_seqs);
+  // A row of no sequence, or beyond the rows that one was said to have, stays as it was.
+  if (static_cast<int32_t>(row) < first || static_cast<int32_t>(row) >= last || info == 0) return;
+  // Shares 0 to prefix - 1 and prefix_splits to `end` - 1 are there.
+  const uint32_t prefix = info & 0xffu, end = a.prefix_splits + (info >> 8);
+  if (lane >= end || (lane >= prefix && lane < a.prefix_splits)) ml = f32x2{kNegInf, 0.0f};
   float m = ml[0];
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) m = fmaxf(m, __shfl_xor(m, step));
@@ -86,34 +75,30 @@ __global__ void __launch_bounds__(kJoinHeads * 64) attend_shared_join_kernel(Att
   float l = ml[1] * factor;
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) l += __shfl_xor(l, step);
-  const uint32_t turn = lane / kLanes, d = lane % kLanes * 4;
   f32x4 o{0, 0, 0, 0};
-  constexpr uint32_t kFlight = 4;  // loads under way together
-  for (uint32_t i0 = 0; i0 < used; i0 += kTurns * kFlight) {
-    f32x4 x[kFlight];
-    float f[kFlight];
+  auto add = [&](uint32_t i0, const f32x4 (&y)[kFlight]) {
 #pragma unroll
     for (uint32_t j = 0; j < kFlight; ++j) {
       const uint32_t i = i0 + j * kTurns + turn;
-      x[j] = f32x4{0, 0, 0, 0};
-      f[j] = __shfl(factor, static_cast<int>(i & 63u));
-      if (turn < kTurns && i < used)
-        x[j] = *reinterpret_cast<const f32x4*>(a.share_o + share(i) * DP + d);
-    }
+      const float f = __shfl(factor, static_cast<int>(i & 63u));
+      const bool there = i < prefix || (i >= a.prefix_splits && i < end);
 #pragma unroll
-    for (uint32_t j = 0; j < kFlight; ++j) {
-      const bool mine = turn < kTurns && i0 + j * kTurns + turn < used;
-#pragma unroll
-      for (int v = 0; v < 4; ++v) o[v] += mine ? x[j][v] * f[j] : 0.0f;
+      for (int v = 0; v < 4; ++v) o[v] += there ? y[j][v] * f : 0.0f;
     }
+  };
+  add(0, x);
+  for (uint32_t i0 = kTurns * kFlight; i0 < places; i0 += kTurns * kFlight) {
+#pragma unroll
+    for (uint32_t j = 0; j < kFlight; ++j) x[j] = part(i0 + j * kTurns + turn);
+    add(i0, x);
   }
   if constexpr (kTurns > 1) {
     f32x4 sum = o;
 #pragma unroll
     for (uint32_t t = 1; t < kTurns; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        sum[j] += __shfl(o[j], static_cast<int>((lane + t * kLanes) & 63u));
+      for (int v = 0; v < 4; ++v)
+        sum[v] += __shfl(o[v], static_cast<int>((lane + t * kLanes) & 63u));
     o = sum;
   }
   if (turn) return;

@@ -69,10 +69,11 @@ struct AttendParams {
   uint32_t num_groups;
   // The launch (plan_shared): the groups' rows go in prefix_units tiles of kManyRows over the
   // shared tokens, in prefix_splits shares of prefix_piece tokens, each sequence's in own_tiles
-  // tiles of kFewRows over its own, in own_splits shares of own_piece.  Every row and query head
-  // then has prefix_splits + own_splits places for shares.
-  uint32_t prefix_units, prefix_splits, prefix_piece, own_tiles, own_splits, own_piece;
+  // tiles of kFewRows over its own, in own_splits shares of own_piece, by own_waves waves each.
+  // Every row and query head then has prefix_splits + own_splits places for shares.
+  uint32_t prefix_units, prefix_splits, prefix_piece, own_tiles, own_splits, own_piece, own_waves;
   float *share_o, *share_ml;  // in the workspace
+  uint32_t* share_info;       // [num_rows], how many shares a row's heads have
 };
 
 constexpr uint32_t kFewRows = 16;        // of attend_few_kernel's tile
@@ -80,6 +81,7 @@ constexpr uint32_t kManyRows = 128;      // of attend_many_kernel's, or where ro
 constexpr uint32_t kWideRows = 256;      // and heads have up to kWideMaxDim values
 constexpr uint32_t kWideMaxDim = 128;
 constexpr uint32_t kFewMaxSplits = 192;
+constexpr uint32_t kFewWaves = 4;        // of a workgroup
 // A count of finished shares has a 128-byte line of its own: adds to one line run one
 // after another.  The first kCounts of them (or a sixteenth of a small workspace) are at
 // the workspace's start.
@@ -109,10 +111,11 @@ inline uint32_t padded_dim(uint32_t dim) {
 // of 10,000 tokens and 8 heads in shares of 256, 512, 1,024 and 2,048 takes 20.5, 16.1,
 // 18.7 and 27.1; of 30,000 (8-bit) 36.7, 26.0, 20.9 and 24.1; of 3,000 12.0, 14.2, 18.1
 // and 22.4.
-inline uint64_t few_piece(uint64_t units, uint64_t longest) {
-  constexpr uint64_t kSlots = 512, kEven = 1024;
-  if (units * longest >= 4 * kSlots * kEven) return kEven;
-  const uint64_t most = units < kSlots ? kSlots / units : 1;
+constexpr uint64_t kFewSlots = 512;
+inline uint64_t few_piece(uint64_t units, uint64_t longest, uint64_t slots = kFewSlots) {
+  constexpr uint64_t kEven = 1024;
+  if (units * longest >= 4 * kFewSlots * kEven) return kEven;
+  const uint64_t most = units < slots ? slots / units : 1;
   const uint64_t whole = (longest + most - 1) / most;
   uint64_t piece = 128;
   while (piece * piece < 37 * longest) piece += 128;
@@ -224,6 +227,31 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
 constexpr uint32_t kSharedRows = 64;
 constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
 
+// Bytes of K and V that sharing has to save before it is worth a second launch and the shares
+// that it writes and reads.  (8 heads of 128 and a group of 4, in us, as attend_few_kernel's
+// and shared: 16 sequences behind 500 bf16 tokens, 31 MB, 14.8 and 17.2, behind 2,000, 123 MB,
+// 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000, 25 MB, 12.9 and 16.6, behind 8,000, 98
+// MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6; e4m3: 64 behind 500, 66 MB, 14.6
+// and 19.4, 128, 133 MB, 24.0 and 21.7.)
+constexpr double kSharedSaves = 96 << 20;
+
+// Workgroups that pass over shared tokens, of the 512 that the chip holds.  Each step of one,
+// 64 tokens of 128 rows, takes some 1.4 us (heads of 128), a launch of them 9 more, and own tokens
+// are read at 4.5 TB/s, on average half of the longest: the fewest that are done with the own ones
+// leave the fewest shares to write and join, more leave too little room beside them.  (64, 128,
+// 256 and 384 of them, in us, 64 bf16 sequences: behind 8,000 shared tokens and up to 500 of
+// their own 58, 40, 34 and 42, with up to 2,000 84, 87, 92 and 99; behind 32,000 and up to 2,000
+// 203, 131, 109 and 128; 16 behind 8,000 and up to 2,000 35, 35, 36 and 36.)  Of the longest
+// prefixes two to a compute unit hide each other's loads: 256 sequences behind 30,000 with 256
+// 195, 384 186.
+inline uint64_t prefix_workgroups(uint64_t steps, uint64_t dim, double own_bytes) {
+  const double step = 1.4 * static_cast<double>(dim) / 128;
+  const double own = 8 + own_bytes / 2 / 4.5e6;
+  uint64_t n = 64;
+  while (n < 256 && 9 + static_cast<double>(steps) / static_cast<double>(n) * step > own) n *= 2;
+  return n == 256 && steps >= 64 * 256 ? 384 : n;
+}
+
 // Shapes the launch of a batch whose groups share up to `most_shared` tokens, whose sequences
 // have up to `most_own` more and `most_new` rows, joining in `bytes` of workspace at `ws`.  Like
 // plan_attend's, lengths may be wrong and rows too few.  False where the batch is better off, or
@@ -232,47 +260,70 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
                         uint64_t most_own, uint64_t ws, uint64_t bytes) {
   const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
   const uint64_t room = static_cast<uint64_t>(p->table_width) * p->pages.block_size;
-  if (most_shared == 0 || most_shared > room) most_shared = room;
-  if (most_own == 0 || most_own > room) most_own = room;
+  if (most_shared == 0) most_shared = room;
   if (most_new == 0 || most_new > p->num_rows) most_new = p->num_rows;
   auto ceil_div = [](uint64_t a, uint64_t b) { return (a + b - 1) / b; };
   if (p->num_groups == 0 || p->num_seqs < 2 || p->window || most_new * group > kSharedRows)
     return false;
-  p->own_tiles = static_cast<uint32_t>(ceil_div(most_new * group, kFewRows));
-  const uint64_t groups = p->num_groups < p->num_rows ? p->num_groups : p->num_rows;
-  const uint64_t tiles = p->num_rows * group / kManyRows + groups;
-  p->prefix_units = static_cast<uint32_t>(tiles);
-  constexpr uint64_t kPrefix = 256;  // workgroups
-  uint64_t splits = kPrefix / (tiles * heads);
+  const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
+  const double token = 2.0 * static_cast<double>(heads * p->pages.dim) * (codes ? 1 : 2);
+  const uint64_t groups = p->num_groups < p->num_seqs ? p->num_groups : p->num_seqs;
+  if (static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token <
+      kSharedSaves)
+    return false;
+  if (most_shared > room) most_shared = room;
+  if (most_own == 0 || most_own > room) most_own = room;
+  // Each group's last tile may be part-filled.
+  const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;
+  const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), dim,
+                                            static_cast<double>(p->num_seqs * most_own) * token);
+  uint64_t splits = prefix / (tiles * heads);
   if (splits < 1) splits = 1;
   if (splits > kSharedMaxSplits) splits = kSharedMaxSplits;
   uint64_t piece = ceil_div(ceil_div(most_shared, splits), 64) * 64;
   if (piece < 256) piece = 256;
   splits = ceil_div(most_shared, piece);
-  uint64_t own_piece = few_piece(p->num_seqs * p->own_tiles * heads, most_own);
+  const uint64_t own_tiles = ceil_div(most_new * group, kFewRows);
+  const uint64_t units = p->num_seqs * own_tiles * heads;
+  const uint64_t slots = kFewSlots - (prefix < 256 ? prefix : 256);
+  uint64_t own_piece = few_piece(units, most_own, slots);
   uint64_t own_splits = ceil_div(most_own, own_piece);
   if (own_splits > kSharedMaxSplits) own_splits = kSharedMaxSplits;
   const uint64_t share = p->num_rows * p->q_heads * (dim * 4 + 8);
   const uint64_t counts = workspace_counts(bytes) * kCountStride * 4;
-  const uint64_t most = (bytes - counts) / share;
+  const uint64_t info = ceil_div(p->num_rows * 4, 16) * 16;
+  if (bytes < counts + info) return false;
+  const uint64_t most = (bytes - counts - info) / share;
   if (most < 2) return false;
   if (own_splits > most / 2) own_splits = most / 2;
   if (splits > most - own_splits) splits = most - own_splits;
   piece = ceil_div(ceil_div(most_shared, splits), 64) * 64;
   own_piece = ceil_div(ceil_div(most_own, own_splits), 128) * 128;
+  // The own tokens' workgroups start together, or nearly so (ragged lengths make room), beside
+  // those of the shared ones, where fewer waves for each allow it: 64 sequences behind 8,000 and
+  // up to 500 of their own 34 us with 2 waves and 39 with 4, and with up to 2,000 (64 workgroups
+  // before them) 93 and 84; 128 behind 8,000 and up to 500 59 with one, 61 with 2, 66 with 4.
+  uint32_t waves = kFewWaves;
+  while (waves > 1 && units * own_splits * waves / kFewWaves + prefix > kFewSlots * 5 / 4) waves /= 2;
+  p->prefix_units = static_cast<uint32_t>(tiles);
   p->prefix_splits = static_cast<uint32_t>(splits);
   p->prefix_piece = static_cast<uint32_t>(piece);
+  p->own_tiles = static_cast<uint32_t>(own_tiles);
   p->own_splits = static_cast<uint32_t>(own_splits);
   p->own_piece = static_cast<uint32_t>(own_piece);
-  p->share_o = reinterpret_cast<float*>(ws + counts);
-  p->share_ml = reinterpret_cast<float*>(ws + counts + (splits + own_splits) * p->num_rows *
-                                                           p->q_heads * dim * 4);
+  p->own_waves = waves;
+  const uint64_t values = (splits + own_splits) * p->num_rows * p->q_heads;
+  p->share_info = reinterpret_cast<uint32_t*>(ws + counts);
+  p->share_o = reinterpret_cast<float*>(ws + counts + info);
+  p->share_ml = reinterpret_cast<float*>(ws + counts + info + values * dim * 4);
   return true;
 }
 inline uint64_t shared_grid(const AttendParams& p) {
-  return (static_cast<uint64_t>(p.prefix_units) * p.prefix_splits +
-          static_cast<uint64_t>(p.num_seqs) * p.own_tiles * p.own_splits) *
-         p.pages.heads;
+  const uint64_t own =
+      static_cast<uint64_t>(p.num_seqs) * p.own_tiles * p.own_splits * p.pages.heads;
+  const uint64_t per = kFewWaves / p.own_waves;
+  return static_cast<uint64_t>(p.prefix_units) * p.prefix_splits * p.pages.heads +
+         (own + per - 1) / per;
 }
 // Heads of a workgroup of attend_shared_join_kernel, one a wave.
 constexpr uint32_t kJoinHeads = 4;

@@ -16,7 +16,8 @@ pytestmark = pytest.mark.gpu
 
 class SharedBatch(Batch):
     """Groups of sequences, ``sizes`` of them behind ``shared`` whole blocks each, and others
-    behind them; blocks that no sequence has, and tokens past each end, hold NaN."""
+    behind them; blocks that no sequence has, and tokens past each end, hold NaN.  ``own`` cached
+    tokens below 0 are missing of the shared ones."""
 
     def __init__(self, sizes, shared, own, new, form, group, seed=0, sharp=1.0, strides="fused"):
         self.kind, self.rows, heads, dim, bs, head_major = form
@@ -28,7 +29,7 @@ class SharedBatch(Batch):
         blocks = [0 if g is None else shared[g] for g in of]
         lens = np.array([b * bs + a + n for b, a, n in zip(blocks, own, new)])
         self.cached = [int(n) - m for n, m in zip(lens, new)]
-        own_blocks = [-(-int(n) // bs) - b for n, b in zip(lens, blocks)]
+        own_blocks = [max(-(-int(n) // bs) - b, 0) for n, b in zip(lens, blocks)]
         nb = sum(shared) + sum(own_blocks) + 4
         pages = oracle.Pages(nb, bs, heads, dim, self.kind, head_major, self.rows)
         if self.kind in oracle.LARGEST:
@@ -56,6 +57,8 @@ class SharedBatch(Batch):
             b, u = blocks[i], own_blocks[i]
             if b:
                 self.table[i, :b] = first[g]
+            if lens[i] < b * bs:
+                b = -(-int(lens[i]) // bs)
             self.table[i, b:b + u] = order[at:at + u]
             if u:
                 fill(order[at:at + u], int(lens[i]) - b * bs)
@@ -86,7 +89,8 @@ class SharedBatch(Batch):
         out, flat, view = device_rows(np.full_like(bits, 0x5a5a), self.strides, self.rows)
         held = device_array(np.full(bits.shape[:2], 77, np.float32), "fp32") if lse else None
         if hints:
-            kw.setdefault("max_shared_len", int(max(self.shared_lens, default=0)))
+            # More than there is: a batch as small as these would not be worth sharing.
+            kw.setdefault("max_shared_len", 1 << 30)
             kw.setdefault("max_own_len", int(self.lens.max()) if len(self.lens) else 0)
             kw.setdefault("max_query_len", max(self.new) if self.new else 0)
         self.attend(q, out, held, device_array(self.starts + front, "int32"), workspace, stream,
@@ -168,18 +172,33 @@ def test_long_prefixes_are_split_and_joined(gpu, workspace, form, group, sizes, 
         b.check(*b.run(workspace=small), every=every)
         small.close()
     for hints in (dict(max_shared_len=1, max_own_len=1), dict(max_shared_len=1 << 40),
+                  dict(max_own_len=1), dict(max_shared_len=max(shared), max_own_len=max(own) + 1),
                   dict(max_own_len=1 << 31), dict(max_shared_len=0, max_own_len=0)):
         b.check(*b.run(workspace=workspace, **hints), every=every)
 
 
 def test_shared_lengths_of_any_size(gpu, workspace):
-    """Lengths that end inside a block, none, negative ones, and ones that reach into new tokens
-    or past the end of a sequence, which are cut to what all have cached."""
-    for shared in ([0, 5], [13, 47], [1, 1 << 30], [150, 64], [160, 2 ** 31 - 1], [-3, -2 ** 31]):
+    """Lengths that end inside a block, none and negative ones."""
+    for shared in ([0, 5], [13, 47], [1, 64], [150, 64], [160, 63], [-3, -2 ** 31]):
         b = SharedBatch([3, 4], [10, 4], [0, 12, 40, 9, 0, 1, 70], [2, 1, 3, 1, 5, 1, 2], FORMS[0],
                         4, seed=4)
         b.shared_lens = np.array(shared, np.int32)
-        b.check(*b.run(workspace=workspace, max_shared_len=160))
+        b.check(*b.run(workspace=workspace))
+
+
+@pytest.mark.parametrize("form,group", [(LLAMA, 4), (FORMS[4], 5)], ids=str)
+def test_sequences_that_have_cached_less(gpu, workspace, form, group):
+    """A sequence shares what it has cached, whatever the others have: its new tokens, and its
+    end, may lie among the shared ones."""
+    bs = form[4]
+    n = [-(-k // bs) for k in (1000, 100)]
+    b = SharedBatch([5, 3], n, [-900, 12, -1, -n[0] * bs, -400, -70, -n[1] * bs + 3, -3],
+                    [2, 1, 3, 1, 2, 1, 2, 1], form, group, seed=15)
+    b.check(*b.run(workspace=workspace))
+    # Sequences that share all they have cached.
+    b = SharedBatch([4], [60], [-50 * bs + 7, -1, -60 * bs + 5, -20 * bs], [2, 3, 1, 1], form, group, seed=16)
+    b.shared_lens[:] = 2 ** 31 - 1
+    b.check(*b.run(workspace=workspace))
 
 
 @pytest.mark.parametrize("form", [FORMS[0], FORMS[4]], ids=str)
@@ -192,7 +211,7 @@ def test_padded_batches(gpu, workspace, form):
                     [0, 1, 0, 2, 1, 0, 0, 1, 3, 1, 1], form, 4, seed=5)
     b.table[0] = -5  # a sequence without rows has a row of the table that says nothing
     b.check(*b.run(workspace=workspace, tail=1))
-    # One that has rows but no tokens: its rows attend nothing, the group shares nothing.
+    # One that has rows but no tokens: its rows attend nothing.
     b.lens[8] = 0
     b.check(*b.run(workspace=workspace))
     b.lens[:] = 0
