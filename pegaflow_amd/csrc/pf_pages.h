@@ -48,6 +48,7 @@ struct CompactParams {
   // that take chunks in turn (1 in place, where a chunk is read before it is overwritten by
   // the next).
   uint32_t cols_shift, strips, scale_strips, turns;
+  bool few;  // at most kCompactFew tokens of a sequence are said to move
 };
 
 constexpr uint32_t kPagesThreads = 256;
@@ -66,18 +67,36 @@ inline uint64_t compact_grid(const CompactParams& p) {
          p.turns;
 }
 
+// Tokens up to which a sequence's moves are few: one chunk, whose launch is all latency.
+constexpr uint64_t kCompactFew = 16;
+
+// Columns of a strip.  A token-major row of 8 heads of 128 is 128 of them, 2 KB that lie together,
+// and moves best whole: 2,500 of 5,000 tokens in 32 layers (bf16) in strips of 16, 32, 64 and 128
+// columns 139, 135, 131 and 129 us, 4 of each of 32 sequences 27, 15.5, 9.7 and 8.4.  In place,
+// though, a strip's tokens move one chunk after another, and strips are all there is to fill
+// the chip: 2,400 tokens of one sequence 89, 91, 135 and 250 us, of four 309, 296, 309 and 329.
+// To other blocks the chunks go to so many workgroups that 8,192 are at work: 2,048 did in 131.
 inline void plan_compact(CompactParams* p, uint64_t most, bool in_place) {
   const uint32_t columns = compact_columns(p->pages);
   const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
   if (most == 0 || most > p->total) most = p->total;
-  p->cols_shift = most <= 16 ? 7 : 4;
-  const uint32_t cols = 1u << p->cols_shift;
-  p->strips = (columns + cols - 1) / cols;
-  p->scale_strips = codes ? (p->pages.heads + cols - 1) / cols : 0;
   p->turns = 1;
-  if (in_place) return;
+  auto cut = [&](uint32_t shift) {
+    const uint32_t cols = 1u << shift;
+    p->cols_shift = shift;
+    p->strips = (columns + cols - 1) / cols;
+    p->scale_strips = codes ? (p->pages.heads + cols - 1) / cols : 0;
+  };
+  cut(7);
+  p->few = most <= kCompactFew;
+  if (p->few) return;
+  if (in_place) {
+    cut(5);
+    if (compact_grid(*p) < 1024) cut(4);
+    return;
+  }
   const uint64_t chunks = (most + compact_chunk(p->cols_shift) - 1) / compact_chunk(p->cols_shift);
-  while (p->turns * 2 <= chunks && compact_grid(*p) < 2048) p->turns *= 2;
+  while (p->turns * 2 <= chunks && compact_grid(*p) < 8192) p->turns *= 2;
 }
 
 hipError_t launch_fork(const ForkParams& p, hipStream_t stream);
