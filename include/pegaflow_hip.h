@@ -786,12 +786,14 @@ typedef struct pf_shared_args {
 /* pf_kv_attend, to the same definition, with the tokens that a group shares passed over once for
  * all its sequences.  That takes a workspace with room for two shares or more of each row
  * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
- * 192, 256), a max_query_len that is not 0 and of at most 64 rows a KV head, and no window; any
- * other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a sequence
- * takes as many as it has cached (in front of its new ones).
- * args->max_seq_len is used where the hints of `shared` are not both given.  The weights of shared
- * tokens are rounded once, those of a sequence's own to twice as many bits.  No bits change from
- * call to call. */
+ * 192, 256), at most 64 rows of a sequence and KV head (max_query_len, or num_rows, says so), no
+ * window, and 96 MiB of K and V or more that are read once instead of again (by num_seqs,
+ * num_groups and the hint of the shared length); any other call runs as pf_kv_attend.  New tokens
+ * are not shared: of shared_lens a sequence takes as many as it has cached (in front of its new
+ * ones).  args->max_seq_len is used where the hints of `shared` are not both given.
+ *
+ * The weights of shared tokens are rounded to 16 bits once, those of a sequence's own to twice as
+ * many; the parts are joined in fp32.  No bits change from call to call. */
 int pf_kv_attend_shared(const pf_kv_pages* pages, const pf_attend_args* args,
                         const pf_shared_args* shared, pf_attend_workspace* workspace,
                         pf_stream stream);

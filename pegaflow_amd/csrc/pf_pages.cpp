@@ -147,7 +147,10 @@ int compact(const pf_kv_layers* layers, const pf_compact_args* a, pf_stream stre
   if (a->table_width == 0) return invalid("the block table has no entries");
   if (static_cast<uint64_t>(a->table_width) * layers->pages.block_size >= kMaxTokens)
     return invalid("the block table spans 2^31 tokens or more");
-  if (a->num_seqs >= (1u << 24) || a->num_kept >= kMaxTokens) return invalid("too many tokens");
+  // A chunk's end stays within 31 bits.
+  if (a->num_seqs >= (1u << 24) || a->num_kept >= kMaxTokens / 2) return invalid("too many tokens");
+  if (a->out_lens && (a->out_lens == a->first || a->out_lens == a->kept_starts))
+    return invalid("out_lens is one of the arrays that are read");
   Ranges ranges;
   if (int rc = add_table("block table", a->block_table, a->num_seqs, a->table_width,
                          a->table_stride, ranges))

@@ -392,9 +392,9 @@ class PagedKVCache:
                                  _stream(stream, q)), "attend")
 
     def attend_shared(self, q, out, block_table, seq_lens, query_starts, group_starts, shared_lens,
-                      *, scale: float | None = None, causal: bool = True, lse=None,
-                      max_shared_len: int = 0, max_own_len: int = 0, max_query_len: int = 0,
-                      workspace: AttentionWorkspace | None = None,
+                      *, scale: float | None = None, causal: bool = True, window: int = 0,
+                      lse=None, max_shared_len: int = 0, max_own_len: int = 0,
+                      max_query_len: int = 0, workspace: AttentionWorkspace | None = None,
                       stream: Stream | None = None) -> None:
         """``attend`` of a batch in which groups of sequences share their first tokens, which
         are passed over once for all of a group (pf_kv_attend_shared).
@@ -404,16 +404,16 @@ class PagedKVCache:
         first ``shared_lens[g]`` tokens lie (int32; none of them new).  Others share nothing.
         ``max_shared_len`` and ``max_own_len``, the most tokens that a group shares and that a
         sequence has behind these, are hints that shape the launch.  Sharing takes a
-        ``workspace`` and a ``max_query_len`` (at most 64 rows a KV head); without, the call
-        runs as ``attend``."""
+        ``workspace``, a ``max_query_len`` (at most 64 rows a KV head), no ``window``, and
+        enough tokens to be worth it; else the call runs as ``attend``."""
         starts = _index(group_starts, 1, "int32", "group_starts")
         lens = _index(shared_lens, 1, "int32", "shared_lens")
         groups = shared_lens.shape[0]
         if group_starts.shape[0] != groups + 1:
             raise ValueError(f"{groups} shared lengths and {group_starts.shape[0]} group starts "
                              "(one more than groups)")
-        args = self._attend_args(q, out, block_table, seq_lens, query_starts, scale, causal, 0,
-                                 lse, 0, max_query_len)
+        args = self._attend_args(q, out, block_table, seq_lens, query_starts, scale, causal,
+                                 window, lse, 0, max_query_len)
         shared = SharedArgs(starts, lens, min(groups, _MOST),
                             _most("max_shared_len", max_shared_len),
                             _most("max_own_len", max_own_len), 0)
