@@ -494,6 +494,19 @@ __device__ __forceinline__ bool many_tile(const AttendParams& a, uint32_t unit, 
   return true;
 }
 
+// The smallest x of a wave, in a scalar: within 16 lanes by cross-lane operands, which cost no trip
+// through LDS.
+__device__ __forceinline__ int32_t wave_min(int32_t x) {
+  constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+  x = min(x, __builtin_amdgcn_mov_dpp(x, kSwap1, 0xf, 0xf, true));
+  x = min(x, __builtin_amdgcn_mov_dpp(x, kSwap2, 0xf, 0xf, true));
+  x = min(x, __builtin_amdgcn_mov_dpp(x, kMirror8, 0xf, 0xf, true));
+  x = min(x, __builtin_amdgcn_mov_dpp(x, kMirror16, 0xf, 0xf, true));
+  const int32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+  const int32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+  return min(min(a, b), min(c, d));
+}
+
 // Groups of sequences that share their first tokens.  Starts are bounded as in seq_of.
 __device__ __forceinline__ int32_t group_start(const AttendParams& a, uint32_t g) {
   return min(max(a.group_starts[g], 0), static_cast<int32_t>(a.num_seqs));
@@ -542,58 +555,60 @@ __device__ __forceinline__ bool group_tile(const AttendParams& a, uint32_t g, ui
   t->s = {first_row, 0, 0};
   t->row = index * ROWS + wave * 32 + (lane & 31u);
   t->valid = t->row < t->rows;
-  const int32_t token = first_row + static_cast<int32_t>(t->row / a.group);
   constexpr int32_t kNone = 0x7fffffff;
   constexpr uint32_t kChunks = 4;  // of 64 sequences, whose loads are under way together
-  int32_t least = kNone, most = -1, mine = 0;
+  int32_t least = kNone, most = -1;
   for (int32_t b0 = first; b0 < last; b0 += 64 * kChunks) {
-    int32_t start[kChunks], cached[kChunks], end[kChunks];
+    int32_t cached[kChunks];
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
       const int32_t b = b0 + static_cast<int32_t>(c * 64 + lane);
-      start[c] = kNone;
-      cached[c] = end[c] = -1;
+      cached[c] = -1;
       if (b < last) {
         const Seq s = seq_of(a, b);
-        start[c] = s.first;
-        end[c] = s.first + s.rows;
         if (s.rows) cached[c] = cached_of(a, s);
       }
     }
 #pragma unroll
     for (uint32_t c = 0; c < kChunks; ++c) {
-      if (b0 + static_cast<int32_t>(c * 64) >= last) break;
-      int32_t lo = cached[c] < 0 ? kNone : cached[c], hi = cached[c];
-#pragma unroll
-      for (int step = 1; step < 64; step *= 2) {
-        lo = min(lo, __shfl_xor(lo, step));
-        hi = max(hi, __shfl_xor(hi, step));
-      }
-      least = min(least, lo);
+      least = min(least, wave_min(cached[c] < 0 ? kNone : cached[c]));
+      const int32_t hi = -wave_min(-cached[c]);
       if (hi > most) {
         most = hi;
         t->seq = b0 + c * 64 + __builtin_ctzll(__ballot(cached[c] == hi));
+      }
+    }
+  }
+  shared = min(shared, most);
+  if (shared <= 0) return false;
+  int32_t mine = shared;
+  if (least < shared) {  // some sequence has cached less: each row's own
+    const int32_t token = first_row + static_cast<int32_t>(t->row / a.group);
+    for (int32_t b0 = first; b0 < last; b0 += 64) {
+      const int32_t b = b0 + static_cast<int32_t>(lane);
+      int32_t start = kNone, end = 0, cached = 0;
+      if (b < last) {
+        const Seq s = seq_of(a, b);
+        start = s.first;
+        end = s.first + s.rows;
+        cached = cached_of(a, s);
       }
       // The last sequence that starts at this lane's token or before: starts ascend.
       int at = 0;
 #pragma unroll
       for (int step = 32; step; step /= 2) {
-        const int32_t then = __shfl(start[c], at + step);
+        const int32_t then = __shfl(start, at + step);
         at += then <= token ? step : 0;
       }
       // All lanes read before any decides: a lane reads nothing of one that does not take part.
-      const int32_t from = __shfl(start[c], at), to = __shfl(end[c], at);
-      const int32_t has = __shfl(cached[c], at);
-      mine = from <= token && token < to ? has : mine;
+      const int32_t from = __shfl(start, at), to = __shfl(end, at), has = __shfl(cached, at);
+      mine = from <= token && token < to ? min(has, shared) : mine;
     }
   }
-  shared = min(shared, most);
-  if (shared <= 0) return false;
-  t->seq = __builtin_amdgcn_readfirstlane(t->seq);
   t->begin = 0;
   t->end = shared;
-  *all_end = __builtin_amdgcn_readfirstlane(min(shared, least));
-  *my_end = t->valid ? min(shared, mine) : 0;
+  *all_end = min(shared, least);
+  *my_end = t->valid ? mine : 0;
   return true;
 }
 
@@ -730,9 +745,12 @@ __device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& 
   const bool wave_rows = wave0 < t.rows;
 
   u32x4 q[DP / 16];
-  const uint64_t q_row = row_address(a, a.q, t);
+  auto load_q = [&] {
+    const uint64_t q_row = row_address(a, a.q, t);
 #pragma unroll
-  for (uint32_t kk = 0; kk < DP / 16; ++kk) q[kk] = load_q8(q_row, kk * 16 + half * 8, a, t.valid);
+    for (uint32_t kk = 0; kk < DP / 16; ++kk) q[kk] = load_q8(q_row, kk * 16 + half * 8, a, t.valid);
+  };
+  if constexpr (!SHARED) load_q();
 
   f32x16 o[DP / 32];
 #pragma unroll
@@ -1035,6 +1053,8 @@ __device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& 
     fill_ring(0);
     __syncthreads();
     load_k(0);
+    // Tokens' places first: a short pass is all latency.
+    if constexpr (SHARED) load_q();
     uint64_t there = tokens_there(0), v_there = ~0ull;
     bool v_masked = false;
     uint32_t n = 0;
@@ -1384,11 +1404,14 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
                                      static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
                                         2;
   u32x4 q[kSteps];
+  auto load_q = [&] {
 #pragma unroll
-  for (uint32_t i = 0; i < kSteps; ++i)
-    q[i] = load_q8(q_row,
-                   kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
-                   valid && active);
+    for (uint32_t i = 0; i < kSteps; ++i)
+      q[i] = load_q8(q_row,
+                     kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
+                     valid && active);
+  };
+  if constexpr (!SHARED) load_q();
   f32x4 o[DP / 16];
 #pragma unroll
   for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
@@ -1626,6 +1649,7 @@ __device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& me
       load_block(t0);
     load(t0);
     load_block(t0 + kStep);
+    if constexpr (SHARED) load_q();  // tokens' places first: a short pass is all latency
   }
   for (; t0 < end; t0 += kStep) tile(t0);
   if constexpr (kLift) {
