@@ -228,11 +228,15 @@ constexpr uint32_t kSharedRows = 64;
 constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
 
 // Bytes of K and V that sharing has to save before it is worth a second launch and the shares
-// that it writes and reads.  (8 heads of 128 and a group of 4, in us, as attend_few_kernel's
+// that it writes and reads, where plan_attend has attend_few_kernel for all.  (8 heads of 128 and a group of 4, in us, as attend_few_kernel's
 // and shared: 16 sequences behind 500 bf16 tokens, 31 MB, 14.8 and 17.2, behind 2,000, 123 MB,
 // 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000, 25 MB, 12.9 and 16.6, behind 8,000, 98
 // MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6; e4m3: 64 behind 500, 66 MB, 14.6
-// and 19.4, 128, 133 MB, 24.0 and 21.7.)
+// and 19.4, 128, 133 MB, 24.0 and 21.7.)  Sequences of more rows it gives tiles of 128 rows, and
+// there tiles of 16 gain whatever is shared (20 rows a head, 8 behind 500 and up to 500 of
+// their own 33.0 and 18.5, 64 55.8 and 38.3; 64 rows, 8 35.2 and 20.5), but for those of more
+// than 48 rows with many own tokens, which four tiles read (64 behind 500 and up to 2,000 133 and
+// 192, 32 87 and 87).
 constexpr double kSharedSaves = 96 << 20;
 
 // Workgroups that pass over shared tokens, of the 512 that the chip holds.  Each step of one,
@@ -268,15 +272,19 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
   const double token = 2.0 * static_cast<double>(heads * p->pages.dim) * (codes ? 1 : 2);
   const uint64_t groups = p->num_groups < p->num_seqs ? p->num_groups : p->num_seqs;
-  if (static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token <
-      kSharedSaves)
-    return false;
+  const double saved =
+      static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token;
   if (most_shared > room) most_shared = room;
   if (most_own == 0 || most_own > room) most_own = room;
+  const double own = static_cast<double>(p->num_seqs * most_own) * token;
+  if (most_new * group <= kFewRows) {
+    if (saved < kSharedSaves) return false;
+  } else if (most_new * group > 3 * kFewRows && own / 2 > kSharedSaves && own / 2 > saved) {
+    return false;
+  }
   // Each group's last tile may be part-filled.
   const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;
-  const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), dim,
-                                            static_cast<double>(p->num_seqs * most_own) * token);
+  const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), dim, own);
   uint64_t splits = prefix / (tiles * heads);
   if (splits < 1) splits = 1;
   if (splits > kSharedMaxSplits) splits = kSharedMaxSplits;

@@ -54,6 +54,7 @@ struct CompactParams {
 constexpr uint32_t kPagesThreads = 256;
 constexpr uint32_t kForkChunks = 4;     // of a thread
 constexpr uint32_t kCompactTokens = 8;  // of a thread
+constexpr uint32_t kMinShift = 3, kMaxShift = 7;
 
 inline uint32_t compact_columns(const PagedView& p) {
   return p.heads * p.dim * (p.type == PF_KV_BF16 || p.type == PF_KV_FP16 ? 2 : 1) / 16;
@@ -70,7 +71,7 @@ inline uint64_t compact_grid(const CompactParams& p) {
 // Tokens up to which a sequence's moves are few: one chunk, whose launch is all latency.
 constexpr uint64_t kCompactFew = 16;
 
-// Columns of a strip.  A token-major row of 8 heads of 128 is 128 of them, 2 KB that lie together,
+// Columns of a strip: a power of two from kMinShift on.  A token-major row of 8 heads of 128 is 128 of them, 2 KB that lie together,
 // and moves best whole: 2,500 of 5,000 tokens in 32 layers (bf16) in strips of 16, 32, 64 and 128
 // columns 139, 135, 131 and 129 us, 4 of each of 32 sequences 27, 15.5, 9.7 and 8.4.  In place,
 // though, a strip's tokens move one chunk after another, and strips are all there is to fill
@@ -87,12 +88,14 @@ inline void plan_compact(CompactParams* p, uint64_t most, bool in_place) {
     p->strips = (columns + cols - 1) / cols;
     p->scale_strips = codes ? (p->pages.heads + cols - 1) / cols : 0;
   };
-  cut(7);
+  uint32_t whole = kMinShift;
+  while (whole < kMaxShift && (1u << whole) < columns) ++whole;
+  cut(whole);
   p->few = most <= kCompactFew;
   if (p->few) return;
   if (in_place) {
-    cut(5);
-    if (compact_grid(*p) < 1024) cut(4);
+    if (whole > 5) cut(5);
+    if (whole > 4 && compact_grid(*p) < 1024) cut(4);
     return;
   }
   const uint64_t chunks = (most + compact_chunk(p->cols_shift) - 1) / compact_chunk(p->cols_shift);

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(CompactParams p) {
   }
 
   const int32_t step = static_cast<int32_t>(kChunk * p.turns);
+  static_assert(kChunk <= kThreads, "a thread for each token of a chunk");
   auto find = [&](int32_t j0, uint32_t buffer) {
     if (tid >= kChunk) return;
     const int32_t j = j0 + static_cast<int32_t>(tid);
@@ -207,10 +208,14 @@ hipError_t launch_fork(const ForkParams& p, hipStream_t stream) {
 }
 
 hipError_t launch_compact(const CompactParams& p, hipStream_t stream) {
-  void (*f)(CompactParams) = p.few               ? compact_kernel<7, false>
-                             : p.cols_shift == 7 ? compact_kernel<7, true>
-                             : p.cols_shift == 5 ? compact_kernel<5, true>
-                                                 : compact_kernel<4, true>;
+  static_assert(kMinShift == 3 && kMaxShift == 7, "a kernel for each strip");
+  using Kernel = void (*)(CompactParams);
+  static constexpr Kernel kKernels[2][5] = {
+      {compact_kernel<3, true>, compact_kernel<4, true>, compact_kernel<5, true>,
+       compact_kernel<6, true>, compact_kernel<7, true>},
+      {compact_kernel<3, false>, compact_kernel<4, false>, compact_kernel<5, false>,
+       compact_kernel<6, false>, compact_kernel<7, false>}};
+  const Kernel f = kKernels[p.few][p.cols_shift - kMinShift];
   hipLaunchKernelGGL(f, dim3(static_cast<uint32_t>(compact_grid(p))), dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }

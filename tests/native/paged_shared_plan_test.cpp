@@ -99,9 +99,9 @@ void any_batch() {
 
 void worth_it() {
   const uint64_t ws = 1ull << 40, bytes = 64ull << 20;
-  auto plan = [&](uint32_t seqs, uint32_t prefix, uint32_t own, uint32_t type) {
-    AttendParams p = batch(seqs, 1, seqs, 8, 128, 4, prefix + own, type);
-    return plan_shared(&p, 1, prefix, own, ws, bytes) ? p : AttendParams{};
+  auto plan = [&](uint32_t seqs, uint32_t prefix, uint32_t own, uint32_t type, uint32_t most = 1) {
+    AttendParams p = batch(seqs, 1, seqs * most, 8, 128, 4, prefix + own, type);
+    return plan_shared(&p, most, prefix, own, ws, bytes) ? p : AttendParams{};
   };
   AttendParams p = plan(64, 8000, 500, PF_KV_BF16);
   EXPECT(p.prefix_splits == 16 && p.own_splits == 1 && p.own_waves == 2);
@@ -114,6 +114,11 @@ void worth_it() {
   EXPECT(plan(4, 16000, 500, PF_KV_BF16).prefix_splits > 1);
   EXPECT(!plan(64, 500, 50, PF_KV_E4M3).prefix_splits);
   EXPECT(plan(128, 800, 50, PF_KV_E4M3).prefix_splits);
+  EXPECT(!plan(8, 500, 500, PF_KV_BF16, 4).prefix_splits);
+  EXPECT(plan(8, 500, 500, PF_KV_BF16, 5).own_tiles == 2);
+  EXPECT(plan(8, 500, 500, PF_KV_BF16, 16).own_tiles == 4);
+  EXPECT(!plan(64, 500, 2000, PF_KV_BF16, 16).prefix_splits);
+  EXPECT(!plan(8, 500, 500, PF_KV_BF16, 17).prefix_splits);
 }
 
 }  // namespace
