@@ -245,15 +245,19 @@ constexpr double kSharedSaves = 96 << 20;
 // leave the fewest shares to write and join, more leave too little room beside them.  (64, 128,
 // 256 and 384 of them, in us, 64 bf16 sequences: behind 8,000 shared tokens and up to 500 of
 // their own 58, 40, 34 and 42, with up to 2,000 84, 87, 92 and 99; behind 32,000 and up to 2,000
-// 203, 131, 109 and 128; 16 behind 8,000 and up to 2,000 35, 35, 36 and 36.)  Of the longest
-// prefixes two to a compute unit hide each other's loads: 256 sequences behind 30,000 with 256
-// 195, 384 186.
-inline uint64_t prefix_workgroups(uint64_t steps, uint64_t dim, double own_bytes) {
+// 203, 131, 109 and 128; 16 behind 8,000 and up to 2,000 35, 35, 36 and 36.)  Of long prefixes two
+// to a compute unit hide each other's loads: 64 sequences behind 32,000 with 256 72, 384 69; 256
+// 210 and 195; but 64 behind 12,000 39 and 43.  Where there are several groups, shorter ones
+// among them leave workgroups out: 64 sequences in four groups behind up to 4,000, with 256, 384
+// and 512, 32, 29 and 32, up to 32,000 138, 108 and 110; 256 in four behind up to 12,000 153,
+// 110 and 98.
+inline uint64_t prefix_workgroups(uint64_t steps, uint64_t groups, uint64_t dim, double own_bytes) {
   const double step = 1.4 * static_cast<double>(dim) / 128;
   const double own = 8 + own_bytes / 2 / 4.5e6;
   uint64_t n = 64;
   while (n < 256 && 9 + static_cast<double>(steps) / static_cast<double>(n) * step > own) n *= 2;
-  return n == 256 && steps >= 64 * 256 ? 384 : n;
+  if (n == 256 && steps >= 24 * 256) return groups > 1 ? 512 : 384;
+  return n == 256 && groups > 1 && steps >= 8 * 256 ? 384 : n;
 }
 
 // Shapes the launch of a batch whose groups share up to `most_shared` tokens, whose sequences
@@ -284,7 +288,8 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   }
   // Each group's last tile may be part-filled.
   const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;
-  const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), dim, own);
+  const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), groups, dim,
+                                            own);
   uint64_t splits = prefix / (tiles * heads);
   if (splits < 1) splits = 1;
   if (splits > kSharedMaxSplits) splits = kSharedMaxSplits;
