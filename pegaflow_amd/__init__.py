@@ -12,7 +12,8 @@ Layers (reference roles in parentheses):
                      store and the per-device save/load workers
                      (pegaflow-core/src/lib.rs, gpu_worker.rs, storage.rs);
   * ``paged_cache`` — writing, reading and attending over a registered layer's
-                     blocks, at 16 bits or as 8-bit codes.
+                     blocks, at 16 bits or as 8-bit codes; rotary positions; forks,
+                     copies and compaction over all layers.
 
 All data movement runs in libpegaflow_hip.so (HIP, gfx950).  Importing this
 package does not touch the GPU; the library is loaded on first use and its

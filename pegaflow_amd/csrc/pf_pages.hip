@@ -18,6 +18,9 @@ typedef __attribute__((address_space(1))) int32_t g_i32;
 
 // Workgroups of a child, its K and V of each layer in `parts`; then one for each child's row
 // of the table.
+//
+// 64 children in 32 layers (e4m3, 121 MB) take 18.5 to 20 us, 6 TB/s (part of it stays in the
+// caches between calls), 4 in 12 layers 3.8.
 template <bool FORK>
 __global__ void __launch_bounds__(kThreads) fork_kernel(ForkParams p) {
   const uint32_t tid = threadIdx.x;
