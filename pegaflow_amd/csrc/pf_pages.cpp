@@ -1,5 +1,6 @@
 // pf_pages.cpp — entry points of the operators on all layers of a cache: the layers' handle,
 // argument checks, and the launches (pf_pages.hip).
+#include <algorithm>
 #include <vector>
 
 #include "pf_paged_args.h"
@@ -39,6 +40,15 @@ int create_layers(int device, const pf_kv_pages* pages, uint32_t n, pf_kv_layers
     if (int rc = ranges.check_device(device)) return rc;
     views[i] = {v.k, v.v};
   }
+  // Twice the same memory would be moved twice, by workgroups that do not wait for each other.
+  std::vector<uint64_t> starts;
+  for (const LayerView& v : views) {
+    starts.push_back(v.k);
+    starts.push_back(v.v);
+  }
+  std::sort(starts.begin(), starts.end());
+  if (std::adjacent_find(starts.begin(), starts.end()) != starts.end())
+    return invalid("two layers are the same memory");
   int prev = 0;
   const bool had = hipGetDevice(&prev) == hipSuccess;
   const int rc = pf_init(device);

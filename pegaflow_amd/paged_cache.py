@@ -453,8 +453,8 @@ class PagedKVCache:
 
 class PagedLayers:
     """All layers of a cache, ``PagedKVCache`` of one shape, for what moves blocks and tokens
-    within them, each layer alike (pf_kv_layers).  The layers' memory is borrowed; close it
-    after the last call, or graph, that uses it."""
+    within them, each layer alike (pf_kv_layers).  The layers' memory, on ``device``, is borrowed;
+    close it after the last call, or graph, that uses it."""
 
     def __init__(self, caches, device: int = 0):
         self.handle = None

@@ -164,7 +164,8 @@ struct Handles {
 Handles handles(int device) {
   Handles h;
   const double f[32] = {1.0, 0.5};
-  const pf_kv_pages p[2] = {pages(), pages()};
+  pf_kv_pages p[2] = {pages(), pages()};
+  p[1].layout.data_ptr += 1 << 20;
   EXPECT(pf_rotary_create(device, f, 32, PF_ROTARY_HALF, 1.0f, &h.rotary) == PF_OK);
   EXPECT(pf_kv_layers_create(device, p, 2, &h.layers) == PF_OK);
   EXPECT(pf_attend_workspace_create(device, 1 << 20, &h.workspace) == PF_OK);
@@ -278,6 +279,9 @@ void arguments() {
   pf_kv_pages p[2] = {pages(), pages()};
   REFUSED("no layers", return pf_kv_layers_create(0, p, 0, &l));
   REFUSED("no layers", return pf_kv_layers_create(0, nullptr, 2, &l));
+  REFUSED("same memory", return pf_kv_layers_create(0, p, 2, &l));
+  p[1].layout.data_ptr += 40960;  // its K the other's V
+  REFUSED("same memory", return pf_kv_layers_create(0, p, 2, &l));
   p[1].block_size = 8;
   REFUSED("another shape", return pf_kv_layers_create(0, p, 2, &l));
   p[1] = pages();

@@ -325,3 +325,53 @@ def test_on_a_stream_and_refusals(gpu, workspace):
     cache.attend(q, out, *batch, max_query_len=3, workspace=workspace)
     synchronize()
     assert np.array_equal(got, out.download())
+
+
+def test_hints_as_they_are(gpu, workspace):
+    """Batches that are worth sharing by their true lengths: many bytes saved, and drafts."""
+    own = [(37 * i) % 200 for i in range(20)]
+    b = SharedBatch([20], [95], own, [1] * 20, LLAMA, 4, seed=20)
+    b.check(*b.run(workspace=workspace, max_shared_len=95 * 16, max_own_len=max(own) + 1), every=3)
+    b = SharedBatch([3, 2], [20, 7], own[:6], [5, 1, 4, 2, 5, 3], FORMS[3], 4, seed=21)
+    b.check(*b.run(workspace=workspace, max_shared_len=320, max_own_len=max(own[:6]) + 5))
+
+
+@pytest.mark.parametrize("kw", [dict(window=7), dict(window=300), dict(workspace=None),
+                                dict(max_query_len=0)], ids=str)
+def test_calls_that_run_as_attend(gpu, workspace, kw):
+    """With a window, without a workspace or with more rows than share: attend's own bits."""
+    b = SharedBatch([4], [30], [0, 70, 3, 12], [30, 2, 1, 3], FORMS[0], 4, seed=22)
+    kw = {"workspace": workspace, **kw}
+    got = b.run(**kw)
+    n, heads, dim = b.q.shape
+    q, _, _ = device_rows(b.q, b.strides, b.rows, offset=8)
+    out, _, _ = device_rows(b.q, "contiguous", b.rows)
+    kw.setdefault("max_query_len", 30)
+    b.dev.cache.attend(q, out, device_array(b.table, "int32"), device_array(b.lens, "int32"),
+                       device_array(b.starts, "int32"),
+                       max_seq_len=min(1 << 30, 2 ** 32 - 1) + int(b.lens.max()), **kw)
+    synchronize()
+    assert np.array_equal(got[0], out.download().view(np.uint16).reshape(n, heads, dim))
+
+
+def test_two_calls_at_once(gpu):
+    """On two streams, each with a workspace of its own."""
+    batches = [SharedBatch([9], [40], [(13 * i) % 90 for i in range(10)], [1 + i % 3 for i in range(10)],
+                           form, 4, seed=23) for form in (LLAMA, FORMS[2])]
+    alone = []
+    calls = []
+    for b in batches:
+        w = AttentionWorkspace()
+        alone.append(b.run(workspace=w)[0])
+        q, _, _ = device_rows(b.q, b.strides, b.rows)
+        out, _, _ = device_rows(b.q, "contiguous", b.rows)
+        arrays = [device_array(x, "int32") for x in (b.table, b.lens, b.starts, b.group_starts,
+                                                     b.shared_lens)]
+        calls.append((b.dev.cache, q, out, arrays, w, Stream()))
+    hints = dict(max_shared_len=1 << 30, max_own_len=int(batches[0].lens.max()), max_query_len=3)
+    for _ in range(20):
+        for cache, q, out, arrays, w, stream in calls:
+            cache.attend_shared(q, out, *arrays, workspace=w, stream=stream, **hints)
+    for (_, _, out, _, _, stream), want in zip(calls, alone):
+        stream.synchronize()
+        assert np.array_equal(out.download().view(np.uint16).reshape(want.shape), want)
