@@ -228,11 +228,11 @@ constexpr uint32_t kSharedRows = 64;
 constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
 
 // Bytes of K and V that sharing has to save before it is worth a second launch and the shares
-// that it writes and reads, where plan_attend has attend_few_kernel for all.  (8 heads of 128 and a group of 4, in us, as attend_few_kernel's
-// and shared: 16 sequences behind 500 bf16 tokens, 31 MB, 14.8 and 17.2, behind 2,000, 123 MB,
-// 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000, 25 MB, 12.9 and 16.6, behind 8,000, 98
-// MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6; e4m3: 64 behind 500, 66 MB, 14.6
-// and 19.4, 128, 133 MB, 24.0 and 21.7.)  Sequences of more rows it gives tiles of 128 rows, and
+// that it writes and reads, where plan_attend has attend_few_kernel for all.  (8 heads of 128 and
+// a group of 4, in us, as attend_few_kernel's and shared: 16 sequences behind 500 bf16 tokens, 31
+// MB, 14.8 and 17.2, behind 2,000, 123 MB, 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000,
+// 25 MB, 12.9 and 16.6, behind 8,000, 98 MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6;
+// e4m3: 64 behind 500, 66 MB, 14.6 and 19.4, 128, 133 MB, 24.0 and 21.7.)  Sequences of more rows it gives tiles of 128 rows, and
 // there tiles of 16 gain whatever is shared (20 rows a head, 8 behind 500 and up to 500 of
 // their own 33.0 and 18.5, 64 55.8 and 38.3; 64 rows, 8 35.2 and 20.5), but for those of more
 // than 48 rows with many own tokens, which four tiles read (64 behind 500 and up to 2,000 133 and

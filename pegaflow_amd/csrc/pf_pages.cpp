@@ -94,7 +94,7 @@ int launch_copies(const pf_kv_layers* layers, ForkParams& p, Ranges& ranges, pf_
   p.segment_chunks = static_cast<uint32_t>(bytes / 16);
   p.parts = (p.segment_chunks + kPagesThreads * kForkChunks - 1) / (kPagesThreads * kForkChunks);
   const uint64_t each = static_cast<uint64_t>(p.num_layers) * 2 * p.parts + 1;
-  if (each * p.num_children > 0x7fffffffull) return invalid("too many blocks to copy");
+  if (p.num_children > 0x7fffffffull / each) return invalid("too many blocks to copy");
   hipStream_t s = static_cast<hipStream_t>(stream);
   OnDevice on;
   if (int rc = enter(on, layers, s, ranges)) return rc;
