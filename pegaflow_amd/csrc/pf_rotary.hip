@@ -31,8 +31,11 @@ constexpr uint32_t kThreads = kRotaryThreads;
 constexpr uint32_t kFlight = 2;  // heads whose loads are under way together
 
 // How rows are cut: kWide, kNarrow: whole runs of 8 pairs, loaded by 16 bytes or value by
-// value; kAny: any even number of turned values, each with a load of its partner.
-enum Path { kWide, kNarrow, kAny };
+// value; kPart: neighbours as pairs, of which the last run has some, by 16 bytes; kAny: any even
+// number of turned values, each with a load of its partner.  (13,900 tokens of 12 heads of 128, fp16,
+// 82 values turned, take 57.8 us by kPart and 118 by kAny; 96 values 54 by kWide, where tests for
+// a run's pairs, as kPart has them, cost 10,000 tokens 5 of 48.)
+enum Path { kWide, kNarrow, kPart, kAny };
 
 // Cosine and sine of t / 2^64 turns.
 __device__ __forceinline__ void turn(uint64_t t, float* c, float* s) {
@@ -80,7 +83,7 @@ __device__ __forceinline__ u32x4 pack8(const float* f) {
 // Workgroup b: tokens (b / parts) * groups + group, part b % parts (RotaryParams).
 template <class Row, uint32_t TYPE, uint32_t LANES, Path PATH>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
-  constexpr bool kAligned = PATH == kWide;
+  constexpr bool kAligned = PATH == kWide || PATH == kPart;
   constexpr uint32_t kAngles = PATH == kAny ? 16 : 8;
   const uint32_t lane = threadIdx.x % LANES, parts = p.q_parts + 2 * p.kv_parts;
   const uint32_t unit = blockIdx.x / parts;
@@ -112,8 +115,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
   }
   // This lane's values: d0 to d0 + 7 and d1 to d1 + 7.
   const bool mine = lane * 16 < dim;
-  const bool turned = !value && (PATH == kAny ? lane * 16 : lane * 16 + 15) < r;
-  const bool half = p.layout == PF_ROTARY_HALF;
+  constexpr bool kRuns = PATH == kWide || PATH == kNarrow;
+  const bool turned = !value && (kRuns ? lane * 16 + 15 : lane * 16) < r;
+  const bool half = PATH != kPart && p.layout == PF_ROTARY_HALF;
+  // Of this lane's 8 pairs, those that are turned.
+  const uint32_t pairs = PATH != kPart ? 8 : turned ? min((r - lane * 16) / 2, 8u) : 0;
   uint32_t d0 = lane * 16, d1 = d0 + 8;
   if (PATH != kAny && turned && half) {
     d0 = lane * 8;
@@ -136,7 +142,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
         if (d0 + i < r) turn(position * p.turns[pair_of(d0 + i)], &c[i], &s[i]);
     } else {
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) turn(position * p.turns[lane * 8 + i], &c[i], &s[i]);
+      for (uint32_t i = 0; i < 8; ++i)
+        if (i < pairs) turn(position * p.turns[lane * 8 + i], &c[i], &s[i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kAngles; ++i) {
@@ -196,25 +203,33 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
           for (int i = 0; i < 8; ++i) rotate(f[0][i], f[1][i], c[i], s[i]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            rotate(f[i / 4][2 * i % 8], f[i / 4][2 * i % 8 + 1], c[i], s[i]);
+          for (uint32_t i = 0; i < 8; ++i)
+            if (i < pairs) rotate(f[i / 4][2 * i % 8], f[i / 4][2 * i % 8 + 1], c[i], s[i]);
         }
       }
+      // Values that are not turned go as they are, bit by bit.
+      auto words = [&](const float* y, u32x4 was, uint32_t d) {
+        if (!turned) return was;
+        u32x4 is = pack8<Row>(y);
+        if (!kRuns)
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) is[i] = d + 2 * i < r ? is[i] : was[i];
+        return is;
+      };
       if (!to_pages) {
         const uint64_t to = p.q_out.data + (row * p.q_out.token_stride + h * p.q_out.head_stride) * 2;
         if (mine) {
-          store_row8<kAligned>(to + d0 * 2, turned ? pack8<Row>(f[0]) : x[j][0]);
-          store_row8<kAligned>(to + d1 * 2, turned ? pack8<Row>(f[1]) : x[j][1]);
+          store_row8<kAligned>(to + d0 * 2, words(f[0], x[j][0], d0));
+          store_row8<kAligned>(to + d1 * 2, words(f[1], x[j][1], d1));
         }
         continue;
       }
       const uint64_t at = segment + static_cast<uint64_t>(token) * p.pages.token_bytes +
                           static_cast<uint64_t>(h) * p.pages.head_bytes;
       if constexpr (TYPE == PF_KV_BF16 || TYPE == PF_KV_FP16) {
-        // Values that are not turned go as they are, bit by bit.
         if (mine) {
-          store_row8<true>(at + d0 * 2, turned ? pack8<Row>(f[0]) : x[j][0]);
-          store_row8<true>(at + d1 * 2, turned ? pack8<Row>(f[1]) : x[j][1]);
+          store_row8<true>(at + d0 * 2, words(f[0], x[j][0], d0));
+          store_row8<true>(at + d1 * 2, words(f[1], x[j][1], d1));
         }
       } else {
         // The largest magnitude, as bits: they order as the values do, with infinity and
@@ -248,7 +263,9 @@ using RotaryKernel = void (*)(RotaryParams);
 
 template <class Row, uint32_t TYPE, uint32_t LANES>
 RotaryKernel pick_path(const RotaryParams& p) {
-  if (p.rotary % 16) return rotary_kernel<Row, TYPE, LANES, kAny>;
+  if (p.rotary % 16)
+    return p.aligned && p.layout == PF_ROTARY_INTERLEAVED ? rotary_kernel<Row, TYPE, LANES, kPart>
+                                                          : rotary_kernel<Row, TYPE, LANES, kAny>;
   return p.aligned ? rotary_kernel<Row, TYPE, LANES, kWide> : rotary_kernel<Row, TYPE, LANES, kNarrow>;
 }
 

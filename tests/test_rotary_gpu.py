@@ -245,6 +245,32 @@ def test_odd_values(gpu, kind):
             assert (np.abs(held[i, h] - want[i, h]) <= step * (1 + 2.0 ** -8) + off + coarse).all()
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("r", [2, 20, 32, 46])
+def test_values_behind_the_turned_ones(gpu, r, layout):
+    """They pass bit by bit, NaN of any payload included, and spoil no pair beside them."""
+    rng = np.random.default_rng(r)
+    x = values(rng, (9, 3, 64), "bf16")
+    x[:, :, r:] = rng.integers(0x7f80, 0x8000, (9, 3, 64 - r)) | rng.integers(0, 2, (9, 3, 64 - r)) << 15
+    positions = rng.integers(0, 10 ** 6, 9)
+    rotary = RotaryPositions(r, layout=layout)
+    xd, _, _ = device_rows(x)
+    out, _, _ = device_rows(x)
+    rotary.rotate(xd, out, device_array(positions, "int64"))
+    pages = DevicePages(oracle.Pages(1, 16, 3, 64, "bf16"))
+    pages.cache.write_rotated(None, None, xd, xd, device_array(positions, "int64"),
+                              device_array(np.arange(9), "int64"), rotary)
+    synchronize()
+    got = out.download().view(np.uint16).reshape(9, 3, 64)
+    mine = oracle.Pages(1, 16, 3, 64, "bf16")
+    mine.bytes = pages.bytes()
+    want, bound = oracle.rotate(oracle.from_bits(x[..., :r], "bf16"), positions, rotary.frequencies,
+                                layout)
+    for bits in (got, np.asarray(mine.values()[0, 0, :9])):
+        assert np.array_equal(bits[..., r:], x[..., r:])
+        check_rows(bits[..., :r], want, bound, "bf16")
+
+
 def test_refusals(gpu):
     rotary = RotaryPositions(64)
     dev = DevicePages(oracle.Pages(2, 16, 2, 64, "bf16"))
