@@ -232,12 +232,33 @@ constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
 // a group of 4, in us, as attend_few_kernel's and shared: 16 sequences behind 500 bf16 tokens, 31
 // MB, 14.8 and 17.2, behind 2,000, 123 MB, 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000,
 // 25 MB, 12.9 and 16.6, behind 8,000, 98 MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6;
-// e4m3: 64 behind 500, 66 MB, 14.6 and 19.4, 128, 133 MB, 24.0 and 21.7.)  Sequences of more rows it gives tiles of 128 rows, and
-// there tiles of 16 gain whatever is shared (20 rows a head, 8 behind 500 and up to 500 of
-// their own 33.0 and 18.5, 64 55.8 and 38.3; 64 rows, 8 35.2 and 20.5), but for those of more
-// than 48 rows with many own tokens, which four tiles read (64 behind 500 and up to 2,000 133 and
-// 192, 32 87 and 87).
+// e4m3: 64 behind 500, 66 MB, 14.6 and 19.4, 128, 133 MB, 24.0 and 21.7.)
 constexpr double kSharedSaves = 96 << 20;
+
+// Sequences of more rows than kFewRows plan_attend gives tiles of kManyRows, and there tiles of 16
+// gain whatever is shared (20 rows a head, 8 sequences behind 500 and up to 500 of their own 33.0
+// and 18.5, 64 55.8 and 38.3; 64 rows, 8 35.2 and 20.5), but for those of three tiles of 16 and
+// more, which read their own tokens as often, in batches that fill the chip with tiles of kManyRows
+// as well: where the own tokens outweigh what is saved (8 heads of 128, bf16; 56 rows, 40 sequences
+// behind 16 to 250 and up to 1,000 of their own 43 to 53 and 81 to 88, 64 rows, 64 behind 500 and
+// up to 2,000 133 and 192; 48 rows, 80 behind 250 and up to 1,000 84 and 106, but of codes only from
+// four tiles on: 35 rows of 192, 80 behind 250 and up to 1,000 121 and 109, and of longer ones: 35
+// rows, 40 behind 250 and up to 4,000 210 and 156), or the shares do (56
+// rows, 40 behind 64 and up to 20 of their own 21.0 and 24.9, 48 rows 20.9 and 23.8; 160 68 and 74,
+// 80 of 35 rows 28 to 31 and 26).
+inline bool own_tiles_outweigh(const AttendParams& p, uint64_t rows, double saved, double own,
+                               uint64_t most_own, bool codes) {
+  const uint64_t tiles = (rows + kFewRows - 1) / kFewRows;
+  const uint64_t units = static_cast<uint64_t>(p.num_seqs) * p.pages.heads;
+  if (tiles < 3) return false;
+  if (tiles > 3 && own / 2 > kSharedSaves && own / 2 > saved) return true;
+  if (units < 256) return false;
+  if ((tiles > 3 || (!codes && own > 160e6 && most_own <= 2048)) && own * 0.8 > saved) return true;
+  // Written once and read once, of the shared and the own tokens.
+  const double shares = 4.0 * static_cast<double>(p.num_rows) * p.q_heads *
+                        (padded_dim(p.pages.dim) * 4 + 8);
+  return units < (tiles > 3 ? 1024u : 512u) && saved < shares;
+}
 
 // Workgroups that pass over shared tokens, of the 512 that the chip holds.  Each step of one,
 // 64 tokens of 128 rows, takes some 1.4 us (heads of 128), a launch of them 9 more, and own tokens
@@ -281,11 +302,10 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   if (most_shared > room) most_shared = room;
   if (most_own == 0 || most_own > room) most_own = room;
   const double own = static_cast<double>(p->num_seqs * most_own) * token;
-  if (most_new * group <= kFewRows) {
-    if (saved < kSharedSaves) return false;
-  } else if (most_new * group > 3 * kFewRows && own / 2 > kSharedSaves && own / 2 > saved) {
+  if (most_new * group <= kFewRows ? saved < kSharedSaves
+                                   : own_tiles_outweigh(*p, most_new * group, saved, own, most_own,
+                                                        codes))
     return false;
-  }
   // Each group's last tile may be part-filled.
   const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;
   const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), groups, dim,

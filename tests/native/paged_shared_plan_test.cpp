@@ -119,6 +119,15 @@ void worth_it() {
   EXPECT(plan(8, 500, 500, PF_KV_BF16, 16).own_tiles == 4);
   EXPECT(!plan(64, 500, 2000, PF_KV_BF16, 16).prefix_splits);
   EXPECT(!plan(8, 500, 500, PF_KV_BF16, 17).prefix_splits);
+  // Many rows: own tokens, or the shares, that outweigh what is shared.
+  EXPECT(!plan(40, 250, 1000, PF_KV_BF16, 14).prefix_splits);
+  EXPECT(plan(40, 1000, 200, PF_KV_BF16, 14).prefix_splits);
+  EXPECT(plan(24, 250, 1000, PF_KV_BF16, 14).prefix_splits);
+  EXPECT(!plan(80, 250, 1000, PF_KV_BF16, 12).prefix_splits);
+  EXPECT(plan(80, 250, 1000, PF_KV_E4M3, 12).prefix_splits);
+  EXPECT(plan(40, 250, 4000, PF_KV_BF16, 9).prefix_splits);
+  EXPECT(!plan(40, 16, 20, PF_KV_BF16, 14).prefix_splits);
+  EXPECT(plan(40, 16, 20, PF_KV_BF16, 8).prefix_splits);
 }
 
 }  // namespace
