@@ -788,11 +788,12 @@ typedef struct pf_shared_args {
  * all its sequences.  That takes a workspace with room for two shares or more of each row
  * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
  * 192, 256), at most 64 rows of a sequence and KV head (max_query_len, or num_rows, says so), no
- * window, and a batch that gains by it: 96 MiB of K and V or more that are read once instead of
- * again (by num_seqs, num_groups and the hint of the shared length), or sequences of more than 16
- * rows, whose own tokens may outweigh it where there are more than 32; any other call runs as
- * pf_kv_attend.  New tokens are not shared: of shared_lens a sequence takes as many as it has
- * cached (in front of its new ones).  args->max_seq_len is used where the hints of `shared` are not both given.
+ * window, and a batch that gains by it: 32 to 96 MiB of K and V or more, by its rows, sequences and
+ * heads, that are read once instead of again (by num_seqs, num_groups and the hint of the shared
+ * length), or sequences of more than 16 rows, whose own tokens may outweigh it where there are more
+ * than 32; any other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
+ * sequence takes as many as it has cached (in front of its new ones).  args->max_seq_len is used
+ * where the hints of `shared` are not both given.
  *
  * The weights of shared tokens are rounded to 16 bits once, those of a sequence's own to twice as
  * many; the parts are joined in fp32.  No bits change from call to call. */

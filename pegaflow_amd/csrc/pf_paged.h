@@ -227,13 +227,25 @@ inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, ui
 constexpr uint32_t kSharedRows = 64;
 constexpr uint32_t kSharedMaxSplits = 32;  // of the prefix, and of own tokens
 
-// Bytes of K and V that sharing has to save before it is worth a second launch and the shares
-// that it writes and reads, where plan_attend has attend_few_kernel for all.  (8 heads of 128 and
-// a group of 4, in us, as attend_few_kernel's and shared: 16 sequences behind 500 bf16 tokens, 31
-// MB, 14.8 and 17.2, behind 2,000, 123 MB, 22.6 and 17.7, behind 8,000 49 and 21; 4 behind 2,000,
-// 25 MB, 12.9 and 16.6, behind 8,000, 98 MB, 22.4 and 19.3; 64 behind 500, 129 MB, 26.3 and 24.6;
-// e4m3: 64 behind 500, 66 MB, 14.6 and 19.4, 128, 133 MB, 24.0 and 21.7.)
+// Bytes of shares, written once and read once, of the shared tokens and the own ones.
+inline double share_bytes(const AttendParams& p) {
+  return 4.0 * static_cast<double>(p.num_rows) * p.q_heads * (padded_dim(p.pages.dim) * 4 + 8);
+}
+
+// Bytes of K and V that sharing has to save before it is worth a second launch and the shares,
+// where plan_attend has attend_few_kernel for all.  Sequences and heads that fill the chip read at
+// its rate; fewer are split there too.  (In us, as attend_few_kernel's and shared, 8 heads of 128,
+// bf16, if nothing else is said: 64 sequences of 4 rows that save 96 MB 16.0 and 18.7, 200 MB 23.4
+// and 19.9; of 16 rows 128 MB 19.1 and 23.1, 200 MB 24.2 and 23.2; 192 of 16 rows of 96 values (int8)
+// 128 MB 32.0 and 35.5, 200 MB 41.4 and 34.2; 16 of 4 rows 32 MB 14.8 and 16.3, 64 MB 17.6 and 16.5;
+// of 16 rows 16 MB 16.2 and 17.7, 64 MB 20.6 and 18.1; 4 of 16 rows 8 MB 14.2 and 15.4, 32 MB 17.8
+// and 16.9; 64 of 15 rows of one head of 192 16 MB 19.4 and 20.9, 64 MB 38.8 and 24.0.)
 constexpr double kSharedSaves = 96 << 20;
+inline double shared_saves(const AttendParams& p, uint64_t rows) {
+  if (static_cast<uint64_t>(p.num_seqs) * p.pages.heads > 256)
+    return kSharedSaves + 2 * share_bytes(p);
+  return rows > kFewRows / 2 ? kSharedSaves / 3 : kSharedSaves / 2;
+}
 
 // Sequences of more rows than kFewRows plan_attend gives tiles of kManyRows, and there tiles of 16
 // gain whatever is shared (20 rows a head, 8 sequences behind 500 and up to 500 of their own 33.0
@@ -254,10 +266,7 @@ inline bool own_tiles_outweigh(const AttendParams& p, uint64_t rows, double save
   if (tiles > 3 && own / 2 > kSharedSaves && own / 2 > saved) return true;
   if (units < 256) return false;
   if ((tiles > 3 || (!codes && own > 160e6 && most_own <= 2048)) && own * 0.8 > saved) return true;
-  // Written once and read once, of the shared and the own tokens.
-  const double shares = 4.0 * static_cast<double>(p.num_rows) * p.q_heads *
-                        (padded_dim(p.pages.dim) * 4 + 8);
-  return units < (tiles > 3 ? 1024u : 512u) && saved < shares;
+  return units < (tiles > 3 ? 1024u : 512u) && saved < share_bytes(p);
 }
 
 // Workgroups that pass over shared tokens, of the 512 that the chip holds.  Each step of one,
@@ -302,7 +311,7 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   if (most_shared > room) most_shared = room;
   if (most_own == 0 || most_own > room) most_own = room;
   const double own = static_cast<double>(p->num_seqs * most_own) * token;
-  if (most_new * group <= kFewRows ? saved < kSharedSaves
+  if (most_new * group <= kFewRows ? saved < shared_saves(*p, most_new * group)
                                    : own_tiles_outweigh(*p, most_new * group, saved, own, most_own,
                                                         codes))
     return false;

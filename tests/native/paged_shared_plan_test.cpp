@@ -119,6 +119,12 @@ void worth_it() {
   EXPECT(plan(8, 500, 500, PF_KV_BF16, 16).own_tiles == 4);
   EXPECT(!plan(64, 500, 2000, PF_KV_BF16, 16).prefix_splits);
   EXPECT(!plan(8, 500, 500, PF_KV_BF16, 17).prefix_splits);
+  // What sharing has to save grows with the shares of a chip that is full.
+  EXPECT(plan(8, 2000, 500, PF_KV_BF16).prefix_splits);
+  EXPECT(!plan(64, 450, 500, PF_KV_BF16, 4).prefix_splits);
+  EXPECT(plan(64, 900, 500, PF_KV_BF16, 4).prefix_splits);
+  EXPECT(plan(4, 3500, 500, PF_KV_BF16, 4).prefix_splits);
+  EXPECT(!plan(4, 3500, 500, PF_KV_BF16, 1).prefix_splits);
   // Many rows: own tokens, or the shares, that outweigh what is shared.
   EXPECT(!plan(40, 250, 1000, PF_KV_BF16, 14).prefix_splits);
   EXPECT(plan(40, 1000, 200, PF_KV_BF16, 14).prefix_splits);
