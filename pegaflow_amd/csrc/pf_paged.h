@@ -280,12 +280,17 @@ inline bool own_tiles_outweigh(const AttendParams& p, uint64_t rows, double save
 // 210 and 195; but 64 behind 12,000 39 and 43.  Where there are several groups, shorter ones
 // among them leave workgroups out: 64 sequences in four groups behind up to 4,000, with 256, 384
 // and 512, 32, 29 and 32, up to 32,000 138, 108 and 110; 256 in four behind up to 12,000 153,
-// 110 and 98.
+// 110 and 98.  Heads of more than 128 values leave room for one workgroup a compute unit, and own
+// tokens wait where shared ones take them all: heads of 192 with 192 and with 256 or 384, 24
+// sequences of 12 rows (e4m3) behind 4,000 and up to 20 of their own 34 and 40, 24 of 4 (bf16) behind
+// 16,000 and up to 300 52 and 59, 120 of 12 behind 16,000 and up to 20 (4 heads) 114 and 126; but 64
+// of 12 behind 16,000 and up to 300 165 and 156.
 inline uint64_t prefix_workgroups(uint64_t steps, uint64_t groups, uint64_t dim, double own_bytes) {
   const double step = 1.4 * static_cast<double>(dim) / 128;
   const double own = 8 + own_bytes / 2 / 4.5e6;
   uint64_t n = 64;
   while (n < 256 && 9 + static_cast<double>(steps) / static_cast<double>(n) * step > own) n *= 2;
+  if (n == 256 && groups == 1 && dim > 128) return 192;
   if (n == 256 && steps >= 24 * 256) return groups > 1 ? 512 : 384;
   return n == 256 && groups > 1 && steps >= 8 * 256 ? 384 : n;
 }
