@@ -38,11 +38,14 @@ inline uint64_t rotary_grid(const RotaryParams& p) {
 // Heads of a workgroup.  Its lanes keep the sines and cosines of their pairs, some 240
 // operations, for all of them: 2,000 tokens (32 heads of 128 on 8, e4m3) take 10.9 us with 2,
 // 9.9 with 4 and 12.2 with 8.  Where keys need no coding 10,000 take 48.9 with 2, 50.9 with 4
-// and 52.2 with 8.  Few tokens fill the chip only with few heads each: 5 take 3.0 us with one
+// and 52.2 with 8.  Halves of a number of turned values that is no multiple of 16 have twice the
+// sines and cosines: 13,900 tokens (12 heads of 128, fp16, 82 values) 76 with 2, 66 with 4 and 67
+// with 12.  Few tokens fill the chip only with few heads each: 5 take 3.0 us with one
 // head and 5.9 with 8, 500 4.7 from 256 workgroups on and 5.0 from 512.
 inline void plan_rotary(RotaryParams* p) {
   const uint64_t units = rotary_units(*p);
-  uint32_t heads = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8 ? 4 : 2;
+  const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
+  uint32_t heads = codes || (p->rotary % 16 && p->layout == PF_ROTARY_HALF) ? 4 : 2;
   auto parts = [&](uint32_t h) { return (h + heads - 1) / heads; };
   while (heads > 1 && units * (parts(p->q_heads) + 2 * parts(p->kv_heads)) < 256) heads /= 2;
   p->part_heads = heads;

@@ -28,14 +28,16 @@ namespace pf {
 namespace {
 
 constexpr uint32_t kThreads = kRotaryThreads;
+typedef uint16_t __attribute__((may_alias)) any_u16;
 constexpr uint32_t kFlight = 2;  // heads whose loads are under way together
 
 // How rows are cut: kWide, kNarrow: whole runs of 8 pairs, loaded by 16 bytes or value by
-// value; kPart: neighbours as pairs, of which the last run has some, by 16 bytes; kAny: any even
-// number of turned values, each with a load of its partner.  (13,900 tokens of 12 heads of 128, fp16,
-// 82 values turned, take 57.8 us by kPart and 118 by kAny; 96 values 54 by kWide, where tests for
-// a run's pairs, as kPart has them, cost 10,000 tokens 5 of 48.)
-enum Path { kWide, kNarrow, kPart, kAny };
+// value; kPart: neighbours as pairs, of which the last run has some, by 16 bytes; kAnyWide, kAny:
+// any even number of turned values, by 16 bytes or value by value, each with a look at its partner
+// in shared memory.  (13,900 tokens of 12 heads of 128, fp16, 82 values turned, take 57.8 us by
+// kPart and 66.4, in halves, by kAnyWide, 112 where values and partners were loaded one by one; 96
+// values 53 by kWide, where tests for a run's pairs, as kPart has them, cost 10,000 tokens 5 of 48.)
+enum Path { kWide, kNarrow, kPart, kAnyWide, kAny };
 
 // Cosine and sine of t / 2^64 turns.
 __device__ __forceinline__ void turn(uint64_t t, float* c, float* s) {
@@ -83,8 +85,14 @@ __device__ __forceinline__ u32x4 pack8(const float* f) {
 // Workgroup b: tokens (b / parts) * groups + group, part b % parts (RotaryParams).
 template <class Row, uint32_t TYPE, uint32_t LANES, Path PATH>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
-  constexpr bool kAligned = PATH == kWide || PATH == kPart;
-  constexpr uint32_t kAngles = PATH == kAny ? 16 : 8;
+  constexpr bool kAligned = PATH != kNarrow && PATH != kAny;
+  constexpr bool kPartners = PATH == kAnyWide || PATH == kAny;
+  constexpr uint32_t kAngles = kPartners ? 16 : 8;
+  // Rows as they were, for a look at partners: 16 bytes between rows put those of 4 lanes that
+  // ask together in other banks.
+  constexpr uint32_t kRowWords = LANES * 8 + 4, kRows = 64 / LANES;
+  __shared__ uint32_t seen[kPartners ? kThreads / 64 : 1][kPartners ? kFlight : 1]
+                          [kPartners ? kRows * kRowWords : 1] __attribute__((aligned(16)));
   const uint32_t lane = threadIdx.x % LANES, parts = p.q_parts + 2 * p.kv_parts;
   const uint32_t unit = blockIdx.x / parts;
   uint32_t part = blockIdx.x % parts;
@@ -121,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
   // Of this lane's 8 pairs, those that are turned.
   const uint32_t pairs = PATH != kPart ? 8 : turned ? min((r - lane * 16) / 2, 8u) : 0;
   uint32_t d0 = lane * 16, d1 = d0 + 8;
-  if (PATH != kAny && turned && half) {
+  if (!kPartners && turned && half) {
     d0 = lane * 8;
     d1 = r / 2 + d0;
   }
@@ -136,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
   }
   if (turned) {
     const uint64_t position = static_cast<uint64_t>(p.positions[row]);
-    if constexpr (PATH == kAny) {
+    if constexpr (kPartners) {
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i)
         if (d0 + i < r) turn(position * p.turns[pair_of(d0 + i)], &c[i], &s[i]);
@@ -147,7 +155,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
     }
 #pragma unroll
     for (uint32_t i = 0; i < kAngles; ++i) {
-      if (PATH == kAny && d0 + i >= r) continue;
+      if (kPartners && d0 + i >= r) continue;
       c[i] *= p.factor;
       s[i] *= p.factor;
     }
@@ -163,20 +171,33 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
       if (mine && h0 + j < last) {
         x[j][0] = load_row8<kAligned>(at + d0 * 2);
         x[j][1] = load_row8<kAligned>(at + d1 * 2);
-        if constexpr (PATH == kAny) {
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i)
-            if (turned && d0 + i < r)
-              other[j][i / 8][i / 2 % 4] |=
-                  static_cast<uint32_t>(
-                      *reinterpret_cast<const g_u16*>(at + partner_of(d0 + i) * 2))
-                  << (i % 2 * 16);
-        }
       }
     }
-    // Rows that are turned in place are read whole, by all lanes of a row, before they are
-    // written.
-    if constexpr (PATH == kAny) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if constexpr (kPartners) {
+      // A row's lanes are of one wave, whose accesses to shared memory are in order.
+#pragma unroll
+      for (uint32_t j = 0; j < kFlight; ++j) {
+        uint32_t* mem = seen[threadIdx.x / 64][j] + threadIdx.x % 64 / LANES * kRowWords;
+        *reinterpret_cast<u32x4*>(mem + lane * 8) = x[j][0];
+        *reinterpret_cast<u32x4*>(mem + lane * 8 + 4) = x[j][1];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      if (turned) {
+#pragma unroll
+        for (uint32_t j = 0; j < kFlight; ++j) {
+          const any_u16* values = reinterpret_cast<const any_u16*>(
+              seen[threadIdx.x / 64][j] + threadIdx.x % 64 / LANES * kRowWords);
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i)
+            if (d0 + i < r)
+              other[j][i / 8][i / 2 % 4] |= static_cast<uint32_t>(values[partner_of(d0 + i)])
+                                            << (i % 2 * 16);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    // Rows that are turned in place are read before they are written.
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (uint32_t j = 0; j < kFlight; ++j) {
@@ -186,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryParams p) {
       unpack8<Row>(x[j][0], f[0]);
       unpack8<Row>(x[j][1], f[1]);
       if (turned) {
-        if constexpr (PATH == kAny) {
+        if constexpr (kPartners) {
           float g[2][8];
           unpack8<Row>(other[j][0], g[0]);
           unpack8<Row>(other[j][1], g[1]);
@@ -265,6 +286,7 @@ template <class Row, uint32_t TYPE, uint32_t LANES>
 RotaryKernel pick_path(const RotaryParams& p) {
   if (p.rotary % 16)
     return p.aligned && p.layout == PF_ROTARY_INTERLEAVED ? rotary_kernel<Row, TYPE, LANES, kPart>
+           : p.aligned                                    ? rotary_kernel<Row, TYPE, LANES, kAnyWide>
                                                           : rotary_kernel<Row, TYPE, LANES, kAny>;
   return p.aligned ? rotary_kernel<Row, TYPE, LANES, kWide> : rotary_kernel<Row, TYPE, LANES, kNarrow>;
 }
