@@ -352,6 +352,10 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   // before them) 93 and 84; 128 behind 8,000 and up to 500 59 with one, 61 with 2, 66 with 4.
   uint32_t waves = kFewWaves;
   while (waves > 1 && units * own_splits * waves / kFewWaves + prefix > kFewSlots * 5 / 4) waves /= 2;
+  // The kernel counts units in 32 bits, of sequences without rows as well, and both kinds make one
+  // grid.
+  constexpr uint64_t kMostUnits = 0x3fffffff;
+  if (units * own_splits > kMostUnits || tiles * splits * heads > kMostUnits) return false;
   p->prefix_units = static_cast<uint32_t>(tiles);
   p->prefix_splits = static_cast<uint32_t>(splits);
   p->prefix_piece = static_cast<uint32_t>(piece);

@@ -1,0 +1,23 @@
+"""Batches of shared tokens of any size that a call accepts, in the kernel's 32-bit counts, on the
+host (CPU only)."""
+
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="g++ is not installed")
+def test_no_count_wraps(tmp_path):
+    """tests/native/paged_shared_bounds_test.cpp: units of own tokens and tiles of shared ones."""
+    exe = str(tmp_path / "paged_shared_bounds_test")
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-D__HIP_PLATFORM_AMD__",
+                    f"-I{rocm}/include", f"-I{ROOT}/include", f"-I{ROOT}/pegaflow_amd/csrc",
+                    os.path.join(ROOT, "tests", "native", "paged_shared_bounds_test.cpp"), "-o",
+                    exe], check=True)
+    r = subprocess.run([exe], timeout=120, stdout=subprocess.PIPE, text=True)
+    assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout
