@@ -656,9 +656,9 @@ int pf_kv_write_rotated(const pf_kv_pages* pages, const pf_rotary* rotary, const
                         uint64_t num_rows, pf_stream stream);
 
 /* All layers of a cache, of pages of one shape, for the calls below that move blocks or
- * tokens within them, each layer alike.  The layers are distinct, lie on `device` (or in pinned
- * memory) and are borrowed: no call, or graph that holds one, may run after one of them has been
- * freed. */
+ * tokens within them, each layer alike.  The layers have no byte of a block in common (others are
+ * refused), lie on `device` (or in pinned memory) and are borrowed: no call, or graph that holds
+ * one, may run after one of them has been freed. */
 typedef struct pf_kv_layers pf_kv_layers;
 int pf_kv_layers_create(int device, const pf_kv_pages* layers, uint32_t num_layers,
                         pf_kv_layers** out);

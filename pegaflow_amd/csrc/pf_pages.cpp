@@ -23,6 +23,13 @@ bool same_shape(const PagedView& a, const PagedView& b) {
          a.token_bytes == b.token_bytes && a.head_bytes == b.head_bytes && a.type == b.type;
 }
 
+// Whether `count` segments of `bytes`, each `step` behind the one before it, have bytes in common
+// with as many that start `apart` behind them.
+bool segments_meet(uint64_t apart, uint64_t step, uint64_t count, uint64_t bytes) {
+  const uint64_t whole = apart / step, rest = apart % step;
+  return (whole < count && rest < bytes) || (whole + 1 < count && step - rest < bytes);
+}
+
 int create_layers(int device, const pf_kv_pages* pages, uint32_t n, pf_kv_layers** out) {
   if (!out) return invalid("null output");
   *out = nullptr;
@@ -41,21 +48,27 @@ int create_layers(int device, const pf_kv_pages* pages, uint32_t n, pf_kv_layers
     views[i] = {v.k, v.v};
   }
   // Twice the same memory would be moved twice, by workgroups that do not wait for each other.
+  // Layers may lie between each other's blocks.
   std::vector<uint64_t> starts;
   for (const LayerView& v : views) {
     starts.push_back(v.k);
     starts.push_back(v.v);
   }
   std::sort(starts.begin(), starts.end());
-  if (std::adjacent_find(starts.begin(), starts.end()) != starts.end())
-    return invalid("two layers are the same memory");
+  uint64_t bytes = 0;
+  if (int rc = segment_bytes(shape.block_size, shape.heads, shape.dim, shape.type, &bytes)) return rc;
+  const uint64_t span = (shape.num_blocks - 1ull) * shape.block_bytes + bytes;
+  for (size_t i = 0; i < starts.size(); ++i)
+    for (size_t j = i + 1; j < starts.size() && starts[j] - starts[i] < span; ++j)
+      if (segments_meet(starts[j] - starts[i], shape.block_bytes, shape.num_blocks, bytes))
+        return invalid("two layers have some of the same memory");
   int prev = 0;
   const bool had = hipGetDevice(&prev) == hipSuccess;
   const int rc = pf_init(device);
-  const uint64_t bytes = n * sizeof(LayerView);
+  const uint64_t table = n * sizeof(LayerView);
   void* p = nullptr;
-  hipError_t e = rc == PF_OK ? hipMalloc(&p, bytes) : hipSuccess;
-  if (p) e = hipMemcpy(p, views.data(), bytes, hipMemcpyHostToDevice);
+  hipError_t e = rc == PF_OK ? hipMalloc(&p, table) : hipSuccess;
+  if (p) e = hipMemcpy(p, views.data(), table, hipMemcpyHostToDevice);
   if (e != hipSuccess && p) (void)hipFree(p);
   if (had && prev != device) (void)hipSetDevice(prev);
   if (rc != PF_OK) return rc;
