@@ -711,7 +711,8 @@ typedef struct pf_compact_args {
   uint64_t num_kept;
   uint64_t kept_starts; /* int32 [num_seqs + 1], device */
   uint64_t first;       /* int32 [num_seqs], device, or 0: every sequence from 0 on */
-  uint64_t out_lens;    /* int32 [num_seqs], device, or 0: receives first + kept tokens */
+  uint64_t out_lens;    /* int32 [num_seqs], device, or 0: receives first + kept tokens (it is */
+                        /* none of the arrays that are read, not even in part)              */
   uint32_t num_seqs;
   uint32_t table_width;
   uint32_t max_kept;    /* most kept tokens of a sequence, as a hint that shapes the launch */

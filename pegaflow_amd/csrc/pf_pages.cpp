@@ -172,8 +172,14 @@ int compact(const pf_kv_layers* layers, const pf_compact_args* a, pf_stream stre
     return invalid("the block table spans 2^31 tokens or more");
   // A chunk's end stays within 31 bits.
   if (a->num_seqs >= (1u << 24) || a->num_kept >= kMaxTokens / 2) return invalid("too many tokens");
-  if (a->out_lens && (a->out_lens == a->first || a->out_lens == a->kept_starts))
-    return invalid("out_lens is one of the arrays that are read");
+  // A sequence's length is written by one workgroup while others still read the arrays.
+  auto written = [&](uint64_t at, uint64_t entries) {
+    return a->out_lens && at && at < a->out_lens + a->num_seqs * 4ull &&
+           a->out_lens < at + entries * 4;
+  };
+  if (written(a->first, a->num_seqs) || written(a->kept_starts, a->num_seqs + 1ull) ||
+      written(a->kept, a->num_kept))
+    return invalid("out_lens is, in part, one of the arrays that are read");
   Ranges ranges;
   if (int rc = add_table("block table", a->block_table, a->num_seqs, a->table_width,
                          a->table_stride, ranges))

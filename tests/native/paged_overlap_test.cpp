@@ -146,10 +146,50 @@ void layers() {
   }
 }
 
+// Lengths that are written may be none of the entries that are read.
+void lengths() {
+  const pf_kv_pages one = pages(1 << 20, 10, 64, 0);
+  pf_kv_layers* l = nullptr;
+  EXPECT(pf_kv_layers_create(0, &one, 1, &l) == PF_OK);
+  const uint32_t seqs = 5, width = 4, kept = 9;
+  const uint64_t out = kBase + 4096, far = kBase + 65536;
+  pf_compact_args args{};
+  args.block_table = args.out_table = far;
+  args.table_stride = args.out_stride = args.table_width = width;
+  args.num_seqs = seqs;
+  args.num_kept = kept;
+  args.out_lens = out;
+  const struct {
+    uint64_t pf_compact_args::*at;
+    int entries;
+  } arrays[] = {{&pf_compact_args::first, seqs},
+                {&pf_compact_args::kept_starts, seqs + 1},
+                {&pf_compact_args::kept, kept}};
+  for (const auto& array : arrays)
+    for (int shift = -12; shift <= 12; ++shift) {
+      pf_compact_args a = args;
+      a.kept = far + 4096;
+      a.kept_starts = far + 8192;
+      a.first = far + 12288;
+      a.*array.at = out + 4 * shift;
+      const bool meet = shift < static_cast<int>(seqs) && shift + array.entries > 0;
+      launches = 0;
+      EXPECT(pf_kv_compact(l, &a, nullptr) == (meet ? PF_ERR_INVALID_ARGUMENT : PF_OK));
+      EXPECT(launches == (meet ? 0 : 1) && (!meet || std::strstr(pf_last_error(), "out_lens")));
+    }
+  pf_compact_args a = args;  // without firsts, and without kept tokens
+  a.kept_starts = far + 8192;
+  a.num_kept = 0;
+  a.kept = out;
+  EXPECT(pf_kv_compact(l, &a, nullptr) == PF_OK);
+  pf_kv_layers_destroy(l);
+}
+
 }  // namespace
 
 int main() {
   layers();
+  lengths();
   if (failures) return 1;
   std::puts("ok");
   return 0;

@@ -14,7 +14,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 @pytest.mark.skipif(not shutil.which("g++"), reason="g++ is not installed")
 def test_memory_given_twice_is_refused(tmp_path):
-    """tests/native/paged_overlap_test.cpp: layers that overlap, anywhere, and none that do not."""
+    """tests/native/paged_overlap_test.cpp: layers that overlap,
+    anywhere, lengths written where others are read, and nothing else."""
     _lib.load()  # built, if it was not
     exe = str(tmp_path / "paged_overlap_test")
     lib = os.path.dirname(build.LIB)
