@@ -785,6 +785,9 @@ typedef struct pf_shared_args {
                            /* the launch (0: unknown)                                         */
   uint32_t reserved;
 } pf_shared_args;
+/* As max_shared_len: share whatever that saves, also nothing.  (Any other length beyond what the
+ * block table holds counts as what it holds.) */
+enum { PF_SHARED_LEN_ANYWAY = 1 << 30 };
 /* pf_kv_attend, to the same definition, with the tokens that a group shares passed over once for
  * all its sequences.  That takes a workspace with room for two shares or more of each row
  * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
@@ -792,7 +795,7 @@ typedef struct pf_shared_args {
  * window, and a batch that gains by it: 32 to 96 MiB of K and V or more, by its rows, sequences and
  * heads, that are read once instead of again (by num_seqs, num_groups and the hint of the shared
  * length), or sequences of more than 16 rows, whose own tokens may outweigh it where there are more
- * than 32; any other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
+ * than 32, or PF_SHARED_LEN_ANYWAY; any other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
  * sequence takes as many as it has cached (in front of its new ones).  args->max_seq_len is used
  * where the hints of `shared` are not both given.
  *

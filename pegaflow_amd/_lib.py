@@ -178,6 +178,7 @@ KV_BF16, KV_FP16, KV_E4M3, KV_INT8 = 1, 2, 3, 4
 KV_TOKEN_MAJOR, KV_HEAD_MAJOR = 0, 1
 ROTARY_HALF, ROTARY_INTERLEAVED = 1, 2
 KV_MAX_HEAD_DIM = 256
+SHARED_LEN_ANYWAY = 1 << 30
 ATTEND_WORKSPACE_DEFAULT = 64 << 20
 
 

@@ -297,8 +297,9 @@ inline uint64_t prefix_workgroups(uint64_t steps, uint64_t groups, uint64_t dim,
 
 // Shapes the launch of a batch whose groups share up to `most_shared` tokens, whose sequences
 // have up to `most_own` more and `most_new` rows, joining in `bytes` of workspace at `ws`.  Like
-// plan_attend's, lengths may be wrong and rows too few.  False where the batch is better off, or
-// has to be, attended by plan_attend's kernels.
+// plan_attend's, lengths may be wrong and rows too few; a shared length counts for what the block
+// table holds, whatever it says, or, from PF_SHARED_LEN_ANYWAY on, for as much as sharing takes.
+// False where the batch is better off, or has to be, attended by plan_attend's kernels.
 inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared,
                         uint64_t most_own, uint64_t ws, uint64_t bytes) {
   const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
@@ -311,14 +312,16 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
   const double token = 2.0 * static_cast<double>(heads * p->pages.dim) * (codes ? 1 : 2);
   const uint64_t groups = p->num_groups < p->num_seqs ? p->num_groups : p->num_seqs;
-  const double saved =
-      static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token;
+  const bool anyway = most_shared >= PF_SHARED_LEN_ANYWAY;
   if (most_shared > room) most_shared = room;
   if (most_own == 0 || most_own > room) most_own = room;
+  const double saved =
+      static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token;
   const double own = static_cast<double>(p->num_seqs * most_own) * token;
-  if (most_new * group <= kFewRows ? saved < shared_saves(*p, most_new * group)
-                                   : own_tiles_outweigh(*p, most_new * group, saved, own, most_own,
-                                                        codes))
+  if (!anyway &&
+      (most_new * group <= kFewRows
+           ? saved < shared_saves(*p, most_new * group)
+           : own_tiles_outweigh(*p, most_new * group, saved, own, most_own, codes)))
     return false;
   // Each group's last tile may be part-filled.
   const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;

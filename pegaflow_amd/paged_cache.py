@@ -33,6 +33,7 @@ KV_TYPES = {"bf16": _lib.KV_BF16, "fp16": _lib.KV_FP16, "e4m3": _lib.KV_E4M3,
 _ROW_NAMES = {"bf16": _lib.KV_BF16, "bfloat16": _lib.KV_BF16, "fp16": _lib.KV_FP16,
               "float16": _lib.KV_FP16}
 _row_types: dict = {}  # a tensor's dtype -> PF_KV_*
+SHARE_ANYWAY = _lib.SHARED_LEN_ANYWAY
 _MOST = 2 ** 32 - 1  # of a 32-bit field, which ctypes fills with a number's low bits
 
 
@@ -405,7 +406,8 @@ class PagedKVCache:
         ``max_shared_len`` and ``max_own_len``, the most tokens that a group shares and that a
         sequence has behind these, are hints that shape the launch.  Sharing takes a
         ``workspace``, a ``max_query_len`` (at most 64 rows a KV head), no ``window``, and
-        enough tokens to be worth it; else the call runs as ``attend``."""
+        enough tokens to be worth it, or a ``max_shared_len`` of ``SHARE_ANYWAY`` or more; else
+        the call runs as ``attend``."""
         starts = _index(group_starts, 1, "int32", "group_starts")
         lens = _index(shared_lens, 1, "int32", "shared_lens")
         groups = shared_lens.shape[0]
@@ -551,5 +553,5 @@ class PagedLayers:
             pass
 
 
-__all__ = ["KV_TYPES", "AttentionWorkspace", "PagedKVCache", "PagedLayers", "RotaryPositions",
-           "segment_bytes"]
+__all__ = ["KV_TYPES", "SHARE_ANYWAY", "AttentionWorkspace", "PagedKVCache", "PagedLayers",
+           "RotaryPositions", "segment_bytes"]
