@@ -680,493 +680,13 @@ __device__ __forceinline__ void many_store(const AttendParams& a, const ManyTile
   many_lse<Row>(a, t, m, l);
 }
 
-// Workgroup `index` of attend_many_kernel, or (SHARED) of attend_shared_kernel's tiles of the
-// tokens that groups of sequences share.
-template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS, bool SHARED>
-__device__ __forceinline__ void attend_many(const AttendParams& a, ManyLds<DP>& lds,
-                                            uint32_t index) {
-  constexpr uint32_t kThreads = 2 * ROWS, kWaves = ROWS / 32;
-  constexpr bool kCodes = is_codes(TYPE);
-  constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
-  constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
-  constexpr uint32_t kPer = kCodes ? 16 : 8;  // values of a 16-byte load
-  // Lanes of a token: a power of two, so that a wave's load stays within 16 tokens.
-  constexpr uint32_t kCols = (DP <= 64 ? 64 : DP <= 128 ? 128 : 256) / kPer;
-  // Tokens of one load of the workgroup, whose threads may be more than a tile needs: then
-  // its halves load and store the same.
-  constexpr uint32_t kLoadTokens = kThreads / kCols < kTileTokens ? kThreads / kCols : kTileTokens;
-  constexpr uint32_t kLoads = kTileTokens / kLoadTokens;
-  constexpr uint32_t kKP = k_pitch(DP), kVP = v_pitch(DP);
-  constexpr int32_t kStep = kTileTokens;
-  using Lds = ManyLds<DP>;
-  const PagedView& pg = a.pages;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, half = lane >> 5;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-  // Heads of one tile are neighbours: with 8 of them each has an XCD's L2 for its pages.
-  const uint32_t head = index % pg.heads;
-  const uint32_t rest = index / pg.heads;
-  uint32_t unit = rest, split = 0, splits = 1;
-  ManyTile t;
-  int32_t all_begin, all_end, my_begin, my_end;
-  if constexpr (SHARED) {
-    splits = a.prefix_splits;
-    split = rest % splits;
-    unit = rest / splits;
-    if (!shared_tile<ROWS>(a, unit, head, wave, &t, &all_end, &my_end)) return;
-  } else {
-    if (rest >= a.many_whole) {
-      splits = a.many_splits;
-      split = (rest - a.many_whole) % splits;
-      unit = a.many_whole + (rest - a.many_whole) / splits;
-    }
-    if (!many_tile<ROWS>(a, unit, head, wave, &t)) return;
-  }
-  int32_t begin = t.begin, end = t.end;
-  const uint32_t used =
-      split_range(begin, end, split, splits, SHARED ? a.prefix_piece : a.many_piece);
-  if (split >= used) return;
-  begin = __builtin_amdgcn_readfirstlane(begin);
-  end = __builtin_amdgcn_readfirstlane(end);
-  const int32_t* table = a.block_table + t.seq * a.table_stride;
-
-  // Tokens that every row of the workgroup attends, and this wave's and row's.
-  const uint32_t wave0 = __builtin_amdgcn_readfirstlane(t.row), group = a.group;
-  const uint32_t tile0 = wave0 - wave * 32, tile_last = min(tile0 + ROWS, t.rows) - 1;
-  if constexpr (SHARED) {
-    all_begin = my_begin = 0;
-  } else {
-    all_begin = row_begin(a, t.pos0 + static_cast<int32_t>(tile_last / group));
-    all_end = row_end(a, t.s.len, t.pos0 + static_cast<int32_t>(tile0 / group));
-    const int32_t pos = t.pos0 + static_cast<int32_t>(t.row / group);
-    my_begin = row_begin(a, pos);
-    my_end = t.valid ? row_end(a, t.s.len, pos) : 0;
-  }
-  const bool wave_rows = wave0 < t.rows;
-
-  u32x4 q[DP / 16];
-  auto load_q = [&] {
-    const uint64_t q_row = row_address(a, a.q, t);
-#pragma unroll
-    for (uint32_t kk = 0; kk < DP / 16; ++kk) q[kk] = load_q8(q_row, kk * 16 + half * 8, a, t.valid);
-  };
-  if constexpr (!SHARED) load_q();
-
-  f32x16 o[DP / 32];
-#pragma unroll
-  for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
-  float m = kNegInf, l = 0.0f;
-  float lift = t.valid ? kLiftStart : kLiftNone, lift_limit = 0.0f;  // kLift
-
-  // This thread's part of a tile: 16 bytes of tokens my_tok + kLoadTokens * i, values
-  // my_d and on, and of 8-bit pages the scales of token 16 * wave + lane (lanes 0 to 15 of
-  // the first 4 waves).
-  const uint32_t my_tok = tid / kCols % kTileTokens, my_d = (tid % kCols) * kPer;
-  const bool my_col = my_d < pg.dim;
-  const uint32_t shift = a.unit_shift, in_unit = (1u << shift) - 1, tile_units = kTileTokens >> shift;
-  // A load's tokens repeat their place in their unit after at most two loads.
-  constexpr uint32_t kOffsets = kLoadTokens < 16 ? 2 : 1;
-  uint32_t lane_at[kOffsets];
-#pragma unroll
-  for (uint32_t i = 0; i < kOffsets; ++i)
-    lane_at[i] = ((my_tok + i * kLoadTokens) & in_unit) * pg.token_bytes +
-                 (my_col ? my_d : 0) * (kCodes ? 1 : 2);
-  const uint32_t lane_scale = (lane & in_unit & 15u) * 4u;
-  u32x4 kr[kLoads], vr[kLoads];
-  float k_sr = 0.0f, v_sr = 0.0f;
-  // The half of the ring that starts with tile n.
-  auto fill_ring = [&](uint32_t n) {
-    if (tid >= kRing / 2) return;
-    const uint32_t unit = n * tile_units + tid;
-    const int32_t tok = begin + static_cast<int32_t>(unit << shift);
-    const uint32_t page = page_of(pg, min(tok, end - 1));
-    const int32_t block = tok < end ? table[page] : -1;
-    uint64_t at, scale_at;
-    const bool in = token_at(pg, block, tok, page, head, &at, &scale_at);
-    lds.at[unit % kRing] = in ? at : 0;
-    if constexpr (kCodes) lds.scale_at[unit % kRing] = in ? scale_at : pg.scale_offset;
-    lds.there[unit % kRing] = in;
-  };
-  auto unit_of = [&](uint32_t n, uint32_t tok) {
-    return (n * tile_units & (kRing - 1)) + (tok >> shift);
-  };
-  auto load_k = [&](uint32_t n) {
-#pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i)
-      kr[i] = *reinterpret_cast<const g_u32x4*>(
-          pg.k + lds.at[unit_of(n, my_tok + i * kLoadTokens)] + lane_at[i % kOffsets]);
-    if constexpr (kCodes)
-      if (lane < 16 && wave < 4) {
-        const uint64_t at = lds.scale_at[unit_of(n, wave * 16 + lane)] + lane_scale;
-        k_sr = *reinterpret_cast<const g_f32*>(pg.k + at);
-        v_sr = *reinterpret_cast<const g_f32*>(pg.v + at);
-      }
-  };
-  auto load_v = [&](uint32_t n) {
-#pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i)
-      vr[i] = *reinterpret_cast<const g_u32x4*>(
-          pg.v + lds.at[unit_of(n, my_tok + i * kLoadTokens)] + lane_at[i % kOffsets]);
-  };
-  auto tokens_there = [&](uint32_t n) { return __ballot(lds.there[unit_of(n, lane)] != 0); };
-  // K into LDS.
-  auto store_k = [&](uint32_t n) {
-    typename Lds::K& tile = lds.k[n % Lds::kBuffers];
-    if (my_col)
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) {
-        u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kKP + my_d * 2);
-        if constexpr (kCodes) {
-          const u32x2 x0 = codes_to_16<Row, TYPE>(kr[i][0]), x1 = codes_to_16<Row, TYPE>(kr[i][1]);
-          const u32x2 x2 = codes_to_16<Row, TYPE>(kr[i][2]), x3 = codes_to_16<Row, TYPE>(kr[i][3]);
-          to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
-          to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
-        } else {
-          to[0] = kr[i];
-        }
-      }
-    if constexpr (kCodes)
-      if (lane < 16 && wave < 4) {
-        tile.k_scale[wave * 16 + lane] = k_sr;
-        tile.v_scale[wave * 16 + lane] = v_sr;
-      }
-  };
-  // V of tile n into LDS; `masked`: some row does not attend every token; bit j of
-  // `there`: token j has a block.
-  auto store_v = [&](uint32_t n, bool masked, uint64_t there) {
-    typename Lds::V& tile = lds.v[n % Lds::kBuffers];
-    if (masked) {
-      bool odd = false;
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) {
-        const uint32_t tok = my_tok + i * kLoadTokens;
-        if (!(there >> tok & 1u) || begin + static_cast<int32_t>(n * kTileTokens + tok) >= end)
-          vr[i] = u32x4{0, 0, 0, 0};
-        odd |= clear_odd<Row, TYPE>(vr[i]);
-      }
-      if (odd && my_col) lds.odd = 1;
-    }
-    if (my_col)
-#pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i) {
-        u32x4* to = reinterpret_cast<u32x4*>(tile.data + (my_tok + i * kLoadTokens) * kVP + my_d * 2);
-        if constexpr (kCodes) {
-          const u32x2 x0 = codes_to_16<Row, TYPE>(vr[i][0]), x1 = codes_to_16<Row, TYPE>(vr[i][1]);
-          const u32x2 x2 = codes_to_16<Row, TYPE>(vr[i][2]), x3 = codes_to_16<Row, TYPE>(vr[i][3]);
-          to[0] = u32x4{x0[0], x0[1], x1[0], x1[1]};
-          to[1] = u32x4{x2[0], x2[1], x3[0], x3[1]};
-        } else {
-          to[0] = vr[i];
-        }
-      }
-  };
-  // S^T of tile n: this lane's row, tokens 32 tt + 8 (i / 4) + 4 half + i % 4.  The reads
-  // of one group of products are under way during the group before.
-  f32x16 s[2];
-  constexpr uint32_t kGroup = 2;  // steps of 16 values: 4 products
-  u32x4 kf[2][kGroup][2];
-  auto read_k = [&](uint32_t n, uint32_t g, u32x4 (&f)[kGroup][2]) {
-    const uint8_t* at = lds.k[n % Lds::kBuffers].data + (lane & 31u) * kKP + half * 16;
-#pragma unroll
-    for (uint32_t j = 0; j < kGroup; ++j)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-        f[j][tt] = *reinterpret_cast<const u32x4*>(at + tt * 32 * kKP + (g * kGroup + j) * 32);
-  };
-  // Scales of the tile: lane i of 16 holds that of this half's token i, and 32 tt on.
-  float ks[2], vs[2];
-  const uint32_t my_scale = 8 * ((lane & 15u) / 4) + 4 * half + (lane & 3u);
-  auto scores = [&](uint32_t n) {
-    if constexpr (kCodes)
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        ks[tt] = lds.k[n % Lds::kBuffers].k_scale[32 * tt + my_scale];
-        vs[tt] = lds.k[n % Lds::kBuffers].v_scale[32 * tt + my_scale];
-      }
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[tt][i] = 0.0f;
-#pragma unroll
-    for (uint32_t g = 0; g < DP / 16 / kGroup; ++g) {
-      if (g + 1 < DP / 16 / kGroup) read_k(n, g + 1, kf[(g + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (uint32_t j = 0; j < kGroup; ++j)
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-          s[tt] = Mat<Row>::mul32(kf[g & 1][j][tt], q[g * kGroup + j], s[tt]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (kCodes) {
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = s[tt][i];
-        scale_by<0>(x, ks[tt], std::make_integer_sequence<int, 16>());
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[tt][i] = x[i];
-      }
-    }
-  };
-  // V^T of 16 tokens of tile n, from 16 u on.  They are taken in the order in which a
-  // lane holds their weights: 4 half + (0..3), then 8 + 4 half + (0..3).
-  const uint32_t quad = lane & 15u;
-  const uint32_t v_lane = (half * 4 + quad / 4) * kVP + ((lane >> 4) & 1u) * 32 + (quad & 3u) * 8;
-  u32x4 vf[2][DP / 32];
-  auto read_v = [&](uint32_t n, int u, u32x4 (&f)[DP / 32]) {
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt) {
-      const uint8_t* from = lds.v[n % Lds::kBuffers].data + v_lane + u * 16 * kVP + dt * 64;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(from + 8 * kVP));
-      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-      f[dt] = u32x4{x[0], x[1], y[0], y[1]};
-    }
-  };
-  // O^T += V^T W^T.
-  auto add_v = [&](const u32x4 (&f)[DP / 32], u32x4 w) {
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt) o[dt] = Mat<Row>::mul32(f[dt], w, o[dt]);
-  };
-  // Tile n's scores and softmax.  Its product with V follows in the next step, under that
-  // tile's softmax: p are the weights of tile n - 1 at first, of tile n at the end.
-  u32x4 p[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) p[u] = u32x4{0, 0, 0, 0};
-  auto step = [&](int32_t t0, uint32_t n, bool masked, uint64_t hole) {
-    __builtin_amdgcn_s_setprio(1);  // ahead of the other workgroup's softmax
-    scores(n);
-    read_v(n + 1, 0, vf[0]);  // the buffer of tile n - 1
-    if (masked) {
-      // Bit j of `seen`: this half's token j, of 64, is attended; its scores are tokens
-      // 32 tt + 8 (i / 4) + i % 4.
-      const int32_t lo = my_begin - t0 - static_cast<int32_t>(4 * half);
-      const int32_t hi = my_end - t0 - static_cast<int32_t>(4 * half);
-      const uint64_t seen = bits_below(hi) & ~bits_below(lo) & ~(hole >> (4 * half));
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const int32_t word = static_cast<int32_t>(seen >> (32 * tt));
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int b = 8 * (i / 4) + i % 4;
-          const uint32_t keep = static_cast<uint32_t>(word << (31 - b) >> 31);
-          const float x = s[tt][i];
-          s[tt][i] = __builtin_bit_cast(
-              float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
-        }
-      }
-    }
-    float top = s[0][0];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tt][i]);
-    top = max32(top);
-    top *= a.scale_log2;
-    bool grown = __any(top - m > lag<Row, DP>());
-    float keep = 1.0f;
-    if (grown) {
-      const float m_new = fmaxf(m, kLift ? floorf(top) : top);
-      keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-    }
-    float base = m == kNegInf ? 0.0f : -m;
-    if constexpr (kLift) {
-      if (__any(fmaxf(vs[0], vs[1]) > lift_limit)) {  // some row may not have room for it
-        const float* scale = lds.k[n % Lds::kBuffers].v_scale + 4 * half;
-        float big = 0.0f;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            big = fmaxf(big, s[tt][i] == kNegInf ? 0.0f : scale[32 * tt + 8 * (i / 4) + i % 4]);
-        keep *= lower_lift(max32(big), &lift, &lift_limit);
-        grown = true;
-      }
-      base += lift;
-    }
-    if constexpr (kFixed) base += kFp16Room;
-    float sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (u < 3) read_v(n + 1, u + 1, vf[(u + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
-      add_v(vf[u & 1], p[u]);
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float z = s[u / 2][8 * (u & 1) + i];
-        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z, a.scale_log2, base));
-        sum += x[i];
-      }
-      if constexpr (kCodes) {
-        if (u & 1)
-          scale_by<8>(x, vs[u / 2], std::make_integer_sequence<int, 8>());
-        else
-          scale_by<0>(x, vs[u / 2], std::make_integer_sequence<int, 8>());
-        if (masked) {  // a hidden token's scale may be anything
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (s[u / 2][8 * (u & 1) + i] == kNegInf) x[i] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[u][j] = Mat<Row>::pack(x[2 * j], x[2 * j + 1]);
-      asm volatile("" : "+v"(p[u]), "+v"(sum));  // here, beside the products
-#pragma unroll
-      for (uint32_t i = 0; i < DP / 32; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
-        __builtin_amdgcn_sched_group_barrier(0x402, 8, 0);  // vector and exponentials
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    __builtin_amdgcn_s_setprio(0);
-    l = l * keep + sum;
-    if (grown) {  // the outputs up to tile n - 1
-#pragma unroll
-      for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= keep;
-    }
-  };
-
-  if (tid == 0) lds.odd = 0;
-  // Values past the head's size, and V before the first tile, which meets weights of 0.
-#pragma unroll
-  for (uint32_t i = 0; i < kLoads; ++i)
-#pragma unroll
-    for (uint32_t j = 0; j < kPer / 8; ++j) {
-      const uint32_t tok = my_tok + i * kLoadTokens;
-      if (my_d >= DP) continue;
-#pragma unroll
-      for (uint32_t b = 0; b < Lds::kBuffers; ++b) {
-        if (!my_col)
-          reinterpret_cast<u32x4*>(lds.k[b].data + tok * kKP + my_d * 2)[j] = u32x4{0, 0, 0, 0};
-        reinterpret_cast<u32x4*>(lds.v[b].data + tok * kVP + my_d * 2)[j] = u32x4{0, 0, 0, 0};
-      }
-    }
-  if (begin < end) {
-    fill_ring(0);
-    __syncthreads();
-    load_k(0);
-    // Tokens' places first: a short pass is all latency.
-    if constexpr (SHARED) load_q();
-    uint64_t there = tokens_there(0), v_there = ~0ull;
-    bool v_masked = false;
-    uint32_t n = 0;
-    for (int32_t t0 = begin; t0 < end; t0 += kStep, ++n) {
-      const bool masked = t0 < all_begin || t0 + kStep > all_end || ~there;
-      if (Lds::kBuffers == 1) __syncthreads();  // the tiles before have been read
-      store_k(n);
-      if (n) store_v(n - 1, v_masked, v_there);
-      if ((n + 1) * tile_units % (kRing / 2) == 0) fill_ring(n + 1);
-      __syncthreads();
-      read_k(n, 0, kf[0]);
-      v_masked = masked;
-      v_there = there;
-      there = tokens_there(n + 1);
-      load_v(n);
-      load_k(n + 1);
-      if (wave_rows) step(t0, n, masked, ~v_there);
-    }
-    if (Lds::kBuffers == 1) __syncthreads();
-    store_v(n - 1, v_masked, v_there);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      read_v(n - 1, u, vf[u & 1]);
-      add_v(vf[u & 1], p[u]);
-    }
-  }
-
-  if constexpr (kLift) {
-    const float down = __builtin_amdgcn_exp2f(-lift);
-    l *= down;
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[dt][i] *= down;
-  }
-  __syncthreads();
-  bool odd = TYPE != PF_KV_INT8 && lds.odd;
-  if constexpr (!kCodes) odd |= __any(t.valid & (l == l) & any_nan<16>(o));
-  // Those of every tile: where none was cleared the products have them already, and once
-  // more changes nothing.
-  if (__builtin_expect(odd, 0)) {
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt) lose_nan<16>(o[dt]);
-    for (int32_t t0 = begin; t0 < end; t0 += kStep) {
-      const uint64_t tokens = odd_tokens<Row, TYPE>(pg, table, head, t0, end);
-      for (uint64_t left = tokens; left; left &= left - 1) {
-        const int32_t tok = t0 + __builtin_ctzll(left);
-        if (tok < my_begin || tok >= my_end) continue;
-        uint64_t at, scale_at;
-        const uint32_t page = page_of(pg, tok);
-        token_at(pg, table[page], tok, page, head, &at, &scale_at);
-#pragma unroll
-        for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            float x[4] = {o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
-            add_odd<Row, TYPE>(pg.v + at, dt * 32 + 8 * i + 4 * half, pg.dim, x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[dt][4 * i + j] = x[j];
-          }
-      }
-      if (!tokens) continue;
-      bool settled = true;  // NaN throughout, which nothing changes
-#pragma unroll
-      for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-          settled &= o[dt][i] != o[dt][i] || dt * 32 + 8 * (i / 4) + 4 * half >= pg.dim;
-      if (!__any(t.valid && !settled)) break;
-    }
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt) restore_nan<16>(o[dt]);
-  }
-
-  l = sum32(l);
-  if constexpr (SHARED) {
-    if (!t.valid) return;
-    const uint32_t token = t.row / group, g = t.row - token * group;
-    const uint64_t at = share_at(a, split, t.s.first + token, head * group + g);
-    f32x4* part = reinterpret_cast<f32x4*>(a.share_o + at * DP) + half;
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        part[dt * 8 + 2 * i] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
-                                     o[dt][4 * i + 3]};
-    if (half == 0) reinterpret_cast<f32x2*>(a.share_ml)[at] = f32x2{m, l};
-    return;
-  }
-  if (used == 1) {
-    many_store<Row, DP>(a, t, o, m, l);
-    return;
-  }
-  // This split's share for attend_many_join_kernel: 16 bytes a lane at a time.
-  if (!wave_rows) return;
-  const uint64_t slot = (rest - a.many_whole) * static_cast<uint64_t>(pg.heads) + head;
-  f32x4* part = reinterpret_cast<f32x4*>(a.many_o) + (slot * kWaves + wave) * (DP / 8) * 64 + lane;
-#pragma unroll
-  for (uint32_t dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      part[(dt * 4 + i) * 64] = f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2],
-                                      o[dt][4 * i + 3]};
-  reinterpret_cast<f32x2*>(a.many_ml)[(slot * kWaves + wave) * 64 + lane] = f32x2{m, l};
-}
-
 template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>
 __global__ void __launch_bounds__(2 * ROWS, DP <= 128 ? 2 : 1)
 attend_many_kernel(AttendParams a) {
   __shared__ ManyLds<DP> lds;
-  attend_many<Row, TYPE, DP, ROWS, false>(a, lds, blockIdx.x);
+  constexpr bool SHARED = false;
+  const uint32_t index = blockIdx.x;
+#include "pf_attend_many.inc"
 }
 
 // Joins the shares of split tiles.  A wave takes 32 rows and 32 values of each, in the
@@ -1305,570 +825,13 @@ struct FewLds {
   bool finished;
 };
 
-// Workgroup `index` of attend_few_kernel, or (SHARED) of attend_shared_kernel's tiles of the
-// tokens that a sequence has to itself, 16 rows each, of which each takes own_waves waves.
-template <class Row, uint32_t TYPE, uint32_t DP, bool SHARED>
-__device__ __forceinline__ void attend_few(const AttendParams& a, FewLds<DP>& mem,
-                                           uint32_t index) {
-  constexpr bool kCodes = is_codes(TYPE);
-  constexpr bool kLift = kCodes && Row::kType == PF_KV_FP16;
-  constexpr bool kFixed = !kCodes && Row::kType == PF_KV_FP16;
-  constexpr uint32_t kPer = kCodes ? 16 : 8;
-  constexpr uint32_t kKLoads = DP / (4 * kPer) + (DP % (4 * kPer) ? 1 : 0);  // of 16 tokens
-  constexpr uint32_t kCols = DP / kPer;
-  constexpr uint32_t kVLoads = (kFewTokens * kCols + 63) / 64;
-  constexpr uint32_t kVP = few_v_pitch(DP);
-  constexpr uint32_t kSteps = kKLoads * (kCodes ? 2 : 1);  // products of 32 values
-  using WaveLds = typename FewLds<DP>::Wave;
-  WaveLds (&lds)[kFewWaves] = mem.wave;
-  float (&join_m)[kFewWaves][16] = mem.join_m, (&join_l)[kFewWaves][16] = mem.join_l;
-  bool& finished = mem.finished;
-  const PagedView& pg = a.pages;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, col = lane & 15u, quarter = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // The waves that share a unit: this one's place among them, and the first.
-  const uint32_t waves = SHARED ? a.own_waves : kFewWaves;
-  const uint32_t turn = SHARED ? wave % waves : wave, wave0 = wave - turn;
-  bool active = true;  // SHARED: of a unit without a share, whose waves only meet the others
-  uint32_t unit = index;
-  if constexpr (SHARED) {
-    unit = index * (kFewWaves / waves) + wave / waves;
-    active = unit < a.num_seqs * a.own_tiles * a.own_splits * pg.heads;
-    if (!active) unit = 0;
-  }
-  const uint32_t head = unit % pg.heads;
-  const uint32_t rest = unit / pg.heads;
-  const uint32_t splits = SHARED ? a.own_splits : a.few_splits, split = rest % splits;
-  const uint32_t seq = SHARED ? rest / splits / a.own_tiles : rest / splits;
-  const uint32_t row0 = SHARED ? rest / splits % a.own_tiles * kFewRows : 0;
-  const int32_t* table = a.block_table + seq * a.table_stride;
-  // Without a window a share starts at a token known from here on: a launch that is all
-  // latency asks for its first block beside the sequence's length (a token behind 10,000
-  // gains 0.8 us; where shares wait for their turn it costs 2%).
-  const bool ask_early = !SHARED && !a.window && gridDim.x <= 512;
-  int32_t early_block = -1;
-  if (ask_early)
-    early_block = table[page_of(pg, min(split * a.few_piece + wave * kFewTokens + (lane & 31u),
-                                        a.table_width * pg.block_size - 1))];
-  const Seq sq = seq_of(a, seq);
-  uint32_t rows = static_cast<uint32_t>(sq.rows) * a.group;
-  int32_t shared = 0;
-  if constexpr (SHARED) {
-    active = active && rows > row0;
-    rows = active ? min(rows - row0, kFewRows) : 1;
-    shared = shared_of(a, static_cast<int32_t>(seq), sq);
-  } else {
-    if (rows > kFewRows) {
-      if (a.many_units) return;  // attend_many_kernel's
-      rows = kFewRows;
-    }
-    if (rows > a.few_rows_most) rows = a.few_rows_most;  // more than the batch was said to have
-    if (rows == 0) return;
-  }
-  const int32_t pos0 = sq.len - sq.rows;
-  uint8_t* v_lds = lds[wave].v;
-
-  const uint32_t row = row0 + col, last = row0 + rows - 1;
-  const bool valid = col < rows;
-  const int32_t pos = pos0 + static_cast<int32_t>(row / a.group);
-  const int32_t my_begin = SHARED ? shared : row_begin(a, pos);
-  const int32_t my_end = valid ? row_end(a, sq.len, pos) : 0;
-  int32_t begin = SHARED ? shared : row_begin(a, pos0) & ~static_cast<int32_t>(kFewTokens - 1);
-  int32_t end = row_end(a, sq.len, pos0 + static_cast<int32_t>(last / a.group));
-  const int32_t all_begin =
-      SHARED ? shared : row_begin(a, pos0 + static_cast<int32_t>(last / a.group));
-  const int32_t all_end = row_end(a, sq.len, pos0 + static_cast<int32_t>(row0 / a.group));
-  uint32_t used = 0;
-  if constexpr (SHARED) {
-    // Shares are those of the sequence, and the same for all its tiles.
-    const int32_t tile_end = end;
-    end = row_end(a, sq.len, pos0 + sq.rows - 1);
-    used = split_range(begin, end, split, splits, a.own_piece);
-    end = min(end, tile_end);
-    active = active && split < used;
-    // The join is told how many there are of each kind, 0 of a row beyond the tiles.
-    if (active && head == 0 && split == 0 && row0 == 0 && turn == 0) {
-      int32_t b = 0, e = shared;
-      const uint32_t prefix = shared ? split_range(b, e, 0, a.prefix_splits, a.prefix_piece) : 0;
-      for (uint32_t i = lane; i < static_cast<uint32_t>(sq.rows); i += 64)
-        a.share_info[sq.first + i] =
-            (i + 1) * a.group <= a.own_tiles * kFewRows ? prefix | used << 8 : 0;
-    }
-    if (!active) end = begin;
-  } else {
-    used = split_range(begin, end, split, splits, a.few_piece);
-    if (split >= used) return;
-  }
-  const uint32_t token = row / a.group, g = row - token * a.group;
-  const uint64_t q_row = a.q.data + ((sq.first + static_cast<uint64_t>(token)) * a.q.token_stride +
-                                     static_cast<uint64_t>(head * a.group + g) * a.q.head_stride) *
-                                        2;
-  u32x4 q[kSteps];
-  auto load_q = [&] {
-#pragma unroll
-    for (uint32_t i = 0; i < kSteps; ++i)
-      q[i] = load_q8(q_row,
-                     kCodes ? (i / 2) * 64 + quarter * 16 + (i & 1) * 8 : i * 32 + quarter * 8, a,
-                     valid && active);
-  };
-  if constexpr (!SHARED) load_q();
-  f32x4 o[DP / 16];
-#pragma unroll
-  for (uint32_t dt = 0; dt < DP / 16; ++dt) o[dt] = f32x4{0, 0, 0, 0};
-  float m = kNegInf, l = 0.0f;
-  bool odd = false;  // some tile attended in part holds V that is not finite
-  float lift = valid ? kLiftStart : kLiftNone, lift_limit = 0.0f;  // kLift
-
-  u32x4 kr[2][kKLoads], vr[kVLoads];
-  // Token t0 + lane of a tile, lanes 0 to 31: its block (of the tile to load next), its
-  // place and, once the tile is on its way, its scales.  A token past the end or
-  // without a block reads some other place: it is masked and its V zeroed.
-  int32_t block = -1;
-  float k_scale = 0.0f, v_scale = 0.0f;
-  uint32_t there = 0;  // bit j: token j of the tile has a block
-  auto load_block = [&](int32_t t0) {
-    const int32_t tok = t0 + static_cast<int32_t>(lane & 31u);
-    block = tok < end ? table[page_of(pg, tok)] : -1;
-  };
-  // d of this lane's part of K and V (some other value where there is none).
-  uint32_t k_at[kKLoads], v_at[kVLoads];
-#pragma unroll
-  for (uint32_t i = 0; i < kKLoads; ++i) {
-    const uint32_t d = (i * 4 + quarter) * kPer;
-    k_at[i] = (d < pg.dim ? d : 0) * (kCodes ? 1 : 2);
-  }
-#pragma unroll
-  for (uint32_t i = 0; i < kVLoads; ++i) {
-    const uint32_t d = (lane + i * 64) % kCols * kPer;
-    v_at[i] = (d < pg.dim ? d : 0) * (kCodes ? 1 : 2);
-  }
-  auto load = [&](int32_t t0) {
-    const int32_t tok = t0 + static_cast<int32_t>(lane & 31u);
-    uint64_t place, scale_place;
-    const bool in =
-        token_at(pg, block, tok, page_of(pg, tok), head, &place, &scale_place);
-    there = static_cast<uint32_t>(__ballot(in));
-    if (lane < 32) {
-      lds[wave].at[lane] = in ? place : 0;
-      if constexpr (kCodes) {
-        if (!in) scale_place = pg.scale_offset;
-        k_scale = *reinterpret_cast<const g_f32*>(pg.k + scale_place);
-        v_scale = *reinterpret_cast<const g_f32*>(pg.v + scale_place);
-      }
-    }
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const uint64_t at = pg.k + lds[wave].at[tt * 16 + col];
-#pragma unroll
-      for (uint32_t i = 0; i < kKLoads; ++i)
-        kr[tt][i] = *reinterpret_cast<const g_u32x4*>(at + k_at[i]);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kVLoads; ++i)
-      vr[i] = *reinterpret_cast<const g_u32x4*>(
-          pg.v + lds[wave].at[(lane + i * 64) / kCols] + v_at[i]);
-  };
-
-  const int32_t kStep = static_cast<int32_t>(kFewTokens * waves);
-  auto tile = [&](int32_t t0) {
-    const bool partial = t0 < all_begin || t0 + static_cast<int32_t>(kFewTokens) > all_end;
-    const bool masked = partial || there != 0xffffffffu;
-    // V into LDS.
-    if (masked) {
-#pragma unroll
-      for (uint32_t i = 0; i < kVLoads; ++i) {
-        const uint32_t j = (lane + i * 64) / kCols;
-        if (!(there >> j & 1u)) vr[i] = u32x4{0, 0, 0, 0};
-        odd |= clear_odd<Row, TYPE>(vr[i]);
-      }
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kVLoads; ++i) {
-      const uint32_t c = lane + i * 64, j = c / kCols, cc = c % kCols;
-      u32x4 v0 = vr[i], v1{0, 0, 0, 0};
-      if constexpr (kCodes) {
-        const u32x2 b0 = codes_to_16<Row, TYPE>(vr[i][0]), b1 = codes_to_16<Row, TYPE>(vr[i][1]);
-        const u32x2 b2 = codes_to_16<Row, TYPE>(vr[i][2]), b3 = codes_to_16<Row, TYPE>(vr[i][3]);
-        v0 = u32x4{b0[0], b0[1], b1[0], b1[1]};
-        v1 = u32x4{b2[0], b2[1], b3[0], b3[1]};
-      }
-      u32x4* vd = reinterpret_cast<u32x4*>(v_lds + j * kVP + cc * (kCodes ? 32 : 16));
-      vd[0] = v0;
-      if constexpr (kCodes) vd[1] = v1;
-    }
-    if constexpr (kCodes) {
-      if (lane < 32) {
-        lds[wave].k_scale[lane] = k_scale;
-        lds[wave].v_scale[lane] = v_scale;
-      }
-    }
-    if (pg.dim != DP) {  // values past the head's size
-#pragma unroll
-      for (uint32_t i = 0; i < kKLoads; ++i)
-        if ((i * 4 + quarter) * kPer >= pg.dim) kr[0][i] = kr[1][i] = u32x4{0, 0, 0, 0};
-    }
-    // S^T: this lane's row `col`, tokens 16 tt + 4 quarter + i.
-    f32x4 s[2];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      s[tt] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (uint32_t i = 0; i < kKLoads; ++i) {
-        if constexpr (kCodes) {
-          const u32x2 a0 = codes_to_16<Row, TYPE>(kr[tt][i][0]);
-          const u32x2 a1 = codes_to_16<Row, TYPE>(kr[tt][i][1]);
-          const u32x2 a2 = codes_to_16<Row, TYPE>(kr[tt][i][2]);
-          const u32x2 a3 = codes_to_16<Row, TYPE>(kr[tt][i][3]);
-          s[tt] = Mat<Row>::mul16(u32x4{a0[0], a0[1], a1[0], a1[1]}, q[2 * i], s[tt]);
-          s[tt] = Mat<Row>::mul16(u32x4{a2[0], a2[1], a3[0], a3[1]}, q[2 * i + 1], s[tt]);
-        } else {
-          s[tt] = Mat<Row>::mul16(kr[tt][i], q[i], s[tt]);
-        }
-      }
-    }
-    float wv[2][4];
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      f32x4 x{1, 1, 1, 1}, y{1, 1, 1, 1};
-      if constexpr (kCodes) {
-        x = *reinterpret_cast<const f32x4*>(lds[wave].k_scale + tt * 16 + quarter * 4);
-        y = *reinterpret_cast<const f32x4*>(lds[wave].v_scale + tt * 16 + quarter * 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (kCodes) s[tt][i] *= x[i];
-        wv[tt][i] = y[i];
-      }
-    }
-    const uint32_t seen_blocks = there;
-    const bool lower = kLift && __any(v_scale > lift_limit);
-    if (t0 + kStep < end) {
-      load(t0 + kStep);
-      load_block(t0 + 2 * kStep);
-    }
-    if (masked) {
-      // Bit 16 tt + i: this lane's token 16 tt + 4 quarter + i is attended.
-      const int32_t at = t0 + static_cast<int32_t>(quarter) * 4;
-      const uint32_t seen =
-          static_cast<uint32_t>(bits_below(my_end - at) & ~bits_below(my_begin - at)) &
-          (seen_blocks >> (quarter * 4));
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t keep =
-              static_cast<uint32_t>(static_cast<int32_t>(seen << (31 - tt * 16 - i)) >> 31);
-          const float x = s[tt][i], y = wv[tt][i];
-          s[tt][i] = __builtin_bit_cast(
-              float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
-          wv[tt][i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & keep);
-        }
-    }
-    float top = kNegInf;
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[tt][i]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = max32(top);
-    top *= a.scale_log2;
-    if (__any(top - m > lag<Row, DP>())) {
-      const float m_new = fmaxf(m, kLift ? floorf(top) : top);
-      const float keep = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-      m = m_new;
-      l *= keep;
-#pragma unroll
-      for (uint32_t dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
-    }
-    float base = m == kNegInf ? 0.0f : -m;
-    if constexpr (kLift) {
-      if (lower) {  // a scale that some row may not have room for; hidden ones are 0 here
-        float big = 0.0f;
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) big = fmaxf(big, wv[tt][i]);
-        big = fmaxf(big, __shfl_xor(big, 16));
-        const float keep = lower_lift(max32(big), &lift, &lift_limit);
-        l *= keep;
-#pragma unroll
-        for (uint32_t dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[dt][i] *= keep;
-      }
-      base += lift;
-    }
-    if constexpr (kFixed) base += kFp16Room;
-#pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, base));
-        l += w;
-        wv[tt][i] *= w;
-      }
-    // Each weight as two numbers of 16 bits, the second what the first's rounding left: the
-    // matrix cores have time here, and outputs are off by little more than their own
-    // rounding (twice that with the first alone, of a few tokens).  The product costs 2% at
-    // 32 sequences behind 1,000 tokens, and nothing measurable elsewhere.
-    u32x4 w, rest;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = wv[i / 2][2 * (i & 1)], y = wv[i / 2][2 * (i & 1) + 1];
-      const uint32_t word = Mat<Row>::pack(x, y);
-      const f32x2 held = Mat<Row>::unpack(word);
-      w[i] = word;
-      float rest_x = x - held[0], rest_y = y - held[1];
-      if constexpr (kCodes) {  // an infinite scale leaves no number
-        rest_x = rest_x == rest_x ? rest_x : 0.0f;
-        rest_y = rest_y == rest_y ? rest_y : 0.0f;
-      }
-      rest[i] = Mat<Row>::pack(rest_x, rest_y);
-    }
-    // Every lane of the wave has stored its part of V before any reads another's.
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const uint8_t* v_from = v_lds + (quarter * 4 + col / 4) * kVP + (col & 3u) * 8;
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt) {
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_from + dt * 32));
-      const s16x4 hi =
-          __builtin_amdgcn_ds_read_tr16_b64_v4i16((l_s16x4*)(v_from + 16 * kVP + dt * 32));
-      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-      o[dt] = Mat<Row>::mul16(u32x4{x[0], x[1], y[0], y[1]}, w, o[dt]);
-      o[dt] = Mat<Row>::mul16(u32x4{x[0], x[1], y[0], y[1]}, rest, o[dt]);
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  };
-  int32_t t0 = begin + static_cast<int32_t>(turn * kFewTokens);
-  if (t0 < end) {
-    if (ask_early)
-      block = t0 + static_cast<int32_t>(lane & 31u) < end ? early_block : -1;
-    else
-      load_block(t0);
-    load(t0);
-    load_block(t0 + kStep);
-    if constexpr (SHARED) load_q();  // tokens' places first: a short pass is all latency
-  }
-  for (; t0 < end; t0 += kStep) tile(t0);
-  if constexpr (kLift) {
-    const float down = __builtin_amdgcn_exp2f(-lift);
-    l *= down;
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[dt][i] *= down;
-  }
-  // Those of all of this wave's tiles, as in attend_many_kernel.
-  if constexpr (!kCodes) odd |= valid & (l == l) & any_nan<4>(o);
-  if (TYPE != PF_KV_INT8 && __builtin_expect(__any(odd), 0)) {
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt) lose_nan<4>(o[dt]);
-    for (int32_t t1 = begin + static_cast<int32_t>(turn * kFewTokens); t1 < end; t1 += kStep) {
-      const uint64_t tokens = odd_tokens<Row, TYPE>(
-          pg, table, head, t1, min(end, t1 + static_cast<int32_t>(kFewTokens)));
-      for (uint64_t left = tokens; left; left &= left - 1) {
-        const int32_t tok = t1 + __builtin_ctzll(left);
-        if (tok < my_begin || tok >= my_end) continue;
-        uint64_t at, scale_at;
-        const uint32_t page = page_of(pg, tok);
-        token_at(pg, table[page], tok, page, head, &at, &scale_at);
-#pragma unroll
-        for (uint32_t dt = 0; dt < DP / 16; ++dt) {
-          float x[4] = {o[dt][0], o[dt][1], o[dt][2], o[dt][3]};
-          add_odd<Row, TYPE>(pg.v + at, dt * 16 + quarter * 4, pg.dim, x);
-          o[dt] = f32x4{x[0], x[1], x[2], x[3]};
-        }
-      }
-      if (!tokens) continue;
-      bool settled = true;
-#pragma unroll
-      for (uint32_t dt = 0; dt < DP / 16; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          settled &= o[dt][i] != o[dt][i] || dt * 16 + quarter * 4 >= pg.dim;
-      if (!__any(valid && !settled)) break;
-    }
-#pragma unroll
-    for (uint32_t dt = 0; dt < DP / 16; ++dt) restore_nan<4>(o[dt]);
-  }
-
-  // Join the waves: each puts its outputs, 16 rows x DP in fp32, into its own part of
-  // LDS (which V no longer needs), and the threads share the sums.
-  l += __shfl_xor(l, 16);
-  l = sum32(l);
-  float* mine = reinterpret_cast<float*>(lds[wave].v);
-  static_assert(sizeof(WaveLds) >= 16 * DP * sizeof(float), "a wave's outputs fit its LDS");
-#pragma unroll
-  for (uint32_t dt = 0; dt < DP / 16; ++dt)
-    *reinterpret_cast<f32x4*>(mine + col * DP + dt * 16 + quarter * 4) = o[dt];
-  if (quarter == 0) {
-    join_m[wave][col] = m;
-    join_l[wave][col] = l;
-  }
-  __syncthreads();
-  const uint64_t slot = (static_cast<uint64_t>(seq) * a.few_splits + split) * pg.heads + head;
-  const __amdgpu_buffer_rsrc_t share = __builtin_amdgcn_make_buffer_rsrc(
-      a.few_o + (!SHARED && used > 1 ? slot * a.few_rows_most * DP : 0), 0,
-      static_cast<int>(a.few_rows_most * DP * 4), 0x00027000);
-  if (!active) return;
-  for (uint32_t i = tid - wave0 * 64; i < 16 * DP / 4; i += waves * 64) {
-    const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (r >= rows) continue;
-    float top = kNegInf;
-#pragma unroll
-    for (uint32_t w = 0; w < kFewWaves; ++w)
-      if (w < waves) top = fmaxf(top, join_m[wave0 + w][r]);
-    float sum = 0.0f;
-    f32x4 x{0, 0, 0, 0};
-#pragma unroll
-    for (uint32_t w = 0; w < kFewWaves; ++w) {
-      if (w >= waves) break;
-      const float mw = join_m[wave0 + w][r], lw = join_l[wave0 + w][r];
-      const float keep = mw == kNegInf ? (lw == 0.0f ? 0.0f : 1.0f)
-                                       : share_factor(mw - top);
-      sum += lw * keep;
-      const f32x4 y = *reinterpret_cast<const f32x4*>(
-          reinterpret_cast<const float*>(lds[wave0 + w].v) + r * DP + d);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += y[j] * keep;
-    }
-    if constexpr (SHARED) {
-      const uint32_t tok = (row0 + r) / a.group, qh = head * a.group + (row0 + r) - tok * a.group;
-      const uint64_t at = share_at(a, a.prefix_splits + split, sq.first + tok, qh);
-      *reinterpret_cast<f32x4*>(a.share_o + at * DP + d) = x;
-      if (d == 0) reinterpret_cast<f32x2*>(a.share_ml)[at] = f32x2{top, sum};
-      continue;
-    }
-    if (used > 1) {
-      // Written through the XCD's L2 (the sc1 policy of agent-scope stores, which the
-      // language offers for at most 8 bytes at a time).
-      constexpr int kSc1 = 16;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), share,
-                                             static_cast<int>((r * DP + d) * 4), 0, kSc1);
-      if (d == 0)
-        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.few_ml) + slot * a.few_rows_most + r,
-                           __builtin_bit_cast(uint64_t, f32x2{top, sum}), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-    } else {
-      few_store<Row>(a, sq, head, r, d, x, top, sum);
-    }
-  }
-  if (SHARED || used == 1) return;
-  // The split that finishes last joins them all, in order.  Shares go through the XCD's
-  // L2 to where every XCD sees them; a workgroup counts itself once its stores have been
-  // acknowledged, and the last one puts the count back to 0 for the next call.
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  uint32_t* count = a.few_count + (static_cast<uint64_t>(seq) * pg.heads + head) * kCountStride;
-  if (tid == 0) {
-    const uint32_t before =
-        __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (before + 1 == used)
-      __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    finished = before + 1 == used;
-  }
-  __syncthreads();
-  if (!finished) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  const uint64_t slot0 = static_cast<uint64_t>(seq) * a.few_splits * pg.heads + head;
-  const f32x2* ml = reinterpret_cast<const f32x2*>(a.few_ml);
-  // 4 values an item; where there are fewer items than threads, groups of threads share
-  // the splits out and add up in LDS.
-  const uint32_t items = rows * (DP / 4);
-  uint32_t groups = 1;
-  while (groups * 2 * items <= kFewThreads) groups *= 2;
-  const uint32_t group = tid / items;
-  const uint64_t stride = static_cast<uint64_t>(pg.heads) * a.few_rows_most * DP;
-  const uint32_t first = groups > 1 ? group : 0;
-  auto part = [&](uint32_t i, uint32_t s) {
-    return *reinterpret_cast<const f32x4*>(a.few_o + (slot0 * a.few_rows_most + i / (DP / 4)) * DP +
-                                           i % (DP / 4) * 4 + s * stride);
-  };
-  // The first shares' values are under way while their factors are computed.
-  constexpr uint32_t kAhead = 8;
-  const uint32_t item = groups > 1 ? tid - group * items : tid;
-  f32x4 ahead[kAhead];
-#pragma unroll
-  for (uint32_t j = 0; j < kAhead; ++j)
-    if (group < groups && item < items && first + j * groups < used)
-      ahead[j] = part(item, first + j * groups);
-  // Each share's factor exp(m - largest m), of every row, and the rows' sums.
-  static_assert(sizeof(lds) >= kFewMaxSplits * 64 + kFewThreads * 16, "factors and sums fit");
-  float* factor = reinterpret_cast<float*>(lds);  // [used][16]
-  for (uint32_t r = wave; r < rows; r += kFewWaves) {
-    constexpr uint32_t kEach = kFewMaxSplits / 64;
-    f32x2 y[kEach];
-    float largest = kNegInf;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-      const uint32_t s = lane + j * 64;
-      y[j] = f32x2{kNegInf, 0.0f};
-      if (s < used) y[j] = ml[(slot0 + s * pg.heads) * a.few_rows_most + r];
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) largest = fmaxf(largest, y[j][0]);
-    // Lanes from `used` on hold nothing.
-    for (uint32_t step = 1; step < 64 && step < used; step *= 2)
-      largest = fmaxf(largest, __shfl_xor(largest, step));
-    float sum = 0.0f;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-      // A share without a maximum attended nothing, or only what is no number.
-      const float f = y[j][0] == kNegInf
-                          ? (y[j][1] == 0.0f ? 0.0f : 1.0f)
-                          : share_factor(y[j][0] - largest);
-      if (lane + j * 64 < used) factor[(lane + j * 64) * 16 + r] = f;
-      sum += y[j][1] * f;
-    }
-    for (uint32_t step = 1; step < 64 && step < used; step *= 2) sum += __shfl_xor(sum, step);
-    if (lane == 0) {
-      join_m[0][r] = largest;
-      join_l[0][r] = sum;
-    }
-  }
-  __syncthreads();
-  f32x4* sums = reinterpret_cast<f32x4*>(factor + used * 16);
-  for (uint32_t i0 = 0; i0 < items; i0 += kFewThreads) {
-    const uint32_t i = groups > 1 ? tid - group * items : i0 + tid;
-    const uint32_t r = i / (DP / 4), d = i % (DP / 4) * 4;
-    const bool mine = groups > 1 ? group < groups : i < items;
-    f32x4 x{0, 0, 0, 0};
-    if (mine) {
-      auto add = [&](uint32_t s, f32x4 y) {
-        const float f = factor[s * 16 + r];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] += y[j] * f;
-      };
-      uint32_t s = first;
-      if (i0 == 0)
-#pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j, s += groups)
-          if (s < used) add(s, ahead[j]);
-#pragma unroll 8
-      for (; s < used; s += groups) add(s, part(i, s));
-    }
-    if (groups > 1) {
-      if (mine) sums[tid] = x;
-      __syncthreads();
-      if (group == 0)
-        for (uint32_t g = 1; g < groups; ++g) {
-          const f32x4 y = sums[g * items + i];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] += y[j];
-        }
-    }
-    if (mine && group * (groups > 1) == 0)
-      few_store<Row>(a, sq, head, r, d, x, join_m[0][r], join_l[0][r]);
-  }
-}
-
 template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
 attend_few_kernel(AttendParams a) {
-  __shared__ FewLds<DP> lds;
-  attend_few<Row, TYPE, DP, false>(a, lds, blockIdx.x);
+  __shared__ FewLds<DP> mem;
+  constexpr bool SHARED = false;
+  const uint32_t index = blockIdx.x;
+#include "pf_attend_few.inc"
 }
 
 template <class Row, uint32_t TYPE, uint32_t DP, uint32_t ROWS>

@@ -26,6 +26,23 @@
 namespace pf {
 namespace {
 
+// Workgroup `index` of the tiles of shared tokens.
+template <class Row, uint32_t TYPE, uint32_t DP>
+__device__ __forceinline__ void attend_shared_tokens(const AttendParams& a, ManyLds<DP>& lds,
+                                                     uint32_t index) {
+  constexpr uint32_t ROWS = kManyRows;
+  constexpr bool SHARED = true;
+#include "pf_attend_many.inc"
+}
+
+// Workgroup `index` of the tiles of sequences' own tokens.
+template <class Row, uint32_t TYPE, uint32_t DP>
+__device__ __forceinline__ void attend_own_tokens(const AttendParams& a, FewLds<DP>& mem,
+                                                  uint32_t index) {
+  constexpr bool SHARED = true;
+#include "pf_attend_few.inc"
+}
+
 template <class Row, uint32_t TYPE, uint32_t DP>
 __global__ void __launch_bounds__(kFewThreads, DP <= 128 ? 2 : 1)
 attend_shared_kernel(AttendParams a) {
@@ -37,9 +54,9 @@ attend_shared_kernel(AttendParams a) {
   // Tiles of shared tokens take the longest: first.
   const uint32_t prefix = a.prefix_units * a.prefix_splits * a.pages.heads;
   if (blockIdx.x < prefix)
-    attend_many<Row, TYPE, DP, kManyRows, true>(a, lds.many, blockIdx.x);
+    attend_shared_tokens<Row, TYPE, DP>(a, lds.many, blockIdx.x);
   else
-    attend_few<Row, TYPE, DP, true>(a, lds.few, blockIdx.x - prefix);
+    attend_own_tokens<Row, TYPE, DP>(a, lds.few, blockIdx.x - prefix);
 }
 
 // Joins the shares of a row: a wave to a query head, 4 values a lane, shares in turn where a
