@@ -796,8 +796,9 @@ enum { PF_SHARED_LEN_ANYWAY = 1 << 30 };
  * heads, that are read once instead of again (by num_seqs, num_groups and the hint of the shared
  * length), or sequences of more than 16 rows, whose own tokens may outweigh it where there are more
  * than 32, or PF_SHARED_LEN_ANYWAY; any other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
- * sequence takes as many as it has cached (in front of its new ones).  args->max_seq_len is used
- * where the hints of `shared` are not both given.
+ * sequence takes as many as it has cached (in front of its new ones).  A call that runs as
+ * pf_kv_attend is shaped by the shorter of args->max_seq_len and the sum of the hints of `shared`,
+ * of those that are given.
  *
  * The weights of shared tokens are rounded to 16 bits once, those of a sequence's own to twice as
  * many; the parts are joined in fp32.  No bits change from call to call. */

@@ -127,8 +127,10 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, const pf_shared_ar
     grid = std::max(shared_grid(p), shared_join_grid(p));
   } else {
     uint64_t longest = a->max_seq_len;
-    if (shared && shared->max_shared_len && shared->max_own_len)
-      longest = static_cast<uint64_t>(shared->max_shared_len) + shared->max_own_len;
+    if (shared && shared->max_shared_len && shared->max_own_len) {
+      const uint64_t both = static_cast<uint64_t>(shared->max_shared_len) + shared->max_own_len;
+      longest = longest ? std::min(longest, both) : both;
+    }
     plan_attend(&p, a->max_query_len, longest, work, bytes);
     const uint64_t left = p.many_units - p.many_whole;
     grid = std::max({static_cast<uint64_t>(p.num_seqs) * p.few_splits,

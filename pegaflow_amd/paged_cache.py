@@ -395,7 +395,8 @@ class PagedKVCache:
     def attend_shared(self, q, out, block_table, seq_lens, query_starts, group_starts, shared_lens,
                       *, scale: float | None = None, causal: bool = True, window: int = 0,
                       lse=None, max_shared_len: int = 0, max_own_len: int = 0,
-                      max_query_len: int = 0, workspace: AttentionWorkspace | None = None,
+                      max_query_len: int = 0, max_seq_len: int = 0,
+                      workspace: AttentionWorkspace | None = None,
                       stream: Stream | None = None) -> None:
         """``attend`` of a batch in which groups of sequences share their first tokens, which
         are passed over once for all of a group (pf_kv_attend_shared).
@@ -407,7 +408,8 @@ class PagedKVCache:
         sequence has behind these, are hints that shape the launch.  Sharing takes a
         ``workspace``, a ``max_query_len`` (at most 64 rows a KV head), no ``window``, and
         enough tokens to be worth it, or a ``max_shared_len`` of ``SHARE_ANYWAY`` or more; else
-        the call runs as ``attend``."""
+        the call runs as ``attend``, shaped by the shorter of these two hints' sum and
+        ``max_seq_len``, if given."""
         starts = _index(group_starts, 1, "int32", "group_starts")
         lens = _index(shared_lens, 1, "int32", "shared_lens")
         groups = shared_lens.shape[0]
@@ -415,7 +417,7 @@ class PagedKVCache:
             raise ValueError(f"{groups} shared lengths and {group_starts.shape[0]} group starts "
                              "(one more than groups)")
         args = self._attend_args(q, out, block_table, seq_lens, query_starts, scale, causal,
-                                 window, lse, 0, max_query_len)
+                                 window, lse, max_seq_len, max_query_len)
         shared = SharedArgs(starts, lens, min(groups, _MOST),
                             _most("max_shared_len", max_shared_len),
                             _most("max_own_len", max_own_len), 0)
