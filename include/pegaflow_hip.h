@@ -792,10 +792,11 @@ enum { PF_SHARED_LEN_ANYWAY = 1 << 30 };
  * all its sequences.  That takes a workspace with room for two shares or more of each row
  * (num_rows * num_q_heads * (4 * head_dim + 8) bytes each, head_dim up to the next of 64, 96, 128,
  * 192, 256), at most 64 rows of a sequence and KV head (max_query_len, or num_rows, says so), no
- * window, and a batch that gains by it: 32 to 96 MiB of K and V or more, by its rows, sequences and
- * heads, that are read once instead of again (by num_seqs, num_groups and the hint of the shared
- * length), or sequences of more than 16 rows, whose own tokens may outweigh it where there are more
- * than 32, or PF_SHARED_LEN_ANYWAY; any other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
+ * window, and a batch that gains by it: of up to 16 rows of a sequence and KV head one that reads 32
+ * to 96 MiB of K and V or more, by its rows, sequences and heads, once instead of again (by num_seqs,
+ * num_groups and the hint of the shared length), of more rows one that is estimated to take no
+ * longer (by these, num_rows and the hint of the own length), and any with PF_SHARED_LEN_ANYWAY; any
+ * other call runs as pf_kv_attend.  New tokens are not shared: of shared_lens a
  * sequence takes as many as it has cached (in front of its new ones).  A call that runs as
  * pf_kv_attend is shaped by the shorter of args->max_seq_len and the sum of the hints of `shared`,
  * of those that are given.

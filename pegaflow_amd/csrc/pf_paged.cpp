@@ -120,8 +120,11 @@ int attend(const pf_kv_pages* pages, const pf_attend_args* a, const pf_shared_ar
   p.aligned = aligned;
   while (p.unit_shift < 4 && !(pv.block_size >> p.unit_shift & 1u)) ++p.unit_shift;
   const uint64_t work = ws ? ws->data : 0, bytes = ws ? ws->bytes : 0;
+  // More rows than the sequences can have are not all theirs.
+  const uint64_t most_new = a->max_query_len ? a->max_query_len : a->num_rows;
+  const uint64_t rows = a->num_rows <= a->num_seqs * most_new ? a->num_rows : 0;
   const bool joined = groups && plan_shared(&p, a->max_query_len, shared->max_shared_len,
-                                            shared->max_own_len, work, bytes);
+                                            shared->max_own_len, work, bytes, rows);
   uint64_t grid = 0;
   if (joined) {
     grid = std::max(shared_grid(p), shared_join_grid(p));

@@ -4,6 +4,8 @@
 
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/pegaflow_hip.h"
@@ -82,6 +84,7 @@ constexpr uint32_t kWideRows = 256;      // and heads have up to kWideMaxDim val
 constexpr uint32_t kWideMaxDim = 128;
 constexpr uint32_t kFewMaxSplits = 192;
 constexpr uint32_t kFewWaves = 4;        // of a workgroup
+constexpr uint32_t kCus = 256;
 // A count of finished shares has a 128-byte line of its own: adds to one line run one
 // after another.  The first kCounts of them (or a sixteenth of a small workspace) are at
 // the workspace's start.
@@ -145,7 +148,6 @@ inline bool wide_tiles(uint64_t seqs, uint64_t rows, uint64_t heads, uint64_t di
 // that a sequence has beyond it may stay as they were.
 inline void plan_attend(AttendParams* p, uint64_t most_new, uint64_t longest, uint64_t ws,
                         uint64_t bytes) {
-  constexpr uint64_t kCus = 256;
   const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
   const uint64_t room = static_cast<uint64_t>(p->table_width) * p->pages.block_size;
   if (longest == 0 || longest > room) longest = room;
@@ -247,26 +249,48 @@ inline double shared_saves(const AttendParams& p, uint64_t rows) {
   return rows > kFewRows / 2 ? kSharedSaves / 3 : kSharedSaves / 2;
 }
 
-// Sequences of more rows than kFewRows plan_attend gives tiles of kManyRows, and there tiles of 16
-// gain whatever is shared (20 rows a head, 8 sequences behind 500 and up to 500 of their own 33.0
-// and 18.5, 64 55.8 and 38.3; 64 rows, 8 35.2 and 20.5), but for those of three tiles of 16 and
-// more, which read their own tokens as often, in batches that fill the chip with tiles of kManyRows
-// as well: where the own tokens outweigh what is saved (8 heads of 128, bf16; 56 rows, 40 sequences
-// behind 16 to 250 and up to 1,000 of their own 43 to 53 and 81 to 88, 64 rows, 64 behind 500 and
-// up to 2,000 133 and 192; 48 rows, 80 behind 250 and up to 1,000 84 and 106, but of codes only from
-// four tiles on: 35 rows of 192, 80 behind 250 and up to 1,000 121 and 109, and of longer ones: 35
-// rows, 40 behind 250 and up to 4,000 210 and 156), or the shares do (56
-// rows, 40 behind 64 and up to 20 of their own 21.0 and 24.9, 48 rows 20.9 and 23.8; 160 68 and 74,
-// 80 of 35 rows 28 to 31 and 26).
-inline bool own_tiles_outweigh(const AttendParams& p, uint64_t rows, double saved, double own,
-                               uint64_t most_own, bool codes) {
-  const uint64_t tiles = (rows + kFewRows - 1) / kFewRows;
-  const uint64_t units = static_cast<uint64_t>(p.num_seqs) * p.pages.heads;
-  if (tiles < 3) return false;
-  if (tiles > 3 && own / 2 > kSharedSaves && own / 2 > saved) return true;
-  if (units < 256) return false;
-  if ((tiles > 3 || (!codes && own > 160e6 && most_own <= 2048)) && own * 0.8 > saved) return true;
-  return units < (tiles > 3 ? 1024u : 512u) && saved < share_bytes(p);
+// For sequences of more rows than kFewRows the times of both ways, in us, are estimated and
+// compared: neither way gains by a simple count of bytes, for attend reads a sequence's own tokens
+// once, in a tile of kManyRows that its rows fill in part, and sharing reads them once for every
+// kFewRows rows.  `most` rows of a sequence and KV head, `mean` on average, stand behind `shared`
+// tokens and up to `own` of their own.  (14,675 random batches of 2 to 320 sequences, 1 to 12 heads
+// of 64 to 256, 17 to 64 rows, timed both ways: by the better way each they take 888 ms, by this rule
+// 902, by attend 1,542, all shared 937; the rule leaves 851 more than 6% slower than the better way and
+// 25 more than 50%.  Of 5,865 others, from which no constant was taken, 367 and 16.)
+
+// attend: the tiles' start, which looks for their sequences; their steps of 64 tokens; of few tiles,
+// in shares of 4 steps or more, the join; and a launch for sequences of up to kFewRows rows, of
+// which there are as many as if rows were spread evenly up to `most`.
+inline double attend_us(const AttendParams& p, double most, double mean, double shared, double own,
+                        bool codes) {
+  const double heads = p.pages.heads, seqs = p.num_seqs, dim = padded_dim(p.pages.dim) / 128.0;
+  const double slots = dim <= 1 ? 2 * kCus : kCus;
+  const double few = std::min(1.0, 2 * (most - mean) / most * (kFewRows / most));
+  const double steps = (shared + own) / 64;
+  const double full = seqs * (1 + mean / kManyRows) * heads / slots;  // the chip, so many times
+  const double shares = std::min(std::max(std::floor(1 / full), 1.0), std::max(steps / 4, 1.0));
+  const double chain = full < 1 ? steps / shares
+                                : std::max(steps, seqs * heads * (1 - few) * steps / slots);
+  const double join = shares > 1 ? 4 + 9.4 * dim * shares * seqs * heads / slots : 0;
+  return 6.4 + std::max(full, 1.0) * (2.9 + 5.4 * seqs / 64) +
+         (codes ? 1.95 : 1.75) * (dim + 0.5) / 1.5 * chain + join +
+         few * (20 + 2.7 * dim * seqs * heads * steps / 1024);
+}
+
+// Sharing, as plan_shared has shaped it: a tile's chain of steps over shared tokens and a wave's over
+// own ones, what all tiles of either kind take of the chip, and the shares' bytes.
+inline double shared_us(const AttendParams& p, double groups, double most, double mean,
+                        double shared, double own, bool codes) {
+  const double heads = p.pages.heads, seqs = p.num_seqs, dim = padded_dim(p.pages.dim) / 128.0;
+  // A sequence's last tile may be part-filled.
+  const double tiles = mean > 0.95 * most ? p.own_tiles
+                                          : std::min(mean / kFewRows + 0.4, 1.0 * p.own_tiles);
+  const double chain = 1.1 * std::min(shared, 1.0 * p.prefix_piece) / 64 +
+                       0.27 * std::min(own, 1.0 * p.own_piece) / 32 / p.own_waves;
+  const double prefix = (seqs * mean / kManyRows + 0.5 * groups) * heads * shared / 64;
+  const double owns = seqs * heads * tiles * own;
+  return 12.4 + dim * (chain + 1.2 * prefix / (2 * kCus) + (codes ? 2.9e-5 : 4.4e-5) * owns) +
+         2.3e-6 * seqs * mean * heads * (512 * dim + 8);
 }
 
 // Workgroups that pass over shared tokens, of the 512 that the chip holds.  Each step of one,
@@ -299,9 +323,10 @@ inline uint64_t prefix_workgroups(uint64_t steps, uint64_t groups, uint64_t dim,
 // have up to `most_own` more and `most_new` rows, joining in `bytes` of workspace at `ws`.  Like
 // plan_attend's, lengths may be wrong and rows too few; a shared length counts for what the block
 // table holds, whatever it says, or, from PF_SHARED_LEN_ANYWAY on, for as much as sharing takes.
+// `rows`: of all sequences together, 0 if that is not known (num_rows may have others behind them).
 // False where the batch is better off, or has to be, attended by plan_attend's kernels.
 inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared,
-                        uint64_t most_own, uint64_t ws, uint64_t bytes) {
+                        uint64_t most_own, uint64_t ws, uint64_t bytes, uint64_t rows = 0) {
   const uint64_t heads = p->pages.heads, group = p->group, dim = padded_dim(p->pages.dim);
   const uint64_t room = static_cast<uint64_t>(p->table_width) * p->pages.block_size;
   if (most_shared == 0) most_shared = room;
@@ -318,11 +343,8 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   const double saved =
       static_cast<double>(p->num_seqs - groups) * static_cast<double>(most_shared) * token;
   const double own = static_cast<double>(p->num_seqs * most_own) * token;
-  if (!anyway &&
-      (most_new * group <= kFewRows
-           ? saved < shared_saves(*p, most_new * group)
-           : own_tiles_outweigh(*p, most_new * group, saved, own, most_own, codes)))
-    return false;
+  const bool few = most_new * group <= kFewRows;
+  if (!anyway && few && saved < shared_saves(*p, most_new * group)) return false;
   // Each group's last tile may be part-filled.
   const uint64_t tiles = (p->num_rows * group + groups * (kManyRows - 1)) / kManyRows;
   const uint64_t prefix = prefix_workgroups(tiles * heads * ceil_div(most_shared, 64), groups, dim,
@@ -366,6 +388,14 @@ inline bool plan_shared(AttendParams* p, uint64_t most_new, uint64_t most_shared
   p->own_splits = static_cast<uint32_t>(own_splits);
   p->own_piece = static_cast<uint32_t>(own_piece);
   p->own_waves = waves;
+  if (!anyway && !few) {
+    const double most = static_cast<double>(most_new * group);
+    const double mean = rows ? std::min(static_cast<double>(rows * group) / p->num_seqs, most) : most / 2;
+    const double s = static_cast<double>(most_shared), o = static_cast<double>(most_own);
+    if (shared_us(*p, static_cast<double>(groups), most, mean, s, o, codes) >
+        1.05 * attend_us(*p, most, mean, s, o, codes))
+      return false;
+  }
   const uint64_t values = (splits + own_splits) * p->num_rows * p->q_heads;
   p->share_info = reinterpret_cast<uint32_t*>(ws + counts);
   p->share_o = reinterpret_cast<float*>(ws + counts + info);
