@@ -12,13 +12,20 @@
 // their shares in fp32, which a second launch joins.
 //
 // 64 sequences behind 10,000 shared tokens and up to 500 of their own (bf16, 32 heads of 128 on 8)
-// take 42 us, 31.7 to 36.6 of them the tiles and 6.8 the join; attend, which reads the shared
-// tokens 64 times, 224.  The bytes alone would take 21 and the products 9: a tile's start is a
+// take 38 to 42 us, 31.7 to 36.6 of them the tiles and 6.8 the join; attend, which reads the shared
+// tokens 64 times, 224 to 231.  The bytes alone would take 21 and the products 9: a tile's start is a
 // chain of loads (groups, lengths, table, K: some 7 us of a cold launch), its steps have one wave
 // a vector unit where own tokens take the other, 1.4 us each, of which half are products and
 // softmax and a third the wait for K and V, and 17 MB of shares are written and read.  256
-// sequences behind 30,000 take 182 to 192 (attend 3,690), 690 TFLOP/s; there tiles of 256 rows
-// were no faster.  64 behind 16,000 and up to 2,000 (e4m3) take 66 to 70 (attend 249).
+// sequences behind 30,000 take 182 to 199 (attend 3,690 to 3,720), 690 TFLOP/s; there tiles of 256
+// rows were no faster.  64 behind 16,000 and up to 2,000 (e4m3) take 66 to 71 (attend 242 to 249).
+//
+// The weights of shared tokens are rounded once to the rows' type, as attend rounds those of more
+// than 16 rows: outputs are off by 0.0022 to 0.0023 relative (bf16; fp16 0.00025 to 0.00029) where
+// the rounding of the output alone takes 0.0017 (0.00021).  The rest of each weight, multiplied as
+// well, brought them to that, but the three batches above took 45, 242 and 74 us instead of 38, 183
+// and 69 (29 drafts behind 4,100, int8, 47 instead of 39), and was left out: who needs it calls
+// attend.
 #pragma once
 
 #include "pf_attend_kernels.h"

@@ -72,11 +72,12 @@ inline uint64_t compact_grid(const CompactParams& p) {
 constexpr uint64_t kCompactFew = 16;
 
 // Columns of a strip: a power of two from kMinShift on.  A token-major row of 8 heads of 128 is 128
-// of them, 2 KB that lie together, and moves best whole: 2,500 of 5,000 tokens in 32 layers (bf16) in strips of 16, 32, 64 and 128
-// columns 139, 135, 131 and 129 us, 4 of each of 32 sequences 27, 15.5, 9.7 and 8.4.  In place,
-// though, a strip's tokens move one chunk after another, and strips are all there is to fill
-// the chip: 2,400 tokens of one sequence 89, 91, 135 and 250 us, of four 309, 296, 309 and 329.
-// To other blocks the chunks go to so many workgroups that 8,192 are at work: 2,048 did in 131.
+// of them, 2 KB that lie together, and moves best whole: 2,500 of 5,000 tokens in 32 layers (bf16)
+// in strips of 16, 32, 64 and 128 columns 139, 135, 131 and 129 us, 4 of each of 32 sequences 27,
+// 15.5, 9.7 and 8.4.  In place, though, a strip's tokens move one chunk after another, and strips
+// are all there is to fill the chip: 2,400 of 4,800 tokens of one sequence (the same layers) 131,
+// 134, 202 and 380 us, of four 529, 507, 511 and 508 (their bytes 123 and 491).  To other blocks the
+// chunks go to so many workgroups that 8,192 are at work: 2,048 did in 131.
 inline void plan_compact(CompactParams* p, uint64_t most, bool in_place) {
   const uint32_t columns = compact_columns(p->pages);
   const bool codes = p->pages.type == PF_KV_E4M3 || p->pages.type == PF_KV_INT8;
