@@ -16,7 +16,7 @@ struct Measured {
 };
 
 // The first 20 of either kind, by a factor of 1.6 or more, of 4,000 random batches that no constant
-// of the rule was taken from; half of the batches with as many new tokens for each sequence.
+// of the rule was taken from; six in ten with as many new tokens for each sequence.
 const Measured kBatches[] = {
     {25, 1, 12, 5, 64, PF_KV_INT8, 9, 225, 80, 104, 24.2, 14.7},
     {3, 1, 12, 5, 128, PF_KV_FP16, 7, 21, 16, 11047, 61.5, 33.4},
